@@ -39,6 +39,8 @@ HIP_SOURCES = [
     "dq_eden.hip", "dq_eden_short.hip",
     "dq_streams.hip",
     "dq_io_floor.hip",
+    "dq_optimizer.hip",
+    "dq_microscale.hip", "dq_microscale_product.hip",
 ]
 
 HIPCC_FLAGS = [

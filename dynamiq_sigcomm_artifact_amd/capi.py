@@ -35,6 +35,8 @@ EXPORTS = [
     "dq_hadamard", "dq_rht_blocked", "dq_rand_diag", "dq_rand_diag_bits", "dq_rht_scaling_compress", "dq_rht_scaling_compress_mfma16", "dq_scaling_decompress_irht", "dq_pack_signs",
     "dq_bins_to_bits", "dq_bits_to_bins", "dq_quantization",
     "dq_eden_work_doubles", "dq_eden_quantize", "dq_eden_quantize_static_max_n", "dq_eden_quantize_static", "dq_eden_dequantize", "dq_eden_dequantize_irht", "dq_eden_slice_bytes", "dq_eden_compress", "dq_eden_decompress", "dq_thc_compress", "dq_thc_compress_drawn", "dq_thc_decompress", "dq_thc_quantize", "dq_thc_dequantize", "dq_thc_rht_quantize", "dq_thc_dequantize_irht",
+    "dq_grad_norm_work_doubles", "dq_grad_norm", "dq_adamw_step", "dq_adamw_coefficients",
+    "dq_mx4_quantize", "dq_mx4_dequantize", "dq_mx4_product",
 ]
 
 STAGE_STATS, STAGE_PLAN, STAGE_COMPRESS, STAGE_DECOMPRESS = 1, 2, 4, 8
@@ -52,6 +54,25 @@ class Bucket(ctypes.Structure):
         ("packed_bytes", ctypes.c_int64), ("out", ctypes.c_void_p), ("hist", ctypes.c_void_p),
         ("hist_ints", ctypes.c_int64), ("seed", ctypes.c_uint64), ("step", ctypes.c_uint64), ("step_dev", ctypes.c_void_p),
     ]
+
+
+class Span(ctypes.Structure):
+    """dq_span_t of include/dynamiq_eden.h"""
+    _fields_ = [("data", ctypes.c_void_p), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """dq_adamw_tensor_t of include/dynamiq_eden.h"""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("n", ctypes.c_int64), ("start", ctypes.c_int64),
+                ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32)]
+
+
+class Adamw(ctypes.Structure):
+    """dq_adamw_t of include/dynamiq_eden.h"""
+    _fields_ = [("state", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("master", ctypes.c_void_p), ("total", ctypes.c_int64),
+                ("bits", ctypes.c_int32), ("reserved", ctypes.c_int32), ("lr", ctypes.c_double), ("beta1", ctypes.c_double),
+                ("beta2", ctypes.c_double), ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64),
+                ("grad_scale", ctypes.c_void_p), ("coefficients", ctypes.c_void_p)]
 
 
 _lib = None
@@ -181,6 +202,20 @@ def lib():
         L.dq_thc_dequantize_irht.argtypes = [vp, vp, i32, vp, i64, i64, f32, vp, vp, i32, vp]
         L.dq_quantization.restype = i32
         L.dq_quantization.argtypes = [vp, i64, i32, f32, f32, u64, vp]
+        L.dq_grad_norm_work_doubles.restype = i64
+        L.dq_grad_norm_work_doubles.argtypes = []
+        L.dq_grad_norm.restype = i32
+        L.dq_grad_norm.argtypes = [c.POINTER(Span), i32, c.c_double, vp, i64, vp, i32, vp]
+        L.dq_adamw_step.restype = i32
+        L.dq_adamw_step.argtypes = [c.POINTER(Adamw), c.POINTER(AdamwTensor), i32, i32, vp]
+        L.dq_adamw_coefficients.restype = i32
+        L.dq_adamw_coefficients.argtypes = [vp, c.c_double, vp, c.c_double, c.c_double, c.c_double, vp, vp, i32, vp]
+        L.dq_mx4_quantize.restype = i32
+        L.dq_mx4_quantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i32, vp, i32, u64, u64, vp, vp, i32, vp]
+        L.dq_mx4_dequantize.restype = i32
+        L.dq_mx4_dequantize.argtypes = [vp, vp, vp, i32, i64, i64, i32, vp]
+        L.dq_mx4_product.restype = i32
+        L.dq_mx4_product.argtypes = [vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, vp]
         _lib = L
     return _lib
 

@@ -180,6 +180,16 @@ inline bool dtype_rand_ok(int dtype)
     return dtype_ok(dtype & 0xf);
 }
 
+// rows x length, the length padded to whole superchunks
+inline bool mx4_size_ok(int64_t rows, int64_t length)
+{
+    return rows >= 1 && length >= 1 && rows <= 0x7fffff00 && length <= 0x7fffff00 && rows * ((length + 255) / 256) < dq::kMxMost / 256;
+}
+inline bool mx4_aligned(const void *codes, const void *scales)
+{
+    return ((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 7)) == 0;
+}
+
 // the production shape: one fused-capable vectorised kernel family
 inline bool hier16_shape(int dtype, int chunk_size, int strategy)
 {
@@ -1103,6 +1113,106 @@ int dq_quantization(float *vec, int64_t n, int device, float div_factor, float t
     int rc;
     if ((rc = select_device(device))) return rc;
     return finish(dq::launch_quantization(vec, n, div_factor, tensor_max, seed, static_cast<hipStream_t>(stream)));
+}
+
+int64_t dq_grad_norm_work_doubles(void) { return 1 + dq::kNormGrid; }
+
+int dq_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work, int64_t work_doubles, float *out, int device,
+                 dq_stream_t stream)
+{
+    if (count < 0) return fail(DQ_ERR_SIZE, "count must not be negative");
+    if ((count && !spans) || !work || !out) return fail(DQ_ERR_NULL);
+    if (!(max_norm > 0)) return fail(DQ_ERR_SIZE, "max_norm must be positive");
+    if (work_doubles < dq_grad_norm_work_doubles()) return fail(DQ_ERR_SIZE, "work buffer is too small (dq_grad_norm_work_doubles)");
+    for (int k = 0; k < count; k++) {
+        if (!dtype_ok(spans[k].dtype)) return fail(DQ_ERR_DTYPE);
+        if (spans[k].n < 0 || spans[k].n >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "n must be in [0, 2^40)");
+        if (spans[k].n && !spans[k].data) return fail(DQ_ERR_NULL);
+    }
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    return finish(dq::launch_grad_norm(spans, count, max_norm, work, out, static_cast<hipStream_t>(stream)));
+}
+
+int dq_adamw_step(const dq_adamw_t *o, const dq_adamw_tensor_t *tensors, int count, int device, dq_stream_t stream)
+{
+    if (count < 0) return fail(DQ_ERR_SIZE, "count must not be negative");
+    if (!o || (count && !tensors)) return fail(DQ_ERR_NULL);
+    if (o->bits != 32 && o->bits != 8) return fail(DQ_ERR_NBITS, "states are held in 32 or in 8 bits");
+    if (o->total < 0 || o->total % dq::kMxBlock || o->total >= (int64_t)1 << 37) return fail(DQ_ERR_SIZE, "total must be a multiple of 32 below 2^37");
+    if (o->total && (!o->state || (o->bits == 8 && !o->scales))) return fail(DQ_ERR_NULL);
+    if ((reinterpret_cast<uintptr_t>(o->state) | reinterpret_cast<uintptr_t>(o->master)) & 15) return fail(DQ_ERR_SIZE, "state and master must be 16-byte aligned");
+    if (!(o->beta1 >= 0 && o->beta1 < 1 && o->beta2 >= 0 && o->beta2 < 1)) return fail(DQ_ERR_SIZE, "beta1 and beta2 must be in [0, 1)");
+    if (!(o->eps >= 0) || !__builtin_isfinite(o->eps)) return fail(DQ_ERR_SIZE, "eps must be a number and not negative");
+    if (!o->coefficients) {
+        if (o->step < 1) return fail(DQ_ERR_SIZE, "step counts from 1");
+        if (!__builtin_isfinite(o->lr) || !__builtin_isfinite(o->weight_decay)) return fail(DQ_ERR_SIZE, "lr and weight_decay must be numbers");
+    }
+    for (int k = 0; k < count; k++) {
+        const dq_adamw_tensor_t &t = tensors[k];
+        if (!dtype_ok(t.param_dtype) || !dtype_ok(t.grad_dtype)) return fail(DQ_ERR_DTYPE);
+        if (o->master && t.param_dtype == DQ_F32) return fail(DQ_ERR_DTYPE, "master weights are for 16-bit parameters");
+        if (t.n < 0 || t.n > dq::kMxMost - 4096) return fail(DQ_ERR_SIZE, "n must be in [0, 2^35 - 4096]");
+        if (t.start < 0 || t.start % dq::kMxBlock || t.start + (t.n + dq::kMxBlock - 1) / dq::kMxBlock * dq::kMxBlock > o->total)
+            return fail(DQ_ERR_SIZE, "start must be a multiple of 32, with room for the tensor in the arenas");
+        if (t.n && (!t.param || !t.grad)) return fail(DQ_ERR_NULL);
+    }
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    return finish(dq::launch_adamw(*o, tensors, count, static_cast<hipStream_t>(stream)));
+}
+
+int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double beta1, double beta2, double weight_decay,
+                          const float *grad_scale, float *coefficients, int device, dq_stream_t stream)
+{
+    if (!steps || !coefficients) return fail(DQ_ERR_NULL);
+    if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1)) return fail(DQ_ERR_SIZE, "beta1 and beta2 must be in [0, 1)");
+    if (!__builtin_isfinite(lr) || !__builtin_isfinite(weight_decay)) return fail(DQ_ERR_SIZE, "lr and weight_decay must be numbers");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    const dq::AdamwCount a = {steps, lr_dev, grad_scale, coefficients, lr, beta1, beta2, weight_decay};
+    return finish(dq::launch_adamw_coefficients(a, static_cast<hipStream_t>(stream)));
+}
+
+int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, int64_t stride, int columns, const uint32_t *sign, int stochastic,
+                    const void *rand_pool, int rand_dtype, uint64_t seed, uint64_t step, uint8_t *codes, uint8_t *scales, int device,
+                    dq_stream_t stream)
+{
+    if (!dtype_ok(dtype) || (rand_pool && !dtype_ok(rand_dtype))) return fail(DQ_ERR_DTYPE);
+    if (!mx4_size_ok(columns ? x_cols : x_rows, columns ? x_rows : x_cols))
+        return fail(DQ_ERR_SIZE, "rows and columns must be positive, with less than 2^35 elements, padding included");
+    if (stride < x_cols || stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
+    if (rand_pool && !stochastic) return fail(DQ_ERR_SIZE, "a rand_pool is for stochastic rounding");
+    if (!x || !codes || !scales) return fail(DQ_ERR_NULL);
+    if (!mx4_aligned(codes, scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    const dq::QuantizeArgs a = {x, x_rows, x_cols, stride, codes, scales, sign, rand_pool, {seed, step}};
+    return finish(dq::launch_mx4_quantize(a, dtype, columns != 0, stochastic != 0, rand_dtype, static_cast<hipStream_t>(stream)));
+}
+
+int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows, int64_t cols, int device, dq_stream_t stream)
+{
+    if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
+    if (!mx4_size_ok(rows, cols)) return fail(DQ_ERR_SIZE, "rows and columns must be positive, with less than 2^35 elements, padding included");
+    if (!out || !codes || !scales) return fail(DQ_ERR_NULL);
+    if (!mx4_aligned(codes, scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    return finish(dq::launch_mx4_dequantize(codes, scales, out, rows, cols, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out, int dtype, int64_t m,
+                   int64_t n, int64_t k, int device, dq_stream_t stream)
+{
+    if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
+    if (!mx4_size_ok(m, k) || !mx4_size_ok(n, k) || !mx4_size_ok(m, n))
+        return fail(DQ_ERR_SIZE, "m, n and k must be positive, with less than 2^35 elements of every matrix, padding included");
+    if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return fail(DQ_ERR_NULL);
+    if (!mx4_aligned(a_codes, a_scales) || !mx4_aligned(b_codes, b_scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    return finish(dq::launch_mx4_product(a_codes, a_scales, b_codes, b_scales, out, m, n, k, dtype, static_cast<hipStream_t>(stream)));
 }
 
 } // extern "C"

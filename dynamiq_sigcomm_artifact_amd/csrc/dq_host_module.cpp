@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/DynamicTypes.h>
@@ -1059,7 +1060,249 @@ PyObject *scaling_decompress_irht(PyObject *, PyObject *const *v, Py_ssize_t hav
     });
 }
 
+// ---- the end of a training step (optimizer.py) and 4-bit matrices (microscale.py) ----------------------------
+// Work goes to the current stream of the tensors' device, and the caller's current device stays what it is.
+
+template <class F> PyObject *answering(Py_ssize_t have, Py_ssize_t want, F body)
+{
+    PyObject *answer = nullptr;
+    PyObject *none = guarded(have, want, [&] { answer = body(); });
+    Py_XDECREF(none);
+    return none ? answer : nullptr;
+}
+
+double number(PyObject *o)
+{
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+    return v;
+}
+
+// the items of a list or tuple
+struct Items {
+    py::object held;
+    PyObject **item;
+    Py_ssize_t count;
+    explicit Items(PyObject *o) : held(py::reinterpret_steal<py::object>(PySequence_Fast(o, "a list of tensors is required")))
+    {
+        if (!held) throw py::error_already_set();
+        item = PySequence_Fast_ITEMS(held.ptr());
+        count = PySequence_Fast_GET_SIZE(held.ptr());
+    }
+};
+
+c10::Device cuda(int device) { return c10::Device(at::kCUDA, (c10::DeviceIndex)device); }
+
+// grads, max_norm, work, out
+PyObject *grad_norm(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return guarded(have, 4, [&] {
+        Args a;
+        const at::Tensor &work = a.typed(v[2], at::kDouble, 0, "work"), &out = a.typed(v[3], at::kFloat, 2, "out");
+        const Items grads(v[0]);
+        std::vector<dq_span_t> spans((size_t)grads.count);
+        for (Py_ssize_t k = 0; k < grads.count; k++) {
+            const at::Tensor &t = a.tensor(grads.item[k]);
+            spans[(size_t)k] = {t.data_ptr(), t.numel(), dtype_code(t), 0};
+        }
+        const double most = number(v[1]);
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const dq_stream_t s = c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream();
+        double *w = work.data_ptr<double>();
+        float *o = out.data_ptr<float>();
+        const int64_t room = work.numel();
+        int rc;
+        {
+            py::gil_scoped_release nogil;
+            rc = dq_grad_norm(spans.data(), (int)spans.size(), most, w, room, o, a.device, s);
+        }
+        check(rc);
+    });
+}
+
+// params, grads, state, scales, master, grad_scale, coefficients, step, lr, beta1, beta2, eps, weight_decay
+PyObject *adamw_step(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return guarded(have, 13, [&] {
+        Args a;
+        const Items params(v[0]), grads(v[1]);
+        if (params.count != grads.count) refuse("adamw_step: as many gradients as parameters are required");
+        dq_adamw_t o;
+        memset(&o, 0, sizeof(o));
+        const at::Tensor &state = a.tensor(v[2]);
+        need(state.dim() == 2 && state.size(0) == 2, "adamw_step: the state has two rows");
+        o.state = state.data_ptr();
+        o.total = state.size(1);
+        if (v[3] == Py_None) {
+            need(state.scalar_type() == at::kFloat, "adamw_step: a state in 32 bits is float32");
+            o.bits = 32;
+        } else {
+            need(state.scalar_type() == at::kByte, "adamw_step: a state in 8 bits is uint8");
+            const at::Tensor &scales = a.typed(v[3], at::kByte, 2 * (o.total / 32), "scales");
+            o.scales = static_cast<uint8_t *>(scales.data_ptr());
+            o.bits = 8;
+        }
+        if (v[4] != Py_None) o.master = a.typed(v[4], at::kFloat, o.total, "master").data_ptr<float>();
+        if (v[5] != Py_None) o.grad_scale = a.typed(v[5], at::kFloat, 1, "grad_scale").data_ptr<float>();
+        if (v[6] != Py_None) o.coefficients = a.typed(v[6], at::kFloat, 4, "coefficients").data_ptr<float>();
+        o.step = integer(v[7]);
+        o.lr = number(v[8]);
+        o.beta1 = number(v[9]);
+        o.beta2 = number(v[10]);
+        o.eps = number(v[11]);
+        o.weight_decay = number(v[12]);
+        std::vector<dq_adamw_tensor_t> tensors;
+        std::vector<Span> spans;
+        tensors.reserve((size_t)params.count);
+        spans.reserve((size_t)params.count);
+        int64_t start = 0;
+        for (Py_ssize_t k = 0; k < params.count; k++) {
+            const at::Tensor &p = a.tensor(params.item[k]);
+            const int64_t n = p.numel();
+            if (grads.item[k] != Py_None) { // no gradient: the parameter and its states stay
+                const at::Tensor &g = a.tensor(grads.item[k]);
+                if (g.numel() != n) refuse("adamw_step: a gradient has as many elements as its parameter");
+                tensors.push_back({p.data_ptr(), g.data_ptr(), n, start, dtype_code(p), dtype_code(g)});
+                if (n) spans.push_back(Span(p, n));
+            }
+            start += (n + 31) / 32 * 32;
+        }
+        if (start != o.total) refuse("adamw_step: the state is of other parameters (adamw_state)");
+        std::sort(spans.begin(), spans.end(), [](const Span &x, const Span &y) { return x.begin < y.begin; });
+        for (size_t k = 1; k < spans.size(); k++)
+            if (spans[k].begin < spans[k - 1].end) refuse("adamw_step: two parameters share memory");
+        if (a.device < 0) refuse("adamw_step: no tensors");
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const dq_stream_t s = c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream();
+        int rc;
+        {
+            py::gil_scoped_release nogil;
+            rc = dq_adamw_step(&o, tensors.data(), (int)tensors.size(), a.device, s);
+        }
+        check(rc);
+        for (Py_ssize_t k = 0; k < params.count; k++) { // what autograd has saved of them is out of date
+            const at::Tensor &p = THPVariable_Unpack(params.item[k]);
+            if (grads.item[k] != Py_None && !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+        }
+    });
+}
+
+// steps, lr (a number or a float32 tensor), beta1, beta2, weight_decay, grad_scale, coefficients
+PyObject *adamw_coefficients(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return guarded(have, 7, [&] {
+        Args a;
+        int64_t *steps = a.typed(v[0], at::kLong, 1, "steps").data_ptr<int64_t>();
+        const float *lr_dev = THPVariable_Check(v[1]) ? a.typed(v[1], at::kFloat, 1, "lr").data_ptr<float>() : nullptr;
+        const double lr = lr_dev ? 0.0 : number(v[1]), beta1 = number(v[2]), beta2 = number(v[3]), decay = number(v[4]);
+        const float *scale = v[5] == Py_None ? nullptr : a.typed(v[5], at::kFloat, 1, "grad_scale").data_ptr<float>();
+        float *out = a.typed(v[6], at::kFloat, 4, "coefficients").data_ptr<float>();
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        check(dq_adamw_coefficients(steps, lr, lr_dev, beta1, beta2, decay, scale, out, a.device,
+                                    c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream()));
+    });
+}
+
+// a 4-bit matrix: codes [rows][128 s], scales [rows][8 s], s = ceil(length / 256)
+struct Matrix4 {
+    const uint8_t *codes, *scales;
+    Matrix4(Args &a, PyObject *c, PyObject *s, int64_t rows, int64_t length)
+    {
+        const int64_t supers = (length + 255) / 256;
+        const at::Tensor &x = a.tensor(c), &y = a.tensor(s);
+        need(x.scalar_type() == at::kByte && y.scalar_type() == at::kByte, "codes and scales are uint8");
+        need(rows >= 0 && length >= 0 && x.numel() == rows * 128 * supers && y.numel() == rows * 8 * supers, "codes and scales do not belong to a matrix of this size");
+        codes = static_cast<const uint8_t *>(x.data_ptr());
+        scales = static_cast<const uint8_t *>(y.data_ptr());
+    }
+};
+
+at::Tensor new_matrix(int device, int64_t rows, int64_t cols, at::ScalarType dtype)
+{
+    return at::empty({rows, cols}, at::TensorOptions().dtype(dtype).device(cuda(device)));
+}
+
+// x, columns, sign, rand_pool, seed (None: no random stream), step -> (codes, scales)
+PyObject *mx4_quantize(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 6, [&]() -> PyObject * {
+        Args a;
+        if (!THPVariable_Check(v[0])) refuse(std::string("a tensor argument is required, got ") + Py_TYPE(v[0])->tp_name);
+        const at::Tensor &x = THPVariable_Unpack(v[0]);
+        if (!x.is_cuda()) refuse("tensor arguments must live on the GPU (got a " + std::string(c10::DeviceTypeName(x.device().type(), true)) + " tensor)");
+        need(x.dim() == 2, "quantize: a matrix is required");
+        const int64_t xr = x.size(0), xc = x.size(1);
+        need((x.stride(1) == 1 || xc <= 1) && (x.stride(0) >= xc || xr <= 1), "quantize: the elements of a row must be consecutive, and the rows apart");
+        a.device = x.device().index();
+        const int code = dtype_code(x);
+        const bool columns = PyObject_IsTrue(v[1]);
+        const int64_t rows = columns ? xc : xr, length = columns ? xr : xc, supers = (length + 255) / 256;
+        const uint32_t *sign = v[2] == Py_None ? nullptr : reinterpret_cast<const uint32_t *>(a.typed(v[2], at::kInt, 8 * supers, "sign").data_ptr<int32_t>());
+        const void *pool = nullptr;
+        int pool_code = 0;
+        if (v[3] != Py_None) {
+            const at::Tensor &p = a.tensor(v[3]);
+            need(p.numel() == rows * 256 * supers, "quantize: rand_pool has one value per element of the result, padding included");
+            need(v[4] == Py_None, "quantize: rand_pool or seed, not both");
+            pool_code = dtype_code(p);
+            pool = p.data_ptr();
+        }
+        const bool stochastic = pool || v[4] != Py_None;
+        const uint64_t seed = v[4] == Py_None ? 0 : word(v[4], true), step = word(v[5], true);
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const at::Tensor codes = new_matrix(a.device, rows, 128 * supers, at::kByte), scales = new_matrix(a.device, rows, 8 * supers, at::kByte);
+        if (rows && length) {
+            const dq_stream_t s = c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream();
+            check(dq_mx4_quantize(x.data_ptr(), code, xr, xc, xr > 1 ? x.stride(0) : xc, columns, sign, stochastic, pool, pool_code, seed, step,
+                                  static_cast<uint8_t *>(codes.data_ptr()), static_cast<uint8_t *>(scales.data_ptr()), a.device, s));
+        }
+        return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(codes)).ptr(), py::reinterpret_steal<py::object>(THPVariable_Wrap(scales)).ptr());
+    });
+}
+
+// codes, scales, rows, cols, a tensor of the element type asked for
+PyObject *mx4_dequantize(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 5, [&]() -> PyObject * {
+        Args a;
+        const int64_t rows = integer(v[2]), cols = integer(v[3]);
+        const Matrix4 q(a, v[0], v[1], rows, cols);
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const at::Tensor out = new_matrix(a.device, rows, cols, THPVariable_Unpack(v[4]).scalar_type());
+        const int code = dtype_code(out);
+        if (rows && cols)
+            check(dq_mx4_dequantize(q.codes, q.scales, out.data_ptr(), code, rows, cols, a.device,
+                                    c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream()));
+        return THPVariable_Wrap(out);
+    });
+}
+
+// codes and scales of a and of b, m, n, k, a tensor of the element type asked for
+PyObject *mx4_product(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 8, [&]() -> PyObject * {
+        Args a;
+        const int64_t m = integer(v[4]), n = integer(v[5]), k = integer(v[6]);
+        const Matrix4 x(a, v[0], v[1], m, k), y(a, v[2], v[3], n, k);
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const at::Tensor out = new_matrix(a.device, m, n, THPVariable_Unpack(v[7]).scalar_type());
+        const int code = dtype_code(out);
+        if (m && n && k)
+            check(dq_mx4_product(x.codes, x.scales, y.codes, y.scales, out.data_ptr(), code, m, n, k, a.device,
+                                 c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream()));
+        else
+            out.zero_();
+        return THPVariable_Wrap(out);
+    });
+}
+
 PyMethodDef kFunctions[] = {
+    {"grad_norm", reinterpret_cast<PyCFunction>(grad_norm), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(adamw_step), METH_FASTCALL, nullptr},
+    {"adamw_coefficients", reinterpret_cast<PyCFunction>(adamw_coefficients), METH_FASTCALL, nullptr},
+    {"mx4_quantize", reinterpret_cast<PyCFunction>(mx4_quantize), METH_FASTCALL, nullptr},
+    {"mx4_dequantize", reinterpret_cast<PyCFunction>(mx4_dequantize), METH_FASTCALL, nullptr},
+    {"mx4_product", reinterpret_cast<PyCFunction>(mx4_product), METH_FASTCALL, nullptr},
     {"scaling_compress", reinterpret_cast<PyCFunction>(scaling_compress), METH_FASTCALL, nullptr},
     {"scaling_decompress", reinterpret_cast<PyCFunction>(scaling_decompress), METH_FASTCALL, nullptr},
     {"scaling_dec_comp", reinterpret_cast<PyCFunction>(scaling_dec_comp), METH_FASTCALL, nullptr},

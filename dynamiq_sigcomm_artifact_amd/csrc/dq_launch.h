@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "dq_device.cuh"
@@ -346,5 +347,59 @@ hipError_t launch_bits_to_bins(int32_t *bins, int64_t nbins, const uint32_t *arr
                                hipStream_t stream);
 hipError_t launch_quantization(float *vec, int64_t n, float div_factor, float tensor_max,
                                uint64_t seed, hipStream_t stream);
+
+// the end of a training step (dq_optimizer.hip): tensors of one launch; their descriptors are kernel arguments
+constexpr int kTensors = 64;
+constexpr int kMxBlock = 32;                       // elements that share a scale
+constexpr int64_t kMxMost = (int64_t)1 << 35;      // elements of a matrix, padding included, or of a tensor: a grid has less than 2^32 threads
+constexpr int kNormGrid = 2048; // workgroups of a launch at most, and partial sums
+struct NormArgs {
+    uint32_t first_tile[kTensors];
+    const void *data[kTensors];
+    int64_t n[kTensors];
+    double *partial;
+    uint32_t *ticket; // how many workgroups of the last launch are done; 0 between calls
+    float *out;       // null in all launches of a call but the last
+    double max_norm;
+    uint32_t tiles, slots_before; // partial sums that earlier launches of the call have left
+};
+struct AdamwArgs {
+    uint32_t first_tile[kTensors];
+    void *param[kTensors];
+    const void *grad[kTensors];
+    int64_t n[kTensors];
+    uint32_t first_block[kTensors]; // start of the tensor in the arenas, in blocks of 32
+    void *state;
+    uint8_t *scales;
+    float *master;
+    int64_t total;
+    const float *grad_scale, *coefficients;
+    float beta1, rest1, beta2, rest2, eps, keep, step, root;
+    uint32_t dither;
+};
+struct AdamwCount {
+    int64_t *count;
+    const float *lr_dev, *grad_scale;
+    float *out;
+    double lr, beta1, beta2, weight_decay;
+};
+hipError_t launch_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work, float *out, hipStream_t stream);
+hipError_t launch_adamw(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, int count, hipStream_t stream);
+hipError_t launch_adamw_coefficients(const AdamwCount &a, hipStream_t stream);
+
+// 4-bit microscaled matrices (dq_microscale.hip) and their product (dq_microscale_product.hip)
+struct QuantizeArgs {
+    const void *x;
+    int64_t rows, cols, stride; // of x
+    uint8_t *codes, *scales;
+    const uint32_t *sign;
+    const void *pool;
+    RandKey key;
+};
+hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, bool stochastic, int pool_dtype, hipStream_t stream);
+hipError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int64_t rows, int64_t cols, int dtype,
+                                 hipStream_t stream);
+hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out,
+                              int64_t m, int64_t n, int64_t k, int dtype, hipStream_t stream);
 
 } // namespace dq

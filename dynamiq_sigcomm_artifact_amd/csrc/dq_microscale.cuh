@@ -1,0 +1,105 @@
+// Microscaled blocks: 32 consecutive elements share a power of two 2^k, stored as the byte k + 127 (255: the block is not a number).
+// What the 4-bit operands of products and the 8-bit optimizer states have in common.
+#pragma once
+
+#include "dq_device.cuh"
+
+namespace dq {
+
+// ---- eight consecutive elements of a vector that may lie anywhere: a view into a gradient bucket is aligned to its elements only, and
+// gfx950 loads and stores 16 bytes from any address ----
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+template <int DT> __device__ __forceinline__ void load8(const void *p, int64_t i, float (&v)[8])
+{
+    if (DT == DQ_F32) {
+        const f32x4_any *q = reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + i);
+        const f32x4_any a = q[0], b = q[1];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = a[j];
+            v[j + 4] = b[j];
+        }
+    } else {
+        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (DT == DQ_BF16) {
+                v[2 * j] = __uint_as_float(a[j] << 16);
+                v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
+            } else {
+                v[2 * j] = f16_bits_to_f32(a[j] & 0xffffu);
+                v[2 * j + 1] = f16_bits_to_f32(a[j] >> 16);
+            }
+        }
+    }
+}
+
+// the first `count` of eight, the others 0
+template <int DT> __device__ __forceinline__ void load8_part(const void *p, int64_t i, int count, float (&v)[8])
+{
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < count ? ElemIO<DT>::load(p, i + j) : 0.0f;
+}
+
+template <int DT> __device__ __forceinline__ void store8(void *p, int64_t i, const float (&v)[8])
+{
+    if (DT == DQ_F32) {
+        f32x4_any *q = reinterpret_cast<f32x4_any *>(static_cast<float *>(p) + i);
+        f32x4_any a, b;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            a[j] = v[j];
+            b[j] = v[j + 4];
+        }
+        q[0] = a;
+        q[1] = b;
+    } else {
+        u32x4_any a;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            a[j] = DT == DQ_BF16 ? f32x2_to_bf16x2(v[2 * j], v[2 * j + 1]) : f32_to_f16_bits(v[2 * j]) | (f32_to_f16_bits(v[2 * j + 1]) << 16);
+        *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(p) + i) = a;
+    }
+}
+
+template <int DT> __device__ __forceinline__ void store8_part(void *p, int64_t i, int count, const float (&v)[8])
+{
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j < count) ElemIO<DT>::store(p, i + j, v[j]);
+}
+
+// ---- the shared power of two ----
+
+// the largest magnitude of a block, which four neighbouring lanes hold eight elements each of, as a bit pattern: magnitudes are ordered
+// like their patterns, and infinities and NaN lie above every number
+__device__ __forceinline__ uint32_t block_max(const float (&v)[8])
+{
+    uint32_t u = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) u = max(u, __float_as_uint(v[j]) & 0x7fffffffu);
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0xB1, 0xf, 0xf, true)); // quad_perm [1,0,3,2]
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x4E, 0xf, 0xf, true)); // quad_perm [2,3,0,1]
+    return u;
+}
+
+// the byte k + 127 for k = floor(log2 largest) - TOP, one more where the mantissa's 23 bits are above LIFT; 0 at the least (and for a
+// block of zeros), 255 for a block that holds an infinity or NaN
+template <int TOP, uint32_t LIFT> __device__ __forceinline__ uint32_t block_scale(uint32_t largest)
+{
+    const int k = (int)(largest >> 23) - TOP + ((largest & 0x7fffffu) > LIFT ? 1 : 0);
+    return largest >= 0x7f800000u ? 255u : (uint32_t)max(k, 0);
+}
+// 2^-k, a normal number for every byte up to 253; 0 for 255
+__device__ __forceinline__ float scale_down(uint32_t byte) { return __uint_as_float(byte == 255u ? 0u : (254u - byte) << 23); }
+// 2^k (2^-127 is subnormal); NaN for 255
+__device__ __forceinline__ float scale_up(uint32_t byte)
+{
+    const uint32_t bits = byte << 23;
+    return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : bits);
+}
+
+} // namespace dq

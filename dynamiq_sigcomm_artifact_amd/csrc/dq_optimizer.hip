@@ -1,0 +1,329 @@
+// The end of a training step: the norm of all gradients with the factor that clips them, and the AdamW step over many tensors.
+//
+// Both stream their tensors once and are bound by memory.  A launch takes up to 64 tensors as kernel arguments (kTensors) and cuts each
+// into tiles; a workgroup finds the tensor of its tile with one load per lane and a ballot.  Nothing about the tensors is kept
+// between calls.
+#include "dq_launch.h"
+#include "dq_microscale.cuh"
+
+namespace dq {
+
+// the tensor that tile `tile` belongs to: the last one that starts at or before it
+__device__ __forceinline__ int tensor_of(const uint32_t (&first_tile)[kTensors], uint32_t tile)
+{
+    const uint64_t before = __builtin_amdgcn_ballot_w64(first_tile[threadIdx.x & 63] <= tile);
+    return __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(before));
+}
+
+// ---- the norm ---------------------------------------------------------------------------------------------
+
+constexpr int kNormTile = 256 * 32;
+
+__device__ __forceinline__ double wave_sum(double v)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+// Squares are taken and added in 64 bits: a gradient beyond 2^64 or below 2^-63 has no square in 32, and a sum of 10^8 terms is as exact as
+// its terms.  A workgroup adds its tiles up and writes one number; in the last launch of a call the workgroup that is done last adds those.
+// Which workgroup that is changes from call to call, the order of the additions does not.
+template <int DT> __global__ __launch_bounds__(256) void grad_norm_kernel(NormArgs a)
+{
+    __shared__ double part[4];
+    __shared__ int last;
+    const int t = threadIdx.x;
+    double sum = 0.0;
+    for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+        const int k = tensor_of(a.first_tile, tile);
+        const void *p = a.data[k];
+        const int64_t n = a.n[k], at = (int64_t)(tile - a.first_tile[k]) * kNormTile;
+        float v[4][8];
+        if (at + kNormTile <= n) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) load8<DT>(p, at + 8 * (256 * j + t), v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t i = at + 8 * (256 * j + t);
+                if (i + 8 <= n)
+                    load8<DT>(p, i, v[j]);
+                else
+                    load8_part<DT>(p, i, (int)max((int64_t)0, n - i), v[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum = __builtin_fma((double)v[j][e], (double)v[j][e], sum);
+    }
+    sum = wave_sum(sum);
+    if ((t & 63) == 0) part[t >> 6] = sum;
+    __syncthreads();
+    if (t == 0) {
+        double *slot = a.partial + blockIdx.x;
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
+        if (blockIdx.x < a.slots_before) sum += *slot;
+        // past this XCD's cache, where the last workgroup may not look
+        __hip_atomic_store(slot, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = a.out && __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    const uint32_t slots = max(a.slots_before, gridDim.x);
+    sum = 0.0;
+    for (uint32_t s = t; s < slots; s += 256) sum += __hip_atomic_load(a.partial + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sum = wave_sum(sum);
+    __syncthreads();
+    if ((t & 63) == 0) part[t >> 6] = sum;
+    __syncthreads();
+    if (t == 0) {
+        const double norm = __builtin_sqrt((part[0] + part[1]) + (part[2] + part[3]));
+        const double factor = __builtin_fmin(1.0, a.max_norm / (norm + 1e-6));
+        a.out[0] = (float)norm;
+        a.out[1] = __builtin_isfinite(norm) ? (float)factor : __builtin_nanf("");
+        __hip_atomic_store(a.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+    }
+}
+
+hipError_t launch_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work, float *out, hipStream_t stream)
+{
+    NormArgs a;
+    a.ticket = reinterpret_cast<uint32_t *>(work);
+    a.partial = work + 1;
+    a.max_norm = max_norm;
+    a.slots_before = 0;
+    hipError_t e = hipSuccess;
+    int k = 0;
+    bool done = false;
+    while (!done && e == hipSuccess) {
+        // tensors of one element type, one after the other
+        const int dtype = k < count ? spans[k].dtype : DQ_F32;
+        int take = 0;
+        int64_t tiles = 0;
+        for (; k < count && take < kTensors && spans[k].dtype == dtype; k++) {
+            const int64_t more = (spans[k].n + kNormTile - 1) / kNormTile;
+            if (take && tiles + more > 0x7fffffff) break;
+            if (more == 0) continue;
+            a.first_tile[take] = (uint32_t)tiles;
+            a.data[take] = spans[k].data;
+            a.n[take++] = spans[k].n;
+            tiles += more;
+        }
+        for (int j = take; j < kTensors; j++) a.first_tile[j] = 0xffffffffu;
+        done = k == count;
+        a.tiles = (uint32_t)tiles;
+        a.out = done ? out : nullptr;
+        const uint32_t grid = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(tiles, kNormGrid));
+        if (tiles == 0 && !done) continue;
+        if (dtype == DQ_F32)
+            e = launch_with(grad_norm_kernel<DQ_F32>, dim3(grid), dim3(256), stream, a);
+        else if (dtype == DQ_BF16)
+            e = launch_with(grad_norm_kernel<DQ_BF16>, dim3(grid), dim3(256), stream, a);
+        else
+            e = launch_with(grad_norm_kernel<DQ_F16>, dim3(grid), dim3(256), stream, a);
+        a.slots_before = std::max(a.slots_before, grid);
+    }
+    return e;
+}
+
+// ---- AdamW ------------------------------------------------------------------------------------------------
+
+constexpr int kStepTile = 256 * 8;
+
+struct Coefficients {
+    float keep, step, root; // 1 - lr decay; lr / (1 - beta1^t); 1 / sqrt(1 - beta2^t)
+    uint32_t dither;        // t times its constant
+};
+
+constexpr uint32_t kDitherElement = 0x9E3779B9u, kDitherStep = 0xB504F333u;
+
+// An 8-bit state is E4M3, eleven to thirteen times 2^-7 apart at most; a moment that decays by a thousandth a step would never leave its code if
+// it were rounded to nearest.  So what is cut away is added up over the steps instead: a dither of 20 bits, the fractions of i phi + t / sqrt 2,
+// is added where the bits are cut, and over the steps of one element, and over the elements of one step, these fractions are spread evenly: the mean
+// error goes to zero as 1 / steps.
+__device__ __forceinline__ uint32_t dither_of(uint32_t element, uint32_t step) { return (element * kDitherElement + step) >> 12; }
+
+// the E4M3 code of y >= 0, y <= 448.  From 2^-6 on the code's bits are the float's upper ones; below, where codes are 2^-9 apart, adding
+// 2^-6 puts them there.
+__device__ __forceinline__ uint32_t e4m3_dithered(float y, uint32_t dither)
+{
+    const bool small = y < 0x1p-6f;
+    return ((__float_as_uint(small ? y + 0x1p-6f : y) + dither) >> 20) - (small ? 968u : 960u);
+}
+
+template <int PD, int GD, int BITS, bool MASTER> __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a)
+{
+    const float scale = a.grad_scale ? *a.grad_scale : 1.0f;
+    if (!__builtin_isfinite(scale)) return;
+    Coefficients c = {a.keep, a.step, a.root, a.dither};
+    if (a.coefficients) {
+        c.keep = a.coefficients[0];
+        c.step = a.coefficients[1];
+        c.root = a.coefficients[2];
+        c.dither = __float_as_uint(a.coefficients[3]);
+    }
+    const int k = tensor_of(a.first_tile, blockIdx.x);
+    const int64_t n = a.n[k], i = (int64_t)(blockIdx.x - a.first_tile[k]) * kStepTile + 8 * threadIdx.x;
+    if (i >= ((n + 31) & ~(int64_t)31)) return;
+    const int64_t at = (int64_t)a.first_block[k] * kMxBlock + i; // in the arenas
+    const int mine = (int)min((int64_t)8, n - i);                // elements of the tensor; 0 or less in its padding
+    float g[8], p[8], m[8], v[8], r[8];
+    if (mine == 8)
+        load8<GD>(a.grad[k], i, g);
+    else
+        load8_part<GD>(a.grad[k], i, mine, g);
+    if (MASTER)
+        load8<DQ_F32>(a.master, at, p);
+    else if (mine == 8)
+        load8<PD>(a.param[k], i, p);
+    else
+        load8_part<PD>(a.param[k], i, mine, p);
+    uint8_t *codes = static_cast<uint8_t *>(a.state);
+    if (BITS == 32) {
+        load8<DQ_F32>(a.state, at, m);
+        load8<DQ_F32>(a.state, a.total + at, v);
+    } else {
+        const uint2 cm = *reinterpret_cast<const uint2 *>(codes + at), cr = *reinterpret_cast<const uint2 *>(codes + a.total + at);
+        const float um = scale_up(a.scales[at >> 5]), ur = scale_up(a.scales[(a.total + at) >> 5]);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t wm = h ? cm.y : cm.x, wr = h ? cr.y : cr.x;
+            const f32x2_t m0 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, true);
+            const f32x2_t r0 = __builtin_amdgcn_cvt_pk_f32_fp8(wr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(wr, true);
+            m[4 * h] = m0.x * um; m[4 * h + 1] = m0.y * um; m[4 * h + 2] = m1.x * um; m[4 * h + 3] = m1.y * um;
+            r[4 * h] = r0.x * ur; r[4 * h + 1] = r0.y * ur; r[4 * h + 2] = r1.x * ur; r[4 * h + 3] = r1.y * ur;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = r[j] * r[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float gj = g[j] * scale;
+        m[j] = m[j] * a.beta1 + gj * a.rest1;
+        v[j] = v[j] * a.beta2 + (gj * gj) * a.rest2;
+        r[j] = __builtin_sqrtf(v[j]);
+        p[j] = p[j] * c.keep - c.step * (m[j] / (r[j] * c.root + a.eps));
+    }
+    if (mine < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j >= mine) p[j] = m[j] = v[j] = r[j] = 0.0f; // the padding is zero, whatever it was
+    }
+    if (BITS == 32) {
+        store8<DQ_F32>(a.state, at, m);
+        store8<DQ_F32>(a.state, a.total + at, v);
+    } else {
+        const uint32_t sm = block_scale<8, 0x600000u>(block_max(m)), sr = block_scale<8, 0x600000u>(block_max(r));
+        const float dm = scale_down(sm), dr = scale_down(sr);
+        uint32_t wm[2] = {0, 0}, wr[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t d = dither_of((uint32_t)i + j, c.dither);
+            const uint32_t em = e4m3_dithered(__builtin_fabsf(m[j]) * dm, d) | (__float_as_uint(m[j]) >> 31 << 7);
+            // a root above zero stays above zero: a step divides by it
+            const uint32_t er = max(e4m3_dithered(r[j] * dr, 0xfffffu - d), r[j] > 0.0f ? 1u : 0u);
+            wm[j >> 2] |= (em & 0xffu) << (8 * (j & 3));
+            wr[j >> 2] |= (er & 0xffu) << (8 * (j & 3));
+        }
+        *reinterpret_cast<uint2 *>(codes + at) = make_uint2(wm[0], wm[1]);
+        *reinterpret_cast<uint2 *>(codes + a.total + at) = make_uint2(wr[0], wr[1]);
+        if ((threadIdx.x & 3) == 0) {
+            a.scales[at >> 5] = (uint8_t)sm;
+            a.scales[(a.total + at) >> 5] = (uint8_t)sr;
+        }
+    }
+    if (MASTER) store8<DQ_F32>(a.master, at, p);
+    if (mine == 8)
+        store8<PD>(a.param[k], i, p);
+    else
+        store8_part<PD>(a.param[k], i, mine, p);
+}
+
+// what a step's kernels take from the step's number, where that number is in device memory: a recorded step counts on
+__global__ void adamw_coefficients_kernel(AdamwCount a)
+{
+    if (a.grad_scale && !__builtin_isfinite(*a.grad_scale)) return;
+    const int64_t t = *a.count + 1;
+    const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+    *a.count = t;
+    a.out[0] = (float)(1.0 - lr * a.weight_decay);
+    a.out[1] = (float)(lr / (1.0 - pow(a.beta1, (double)t)));
+    a.out[2] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+    a.out[3] = __uint_as_float((uint32_t)t * kDitherStep);
+}
+
+hipError_t launch_adamw_coefficients(const AdamwCount &a, hipStream_t stream)
+{
+    return launch_with(adamw_coefficients_kernel, dim3(1), dim3(1), stream, a);
+}
+
+template <int PD, int GD> static hipError_t launch_step(const AdamwArgs &a, int bits, uint32_t grid, hipStream_t stream)
+{
+    if constexpr (PD != DQ_F32) {
+        if (a.master) {
+            return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, true>, dim3(grid), dim3(256), stream, a)
+                              : launch_with(adamw_kernel<PD, GD, 8, true>, dim3(grid), dim3(256), stream, a);
+        }
+    }
+    return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, false>, dim3(grid), dim3(256), stream, a)
+                      : launch_with(adamw_kernel<PD, GD, 8, false>, dim3(grid), dim3(256), stream, a);
+}
+
+template <int PD> static hipError_t launch_step_of(int grad, const AdamwArgs &a, int bits, uint32_t grid, hipStream_t stream)
+{
+    return grad == DQ_F32 ? launch_step<PD, DQ_F32>(a, bits, grid, stream)
+         : grad == DQ_BF16 ? launch_step<PD, DQ_BF16>(a, bits, grid, stream) : launch_step<PD, DQ_F16>(a, bits, grid, stream);
+}
+
+hipError_t launch_adamw(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, int count, hipStream_t stream)
+{
+    AdamwArgs a;
+    a.state = o.state;
+    a.scales = o.scales;
+    a.master = o.master;
+    a.total = o.total;
+    a.grad_scale = o.grad_scale;
+    a.coefficients = o.coefficients;
+    a.beta1 = (float)o.beta1;
+    a.rest1 = (float)(1.0 - o.beta1);
+    a.beta2 = (float)o.beta2;
+    a.rest2 = (float)(1.0 - o.beta2);
+    a.eps = (float)o.eps;
+    a.keep = a.step = a.root = 0.0f;
+    a.dither = 0;
+    if (!o.coefficients) {
+        a.keep = (float)(1.0 - o.lr * o.weight_decay);
+        a.step = (float)(o.lr / (1.0 - pow(o.beta1, (double)o.step)));
+        a.root = (float)(1.0 / sqrt(1.0 - pow(o.beta2, (double)o.step)));
+        a.dither = (uint32_t)o.step * kDitherStep;
+    }
+    hipError_t e = hipSuccess;
+    int k = 0;
+    while (k < count && e == hipSuccess) {
+        const int param = tensors[k].param_dtype, grad = tensors[k].grad_dtype;
+        int take = 0;
+        int64_t tiles = 0;
+        for (; k < count && take < kTensors && tensors[k].param_dtype == param && tensors[k].grad_dtype == grad; k++) {
+            const dq_adamw_tensor_t &x = tensors[k];
+            const int64_t more = (x.n + kStepTile - 1) / kStepTile;
+            if (take && tiles + more > dq::kMxMost / kStepTile - 1) break;
+            if (more == 0) continue;
+            a.first_tile[take] = (uint32_t)tiles;
+            a.param[take] = x.param;
+            a.grad[take] = x.grad;
+            a.n[take] = x.n;
+            a.first_block[take++] = (uint32_t)(x.start / kMxBlock);
+            tiles += more;
+        }
+        for (int j = take; j < kTensors; j++) a.first_tile[j] = 0xffffffffu;
+        if (tiles == 0) continue;
+        e = param == DQ_F32 ? launch_step_of<DQ_F32>(grad, a, o.bits, (uint32_t)tiles, stream)
+          : param == DQ_BF16 ? launch_step_of<DQ_BF16>(grad, a, o.bits, (uint32_t)tiles, stream)
+                             : launch_step_of<DQ_F16>(grad, a, o.bits, (uint32_t)tiles, stream);
+    }
+    return e;
+}
+
+} // namespace dq

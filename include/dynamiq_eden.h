@@ -733,6 +733,115 @@ int dq_bits_to_bins(int32_t *bins, int64_t nbins, const uint32_t *arr, int64_t n
 int dq_quantization(float *vec, int64_t n, int device, float div_factor, float tensor_max,
                     uint64_t seed, dq_stream_t stream);
 
+/* ---- the end of a training step: clipping and AdamW ---------------------
+ *
+ * No counterpart in the reference, whose training scripts leave both to torch.
+ * Tensors may start at any element (views into a gradient bucket), be of any
+ * length (0 included) and of different element types in one call. */
+typedef struct dq_span {
+    const void *data;
+    int64_t n;     /* elements, in [0, 2^40) */
+    int32_t dtype; /* dq_dtype */
+    int32_t reserved;
+} dq_span_t;
+
+/* float64 entries of the work buffer: zeroed once, then kept from call to call
+ * (a call leaves in it what the next one expects).  Calls that may overlap --
+ * on different streams, or replays of different graphs -- need one each. */
+int64_t dq_grad_norm_work_doubles(void);
+/* out[0] = norm = sqrt(sum of the squares of all elements), summed in 64 bits in
+ * an order that does not change from call to call; out[1] = min(1, max_norm /
+ * (norm + 1e-6)), NaN where the norm is not finite -- the gradient factor of
+ * dq_adamw_step, which a NaN makes do nothing.  max_norm > 0 or infinite (no
+ * clipping).  One launch per 64 tensors, and per change of element type along
+ * the list. */
+int dq_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work,
+                 int64_t work_doubles, float *out, int device, dq_stream_t stream);
+
+/* One AdamW step (decoupled weight decay).  With g the gradient times
+ * *grad_scale and t the number of the step, counted from 1:
+ *   m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in binary32.  The states of all tensors lie in arenas of `total` elements, a
+ * tensor's from element `start` on, a multiple of 32; the gap up to the next
+ * multiple of 32 is set to zero.
+ *   bits 32: state = float [2][total], m and v; scales unused.
+ *   bits 8:  state = uint8 [2][total], E4M3 codes of m and of r = sqrt(v);
+ *            scales = uint8 [2][total / 32], the byte k + 127 of a block of 32:
+ *            its values are the codes' times 2^k, k the least that keeps them
+ *            up to 448 (255: the block holds an infinity or NaN, and is NaN).
+ *            A magnitude is cut off after 20 bits of dither have been added in the
+ *            place of the bits cut away, d = ((i 0x9E3779B9 + t 0xB504F333) mod
+ *            2^32) >> 12 for m and 2^20 - 1 - d for r, i the element's index in
+ *            its tensor; r > 0 is stored as no less than the smallest code.
+ * master (nullable): float [total], the weights that the step reads and writes;
+ * the 16-bit params then only receive them, rounded to nearest.  Without it 16-bit
+ * params are read, and rounded to nearest as well. */
+typedef struct dq_adamw_tensor {
+    void *param;
+    const void *grad;
+    int64_t n;     /* elements, in [0, 2^35 - 4096] */
+    int64_t start; /* of its states in the arenas */
+    int32_t param_dtype, grad_dtype;
+} dq_adamw_tensor_t;
+typedef struct dq_adamw {
+    void *state; /* 16-byte aligned */
+    uint8_t *scales;
+    float *master; /* 16-byte aligned */
+    int64_t total; /* a multiple of 32 below 2^37 */
+    int32_t bits;
+    int32_t reserved;
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;              /* t; unused with coefficients */
+    const float *grad_scale;   /* device memory, nullable: 1; infinite or NaN: the step changes nothing */
+    const float *coefficients; /* device memory, nullable: of dq_adamw_coefficients, in place of lr, weight_decay and step */
+} dq_adamw_t;
+int dq_adamw_step(const dq_adamw_t *adamw, const dq_adamw_tensor_t *tensors, int count, int device, dq_stream_t stream);
+/* For steps that are recorded into a graph: advances *steps in device memory (the
+ * steps done so far) and writes what the next dq_adamw_step takes as
+ * `coefficients`, float [4] -- nothing where *grad_scale (nullable) is infinite or NaN.
+ * lr_dev (nullable): the learning rate in device memory, in place of lr. */
+int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double beta1, double beta2,
+                          double weight_decay, const float *grad_scale, float *coefficients, int device,
+                          dq_stream_t stream);
+
+/* ---- 4-bit microscaled matrices ------------------------------------------
+ *
+ * No counterpart in the reference.  A matrix of `rows` vectors along the axis that
+ * a product contracts: blocks of 32 elements share a power of two 2^k, elements are
+ * E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; the OCP microscaling format MXFP4).
+ * A row is padded with zeros to s = ceil(length / 256) superchunks:
+ *   codes  uint8 [rows][128 s], two elements a byte, the first one in the low half
+ *   scales uint8 [rows][8 s], k + 127 (255: the block is NaN)
+ * codes 16-byte, scales 8-byte aligned.  A matrix has less than 2^35 elements, padding
+ * included. */
+
+/* x: [x_rows][x_cols], row i from element i * stride on.  columns = 0: the rows of
+ * the result are those of x; columns = 1: its columns (what the product with the
+ * transposed matrix takes).
+ * sign (nullable): one bit per element of a result's row, as dq_pack_signs writes
+ * them, ceil(length / 256) * 8 words.  A block x becomes H (s x) / sqrt(32), H the
+ * Walsh-Hadamard matrix, s = -1 where the bit is set: a product of two matrices
+ * rotated alike is that of the matrices.
+ * Rounding: to nearest, ties to even, with k = floor(log2 max) - 2 (magnitudes beyond 6 2^k
+ * become 6 2^k); or, stochastic != 0, up with the probability of the share of
+ * the way from one value to the next: where u is below it, with the least k for
+ * which max <= 6 2^k.  u: rand_pool (rand_dtype; [result's rows][256 s], in [0, 1)), or
+ * with rand_pool = NULL the in-kernel stream of dq_scaling_compress_philox, keyed by
+ * (seed, step, chunk of 16 elements of that layout).
+ * A block that holds an infinity or NaN is NaN. */
+int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, int64_t stride, int columns,
+                    const uint32_t *sign, int stochastic, const void *rand_pool, int rand_dtype, uint64_t seed,
+                    uint64_t step, uint8_t *codes, uint8_t *scales, int device, dq_stream_t stream);
+/* out: `dtype` [rows][cols], the values rounded to nearest */
+int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows,
+                      int64_t cols, int device, dq_stream_t stream);
+/* out[i][j] = sum over the contraction of a[i] b[j], `dtype` [m][n], summed in
+ * binary32; k: the rows' length, padding excluded. */
+int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes,
+                   const uint8_t *b_scales, void *out, int dtype, int64_t m, int64_t n, int64_t k, int device,
+                   dq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,366 @@
+"""4-bit microscaled matrices against their definition (ref_operators.py): bytes to the bit, products in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import ref_operators as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ms(capi):
+    from dynamiq_sigcomm_artifact_amd import microscale
+    return microscale
+
+
+def matrix(r, c, dtype, seed=0, spread=3.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(r, c, generator=g, device=DEV) * torch.exp(spread * torch.randn(r, c, generator=g, device=DEV))
+    return x.clamp(-6e4, 6e4).to(dtype)
+
+
+def signs(capi, n, seed):
+    bits = torch.empty(-(-n // 256) * 8, dtype=torch.int32, device=DEV)
+    capi.rand_diag_bits(bits, bits.numel() * 32, seed)
+    s = 1.0 - 2.0 * ((bits.cpu().numpy().view(np.uint32)[:, None] >> np.arange(32)) & 1).reshape(-1)
+    return bits, s
+
+
+def pool(rows, n, dtype, seed=5):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.rand(rows, -(-n // 256) * 256, generator=g, device=DEV).mul_(0.99).to(dtype)
+
+
+def same(q, values, scales):
+    assert np.array_equal(q.scales.cpu().numpy(), scales)
+    live = np.repeat(scales, 32, axis=1) != 255
+    got = R.unpack4(q.codes.cpu().numpy(), scales)
+    assert np.array_equal(got[live], values[live])
+
+
+SHAPES = [(1, 1), (1, 32), (3, 31), (5, 33), (7, 256), (130, 257), (129, 300), (257, 131), (64, 1000)]
+
+
+@pytest.mark.parametrize("r,c", SHAPES)
+@pytest.mark.parametrize("columns", [False, True])
+@pytest.mark.parametrize("dtype", [FP, BF, HF], ids=str)
+def test_nearest(ms, r, c, columns, dtype):
+    x = matrix(r, c, dtype, r + c)
+    q = ms.quantize(x, columns=columns)
+    assert q.shape == ((c, r) if columns else (r, c))
+    v = x.float().cpu().numpy()
+    values, scales = R.quantize4(v.T if columns else v)
+    same(q, values, scales)
+    for out in (FP, BF, HF):
+        got = ms.dequantize(q, out)
+        want = torch.from_numpy(values[:, :q.cols]).to(out)          # one rounding, of a value with two significant bits
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("r,c", [(3, 31), (130, 257), (257, 131)])
+@pytest.mark.parametrize("columns", [False, True])
+@pytest.mark.parametrize("rotate", [False, True])
+@pytest.mark.parametrize("source", [FP, BF, HF, "philox"], ids=str)
+def test_stochastic_and_rotated(ms, capi, r, c, columns, rotate, source):
+    dtype = BF if rotate else FP
+    x = matrix(r, c, dtype, 7)
+    rows, n = (c, r) if columns else (r, c)
+    bits, s = signs(capi, n, 11) if rotate else (None, None)
+    if source == "philox":
+        q = ms.quantize(x, columns, bits, seed=123, step=9)
+        u = torch.empty(rows * (-(-n // 256) * 256), dtype=FP, device=DEV)
+        capi.philox_uniform(u, 123, 9)
+    else:
+        u = pool(rows, n, source)
+        q = ms.quantize(x, columns, bits, rand_pool=u)
+    v = x.float().cpu().numpy()
+    same(q, *R.quantize4(v.T if columns else v, s, u.float().cpu().numpy()))
+
+
+@pytest.mark.parametrize("columns", [False, True])
+def test_rotation_to_nearest(ms, capi, columns):
+    x = matrix(100, 300, FP, 3, spread=1.0)
+    n = 100 if columns else 300
+    bits, s = signs(capi, n, 4)
+    v = x.cpu().numpy()
+    same(ms.quantize(x, columns, bits), *R.quantize4(v.T if columns else v, s))
+
+
+@pytest.mark.parametrize("columns", [False, True])
+def test_borders(ms, columns):
+    """ties, saturation, subnormal numbers, the largest and smallest scales, blocks of zeros"""
+    halves = np.concatenate([np.arange(0, 33) / 4.0, -np.arange(0, 33) / 4.0, np.nextafter(np.float32([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]), np.float32(9)),
+                             np.nextafter(np.float32([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]), np.float32(0))]).astype(np.float32)
+    rows = []
+    for k in (0, 1, -1, 100, -100, 124, -126, -130, -140, -149):
+        for top in (4.0, 6.0, 7.999, 7.0):
+            with np.errstate(all="ignore"):
+                for at in range(0, len(halves), 31):
+                    b = np.zeros(32, np.float32)
+                    part = halves[at:at + 31]
+                    b[:len(part)] = np.clip(part, -top, top)
+                    b[31] = top
+                    rows.append(np.ldexp(b, k).astype(np.float32))
+    rows.append(np.zeros(32, np.float32))
+    rows.append(np.full(32, 1e-45, np.float32))
+    rows.append(np.full(32, np.finfo(np.float32).max))
+    x = np.concatenate(rows).reshape(1, -1)
+    x[~np.isfinite(x)] = 1.0
+    t = torch.from_numpy(x).to(DEV)
+    q = ms.quantize(t.t().contiguous() if columns else t, columns)
+    same(q, *R.quantize4(x))
+    u = np.full((1, -(-x.shape[1] // 256) * 256), 0.5, np.float32)
+    q = ms.quantize(t.t().contiguous() if columns else t, columns, rand_pool=torch.from_numpy(u).to(DEV))
+    same(q, *R.quantize4(x, None, u))
+
+
+@pytest.mark.parametrize("columns", [False, True])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_what_is_not_finite(ms, columns, bad):
+    """its block is NaN, and so is every product with it, and nothing else"""
+    x = torch.ones(70, 300, device=DEV)
+    x[33, 40] = bad
+    for kw in (dict(), dict(seed=1)):
+        q = ms.quantize(x, columns, **kw)
+        rows, n = q.shape
+        row, at = (40, 33) if columns else (33, 40)
+        values = ms.dequantize(q)
+        nan = torch.zeros(rows, n, dtype=torch.bool, device=DEV)
+        nan[row, at // 32 * 32:min(n, at // 32 * 32 + 32)] = True
+        assert torch.equal(torch.isnan(values), nan)
+        y = ms.product(q, ms.quantize(torch.zeros(5, n, device=DEV)), FP)
+        assert torch.isnan(y[row]).all() and int(torch.isnan(y).sum()) == 5
+        y = ms.product(ms.quantize(torch.ones(40, n, device=DEV)), q, FP)
+        assert torch.isnan(y[:, row]).all() and int(torch.isnan(y).sum()) == 40
+
+
+def test_views(ms):
+    """rows apart, and elements at any address"""
+    big = matrix(40, 1001, BF, 1)
+    for x in (big[:, 3:600], big[5:6, 1:], big[::2, 7:8], big[3:, :]):
+        for columns in (False, True):
+            q, w = ms.quantize(x, columns), ms.quantize(x.clone(memory_format=torch.contiguous_format), columns)
+            assert torch.equal(q.codes, w.codes) and torch.equal(q.scales, w.scales)
+    with pytest.raises(RuntimeError, match="consecutive"):
+        ms.quantize(big.t())
+    with pytest.raises(RuntimeError, match="consecutive"):
+        ms.quantize(big[:1].expand(4, 1001))
+    with pytest.raises(RuntimeError, match="a matrix is required"):
+        ms.quantize(big[0])
+
+
+def test_refusals(ms, capi):
+    x = matrix(4, 300, BF)
+    with pytest.raises(RuntimeError, match="unsupported element dtype"):
+        ms.quantize(x.double())
+    with pytest.raises(RuntimeError, match="sign: wrong dtype or too few"):
+        ms.quantize(x, sign=torch.zeros(15, dtype=torch.int32, device=DEV))
+    with pytest.raises(RuntimeError, match="rand_pool has one value"):
+        ms.quantize(x, rand_pool=torch.zeros(4, 300, device=DEV))
+    with pytest.raises(RuntimeError, match="not both"):
+        ms.quantize(x, rand_pool=torch.zeros(4, 512, device=DEV), seed=1)
+    with pytest.raises(RuntimeError, match="unsupported element dtype"):
+        ms.quantize(x, rand_pool=torch.zeros(4, 512, dtype=torch.uint8, device=DEV))
+    q = ms.quantize(x)
+    with pytest.raises(RuntimeError, match="do not belong"):
+        ms.dequantize(ms.Microscaled(q.codes, q.scales, 4, 700))
+    with pytest.raises(RuntimeError, match="do not belong"):
+        ms.product(q, ms.Microscaled(q.codes, q.scales, 5, 300))
+    with pytest.raises(RuntimeError, match="uint8"):
+        ms.dequantize(ms.Microscaled(q.codes.int(), q.scales, 4, 300))
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ms.dequantize(ms.Microscaled(torch.zeros(4, 512, dtype=torch.uint8, device=DEV)[:, ::2], q.scales, 4, 300))
+
+
+def test_empty(ms):
+    x = torch.ones(3, 40, device=DEV)
+    none = ms.quantize(x[:0])
+    assert none.shape == (0, 40) and ms.dequantize(none).shape == (0, 40)
+    assert ms.product(none, ms.quantize(x)).shape == (0, 3) and ms.product(ms.quantize(x), none).shape == (3, 0)
+    flat = ms.quantize(x[:, :0])
+    assert torch.equal(ms.product(flat, flat, FP), torch.zeros(3, 3, device=DEV))
+
+
+# ---- products ----
+
+def packed(ms, r, n, seed):
+    """a matrix of all codes and many scales, and its values"""
+    rng = np.random.default_rng(seed)
+    values, scales = R.quantize4(rng.standard_normal((r, n)) * np.exp(rng.standard_normal((r, n))))
+    return ms.Microscaled(torch.from_numpy(R.pack4(values, scales)).to(DEV), torch.from_numpy(scales).to(DEV), r, n), values[:, :n]
+
+
+PRODUCTS = [(1, 1, 1), (1, 16, 256), (1, 1000, 4096), (2, 33, 31), (3, 17, 4000), (15, 64, 512), (16, 100, 768), (17, 48, 300), (31, 129, 1024), (33, 255, 513), (64, 64, 64),
+            (65, 130, 2048), (100, 1, 777), (127, 129, 255), (128, 128, 1024), (129, 257, 2304), (256, 256, 256), (300, 500, 4100), (513, 1030, 1500), (1025, 777, 300)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_product(ms, m, n, k):
+    a, x = packed(ms, m, k, m + k)
+    b, y = packed(ms, n, k, n)
+    want, size = x @ y.T, np.abs(x) @ np.abs(y).T
+    # products of two E2M1 numbers and two powers of two are exact; k additions in binary32, in whatever order, are off by k half steps of the sum of magnitudes at most
+    # (the matrix core may cut instead of rounding: a whole step each)
+    bound = k * 2.0 ** -23 * size
+    for dtype in (FP, BF, HF):
+        got = ms.product(a, b, dtype).double().cpu().numpy()
+        err = bound + (torch.finfo(dtype).eps / 2 * (np.abs(want) + bound) + (2.0 ** -25 if dtype == HF else 0) if dtype != FP else 0)
+        assert np.all(np.abs(got - want) <= err), float(np.max(np.abs(got - want) - err))
+
+
+def test_exact_sums(ms):
+    """small whole numbers: every sum is exact, so every element must be right to the bit"""
+    for m, n, k in ((1, 300, 1000), (20, 70, 512), (140, 300, 1111), (600, 520, 256)):
+        rng = np.random.default_rng(k)
+        x, y = rng.integers(-4, 5, (m, k)).astype(np.float32), rng.integers(-4, 5, (n, k)).astype(np.float32)
+        x[:, ::32], y[:, ::32] = 4, 4                       # no block's largest below 4: scale 1
+        got = ms.product(ms.quantize(torch.from_numpy(x).to(DEV)), ms.quantize(torch.from_numpy(y).to(DEV)), FP)
+        assert np.array_equal(got.cpu().numpy(), x @ y.T)
+
+
+def test_scales_of_the_product(ms):
+    """the extreme scales, and each of a row's"""
+    x = torch.ones(40, 512, device=DEV) * torch.exp2(torch.arange(16, device=DEV).repeat_interleave(32).float() - 8)
+    y = torch.ones(24, 512, device=DEV) * torch.exp2(-2.0 * torch.arange(16, device=DEV).repeat_interleave(32).float() + 3)
+    got = ms.product(ms.quantize(x), ms.quantize(y), FP)
+    assert torch.equal(got, (x.double() @ y.double().t()).float())
+    # (2^-149 is below a quarter of the smallest scale, 2^-127: a zero; 2^-128 is half of it)
+    for a, b, want in ((2.0 ** 120, 2.0 ** -120, 256.0), (2.0 ** -126, 2.0 ** 100, 2.0 ** -18), (2.0 ** -128, 2.0 ** 126, 64.0), (2.0 ** -149, 2.0 ** 126, 0.0)):
+        got = ms.product(ms.quantize(torch.full((33, 256), a, device=DEV)), ms.quantize(torch.full((20, 256), b, device=DEV)), FP)
+        assert torch.equal(got, torch.full_like(got, want))
+
+
+def test_order_does_not_change(ms):
+    a, _ = packed(ms, 100, 3000, 1)
+    b, _ = packed(ms, 200, 3000, 2)
+    first = ms.product(a, b, FP)
+    assert all(torch.equal(ms.product(a, b, FP), first) for _ in range(5))
+
+
+# ---- the layer ----
+
+def plain_linear(x, w, dy, sn, sm, pr, pc):
+    q = lambda t, s=None, u=None: R.quantize4(t, s, u)[0]          # noqa: E731
+    f = lambda t: t.float().cpu().numpy()                          # noqa: E731
+    k, n, m = x.shape[1], w.shape[0], x.shape[0]
+    y = q(f(x)) @ q(f(w)).T
+    dx = q(f(dy), sn, None if pr is None else f(pr)) @ q(f(w).T, sn).T
+    dw = q(f(dy).T, sm, None if pc is None else f(pc)) @ q(f(x).T, sm).T
+    return y, dx[:, :k], dw[:, :k]
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (70, 33, 300), (300, 257, 96)])
+@pytest.mark.parametrize("rotate,rounding", [(False, "nearest"), (True, "pool"), (True, "philox")])
+@pytest.mark.parametrize("dtype", [BF, FP], ids=str)
+def test_linear(ms, capi, m, n, k, rotate, rounding, dtype):
+    x, w, dy = matrix(m, k, dtype, 1, 1.0).requires_grad_(), matrix(n, k, dtype, 2, 1.0).requires_grad_(), matrix(m, n, dtype, 3, 1.0)
+    (bn, sn), (bm, sm) = (signs(capi, n, 5), signs(capi, m, 6)) if rotate else ((None, None),) * 2
+    pools = (pool(m, n, BF, 1), pool(n, m, BF, 2)) if rounding == "pool" else None
+    kw = dict(seed=77, step=3) if rounding == "philox" else {}
+    y = ms.linear(x, w, sign=(bn, bm) if rotate else None, rand_pool=pools, **kw)
+    y.backward(dy)
+    if rounding == "philox":
+        pools = tuple(torch.empty(r, -(-c // 256) * 256, device=DEV) for r, c in ((m, n), (n, m)))
+        capi.philox_uniform(pools[0], 77, 6)
+        capi.philox_uniform(pools[1], 77, 7)
+    want = plain_linear(x.detach(), w.detach(), dy, sn, sm, *(pools or (None, None)))
+    for got, t, length in ((y, want[0], k), (x.grad, want[1], n), (w.grad, want[2], m)):
+        assert got.dtype == dtype
+        g = got.detach().double().cpu().numpy()
+        # as in test_product, with the operands' magnitudes bounded by their norms
+        size = np.abs(t).max() * 4 + 1e-30
+        assert np.all(np.abs(g - t) <= torch.finfo(dtype).eps / 2 * np.abs(t) + length * 2.0 ** -23 * size * 8)
+
+
+def test_linear_shapes_and_partial_gradients(ms):
+    x, w = matrix(12, 64, BF, 1).view(3, 4, 64), matrix(10, 64, BF, 2)
+    y = ms.linear(x, w)
+    assert y.shape == (3, 4, 10) and torch.equal(y.view(12, 10), ms.product(ms.quantize(x.view(12, 64)), ms.quantize(w)))
+    wg = w.clone().requires_grad_()
+    ms.linear(x, wg).sum().backward()                       # an expanded gradient
+    assert wg.grad.shape == (10, 64)
+    xg = x.clone().requires_grad_()
+    ms.linear(xg, w, seed=1).float().square().sum().backward()
+    assert xg.grad.shape == x.shape
+    assert ms.linear(x.transpose(0, 1), w).shape == (4, 3, 10)
+
+
+def test_gradients_against_differences(ms):
+    """with operands that 4 bits hold exactly, the layer is the plain product, and its gradients are its differences"""
+    rng = np.random.default_rng(0)
+    x0, w0 = (rng.integers(-2, 3, s).astype(np.float32) for s in ((8, 64), (32, 64)))
+    c = rng.integers(-4, 5, (8, 32)).astype(np.float32)
+    for t in (x0, w0, c):
+        t[:, 0] = 4
+    x0[0], w0[0], c[0] = 4, 4, 4
+    x, w = (torch.from_numpy(t).to(DEV).requires_grad_() for t in (x0, w0))
+    dy = torch.from_numpy(c).to(DEV)
+    (ms.linear(x, w) * dy).sum().backward()
+    value = lambda a, b: float((ms.linear(a, b) * dy).sum())       # noqa: E731
+    with torch.no_grad():
+        for i, j in ((1, 3), (7, 60), (2, 2), (5, 33)):
+            a, b = x.clone(), w.clone()
+            a[i, j], b[i, j] = 0, 0
+            assert value(x, w) - value(a, w) == float(x[i, j] * x.grad[i, j])
+            assert value(x, w) - value(x, b) == float(w[i, j] * w.grad[i, j])
+
+
+def test_rounding_has_no_bias(ms):
+    """the mean of many stochastic roundings is the value: 4096 draws, six standard deviations of half a step at most"""
+    x = matrix(1, 256, FP, 1, 1.0)
+    mean = sum(ms.dequantize(ms.quantize(x, seed=s)).double() for s in range(4096)) / 4096
+    step = torch.exp2(ms.quantize(x, seed=0).scales.double().repeat_interleave(32, 1) - 127) * 2
+    # a uniform value is a multiple of 1/256: half of that is the bias of one rounding at most
+    assert torch.all((mean - x.double()).abs() <= step * (6 * 0.5 / 64 + 1 / 256))
+
+
+def test_graph_and_streams(ms, capi):
+    x, w = matrix(70, 512, BF, 1), matrix(300, 512, BF, 2)
+    bits, _ = signs(capi, 70, 3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(5_000_000)
+        x.mul_(2)
+        y = ms.product(ms.quantize(x), ms.quantize(w))
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, ms.product(ms.quantize(x), ms.quantize(w)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = ms.quantize(x, True, bits, seed=5, step=1)
+        z = ms.product(ms.quantize(x), ms.quantize(w))
+        values = ms.dequantize(q, BF)
+    for k in range(4):
+        x.copy_(matrix(70, 512, BF, 10 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(z, ms.product(ms.quantize(x), ms.quantize(w)))
+        assert torch.equal(values, ms.dequantize(ms.quantize(x, True, bits, seed=5, step=1), BF))
+
+
+def test_layer_in_a_graph(ms, capi):
+    """forward and backward recorded together"""
+    x0, w0, dy = matrix(40, 96, BF, 1, 1.0), matrix(50, 96, BF, 2, 1.0), matrix(40, 50, BF, 3, 1.0)
+    x, w = x0.clone().requires_grad_(), w0.clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ms.linear(x, w, seed=1, step=2), (x, w), dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ms.linear(x, w, seed=1, step=2)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(x0 * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        a, b = (x0 * (k + 1)).requires_grad_(), w0.clone().requires_grad_()
+        e = ms.linear(a, b, seed=1, step=2)
+        assert torch.equal(y, e) and all(torch.equal(s, t) for s, t in zip((dx, dw), torch.autograd.grad(e, (a, b), dy)))
