@@ -12,6 +12,7 @@ struct ProductArgs {
     void *out;
     int64_t m, n;
     int superchunks;
+    uint32_t tiles_n;
 };
 
 __device__ __forceinline__ i32x8 operand(uint4 v)
@@ -50,15 +51,171 @@ template <int DT> __global__ __launch_bounds__(64) void mx4_product_kernel(Produ
     }
 }
 
+// ---- many rows: tiles through LDS --------------------------------------------------------------------------
+
+// 16 (4) bytes a lane from base + offset to LDS, lane after lane from byte `to` on.  Written out: the compiler takes a read of any part of LDS for one of
+// what is on its way there, and waits.  Whoever reads waits for vmcnt himself.
+__device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to));
+}
+__device__ __forceinline__ void load_lds4(const uint8_t *base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(to));
+}
+
+// A workgroup of four waves, 2 x 2, takes a tile of T x T, superchunk by superchunk: rows of 128 bytes of codes and 8 of scales, which lie in LDS twice, one
+// being computed with while the next arrives.  Piece b of row r lies in slot b ^ (r / 2 % 8): the sixteen lanes that read at a time, one piece of sixteen rows,
+// then find sixteen different groups of banks.  The operands of a step are read during the products of the step before; the waves meet before the last step
+// of a superchunk, when everything of it is in registers.
+template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void mx4_tile_kernel(ProductArgs p)
+{
+    constexpr int F = T / 64; // 32 x 32 products of a wave, each way
+    constexpr int kCodes = T * 128, kScales = T * 8, kStage = 2 * (kCodes + kScales);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
+    const int64_t i0 = (int64_t)(blockIdx.x / p.tiles_n) * T, j0 = (int64_t)(blockIdx.x % p.tiles_n) * T;
+    const uint32_t pitch = p.superchunks * 128u, scale_pitch = p.superchunks * 8u;
+
+    // what this lane fetches: pieces of 16 bytes, eight rows a wave and instruction; scale words, 32 rows likewise.  Rows past the end are the last one's.
+    constexpr int kLoads = T / 32, kScaleLoads = T / 128;
+    uint32_t from_a[kLoads], from_b[kLoads], scale_a[kScaleLoads], scale_b[kScaleLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; k++) {
+        const int r = 8 * (4 * k + wave) + (lane >> 3);
+        const uint32_t piece = ((lane & 7) ^ (r >> 1 & 7)) * 16;
+        from_a[k] = (uint32_t)min((int64_t)r, p.m - 1 - i0) * pitch + piece;
+        from_b[k] = (uint32_t)min((int64_t)r, p.n - 1 - j0) * pitch + piece;
+    }
+#pragma unroll
+    for (int k = 0; k < kScaleLoads; k++) {
+        const int r = 32 * (4 * k + wave) + (lane >> 1);
+        scale_a[k] = (uint32_t)min((int64_t)r, p.m - 1 - i0) * scale_pitch + 4 * (lane & 1);
+        scale_b[k] = (uint32_t)min((int64_t)r, p.n - 1 - j0) * scale_pitch + 4 * (lane & 1);
+    }
+    const uint8_t *a = p.a_codes + i0 * pitch, *b = p.b_codes + j0 * pitch;
+    const uint8_t *as = p.a_scales + i0 * scale_pitch, *bs = p.b_scales + j0 * scale_pitch;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    auto fetch = [&](uint32_t stage) {
+        const uint32_t to = lds_at + stage;
+#pragma unroll
+        for (int k = 0; k < kLoads; k++) {
+            load_lds16(a, from_a[k], to + 1024 * (4 * k + wave));
+            load_lds16(b, from_b[k], to + kCodes + 1024 * (4 * k + wave));
+        }
+#pragma unroll
+        for (int k = 0; k < kScaleLoads; k++) {
+            load_lds4(as, scale_a[k], to + 2 * kCodes + 256 * (4 * k + wave));
+            load_lds4(bs, scale_b[k], to + 2 * kCodes + kScales + 256 * (4 * k + wave));
+        }
+        a += 128, b += 128, as += 8, bs += 8;
+    };
+
+    f32x16 acc[F][F] = {};
+    uint4 x[2][F], y[2][F];
+    int sa[F], sb[F], next_sa[F], next_sb[F];
+    const int ra = (wave >> 1) * (T / 2) + (lane & 31), rb = (wave & 1) * (T / 2) + (lane & 31);
+    const uint8_t *at_a = lds + ra * 128, *at_b = lds + kCodes + rb * 128, *at_sa = lds + 2 * kCodes + ra * 8 + 4 * half,
+                  *at_sb = lds + 2 * kCodes + kScales + rb * 8 + 4 * half;
+    uint32_t slot[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) slot[k] = ((4 * half + k) ^ (lane >> 1 & 7)) * 16;
+    auto read = [&](int to, int step, uint32_t stage) {
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            x[to][f] = *reinterpret_cast<const uint4 *>(at_a + stage + slot[step] + 4096 * f);
+            y[to][f] = *reinterpret_cast<const uint4 *>(at_b + stage + slot[step] + 4096 * f);
+        }
+    };
+    auto read_scales = [&](uint32_t stage) {
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            next_sa[f] = *reinterpret_cast<const int *>(at_sa + stage + 256 * f);
+            next_sb[f] = *reinterpret_cast<const int *>(at_sb + stage + 256 * f);
+        }
+    };
+    // every wave has what it fetched, and is done with what it read
+    auto meet = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#define DQ_PRODUCTS(FROM, S)                                                                                                                    \
+    _Pragma("unroll") for (int f = 0; f < F; f++)                                                                                               \
+        _Pragma("unroll") for (int h = 0; h < F; h++)                                                                                           \
+            acc[f][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(y[FROM][h]), operand(x[FROM][f]), acc[f][h], 4, 4, S, sb[h], S, sa[f]);
+    // one read, then as many products as there are to a read
+#define DQ_INTERLEAVE(READS)                                                                                                                    \
+    _Pragma("unroll") for (int k = 0; k < 2 * F; k++) {                                                                                         \
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);                                                                                  \
+        __builtin_amdgcn_sched_group_barrier(0x008, F / 2, 0);                                                                                  \
+    }                                                                                                                                           \
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(0);
+    meet();
+    if (p.superchunks > 1) fetch(kStage);
+    read(0, 0, 0);
+    read_scales(0);
+    uint32_t stage = 0;
+    // (one block of code each, without a branch: products would wander behind it)
+#define DQ_SUPERCHUNK(FETCH)                                                                                                                    \
+    {                                                                                                                                           \
+        _Pragma("unroll") for (int f = 0; f < F; f++) sa[f] = next_sa[f], sb[f] = next_sb[f];                                                   \
+        read(1, 1, stage);                                                                                                                      \
+        DQ_PRODUCTS(0, 0)                                                                                                                       \
+        DQ_INTERLEAVE(1)                                                                                                                        \
+        read(0, 2, stage);                                                                                                                      \
+        DQ_PRODUCTS(1, 1)                                                                                                                       \
+        DQ_INTERLEAVE(1)                                                                                                                        \
+        read(1, 3, stage);                                                                                                                      \
+        DQ_PRODUCTS(0, 2)                                                                                                                       \
+        DQ_INTERLEAVE(1)                                                                                                                        \
+        meet();                                                                                                                                 \
+        FETCH;                                                                                                                                  \
+        stage = kStage - stage;                                                                                                                 \
+        read(0, 0, stage);                                                                                                                      \
+        read_scales(stage);                                                                                                                     \
+        DQ_PRODUCTS(1, 3)                                                                                                                       \
+        DQ_INTERLEAVE(2)                                                                                                                        \
+    }
+    for (int s = 2; s < p.superchunks; s++) DQ_SUPERCHUNK(fetch(stage))
+    if (p.superchunks > 1) DQ_SUPERCHUNK()
+    DQ_SUPERCHUNK() // (what it reads ahead is of the superchunk before, and not used)
+#undef DQ_SUPERCHUNK
+#undef DQ_PRODUCTS
+#undef DQ_INTERLEAVE
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+        const int64_t i = i0 + ra + 32 * f;
+        if (i < p.m) {
+#pragma unroll
+            for (int h = 0; h < F; h++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const int64_t c = j0 + (wave & 1) * (T / 2) + 32 * h + (k >> 2) * 8 + half * 4 + (k & 3);
+                    if (c < p.n) ElemIO<DT>::store(p.out, i * p.n + c, acc[f][h][k]);
+                }
+        }
+    }
+}
+
+template <int DT> static hipError_t launch_product(ProductArgs p, hipStream_t stream)
+{
+    if (p.m > 64) {
+        const int tile = 256;
+        p.tiles_n = (uint32_t)((p.n + tile - 1) / tile);
+        const dim3 grid((uint32_t)((p.m + tile - 1) / tile) * p.tiles_n);
+        return launch_with(mx4_tile_kernel<DT, 256>, grid, dim3(256), stream, p);
+    }
+    const dim3 grid((uint32_t)((p.n + 31) >> 5), (uint32_t)((p.m + 31) >> 5));
+    return launch_with(mx4_product_kernel<DT>, grid, dim3(64), stream, p);
+}
+
 hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out, int64_t m,
                               int64_t n, int64_t k, int dtype, hipStream_t stream)
 {
-    const ProductArgs p = {a_codes, a_scales, b_codes, b_scales, out, m, n, (int)((k + 255) >> 8)};
-    const dim3 grid((uint32_t)((n + 31) >> 5), (uint32_t)((m + 31) >> 5));
-    if (dtype == DQ_F32)
-        return launch_with(mx4_product_kernel<DQ_F32>, grid, dim3(64), stream, p);
-    return dtype == DQ_BF16 ? launch_with(mx4_product_kernel<DQ_BF16>, grid, dim3(64), stream, p)
-                            : launch_with(mx4_product_kernel<DQ_F16>, grid, dim3(64), stream, p);
+    const ProductArgs p = {a_codes, a_scales, b_codes, b_scales, out, m, n, (int)((k + 255) >> 8), 0};
+    return dtype == DQ_F32 ? launch_product<DQ_F32>(p, stream) : dtype == DQ_BF16 ? launch_product<DQ_BF16>(p, stream) : launch_product<DQ_F16>(p, stream);
 }
 
 } // namespace dq
