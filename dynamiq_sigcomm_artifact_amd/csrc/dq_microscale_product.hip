@@ -64,6 +64,18 @@ __device__ __forceinline__ void load_lds4(const uint8_t *base, uint32_t offset, 
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(to));
 }
 
+// Which tile a workgroup takes.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that lie together, four rows of tiles high, so that
+// what its 32 CUs work on at a time shares operands in its L2.
+__device__ __forceinline__ uint2 tile_of(uint32_t id, uint32_t tiles, uint32_t tiles_m, uint32_t tiles_n)
+{
+    const uint32_t xcd = id & 7, each = tiles >> 3, more = tiles & 7;
+    const uint32_t k = xcd * each + min(xcd, more) + (id >> 3);
+    const uint32_t band = k / (4 * tiles_n), in_band = k - band * 4 * tiles_n;
+    const uint32_t high = min(4u, tiles_m - 4 * band);
+    // (divided in vector registers, the same in every lane)
+    return make_uint2(__builtin_amdgcn_readfirstlane(4 * band + in_band % high), __builtin_amdgcn_readfirstlane(in_band / high));
+}
+
 // A workgroup of four waves, 2 x 2, takes a tile of T x T, superchunk by superchunk: rows of 128 bytes of codes and 8 of scales, which lie in LDS twice, one
 // being computed with while the next arrives.  Piece b of row r lies in slot b ^ (r / 2 % 8): the sixteen lanes that read at a time, one piece of sixteen rows,
 // then find sixteen different groups of banks.  The operands of a step are read during the products of the step before; the waves meet before the last step
@@ -74,7 +86,8 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
     constexpr int kCodes = T * 128, kScales = T * 8, kStage = 2 * (kCodes + kScales);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
-    const int64_t i0 = (int64_t)(blockIdx.x / p.tiles_n) * T, j0 = (int64_t)(blockIdx.x % p.tiles_n) * T;
+    const uint2 at = tile_of(blockIdx.x, gridDim.x, (uint32_t)((p.m + T - 1) / T), p.tiles_n);
+    const int64_t i0 = (int64_t)at.x * T, j0 = (int64_t)at.y * T;
     const uint32_t pitch = p.superchunks * 128u, scale_pitch = p.superchunks * 8u;
 
     // what this lane fetches: pieces of 16 bytes, eight rows a wave and instruction; scale words, 32 rows likewise.  Rows past the end are the last one's.
@@ -96,19 +109,27 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
     const uint8_t *a = p.a_codes + i0 * pitch, *b = p.b_codes + j0 * pitch;
     const uint8_t *as = p.a_scales + i0 * scale_pitch, *bs = p.b_scales + j0 * scale_pitch;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    auto fetch = [&](uint32_t stage) {
+    constexpr int kParts = 2 * (kLoads + kScaleLoads);
+    auto fetch_part = [&](uint32_t stage, int part) {
         const uint32_t to = lds_at + stage;
-#pragma unroll
-        for (int k = 0; k < kLoads; k++) {
-            load_lds16(a, from_a[k], to + 1024 * (4 * k + wave));
-            load_lds16(b, from_b[k], to + kCodes + 1024 * (4 * k + wave));
+        const int k = part >> 1;
+        if (k < kLoads) {
+            if (part & 1)
+                load_lds16(b, from_b[k], to + kCodes + 1024 * (4 * k + wave));
+            else
+                load_lds16(a, from_a[k], to + 1024 * (4 * k + wave));
+        } else {
+            if (part & 1)
+                load_lds4(bs, scale_b[k - kLoads], to + 2 * kCodes + kScales + 256 * (4 * (k - kLoads) + wave));
+            else
+                load_lds4(as, scale_a[k - kLoads], to + 2 * kCodes + 256 * (4 * (k - kLoads) + wave));
         }
+    };
+    auto fetched = [&] { a += 128, b += 128, as += 8, bs += 8; };
+    auto fetch = [&](uint32_t stage) {
 #pragma unroll
-        for (int k = 0; k < kScaleLoads; k++) {
-            load_lds4(as, scale_a[k], to + 2 * kCodes + 256 * (4 * k + wave));
-            load_lds4(bs, scale_b[k], to + 2 * kCodes + kScales + 256 * (4 * k + wave));
-        }
-        a += 128, b += 128, as += 8, bs += 8;
+        for (int k = 0; k < kParts; k++) fetch_part(stage, k);
+        fetched();
     };
 
     f32x16 acc[F][F] = {};
@@ -125,13 +146,6 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
         for (int f = 0; f < F; f++) {
             x[to][f] = *reinterpret_cast<const uint4 *>(at_a + stage + slot[step] + 4096 * f);
             y[to][f] = *reinterpret_cast<const uint4 *>(at_b + stage + slot[step] + 4096 * f);
-        }
-    };
-    auto read_scales = [&](uint32_t stage) {
-#pragma unroll
-        for (int f = 0; f < F; f++) {
-            next_sa[f] = *reinterpret_cast<const int *>(at_sa + stage + 256 * f);
-            next_sb[f] = *reinterpret_cast<const int *>(at_sb + stage + 256 * f);
         }
     };
     // every wave has what it fetched, and is done with what it read
@@ -155,7 +169,11 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
     meet();
     if (p.superchunks > 1) fetch(kStage);
     read(0, 0, 0);
-    read_scales(0);
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+        next_sa[f] = *reinterpret_cast<const int *>(at_sa + 256 * f);
+        next_sb[f] = *reinterpret_cast<const int *>(at_sb + 256 * f);
+    }
     uint32_t stage = 0;
     // (one block of code each, without a branch: products would wander behind it)
 #define DQ_SUPERCHUNK(FETCH)                                                                                                                    \
@@ -171,31 +189,75 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
         DQ_PRODUCTS(0, 2)                                                                                                                       \
         DQ_INTERLEAVE(1)                                                                                                                        \
         meet();                                                                                                                                 \
-        FETCH;                                                                                                                                  \
+        const uint32_t free_stage = stage;                                                                                                      \
         stage = kStage - stage;                                                                                                                 \
-        read(0, 0, stage);                                                                                                                      \
-        read_scales(stage);                                                                                                                     \
-        DQ_PRODUCTS(1, 3)                                                                                                                       \
-        DQ_INTERLEAVE(2)                                                                                                                        \
+        /* the first operands of the next superchunk, and what is fetched for the one after it, between the last products of this one */       \
+        _Pragma("unroll") for (int f = 0; f < F; f++)                                                                                           \
+        {                                                                                                                                       \
+            x[0][f] = *reinterpret_cast<const uint4 *>(at_a + stage + slot[0] + 4096 * f);                                                      \
+            y[0][f] = *reinterpret_cast<const uint4 *>(at_b + stage + slot[0] + 4096 * f);                                                      \
+            next_sa[f] = *reinterpret_cast<const int *>(at_sa + stage + 256 * f);                                                               \
+            next_sb[f] = *reinterpret_cast<const int *>(at_sb + stage + 256 * f);                                                               \
+            _Pragma("unroll") for (int h = 0; h < F; h++)                                                                                       \
+            {                                                                                                                                   \
+                acc[f][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(y[1][h]), operand(x[1][f]), acc[f][h], 4, 4, 3, sb[h], 3, sa[f]); \
+                if (FETCH) {                                                                                                                    \
+                    _Pragma("unroll") for (int k = (F * f + h) * kParts / (F * F); k < (F * f + h + 1) * kParts / (F * F); k++) fetch_part(free_stage, k); \
+                }                                                                                                                               \
+                __builtin_amdgcn_sched_barrier(0);                                                                                              \
+            }                                                                                                                                   \
+        }                                                                                                                                       \
+        if (FETCH) fetched();                                                                                                                   \
     }
-    for (int s = 2; s < p.superchunks; s++) DQ_SUPERCHUNK(fetch(stage))
-    if (p.superchunks > 1) DQ_SUPERCHUNK()
-    DQ_SUPERCHUNK() // (what it reads ahead is of the superchunk before, and not used)
+    for (int s = 2; s < p.superchunks; s++) DQ_SUPERCHUNK(true)
+    if (p.superchunks > 1) DQ_SUPERCHUNK(false)
+    DQ_SUPERCHUNK(false) // (what it reads ahead is of the superchunk before, and not used)
 #undef DQ_SUPERCHUNK
 #undef DQ_PRODUCTS
 #undef DQ_INTERLEAVE
+    // The result leaves through LDS as runs of whole rows: 32 rows x T / 2 columns of a wave at a time.  (All waves have passed the last meeting: what lay there
+    // is in registers.)  A lane writes four columns of a row; rows are 16 bytes further apart than long, so that sixteen of them use all banks.
+    typedef typename ElemIO<DT>::storage Elem;
+    constexpr int kRow = T / 2 * sizeof(Elem), kApart = kRow + 16, kPer = 16 / sizeof(Elem), kLanes = kRow / 16;
+    static_assert(4 * 32 * kApart <= 2 * kStage, "the waves' rows fit");
+    uint8_t *mine = lds + wave * 32 * kApart;
+    const int64_t col0 = j0 + (wave & 1) * (T / 2) + lane % kLanes * kPer;
 #pragma unroll
     for (int f = 0; f < F; f++) {
-        const int64_t i = i0 + ra + 32 * f;
-        if (i < p.m) {
 #pragma unroll
-            for (int h = 0; h < F; h++)
+        for (int h = 0; h < F; h++)
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const int64_t c = j0 + (wave & 1) * (T / 2) + 32 * h + (k >> 2) * 8 + half * 4 + (k & 3);
-                    if (c < p.n) ElemIO<DT>::store(p.out, i * p.n + c, acc[f][h][k]);
+            for (int k = 0; k < 4; k++) {
+                uint8_t *to = mine + (lane & 31) * kApart + (32 * h + 8 * k + 4 * half) * sizeof(Elem);
+                const f32x16 v = acc[f][h];
+                if (DT == DQ_F32)
+                    *reinterpret_cast<float4 *>(to) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                else if (DT == DQ_BF16)
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(f32x2_to_bf16x2(v[4 * k], v[4 * k + 1]), f32x2_to_bf16x2(v[4 * k + 2], v[4 * k + 3]));
+                else
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(f32_to_f16_bits(v[4 * k]) | f32_to_f16_bits(v[4 * k + 1]) << 16,
+                                                                f32_to_f16_bits(v[4 * k + 2]) | f32_to_f16_bits(v[4 * k + 3]) << 16);
+            }
+        wave_lds_sync();
+#pragma unroll
+        for (int k = 0; k < 32 * kLanes / 64; k++) {
+            const int r = 64 / kLanes * k + lane / kLanes;
+            const int64_t i = i0 + (wave >> 1) * (T / 2) + 32 * f + r;
+            const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * kApart + lane % kLanes * 16);
+            if (i < p.m) {
+                Elem *to = static_cast<Elem *>(p.out) + i * p.n + col0;
+                if (col0 + kPer <= p.n) {
+                    const u32x4_any w = {v.x, v.y, v.z, v.w};
+                    *reinterpret_cast<u32x4_any *>(to) = w;
+                } else {
+                    const Elem *e = reinterpret_cast<const Elem *>(&v);
+#pragma unroll
+                    for (int c = 0; c < kPer; c++)
+                        if (col0 + c < p.n) to[c] = e[c];
                 }
+            }
         }
+        wave_lds_sync();
     }
 }
 
