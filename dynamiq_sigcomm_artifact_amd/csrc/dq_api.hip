@@ -1208,6 +1208,7 @@ int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_
     if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
     if (!mx4_size_ok(m, k) || !mx4_size_ok(n, k) || !mx4_size_ok(m, n))
         return fail(DQ_ERR_SIZE, "m, n and k must be positive, with less than 2^35 elements of every matrix, padding included");
+    if (k > 1 << 24) return fail(DQ_ERR_SIZE, "k must be at most 2^24");
     if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return fail(DQ_ERR_NULL);
     if (!mx4_aligned(a_codes, a_scales) || !mx4_aligned(b_codes, b_scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
     int rc;

@@ -6,6 +6,7 @@ namespace dq {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct ProductArgs {
     const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
@@ -14,6 +15,9 @@ struct ProductArgs {
     int superchunks;
     uint32_t tiles_n;
 };
+struct NarrowArgs : ProductArgs {
+    int dtype;
+};
 
 __device__ __forceinline__ i32x8 operand(uint4 v)
 {
@@ -21,32 +25,122 @@ __device__ __forceinline__ i32x8 operand(uint4 v)
     return x;
 }
 
-// v_mfma_scale_f32_32x32x64_f8f6f4 on E2M1: lane l holds 32 consecutive elements of row l % 32, and their scale is byte S of its scale word.  The
-// order of the contraction is free as long as both sides keep it: step s takes block s of the superchunk's first half from lanes 0 .. 31 and block s of
-// its second half from lanes 32 .. 63, so that a lane's four scales are one word and its four blocks 64 bytes in a row.
-template <int DT> __global__ __launch_bounds__(64) void mx4_product_kernel(ProductArgs p)
-{
-    const int lane = threadIdx.x, half = lane >> 5, row = lane & 31;
-    const int64_t i0 = (int64_t)blockIdx.y * 32, j0 = (int64_t)blockIdx.x * 32;
-    const int64_t i = min(i0 + row, p.m - 1), j = min(j0 + row, p.n - 1);
-    const uint4 *a = reinterpret_cast<const uint4 *>(p.a_codes + i * p.superchunks * 128 + half * 64);
-    const uint4 *b = reinterpret_cast<const uint4 *>(p.b_codes + j * p.superchunks * 128 + half * 64);
-    const uint32_t *as = reinterpret_cast<const uint32_t *>(p.a_scales + i * p.superchunks * 8 + half * 4);
-    const uint32_t *bs = reinterpret_cast<const uint32_t *>(p.b_scales + j * p.superchunks * 8 + half * 4);
-    f32x16 acc = {};
-    for (int s = 0; s < p.superchunks; s++) {
-        const int sa = (int)as[2 * s], sb = (int)bs[2 * s];
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[8 * s]), operand(a[8 * s]), acc, 4, 4, 0, sb, 0, sa);
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[8 * s + 1]), operand(a[8 * s + 1]), acc, 4, 4, 1, sb, 1, sa);
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[8 * s + 2]), operand(a[8 * s + 2]), acc, 4, 4, 2, sb, 2, sa);
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[8 * s + 3]), operand(a[8 * s + 3]), acc, 4, 4, 3, sb, 3, sa);
+// ---- few rows, or a small result: operands straight from memory -------------------------------------------------
+
+// v_mfma_scale_f32_16x16x128_f8f6f4 on E2M1: lane l holds 32 consecutive elements, one block, of row l % 16, and its scale is byte S of its scale word.  The order of
+// the contraction is free as long as both sides keep it: of a superchunk's eight blocks the lanes l / 16 = g take blocks 2 g and 2 g + 1, so that what a lane
+// loads is 32 bytes of codes in a row and two of scales.
+struct Rows16 {
+    uint4 codes[2];
+    int scales;
+    __device__ __forceinline__ void load(const uint8_t *c, const uint8_t *s)
+    {
+        codes[0] = reinterpret_cast<const uint4 *>(c)[0];
+        codes[1] = reinterpret_cast<const uint4 *>(c)[1];
+        scales = *reinterpret_cast<const uint16_t *>(s);
     }
-    // b is the left operand: a lane holds column `row` of the transposed tile, four consecutive columns of the result at a time
-    if (i0 + row < p.m) {
+};
+
+// A workgroup takes 16 MF x 16 NF of the result; its waves share the superchunks out, one after the other, and add their sums up in LDS, in the order of the
+// waves.  Bound by memory, or by the time to the first byte: every wave has U superchunks on their way at a time.
+template <int MF, int NF, int W, int U> __global__ __launch_bounds__(64 * W) void mx4_narrow_kernel(NarrowArgs p)
+{
+    __shared__ __attribute__((aligned(16))) float sums[W][MF * NF][64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, group = lane >> 4;
+    const int64_t i0 = (int64_t)(blockIdx.x / p.tiles_n) * (16 * MF), j0 = (int64_t)(blockIdx.x % p.tiles_n) * (16 * NF);
+    const uint8_t *a[MF], *as[MF], *b[NF], *bs[NF];
 #pragma unroll
-        for (int k = 0; k < 16; k++) {
-            const int64_t c = j0 + (k >> 2) * 8 + half * 4 + (k & 3);
-            if (c < p.n) ElemIO<DT>::store(p.out, (i0 + row) * p.n + c, acc[k]);
+    for (int f = 0; f < MF; f++) {
+        const int64_t at = min(i0 + 16 * f + row, p.m - 1) * p.superchunks + wave;
+        a[f] = p.a_codes + at * 128 + group * 32;
+        as[f] = p.a_scales + at * 8 + group * 2;
+    }
+#pragma unroll
+    for (int h = 0; h < NF; h++) {
+        const int64_t at = min(j0 + 16 * h + row, p.n - 1) * p.superchunks + wave;
+        b[h] = p.b_codes + at * 128 + group * 32;
+        bs[h] = p.b_scales + at * 8 + group * 2;
+    }
+    f32x4 acc[MF][NF] = {};
+    auto products = [&](const Rows16 (&x)[MF], const Rows16 (&y)[NF]) {
+#pragma unroll
+        for (int f = 0; f < MF; f++)
+#pragma unroll
+            for (int h = 0; h < NF; h++) {
+                acc[f][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(y[h].codes[0]), operand(x[f].codes[0]), acc[f][h], 4, 4, 0, y[h].scales, 0, x[f].scales);
+                acc[f][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(y[h].codes[1]), operand(x[f].codes[1]), acc[f][h], 4, 4, 1, y[h].scales, 1, x[f].scales);
+            }
+    };
+    int s = wave;
+    for (; s + (U - 1) * W < p.superchunks; s += U * W) {
+        Rows16 x[U][MF], y[U][NF];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int h = 0; h < NF; h++) y[u][h].load(b[h] + u * W * 128, bs[h] + u * W * 8);
+#pragma unroll
+            for (int f = 0; f < MF; f++) x[u][f].load(a[f] + u * W * 128, as[f] + u * W * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) products(x[u], y[u]);
+#pragma unroll
+        for (int h = 0; h < NF; h++) b[h] += U * W * 128, bs[h] += U * W * 8;
+#pragma unroll
+        for (int f = 0; f < MF; f++) a[f] += U * W * 128, as[f] += U * W * 8;
+    }
+    for (; s < p.superchunks; s += W) {
+        Rows16 x[MF], y[NF];
+#pragma unroll
+        for (int h = 0; h < NF; h++) {
+            y[h].load(b[h], bs[h]);
+            b[h] += W * 128, bs[h] += W * 8;
+        }
+#pragma unroll
+        for (int f = 0; f < MF; f++) {
+            x[f].load(a[f], as[f]);
+            a[f] += W * 128, as[f] += W * 8;
+        }
+        products(x, y);
+    }
+#pragma unroll
+    for (int f = 0; f < MF; f++)
+#pragma unroll
+        for (int h = 0; h < NF; h++) *reinterpret_cast<f32x4 *>(sums[wave][f * NF + h][lane]) = acc[f][h];
+    __syncthreads();
+    // b is the left operand: what a lane holds are four consecutive columns of a row of the result
+#pragma unroll
+    for (int k = 0; k < (MF * NF + W - 1) / W; k++) {
+        const int block = k * W + wave;
+        if (MF * NF % W != 0 && block >= MF * NF) continue;
+        f32x4 v = *reinterpret_cast<const f32x4 *>(sums[0][block][lane]);
+#pragma unroll
+        for (int w = 1; w < W; w++) v += *reinterpret_cast<const f32x4 *>(sums[w][block][lane]);
+        const int64_t i = i0 + 16 * (block / NF) + row, j = j0 + 16 * (block % NF) + 4 * group;
+        if (i >= p.m) continue;
+        const int64_t to = i * p.n + j;
+        if (j + 4 <= p.n) {
+            if (p.dtype == DQ_F32) {
+                *reinterpret_cast<f32x4_any *>(static_cast<float *>(p.out) + to) = v;
+            } else {
+                typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+                u32x2_any w;
+                if (p.dtype == DQ_BF16)
+                    w = u32x2_any{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+                else
+                    w = u32x2_any{f32_to_f16_bits(v[0]) | f32_to_f16_bits(v[1]) << 16, f32_to_f16_bits(v[2]) | f32_to_f16_bits(v[3]) << 16};
+                *reinterpret_cast<u32x2_any *>(static_cast<uint16_t *>(p.out) + to) = w;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (j + c < p.n) {
+                    if (p.dtype == DQ_F32)
+                        ElemIO<DQ_F32>::store(p.out, to + c, v[c]);
+                    else if (p.dtype == DQ_BF16)
+                        ElemIO<DQ_BF16>::store(p.out, to + c, v[c]);
+                    else
+                        ElemIO<DQ_F16>::store(p.out, to + c, v[c]);
+                }
         }
     }
 }
@@ -261,23 +355,47 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
     }
 }
 
-template <int DT> static hipError_t launch_product(ProductArgs p, hipStream_t stream)
+template <int MF, int NF, int W, int U> static hipError_t launch_narrow(const ProductArgs &p, int dtype, hipStream_t stream)
 {
-    if (p.m > 64) {
-        const int tile = 256;
-        p.tiles_n = (uint32_t)((p.n + tile - 1) / tile);
-        const dim3 grid((uint32_t)((p.m + tile - 1) / tile) * p.tiles_n);
-        return launch_with(mx4_tile_kernel<DT, 256>, grid, dim3(256), stream, p);
-    }
-    const dim3 grid((uint32_t)((p.n + 31) >> 5), (uint32_t)((p.m + 31) >> 5));
-    return launch_with(mx4_product_kernel<DT>, grid, dim3(64), stream, p);
+    NarrowArgs a;
+    static_cast<ProductArgs &>(a) = p;
+    a.dtype = dtype;
+    a.tiles_n = (uint32_t)((p.n + 16 * NF - 1) / (16 * NF));
+    return launch_with(mx4_narrow_kernel<MF, NF, W, U>, dim3((uint32_t)((p.m + 16 * MF - 1) / (16 * MF)) * a.tiles_n), dim3(64 * W), stream, a);
+}
+
+template <int DT, int T> static hipError_t launch_tiles(ProductArgs p, hipStream_t stream)
+{
+    p.tiles_n = (uint32_t)((p.n + T - 1) / T);
+    return launch_with(mx4_tile_kernel<DT, T>, dim3((uint32_t)((p.m + T - 1) / T) * p.tiles_n), dim3(256), stream, p);
+}
+
+// Which kernel.  Tiles of 256 x 256 fetch the least per product, but one takes a CU: at 192 of them, three quarters of the CUs, they draw level with tiles of 128,
+// of which two share a CU (2048 x 4096 x 4096, 128 of 256: 33.6 us against 32.3; 4096 x 4096 x 1000, 256: 18.3 against 19.9).  Below 96 tiles of 128 the contraction
+// is shared out among the waves of a workgroup instead (256 x 4096 x 4096, 64 tiles: 16.4 us, split 14.7; 512 x 4096 x 4096, 128 tiles: 17.0, split 28.8), in the
+// largest blocks that leave 192 workgroups: with fewer, CUs have nothing to do (16 x 4096 x 4096, blocks of 16 x 16: 5.4 us, 16 x 64: 9.2), with more the
+// operands are read more often (16 x 14336 x 4096: 13.3 and 9.6 us).
+template <int MF, int NF, int U> static bool try_narrow(const ProductArgs &p, bool last, int dtype, hipStream_t stream, hipError_t &e)
+{
+    const int64_t blocks = ((p.m + 16 * MF - 1) / (16 * MF)) * ((p.n + 16 * NF - 1) / (16 * NF));
+    if (!last && (blocks < 192 || 8 * MF >= p.m || 8 * NF >= p.n)) return false;
+    e = launch_narrow<MF, NF, 8, U>(p, dtype, stream);
+    return true;
 }
 
 hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out, int64_t m,
                               int64_t n, int64_t k, int dtype, hipStream_t stream)
 {
     const ProductArgs p = {a_codes, a_scales, b_codes, b_scales, out, m, n, (int)((k + 255) >> 8), 0};
-    return dtype == DQ_F32 ? launch_product<DQ_F32>(p, stream) : dtype == DQ_BF16 ? launch_product<DQ_BF16>(p, stream) : launch_product<DQ_F16>(p, stream);
+    const auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+    if (m > 64 && n > 64 && tiles(256) >= 192)
+        return dtype == DQ_F32 ? launch_tiles<DQ_F32, 256>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 256>(p, stream) : launch_tiles<DQ_F16, 256>(p, stream);
+    if (m > 64 && n > 64 && tiles(128) >= 96)
+        return dtype == DQ_F32 ? launch_tiles<DQ_F32, 128>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 128>(p, stream) : launch_tiles<DQ_F16, 128>(p, stream);
+    hipError_t e = hipSuccess;
+    (void)(try_narrow<4, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 2, 1>(p, false, dtype, stream, e) ||
+           try_narrow<1, 4, 1>(p, false, dtype, stream, e) || try_narrow<1, 2, 2>(p, false, dtype, stream, e) || try_narrow<1, 1, 2>(p, true, dtype, stream, e));
+    return e;
 }
 
 } // namespace dq

@@ -837,7 +837,7 @@ int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, in
 int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows,
                       int64_t cols, int device, dq_stream_t stream);
 /* out[i][j] = sum over the contraction of a[i] b[j], `dtype` [m][n], summed in
- * binary32; k: the rows' length, padding excluded. */
+ * binary32; k: the rows' length, padding excluded, at most 2^24. */
 int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes,
                    const uint8_t *b_scales, void *out, int dtype, int64_t m, int64_t n, int64_t k, int device,
                    dq_stream_t stream);

@@ -86,6 +86,7 @@ def test_matrices_refuse(L):
     refused(L, L.dq_mx4_product(P, P, P, P, P, 9, 1, 1, 1, 0, S), "dtype")
     for m, n, k in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1 << 27, 1, 1), (1 << 20, 1 << 20, 1)):
         refused(L, L.dq_mx4_product(P, P, P, P, P, 1, m, n, k, 0, S), "positive")
+    refused(L, L.dq_mx4_product(P, P, P, P, P, 1, 1, 1, (1 << 24) + 1, 0, S), "2^24")
     refused(L, L.dq_mx4_product(P, P, N, P, P, 1, 1, 1, 1, 0, S), "null")
     refused(L, L.dq_mx4_product(P, P, odd, P, P, 1, 1, 1, 1, 0, S), "aligned")
 
