@@ -1115,7 +1115,7 @@ int dq_quantization(float *vec, int64_t n, int device, float div_factor, float t
     return finish(dq::launch_quantization(vec, n, div_factor, tensor_max, seed, static_cast<hipStream_t>(stream)));
 }
 
-int64_t dq_grad_norm_work_doubles(void) { return 1 + dq::kNormGrid; }
+int64_t dq_grad_norm_work_doubles(void) { return dq::kNormGrid; }
 
 int dq_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work, int64_t work_doubles, float *out, int device,
                  dq_stream_t stream)

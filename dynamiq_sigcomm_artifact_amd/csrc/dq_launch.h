@@ -348,27 +348,31 @@ hipError_t launch_bits_to_bins(int32_t *bins, int64_t nbins, const uint32_t *arr
 hipError_t launch_quantization(float *vec, int64_t n, float div_factor, float tensor_max,
                                uint64_t seed, hipStream_t stream);
 
-// the end of a training step (dq_optimizer.hip): tensors of one launch; their descriptors are kernel arguments
-constexpr int kTensors = 64;
-constexpr int kMxBlock = 32;                       // elements that share a scale
-constexpr int64_t kMxMost = (int64_t)1 << 35;      // elements of a matrix, padding included, or of a tensor: a grid has less than 2^32 threads
-constexpr int kNormGrid = 2048; // workgroups of a launch at most, and partial sums
-struct NormArgs {
-    uint32_t first_tile[kTensors];
-    const void *data[kTensors];
-    int64_t n[kTensors];
+// the end of a training step (dq_optimizer.hip).  The descriptors of a launch's tensors are kernel arguments: few, or as many as 4 KiB hold.
+constexpr int kMxBlock = 32;                  // elements that share a scale
+constexpr int64_t kMxMost = (int64_t)1 << 35; // elements of a matrix, padding included, or of a tensor: a grid has less than 2^32 threads
+constexpr int kNormGrid = 2048;               // workgroups of a launch at most, and partial sums
+template <int TENSORS> struct NormArgs {
+    uint32_t first_tile[TENSORS];
+    const void *data[TENSORS];
+    int64_t n[TENSORS];
     double *partial;
-    uint32_t *ticket; // how many workgroups of the last launch are done; 0 between calls
-    float *out;       // null in all launches of a call but the last
+    float *out; // set: the one workgroup of the call finishes it
     double max_norm;
     uint32_t tiles, slots_before; // partial sums that earlier launches of the call have left
 };
-struct AdamwArgs {
-    uint32_t first_tile[kTensors];
-    void *param[kTensors];
-    const void *grad[kTensors];
-    int64_t n[kTensors];
-    uint32_t first_block[kTensors]; // start of the tensor in the arenas, in blocks of 32
+struct NormEnd {
+    const double *partial;
+    float *out;
+    double max_norm;
+    uint32_t slots;
+};
+template <int TENSORS> struct AdamwArgs {
+    uint32_t first_tile[TENSORS];
+    void *param[TENSORS];
+    const void *grad[TENSORS];
+    int64_t n[TENSORS];
+    uint32_t first_block[TENSORS]; // start of the tensor in the arenas, in blocks of 32
     void *state;
     uint8_t *scales;
     float *master;

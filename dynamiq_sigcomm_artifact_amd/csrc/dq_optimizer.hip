@@ -1,18 +1,21 @@
 // The end of a training step: the norm of all gradients with the factor that clips them, and the AdamW step over many tensors.
 //
-// Both stream their tensors once and are bound by memory.  A launch takes up to 64 tensors as kernel arguments (kTensors) and cuts each
-// into tiles; a workgroup finds the tensor of its tile with one load per lane and a ballot.  Nothing about the tensors is kept
-// between calls.
+// Both stream their tensors once and are bound by memory.  A launch takes its tensors as kernel arguments and cuts each into tiles; a workgroup finds
+// the tensor of its tile with a load or two per lane and a ballot.  Nothing about the tensors is kept between calls.
 #include "dq_launch.h"
 #include "dq_microscale.cuh"
 
 namespace dq {
 
 // the tensor that tile `tile` belongs to: the last one that starts at or before it
-__device__ __forceinline__ int tensor_of(const uint32_t (&first_tile)[kTensors], uint32_t tile)
+template <int TENSORS> __device__ __forceinline__ int tensor_of(const uint32_t (&first_tile)[TENSORS], uint32_t tile)
 {
-    const uint64_t before = __builtin_amdgcn_ballot_w64(first_tile[threadIdx.x & 63] <= tile);
-    return __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(before));
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < TENSORS; k += 64)
+        before += __builtin_popcountll(__builtin_amdgcn_ballot_w64((TENSORS % 64 == 0 || k + lane < TENSORS) && first_tile[min(k + lane, TENSORS - 1)] <= tile));
+    return __builtin_amdgcn_readfirstlane(before - 1);
 }
 
 // ---- the norm ---------------------------------------------------------------------------------------------
@@ -26,13 +29,28 @@ __device__ __forceinline__ double wave_sum(double v)
     return v;
 }
 
-// Squares are taken and added in 64 bits: a gradient beyond 2^64 or below 2^-63 has no square in 32, and a sum of 10^8 terms is as exact as
-// its terms.  A workgroup adds its tiles up and writes one number; in the last launch of a call the workgroup that is done last adds those.
-// Which workgroup that is changes from call to call, the order of the additions does not.
-template <int DT> __global__ __launch_bounds__(256) void grad_norm_kernel(NormArgs a)
+// the sum over a workgroup's threads, in its first one
+__device__ __forceinline__ double group_sum(double v)
 {
     __shared__ double part[4];
-    __shared__ int last;
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__device__ __forceinline__ void put_norm(double sum, double max_norm, float *out)
+{
+    const double norm = __builtin_sqrt(sum), factor = __builtin_fmin(1.0, max_norm / (norm + 1e-6));
+    out[0] = (float)norm;
+    out[1] = __builtin_isfinite(norm) ? (float)factor : __builtin_nanf("");
+}
+
+// Squares are taken and added in 64 bits: a gradient beyond 2^64 or below 2^-63 has no square in 32, and a sum of 10^8 terms is as exact as
+// its terms.  A workgroup adds its tiles up and leaves one number for grad_norm_end_kernel, which adds those.  (Workgroups that count themselves, the last of which
+// adds, take longer than a second launch: 800 of them 27 us where the two launches take 9, an atomic on one address being some 30 ns.)
+template <int DT, int TENSORS> __global__ __launch_bounds__(256) void grad_norm_kernel(NormArgs<TENSORS> a)
+{
     const int t = threadIdx.x;
     double sum = 0.0;
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
@@ -58,74 +76,89 @@ template <int DT> __global__ __launch_bounds__(256) void grad_norm_kernel(NormAr
 #pragma unroll
             for (int e = 0; e < 8; e++) sum = __builtin_fma((double)v[j][e], (double)v[j][e], sum);
     }
-    sum = wave_sum(sum);
-    if ((t & 63) == 0) part[t >> 6] = sum;
-    __syncthreads();
+    sum = group_sum(sum);
     if (t == 0) {
-        double *slot = a.partial + blockIdx.x;
-        sum = (part[0] + part[1]) + (part[2] + part[3]);
-        if (blockIdx.x < a.slots_before) sum += *slot;
-        // past this XCD's cache, where the last workgroup may not look
-        __hip_atomic_store(slot, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = a.out && __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        if (blockIdx.x < a.slots_before) sum += a.partial[blockIdx.x];
+        a.partial[blockIdx.x] = sum;
+        if (a.out) put_norm(sum, a.max_norm, a.out);
     }
-    __syncthreads();
-    if (!last) return;
-    const uint32_t slots = max(a.slots_before, gridDim.x);
-    sum = 0.0;
-    for (uint32_t s = t; s < slots; s += 256) sum += __hip_atomic_load(a.partial + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sum = wave_sum(sum);
-    __syncthreads();
-    if ((t & 63) == 0) part[t >> 6] = sum;
-    __syncthreads();
-    if (t == 0) {
-        const double norm = __builtin_sqrt((part[0] + part[1]) + (part[2] + part[3]));
-        const double factor = __builtin_fmin(1.0, a.max_norm / (norm + 1e-6));
-        a.out[0] = (float)norm;
-        a.out[1] = __builtin_isfinite(norm) ? (float)factor : __builtin_nanf("");
-        __hip_atomic_store(a.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+}
+
+__global__ __launch_bounds__(256) void grad_norm_end_kernel(NormEnd a)
+{
+    double v[kNormGrid / 256];
+#pragma unroll
+    for (int k = 0; k < kNormGrid / 256; k++) {
+        const uint32_t s = 256 * k + threadIdx.x;
+        v[k] = a.partial[min(s, a.slots - 1)];
+        if (s >= a.slots) v[k] = 0.0;
     }
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kNormGrid / 256; k++) sum += v[k];
+    sum = group_sum(sum);
+    if (threadIdx.x == 0) put_norm(sum, a.max_norm, a.out);
+}
+
+struct NormCall {
+    const dq_span_t *spans;
+    int count, next;
+    double *partial;
+    double max_norm;
+    float *out;
+    uint32_t slots;
+    hipStream_t stream;
+};
+
+// one launch: tensors of one element type, one after the other, from c.next on
+template <int TENSORS> static hipError_t launch_norm(NormCall &c)
+{
+    NormArgs<TENSORS> a;
+    const int dtype = c.spans[c.next].dtype;
+    int take = 0;
+    int64_t tiles = 0;
+    const bool first = c.next == 0;
+    for (; c.next < c.count && take < TENSORS && c.spans[c.next].dtype == dtype; c.next++) {
+        const dq_span_t &x = c.spans[c.next];
+        const int64_t more = (x.n + kNormTile - 1) / kNormTile;
+        if (take && tiles + more > 0x7fffffff) break;
+        if (more == 0) continue;
+        a.first_tile[take] = (uint32_t)tiles;
+        a.data[take] = x.data;
+        a.n[take++] = x.n;
+        tiles += more;
+    }
+    const bool alone = first && c.next == c.count && tiles <= 2; // the whole call is work for one workgroup
+    if (tiles == 0 && !alone) return hipSuccess;
+    for (int j = take; j < TENSORS; j++) a.first_tile[j] = 0xffffffffu;
+    a.partial = c.partial;
+    a.out = alone ? c.out : nullptr;
+    a.max_norm = c.max_norm;
+    a.tiles = (uint32_t)tiles;
+    a.slots_before = c.slots;
+    const uint32_t grid = alone ? 1 : (uint32_t)std::min<int64_t>(tiles, kNormGrid);
+    c.slots = std::max(c.slots, grid);
+    if (alone) c.out = nullptr;
+    return dtype == DQ_F32 ? launch_with(grad_norm_kernel<DQ_F32, TENSORS>, dim3(grid), dim3(256), c.stream, a)
+         : dtype == DQ_BF16 ? launch_with(grad_norm_kernel<DQ_BF16, TENSORS>, dim3(grid), dim3(256), c.stream, a)
+                            : launch_with(grad_norm_kernel<DQ_F16, TENSORS>, dim3(grid), dim3(256), c.stream, a);
 }
 
 hipError_t launch_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work, float *out, hipStream_t stream)
 {
-    NormArgs a;
-    a.ticket = reinterpret_cast<uint32_t *>(work);
-    a.partial = work + 1;
-    a.max_norm = max_norm;
-    a.slots_before = 0;
+    const dq_span_t nothing = {nullptr, 0, DQ_F32, 0};
+    NormCall c = {count ? spans : &nothing, std::max(count, 1), 0, work, max_norm, out, 0, stream};
     hipError_t e = hipSuccess;
-    int k = 0;
-    bool done = false;
-    while (!done && e == hipSuccess) {
-        // tensors of one element type, one after the other
-        const int dtype = k < count ? spans[k].dtype : DQ_F32;
-        int take = 0;
-        int64_t tiles = 0;
-        for (; k < count && take < kTensors && spans[k].dtype == dtype; k++) {
-            const int64_t more = (spans[k].n + kNormTile - 1) / kNormTile;
-            if (take && tiles + more > 0x7fffffff) break;
-            if (more == 0) continue;
-            a.first_tile[take] = (uint32_t)tiles;
-            a.data[take] = spans[k].data;
-            a.n[take++] = spans[k].n;
-            tiles += more;
-        }
-        for (int j = take; j < kTensors; j++) a.first_tile[j] = 0xffffffffu;
-        done = k == count;
-        a.tiles = (uint32_t)tiles;
-        a.out = done ? out : nullptr;
-        const uint32_t grid = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(tiles, kNormGrid));
-        if (tiles == 0 && !done) continue;
-        if (dtype == DQ_F32)
-            e = launch_with(grad_norm_kernel<DQ_F32>, dim3(grid), dim3(256), stream, a);
-        else if (dtype == DQ_BF16)
-            e = launch_with(grad_norm_kernel<DQ_BF16>, dim3(grid), dim3(256), stream, a);
-        else
-            e = launch_with(grad_norm_kernel<DQ_F16>, dim3(grid), dim3(256), stream, a);
-        a.slots_before = std::max(a.slots_before, grid);
+    while (c.next < c.count && e == hipSuccess) e = c.count - c.next <= 8 ? launch_norm<8>(c) : launch_norm<192>(c);
+    if (e != hipSuccess || !c.out) return e;
+    if (c.slots == 0) { // several types, all of nothing
+        c.next = c.count = 1;
+        c.spans = &nothing;
+        c.next = 0;
+        return launch_norm<8>(c);
     }
-    return e;
+    const NormEnd end = {work, out, max_norm, c.slots};
+    return launch_with(grad_norm_end_kernel, dim3(1), dim3(256), stream, end);
 }
 
 // ---- AdamW ------------------------------------------------------------------------------------------------
@@ -153,7 +186,7 @@ __device__ __forceinline__ uint32_t e4m3_dithered(float y, uint32_t dither)
     return ((__float_as_uint(small ? y + 0x1p-6f : y) + dither) >> 20) - (small ? 968u : 960u);
 }
 
-template <int PD, int GD, int BITS, bool MASTER> __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a)
+template <int PD, int GD, int BITS, bool MASTER, int TENSORS> __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs<TENSORS> a)
 {
     const float scale = a.grad_scale ? *a.grad_scale : 1.0f;
     if (!__builtin_isfinite(scale)) return;
@@ -259,27 +292,28 @@ hipError_t launch_adamw_coefficients(const AdamwCount &a, hipStream_t stream)
     return launch_with(adamw_coefficients_kernel, dim3(1), dim3(1), stream, a);
 }
 
-template <int PD, int GD> static hipError_t launch_step(const AdamwArgs &a, int bits, uint32_t grid, hipStream_t stream)
+template <int PD, int GD, int TENSORS> static hipError_t launch_step(const AdamwArgs<TENSORS> &a, int bits, uint32_t grid, hipStream_t stream)
 {
     if constexpr (PD != DQ_F32) {
         if (a.master) {
-            return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, true>, dim3(grid), dim3(256), stream, a)
-                              : launch_with(adamw_kernel<PD, GD, 8, true>, dim3(grid), dim3(256), stream, a);
+            return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, true, TENSORS>, dim3(grid), dim3(256), stream, a)
+                              : launch_with(adamw_kernel<PD, GD, 8, true, TENSORS>, dim3(grid), dim3(256), stream, a);
         }
     }
-    return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, false>, dim3(grid), dim3(256), stream, a)
-                      : launch_with(adamw_kernel<PD, GD, 8, false>, dim3(grid), dim3(256), stream, a);
+    return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, false, TENSORS>, dim3(grid), dim3(256), stream, a)
+                      : launch_with(adamw_kernel<PD, GD, 8, false, TENSORS>, dim3(grid), dim3(256), stream, a);
 }
 
-template <int PD> static hipError_t launch_step_of(int grad, const AdamwArgs &a, int bits, uint32_t grid, hipStream_t stream)
+template <int PD, int TENSORS> static hipError_t launch_step_of(int grad, const AdamwArgs<TENSORS> &a, int bits, uint32_t grid, hipStream_t stream)
 {
     return grad == DQ_F32 ? launch_step<PD, DQ_F32>(a, bits, grid, stream)
          : grad == DQ_BF16 ? launch_step<PD, DQ_BF16>(a, bits, grid, stream) : launch_step<PD, DQ_F16>(a, bits, grid, stream);
 }
 
-hipError_t launch_adamw(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, int count, hipStream_t stream)
+// one launch: tensors of the same element types, one after the other, from *next on
+template <int TENSORS> static hipError_t launch_tensors(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, int count, int *next, hipStream_t stream)
 {
-    AdamwArgs a;
+    AdamwArgs<TENSORS> a;
     a.state = o.state;
     a.scales = o.scales;
     a.master = o.master;
@@ -299,30 +333,34 @@ hipError_t launch_adamw(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, i
         a.root = (float)(1.0 / sqrt(1.0 - pow(o.beta2, (double)o.step)));
         a.dither = (uint32_t)o.step * kDitherStep;
     }
-    hipError_t e = hipSuccess;
-    int k = 0;
-    while (k < count && e == hipSuccess) {
-        const int param = tensors[k].param_dtype, grad = tensors[k].grad_dtype;
-        int take = 0;
-        int64_t tiles = 0;
-        for (; k < count && take < kTensors && tensors[k].param_dtype == param && tensors[k].grad_dtype == grad; k++) {
-            const dq_adamw_tensor_t &x = tensors[k];
-            const int64_t more = (x.n + kStepTile - 1) / kStepTile;
-            if (take && tiles + more > dq::kMxMost / kStepTile - 1) break;
-            if (more == 0) continue;
-            a.first_tile[take] = (uint32_t)tiles;
-            a.param[take] = x.param;
-            a.grad[take] = x.grad;
-            a.n[take] = x.n;
-            a.first_block[take++] = (uint32_t)(x.start / kMxBlock);
-            tiles += more;
-        }
-        for (int j = take; j < kTensors; j++) a.first_tile[j] = 0xffffffffu;
-        if (tiles == 0) continue;
-        e = param == DQ_F32 ? launch_step_of<DQ_F32>(grad, a, o.bits, (uint32_t)tiles, stream)
-          : param == DQ_BF16 ? launch_step_of<DQ_BF16>(grad, a, o.bits, (uint32_t)tiles, stream)
-                             : launch_step_of<DQ_F16>(grad, a, o.bits, (uint32_t)tiles, stream);
+    const int param = tensors[*next].param_dtype, grad = tensors[*next].grad_dtype;
+    int take = 0;
+    int64_t tiles = 0;
+    for (; *next < count && take < TENSORS && tensors[*next].param_dtype == param && tensors[*next].grad_dtype == grad; ++*next) {
+        const dq_adamw_tensor_t &x = tensors[*next];
+        const int64_t more = (x.n + kStepTile - 1) / kStepTile;
+        if (take && tiles + more > kMxMost / kStepTile - 1) break;
+        if (more == 0) continue;
+        a.first_tile[take] = (uint32_t)tiles;
+        a.param[take] = x.param;
+        a.grad[take] = x.grad;
+        a.n[take] = x.n;
+        a.first_block[take++] = (uint32_t)(x.start / kMxBlock);
+        tiles += more;
     }
+    if (tiles == 0) return hipSuccess;
+    for (int j = take; j < TENSORS; j++) a.first_tile[j] = 0xffffffffu;
+    return param == DQ_F32 ? launch_step_of<DQ_F32>(grad, a, o.bits, (uint32_t)tiles, stream)
+         : param == DQ_BF16 ? launch_step_of<DQ_BF16>(grad, a, o.bits, (uint32_t)tiles, stream)
+                            : launch_step_of<DQ_F16>(grad, a, o.bits, (uint32_t)tiles, stream);
+}
+
+hipError_t launch_adamw(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, int count, hipStream_t stream)
+{
+    hipError_t e = hipSuccess;
+    int next = 0;
+    while (next < count && e == hipSuccess)
+        e = count - next <= 32 ? launch_tensors<32>(o, tensors, count, &next, stream) : launch_tensors<112>(o, tensors, count, &next, stream);
     return e;
 }
 

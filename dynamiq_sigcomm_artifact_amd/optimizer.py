@@ -1,7 +1,7 @@
 """What follows the all-reduce in a training step: the norm of the gradients with the factor that clips them, and the AdamW step,
 its states in 32 bits or in 8.
 
-``grad_norm`` and ``adamw_step`` are the operators, on lists of tensors of any sizes, each a launch per 64 tensors (one element
+``grad_norm`` and ``adamw_step`` are the operators, on lists of tensors of any sizes, a launch for every 192 and 112 of them (of one element
 type at a time); ``AdamW`` keeps the states and the count of the steps for them.  ``include/dynamiq_eden.h`` (dq_grad_norm, dq_adamw_step) has the
 formulas and the 8-bit format to the bit.  Everything runs on the current stream of the tensors' device and nothing is read back."""
 import torch
@@ -13,13 +13,13 @@ _HALF = (torch.float16, torch.bfloat16)
 
 def norm_work(device):
     """the work buffer of grad_norm: kept from call to call, one for every stream (or recorded graph) whose calls may overlap"""
-    return torch.zeros(int(capi.lib().dq_grad_norm_work_doubles()), dtype=torch.float64, device=device)
+    return torch.empty(int(capi.lib().dq_grad_norm_work_doubles()), dtype=torch.float64, device=device)
 
 
 def grad_norm(grads, max_norm=None, work=None, out=None):
     """float32 [2] on the device: the 2-norm of all tensors together, summed in 64 bits, and min(1, max_norm / (norm + 1e-6)), the
     ``grad_scale`` of a step that clips (1 without max_norm).  Where the norm is not finite the factor is NaN, and the step
-    changes nothing.  work: from norm_work(); without it the call makes and clears one."""
+    changes nothing.  work: from norm_work(); without it the call makes one."""
     grads = list(grads)
     if not grads:
         raise RuntimeError("grad_norm: no tensors")

@@ -745,16 +745,15 @@ typedef struct dq_span {
     int32_t reserved;
 } dq_span_t;
 
-/* float64 entries of the work buffer: zeroed once, then kept from call to call
- * (a call leaves in it what the next one expects).  Calls that may overlap --
- * on different streams, or replays of different graphs -- need one each. */
+/* float64 entries of the work buffer.  Calls that may overlap -- on different
+ * streams, or replays of different graphs -- need one each. */
 int64_t dq_grad_norm_work_doubles(void);
 /* out[0] = norm = sqrt(sum of the squares of all elements), summed in 64 bits in
  * an order that does not change from call to call; out[1] = min(1, max_norm /
  * (norm + 1e-6)), NaN where the norm is not finite -- the gradient factor of
  * dq_adamw_step, which a NaN makes do nothing.  max_norm > 0 or infinite (no
- * clipping).  One launch per 64 tensors, and per change of element type along
- * the list. */
+ * clipping).  A launch per 192 tensors, and per change of element type along
+ * the list, and one to end with. */
 int dq_grad_norm(const dq_span_t *spans, int count, double max_norm, double *work,
                  int64_t work_doubles, float *out, int device, dq_stream_t stream);
 
