@@ -6,69 +6,96 @@
 
 namespace dq {
 
-// ---- eight consecutive elements of a vector that may lie anywhere: a view into a gradient bucket is aligned to its elements only, and
-// gfx950 loads and stores 16 bytes from any address ----
+// ---- four or eight consecutive elements of a vector that may lie anywhere: a view into a gradient bucket is aligned to its elements only, and
+// gfx950 loads and stores 16 bytes from any address.  PASSING: with the hint that nothing of it is wanted again soon ----
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+template <int DT> __device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b)
+{
+    if (DT == DQ_BF16) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    } else {
+        a = f16_bits_to_f32(w & 0xffffu);
+        b = f16_bits_to_f32(w >> 16);
+    }
+}
+template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    return DT == DQ_BF16 ? f32x2_to_bf16x2(a, b) : f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16);
+}
+
+template <int DT, bool PASSING = false> __device__ __forceinline__ void load4(const void *p, int64_t i, float *v)
+{
+    if (DT == DQ_F32) {
+        const f32x4_any *q = reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + i);
+        const f32x4_any a = PASSING ? __builtin_nontemporal_load(q) : *q;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = a[j];
+    } else {
+        const u32x2_any *q = reinterpret_cast<const u32x2_any *>(static_cast<const uint16_t *>(p) + i);
+        const u32x2_any a = PASSING ? __builtin_nontemporal_load(q) : *q;
+        unpack2<DT>(a[0], v[0], v[1]);
+        unpack2<DT>(a[1], v[2], v[3]);
+    }
+}
 
 template <int DT> __device__ __forceinline__ void load8(const void *p, int64_t i, float (&v)[8])
 {
     if (DT == DQ_F32) {
-        const f32x4_any *q = reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + i);
-        const f32x4_any a = q[0], b = q[1];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            v[j] = a[j];
-            v[j + 4] = b[j];
-        }
+        load4<DT>(p, i, v);
+        load4<DT>(p, i + 4, v + 4);
     } else {
         const u32x4_any a = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p) + i);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (DT == DQ_BF16) {
-                v[2 * j] = __uint_as_float(a[j] << 16);
-                v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
-            } else {
-                v[2 * j] = f16_bits_to_f32(a[j] & 0xffffu);
-                v[2 * j + 1] = f16_bits_to_f32(a[j] >> 16);
-            }
-        }
+        for (int j = 0; j < 4; j++) unpack2<DT>(a[j], v[2 * j], v[2 * j + 1]);
     }
 }
 
-// the first `count` of eight, the others 0
-template <int DT> __device__ __forceinline__ void load8_part(const void *p, int64_t i, int count, float (&v)[8])
+// the first `count` of N, the others 0
+template <int DT, int N> __device__ __forceinline__ void load_part(const void *p, int64_t i, int count, float *v)
 {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = j < count ? ElemIO<DT>::load(p, i + j) : 0.0f;
+    for (int j = 0; j < N; j++) v[j] = j < count ? ElemIO<DT>::load(p, i + j) : 0.0f;
+}
+
+template <int DT, bool PASSING = false> __device__ __forceinline__ void store4(void *p, int64_t i, const float *v)
+{
+    if (DT == DQ_F32) {
+        const f32x4_any a = {v[0], v[1], v[2], v[3]};
+        f32x4_any *q = reinterpret_cast<f32x4_any *>(static_cast<float *>(p) + i);
+        if (PASSING)
+            __builtin_nontemporal_store(a, q);
+        else
+            *q = a;
+    } else {
+        const u32x2_any a = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+        u32x2_any *q = reinterpret_cast<u32x2_any *>(static_cast<uint16_t *>(p) + i);
+        if (PASSING)
+            __builtin_nontemporal_store(a, q);
+        else
+            *q = a;
+    }
 }
 
 template <int DT> __device__ __forceinline__ void store8(void *p, int64_t i, const float (&v)[8])
 {
     if (DT == DQ_F32) {
-        f32x4_any *q = reinterpret_cast<f32x4_any *>(static_cast<float *>(p) + i);
-        f32x4_any a, b;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            a[j] = v[j];
-            b[j] = v[j + 4];
-        }
-        q[0] = a;
-        q[1] = b;
+        store4<DT>(p, i, v);
+        store4<DT>(p, i + 4, v + 4);
     } else {
-        u32x4_any a;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            a[j] = DT == DQ_BF16 ? f32x2_to_bf16x2(v[2 * j], v[2 * j + 1]) : f32_to_f16_bits(v[2 * j]) | (f32_to_f16_bits(v[2 * j + 1]) << 16);
+        const u32x4_any a = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])};
         *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(p) + i) = a;
     }
 }
 
-template <int DT> __device__ __forceinline__ void store8_part(void *p, int64_t i, int count, const float (&v)[8])
+template <int DT, int N> __device__ __forceinline__ void store_part(void *p, int64_t i, int count, const float *v)
 {
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+    for (int j = 0; j < N; j++)
         if (j < count) ElemIO<DT>::store(p, i + j, v[j]);
 }
 

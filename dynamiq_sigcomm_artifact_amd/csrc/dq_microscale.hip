@@ -96,7 +96,7 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
     if (col + 8 <= a.cols)
         load8<DT>(a.x, at, v);
     else
-        load8_part<DT>(a.x, at, (int)max((int64_t)0, a.cols - col), v);
+        load_part<DT, 8>(a.x, at, (int)max((int64_t)0, a.cols - col), v);
     uniform8<RAND>(a, e, u);
     if (ROTATE) rotate_block(v, a.sign[col >> 5], g);
     uint32_t scale;
@@ -122,7 +122,7 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void 
         if (row + j < a.rows && cols == 8)
             load8<DT>(a.x, (row + j) * a.stride + col, x[j]);
         else
-            load8_part<DT>(a.x, (row + j) * a.stride + col, row + j < a.rows ? cols : 0, x[j]);
+            load_part<DT, 8>(a.x, (row + j) * a.stride + col, row + j < a.rows ? cols : 0, x[j]);
     }
     const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u;
 #pragma unroll
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void mx4_values_kernel(const uint32_t *__restr
     if (col + 8 <= cols)
         store8<DT>(out, row * cols + col, v);
     else
-        store8_part<DT>(out, row * cols + col, (int)(cols - col), v);
+        store_part<DT, 8>(out, row * cols + col, (int)(cols - col), v);
 }
 
 hipError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int64_t rows, int64_t cols, int dtype, hipStream_t stream)

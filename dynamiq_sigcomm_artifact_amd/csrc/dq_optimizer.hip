@@ -57,24 +57,28 @@ template <int DT, int TENSORS> __global__ __launch_bounds__(256) void grad_norm_
         const int k = tensor_of(a.first_tile, tile);
         const void *p = a.data[k];
         const int64_t n = a.n[k], at = (int64_t)(tile - a.first_tile[k]) * kNormTile;
-        float v[4][8];
+        constexpr int kPer = DT == DQ_F32 ? 4 : 8; // elements of 16 bytes
+        float v[32 / kPer][8];
         if (at + kNormTile <= n) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) load8<DT>(p, at + 8 * (256 * j + t), v[j]);
+            for (int j = 0; j < 32 / kPer; j++) {
+                const int64_t i = at + kPer * (256 * j + t);
+                if (DT == DQ_F32)
+                    load4<DT>(p, i, v[j]);
+                else
+                    load8<DT>(p, i, v[j]);
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int64_t i = at + 8 * (256 * j + t);
-                if (i + 8 <= n)
-                    load8<DT>(p, i, v[j]);
-                else
-                    load8_part<DT>(p, i, (int)max((int64_t)0, n - i), v[j]);
+            for (int j = 0; j < 32 / kPer; j++) {
+                const int64_t i = at + kPer * (256 * j + t);
+                load_part<DT, kPer>(p, i, (int)max((int64_t)0, min((int64_t)kPer, n - i)), v[j]);
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < 32 / kPer; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum = __builtin_fma((double)v[j][e], (double)v[j][e], sum);
+            for (int e = 0; e < kPer; e++) sum = __builtin_fma((double)v[j][e], (double)v[j][e], sum);
     }
     sum = group_sum(sum);
     if (t == 0) {
@@ -172,21 +176,74 @@ struct Coefficients {
 
 constexpr uint32_t kDitherElement = 0x9E3779B9u, kDitherStep = 0xB504F333u;
 
-// An 8-bit state is E4M3, eleven to thirteen times 2^-7 apart at most; a moment that decays by a thousandth a step would never leave its code if
-// it were rounded to nearest.  So what is cut away is added up over the steps instead: a dither of 20 bits, the fractions of i phi + t / sqrt 2,
-// is added where the bits are cut, and over the steps of one element, and over the elements of one step, these fractions are spread evenly: the mean
-// error goes to zero as 1 / steps.
-__device__ __forceinline__ uint32_t dither_of(uint32_t element, uint32_t step) { return (element * kDitherElement + step) >> 12; }
+// An 8-bit state is E4M3, whose codes are a sixteenth to an eighth apart; a moment that decays by a thousandth a step would never leave its code if it were
+// rounded to nearest.  So what is cut away is added up over the steps instead: a dither of 20 bits, the fractions of i phi + t / sqrt 2, is added where the
+// bits are cut, and over the steps of one element, and over the elements of one step, these fractions are spread evenly: the mean error goes to zero as
+// 1 / steps.  v_cvt_sr_fp8_f32 adds the upper 20 bits of its seed in this way, at normal and at subnormal codes.
+template <int J> __device__ __forceinline__ uint32_t cut_e4m3(float y, uint32_t seed, uint32_t word) { return __builtin_amdgcn_cvt_sr_fp8_f32(y, seed, word, J); }
 
-// the E4M3 code of y >= 0, y <= 448.  From 2^-6 on the code's bits are the float's upper ones; below, where codes are 2^-9 apart, adding
-// 2^-6 puts them there.
-__device__ __forceinline__ uint32_t e4m3_dithered(float y, uint32_t dither)
+__device__ __forceinline__ uint32_t cut4(const float (&y)[4], uint32_t seed, uint32_t flip)
 {
-    const bool small = y < 0x1p-6f;
-    return ((__float_as_uint(small ? y + 0x1p-6f : y) + dither) >> 20) - (small ? 968u : 960u);
+    uint32_t w = 0;
+    w = cut_e4m3<0>(y[0], seed ^ flip, w);
+    w = cut_e4m3<1>(y[1], (seed + kDitherElement) ^ flip, w);
+    w = cut_e4m3<2>(y[2], (seed + 2u * kDitherElement) ^ flip, w);
+    return cut_e4m3<3>(y[3], (seed + 3u * kDitherElement) ^ flip, w);
 }
 
-template <int PD, int GD, int BITS, bool MASTER, int TENSORS> __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs<TENSORS> a)
+// the largest magnitude of a block that eight neighbouring lanes hold four elements each of, as a bit pattern
+__device__ __forceinline__ uint32_t block_max4(const float *v)
+{
+    uint32_t u = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) u = max(u, __float_as_uint(v[j]) & 0x7fffffffu);
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x141, 0xf, 0xf, true)); // row_half_mirror
+    return u;
+}
+
+template <bool PASSING> __device__ __forceinline__ uint32_t load_word(const uint8_t *p)
+{
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+    return PASSING ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool PASSING> __device__ __forceinline__ void store_word(uint8_t *p, uint32_t w)
+{
+    uint32_t *q = reinterpret_cast<uint32_t *>(p);
+    if (PASSING)
+        __builtin_nontemporal_store(w, q);
+    else
+        *q = w;
+}
+
+// Square roots of eight numbers that are not negative.  Between 2^-100 and 2^120, and of 0: v / sqrt(v) from v_rsq_f32, corrected by half of what its square lacks times
+// 1 / sqrt(v), which leaves it rounded to nearest (but for one in millions, whose two neighbours are all but equally near); 8 issue cycles an element where the
+// compiler's root, which also handles what is outside, takes 17.  Anything outside takes that one, for the whole wave.
+__device__ __forceinline__ void roots8(const float (&v)[8], float (&r)[8])
+{
+    uint32_t least = ~0u, most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        least = min(least, __float_as_uint(v[j]) - 1u); // (0 is above all)
+        most = max(most, __float_as_uint(v[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float s = __builtin_amdgcn_rsqf(__builtin_fmaxf(v[j], 0x1p-126f)), q = v[j] * s;
+        r[j] = __builtin_fmaf(__builtin_fmaf(-q, q, v[j]), 0.5f * s, q);
+    }
+    if (DQ_UNLIKELY(__builtin_amdgcn_ballot_w64(least < 0x0d800000u - 1u || most >= 0x7b800000u) != 0)) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) r[j] = __builtin_sqrtf(v[j]);
+    }
+}
+
+// PASSING: more than the 256 MB of cache in front of the memory hold, so that nothing of it is there at the next step.  With the hint that says so on every load and
+// store 124,439,808 binary32 weights take 593 us with 32-bit states and 328 with 8-bit ones where they take 667 and 385 without it (5.9 and 6.1 TB/s for 5.2; in 148
+// tensors at odd addresses 622 and 358 for 671 and 376; on the loads or the stores alone it gains little or loses).  A bucket of 6,553,600, whose 183 MB stay, takes
+// 32 us without the hint and 39 with it.
+template <int PD, int GD, int BITS, bool MASTER, int TENSORS, bool PASSING> __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs<TENSORS> a)
 {
     const float scale = a.grad_scale ? *a.grad_scale : 1.0f;
     if (!__builtin_isfinite(scale)) return;
@@ -197,37 +254,49 @@ template <int PD, int GD, int BITS, bool MASTER, int TENSORS> __global__ __launc
         c.root = a.coefficients[2];
         c.dither = __float_as_uint(a.coefficients[3]);
     }
+    // A lane takes four elements in each half of the tile, so that what a wave loads or stores with an instruction lies together.
     const int k = tensor_of(a.first_tile, blockIdx.x);
-    const int64_t n = a.n[k], i = (int64_t)(blockIdx.x - a.first_tile[k]) * kStepTile + 8 * threadIdx.x;
-    if (i >= ((n + 31) & ~(int64_t)31)) return;
-    const int64_t at = (int64_t)a.first_block[k] * kMxBlock + i; // in the arenas
-    const int mine = (int)min((int64_t)8, n - i);                // elements of the tensor; 0 or less in its padding
+    const int64_t n = a.n[k], i = (int64_t)(blockIdx.x - a.first_tile[k]) * kStepTile + 4 * threadIdx.x;
+    const int64_t at = (int64_t)a.first_block[k] * kMxBlock + i;  // in the arenas
+    const int64_t end = (n + kMxBlock - 1) & ~(int64_t)(kMxBlock - 1); // of its states
+    int mine[2];                                                  // elements of the tensor; 0 or less in its padding and behind
+    bool live[2];
     float g[8], p[8], m[8], v[8], r[8];
-    if (mine == 8)
-        load8<GD>(a.grad[k], i, g);
-    else
-        load8_part<GD>(a.grad[k], i, mine, g);
-    if (MASTER)
-        load8<DQ_F32>(a.master, at, p);
-    else if (mine == 8)
-        load8<PD>(a.param[k], i, p);
-    else
-        load8_part<PD>(a.param[k], i, mine, p);
     uint8_t *codes = static_cast<uint8_t *>(a.state);
-    if (BITS == 32) {
-        load8<DQ_F32>(a.state, at, m);
-        load8<DQ_F32>(a.state, a.total + at, v);
-    } else {
-        const uint2 cm = *reinterpret_cast<const uint2 *>(codes + at), cr = *reinterpret_cast<const uint2 *>(codes + a.total + at);
-        const float um = scale_up(a.scales[at >> 5]), ur = scale_up(a.scales[(a.total + at) >> 5]);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const uint32_t wm = h ? cm.y : cm.x, wr = h ? cr.y : cr.x;
-            const f32x2_t m0 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, true);
-            const f32x2_t r0 = __builtin_amdgcn_cvt_pk_f32_fp8(wr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(wr, true);
-            m[4 * h] = m0.x * um; m[4 * h + 1] = m0.y * um; m[4 * h + 2] = m1.x * um; m[4 * h + 3] = m1.y * um;
-            r[4 * h] = r0.x * ur; r[4 * h + 1] = r0.y * ur; r[4 * h + 2] = r1.x * ur; r[4 * h + 3] = r1.y * ur;
+    for (int h = 0; h < 2; h++) {
+        const int64_t e = i + kStepTile / 2 * h, s = at + kStepTile / 2 * h;
+        mine[h] = (int)max((int64_t)0, min((int64_t)4, n - e));
+        live[h] = e < end;
+        if (mine[h] == 4)
+            load4<GD, PASSING>(a.grad[k], e, g + 4 * h);
+        else
+            load_part<GD, 4>(a.grad[k], e, mine[h], g + 4 * h);
+        if (!MASTER) {
+            if (mine[h] == 4)
+                load4<PD, PASSING>(a.param[k], e, p + 4 * h);
+            else
+                load_part<PD, 4>(a.param[k], e, mine[h], p + 4 * h);
         }
+        if (live[h]) {
+            if (MASTER) load4<DQ_F32, PASSING>(a.master, s, p + 4 * h);
+            if (BITS == 32) {
+                load4<DQ_F32, PASSING>(a.state, s, m + 4 * h);
+                load4<DQ_F32, PASSING>(a.state, a.total + s, v + 4 * h);
+            } else {
+                const uint32_t wm = load_word<PASSING>(codes + s), wr = load_word<PASSING>(codes + a.total + s);
+                const float um = scale_up(a.scales[s >> 5]), ur = scale_up(a.scales[(a.total + s) >> 5]);
+                const f32x2_t m0 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, true);
+                const f32x2_t r0 = __builtin_amdgcn_cvt_pk_f32_fp8(wr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(wr, true);
+                m[4 * h] = m0.x * um; m[4 * h + 1] = m0.y * um; m[4 * h + 2] = m1.x * um; m[4 * h + 3] = m1.y * um;
+                r[4 * h] = r0.x * ur; r[4 * h + 1] = r0.y * ur; r[4 * h + 2] = r1.x * ur; r[4 * h + 3] = r1.y * ur;
+            }
+        } else {
+#pragma unroll
+            for (int j = 4 * h; j < 4 * h + 4; j++) p[j] = m[j] = v[j] = r[j] = 0.0f;
+        }
+    }
+    if (BITS == 8) {
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = r[j] * r[j];
     }
@@ -236,42 +305,65 @@ template <int PD, int GD, int BITS, bool MASTER, int TENSORS> __global__ __launc
         const float gj = g[j] * scale;
         m[j] = m[j] * a.beta1 + gj * a.rest1;
         v[j] = v[j] * a.beta2 + (gj * gj) * a.rest2;
-        r[j] = __builtin_sqrtf(v[j]);
-        p[j] = p[j] * c.keep - c.step * (m[j] / (r[j] * c.root + a.eps));
     }
-    if (mine < 8) {
+    roots8(v, r);
+    // The quotient only moves the weight: by the reciprocal, good to 1 ulp, unless some divisor of the wave is subnormal, zero or so large that its reciprocal is.
+    float q[8];
+    uint32_t least = ~0u, most = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j >= mine) p[j] = m[j] = v[j] = r[j] = 0.0f; // the padding is zero, whatever it was
+    for (int j = 0; j < 8; j++) {
+        const float under = r[j] * c.root + a.eps;
+        least = min(least, __float_as_uint(under));
+        most = max(most, __float_as_uint(under));
+        q[j] = m[j] * __builtin_amdgcn_rcpf(under);
     }
-    if (BITS == 32) {
-        store8<DQ_F32>(a.state, at, m);
-        store8<DQ_F32>(a.state, a.total + at, v);
-    } else {
-        const uint32_t sm = block_scale<8, 0x600000u>(block_max(m)), sr = block_scale<8, 0x600000u>(block_max(r));
-        const float dm = scale_down(sm), dr = scale_down(sr);
-        uint32_t wm[2] = {0, 0}, wr[2] = {0, 0};
+    if (DQ_UNLIKELY(__builtin_amdgcn_ballot_w64(least < 0x00800000u || most >= 0x7e800000u) != 0)) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t d = dither_of((uint32_t)i + j, c.dither);
-            const uint32_t em = e4m3_dithered(__builtin_fabsf(m[j]) * dm, d) | (__float_as_uint(m[j]) >> 31 << 7);
-            // a root above zero stays above zero: a step divides by it
-            const uint32_t er = max(e4m3_dithered(r[j] * dr, 0xfffffu - d), r[j] > 0.0f ? 1u : 0u);
-            wm[j >> 2] |= (em & 0xffu) << (8 * (j & 3));
-            wr[j >> 2] |= (er & 0xffu) << (8 * (j & 3));
-        }
-        *reinterpret_cast<uint2 *>(codes + at) = make_uint2(wm[0], wm[1]);
-        *reinterpret_cast<uint2 *>(codes + a.total + at) = make_uint2(wr[0], wr[1]);
-        if ((threadIdx.x & 3) == 0) {
-            a.scales[at >> 5] = (uint8_t)sm;
-            a.scales[(a.total + at) >> 5] = (uint8_t)sr;
-        }
+        for (int j = 0; j < 8; j++) q[j] = m[j] / (r[j] * c.root + a.eps);
     }
-    if (MASTER) store8<DQ_F32>(a.master, at, p);
-    if (mine == 8)
-        store8<PD>(a.param[k], i, p);
-    else
-        store8_part<PD>(a.param[k], i, mine, p);
+#pragma unroll
+    for (int j = 0; j < 8; j++) p[j] = p[j] * c.keep - c.step * q[j];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int64_t e = i + kStepTile / 2 * h, s = at + kStepTile / 2 * h;
+        if (mine[h] < 4) { // the padding is zero, whatever it was
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j >= mine[h]) p[4 * h + j] = m[4 * h + j] = v[4 * h + j] = r[4 * h + j] = 0.0f;
+        }
+        if (BITS == 8) { // (every lane: a block lies in eight of them)
+            const uint32_t sm = block_scale<8, 0x600000u>(block_max4(m + 4 * h)), sr = block_scale<8, 0x600000u>(block_max4(r + 4 * h));
+            const float dm = scale_down(sm), dr = scale_down(sr);
+            const uint32_t seed = (uint32_t)e * kDitherElement + c.dither;
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = m[4 * h + j] * dm;
+            const uint32_t wm = cut4(y, seed, 0);
+            // A root above zero stays above zero, since a step divides by it: no less than 2^-9, the smallest code.  (Roots above zero are 2^-75 and more.)
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = __builtin_amdgcn_fmed3f(r[4 * h + j] * dr, 0x1p-9f, r[4 * h + j] * 0x1p127f);
+            const uint32_t wr = cut4(y, seed, ~0u);
+            if (live[h]) {
+                store_word<PASSING>(codes + s, wm);
+                store_word<PASSING>(codes + a.total + s, wr);
+                if ((threadIdx.x & 7) == 0) {
+                    a.scales[s >> 5] = (uint8_t)sm;
+                    a.scales[(a.total + s) >> 5] = (uint8_t)sr;
+                }
+            }
+        }
+        if (live[h]) {
+            if (BITS == 32) {
+                store4<DQ_F32, PASSING>(a.state, s, m + 4 * h);
+                store4<DQ_F32, PASSING>(a.state, a.total + s, v + 4 * h);
+            }
+            if (MASTER) store4<DQ_F32, PASSING>(a.master, s, p + 4 * h);
+        }
+        if (mine[h] == 4)
+            store4<PD, PASSING>(a.param[k], e, p + 4 * h);
+        else
+            store_part<PD, 4>(a.param[k], e, mine[h], p + 4 * h);
+    }
 }
 
 // what a step's kernels take from the step's number, where that number is in device memory: a recorded step counts on
@@ -292,22 +384,27 @@ hipError_t launch_adamw_coefficients(const AdamwCount &a, hipStream_t stream)
     return launch_with(adamw_coefficients_kernel, dim3(1), dim3(1), stream, a);
 }
 
-template <int PD, int GD, int TENSORS> static hipError_t launch_step(const AdamwArgs<TENSORS> &a, int bits, uint32_t grid, hipStream_t stream)
+template <int PD, int GD, bool MASTER, int TENSORS> static hipError_t launch_step_with(const AdamwArgs<TENSORS> &a, int bits, bool passing, uint32_t grid, hipStream_t stream)
 {
-    if constexpr (PD != DQ_F32) {
-        if (a.master) {
-            return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, true, TENSORS>, dim3(grid), dim3(256), stream, a)
-                              : launch_with(adamw_kernel<PD, GD, 8, true, TENSORS>, dim3(grid), dim3(256), stream, a);
-        }
-    }
-    return bits == 32 ? launch_with(adamw_kernel<PD, GD, 32, false, TENSORS>, dim3(grid), dim3(256), stream, a)
-                      : launch_with(adamw_kernel<PD, GD, 8, false, TENSORS>, dim3(grid), dim3(256), stream, a);
+    if (bits == 32)
+        return passing ? launch_with(adamw_kernel<PD, GD, 32, MASTER, TENSORS, true>, dim3(grid), dim3(256), stream, a)
+                       : launch_with(adamw_kernel<PD, GD, 32, MASTER, TENSORS, false>, dim3(grid), dim3(256), stream, a);
+    return passing ? launch_with(adamw_kernel<PD, GD, 8, MASTER, TENSORS, true>, dim3(grid), dim3(256), stream, a)
+                   : launch_with(adamw_kernel<PD, GD, 8, MASTER, TENSORS, false>, dim3(grid), dim3(256), stream, a);
 }
 
-template <int PD, int TENSORS> static hipError_t launch_step_of(int grad, const AdamwArgs<TENSORS> &a, int bits, uint32_t grid, hipStream_t stream)
+template <int PD, int GD, int TENSORS> static hipError_t launch_step(const AdamwArgs<TENSORS> &a, int bits, bool passing, uint32_t grid, hipStream_t stream)
 {
-    return grad == DQ_F32 ? launch_step<PD, DQ_F32>(a, bits, grid, stream)
-         : grad == DQ_BF16 ? launch_step<PD, DQ_BF16>(a, bits, grid, stream) : launch_step<PD, DQ_F16>(a, bits, grid, stream);
+    if constexpr (PD != DQ_F32) {
+        if (a.master) return launch_step_with<PD, GD, true>(a, bits, passing, grid, stream);
+    }
+    return launch_step_with<PD, GD, false>(a, bits, passing, grid, stream);
+}
+
+template <int PD, int TENSORS> static hipError_t launch_step_of(int grad, const AdamwArgs<TENSORS> &a, int bits, bool passing, uint32_t grid, hipStream_t stream)
+{
+    return grad == DQ_F32 ? launch_step<PD, DQ_F32>(a, bits, passing, grid, stream)
+         : grad == DQ_BF16 ? launch_step<PD, DQ_BF16>(a, bits, passing, grid, stream) : launch_step<PD, DQ_F16>(a, bits, passing, grid, stream);
 }
 
 // one launch: tensors of the same element types, one after the other, from *next on
@@ -350,9 +447,11 @@ template <int TENSORS> static hipError_t launch_tensors(const dq_adamw_t &o, con
     }
     if (tiles == 0) return hipSuccess;
     for (int j = take; j < TENSORS; j++) a.first_tile[j] = 0xffffffffu;
-    return param == DQ_F32 ? launch_step_of<DQ_F32>(grad, a, o.bits, (uint32_t)tiles, stream)
-         : param == DQ_BF16 ? launch_step_of<DQ_BF16>(grad, a, o.bits, (uint32_t)tiles, stream)
-                            : launch_step_of<DQ_F16>(grad, a, o.bits, (uint32_t)tiles, stream);
+    const int64_t bytes = (o.master ? 4 : 0) + (param == DQ_F32 ? 4 : 2) + (grad == DQ_F32 ? 4 : 2) + (o.bits == 32 ? 8 : 2);
+    const bool passing = tiles * kStepTile * bytes > (int64_t)256 << 20;
+    return param == DQ_F32 ? launch_step_of<DQ_F32>(grad, a, o.bits, passing, (uint32_t)tiles, stream)
+         : param == DQ_BF16 ? launch_step_of<DQ_BF16>(grad, a, o.bits, passing, (uint32_t)tiles, stream)
+                            : launch_step_of<DQ_F16>(grad, a, o.bits, passing, (uint32_t)tiles, stream);
 }
 
 hipError_t launch_adamw(const dq_adamw_t &o, const dq_adamw_tensor_t *tensors, int count, hipStream_t stream)

@@ -129,9 +129,11 @@ def test_steps(opt, pd, gd, master, bits):
                 for p, g, m, v in zip(p0, host(grads), m0, v0)]
         got_p = arena_parts(weights.double().cpu().numpy(), SIZES) if master else host(params)
         for k, (p, m, v) in enumerate(want):
-            # The weight: two products, a difference; the step's quotient to 8 roundings, its two terms of the moments among them, which may cancel
+            # The weight: two products and a difference, three half steps of it at most.  The step: the moment's four roundings (of terms that may cancel: `step` takes
+            # their magnitudes), v's seven, halved by the root, whose own is one, the product with the correction and the sum with eps two; then the reciprocal, good to a
+            # whole step, two products, and three constants that are rounded themselves.
             step = HYPER["lr"] / (1 - 0.9 ** t) * (0.9 * np.abs(m0[k]) + 0.1 * np.abs(0.25 * host(grads)[k])) / (np.sqrt(v) / math.sqrt(1 - 0.99 ** t) + HYPER["eps"])
-            err = (3 * np.abs(p) + 12 * step) * 2.0 ** -24
+            err = (3 * np.abs(p) + (4 + 3.5 + 1 + 2 + 2 + 2 + 3) * step) * 2.0 ** -24
             if not master:
                 err = err + half_step(pd) * (np.abs(p) + err) + (2.0 ** -25 if pd == HF else 0)
             assert np.all(np.abs(got_p[k] - p) <= err), (t, k, float(np.max(np.abs(got_p[k] - p) - err)))
@@ -162,6 +164,35 @@ def test_steps(opt, pd, gd, master, bits):
                 assert np.all(((codes >> 7) == (x < 0)) | (np.abs(x) <= off))
 
 
+@pytest.mark.parametrize("pd,gd,master", [(FP, FP, False), (BF, BF, True)], ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_one_large_call_is_many_small_ones(opt, pd, gd, master, bits):
+    """beyond the cache, and beyond what one launch takes"""
+    sizes = [40_000_001, 31] + [1000 + 7 * k for k in range(300)]
+    results = []
+    for parts in (1, 2):
+        params, grads = views(sizes, pd, 1, 0.1), views(sizes, gd, 2, 1e-2)
+        state, weights = opt.adamw_state(params, bits), opt.master_weights(params) if master else None
+        total = opt.padded_elements(params)
+        if parts == 1:
+            opt.adamw_step(params, grads, state, 3, master=weights)
+        else:
+            at = 0
+            for p, g in zip(params, grads):
+                n = -(-p.numel() // 32) * 32
+                cut = [t[:, s:s + m].contiguous() for t, s, m in ([(state, at, n)] if bits == 32 else [(state[0], at, n), (state[1], at // 32, n // 32)])]
+                w = weights[at:at + n].clone() if master else None
+                opt.adamw_step([p], [g], cut[0] if bits == 32 else tuple(cut), 3, master=w)
+                for t, c, s in zip([state] if bits == 32 else state, cut, (at, at // 32)):
+                    t[:, s:s + c.shape[1]] = c
+                if master:
+                    weights[at:at + n] = w
+                at += n
+            assert at == total
+        results.append([params[0], params[-1], torch.cat(params)] + ([state] if bits == 32 else list(state)) + ([weights] if master else []))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_zero_gradients_and_padding(opt, bits):
     """nothing moves a weight whose gradients are all zero, whatever lies in the arenas' gaps"""
@@ -174,6 +205,34 @@ def test_zero_gradients_and_padding(opt, bits):
     opt.adamw_step(params, [torch.zeros_like(p) for p in params], state, 1, weight_decay=0.0)
     assert all(torch.equal(p, w) for p, w in zip(params, was))
     assert all(int((t != 0).sum()) == 0 for t in tensors)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e-10, 1e10, 1e15, 1e19])
+@pytest.mark.parametrize("eps", [1e-8, 0.0])
+def test_extreme_sizes(opt, size, eps):
+    """moments at both ends of binary32, beside ordinary ones and zeros"""
+    n, t = 4096, 3
+    g = torch.randn(n, device=DEV)
+    g[1::2] *= size
+    g[::64] = 0
+    p, state = torch.randn(n, device=DEV), opt.adamw_state([g])
+    p0, g0 = p.double().cpu().numpy(), g.double().cpu().numpy()
+    opt.adamw_step([p], [g], state, t, lr=1e-2, eps=eps, weight_decay=0.0)
+    m, v = 0.1 * g0, 0.001 * g0 * g0
+    got_m, got_v = state.double().cpu().numpy()
+    # (1 - beta is rounded; a square below 2^-126 has fewer bits, to a half step of 2^-149, and one of 2^128 and more is infinite in binary32)
+    beyond = g0 * g0 >= 2.0 ** 128
+    assert np.all(np.abs(got_m - m) <= 4 * 2.0 ** -24 * np.abs(m)) and np.all(np.isinf(got_v[beyond]))
+    assert np.all((np.abs(got_v - v) <= 6 * 2.0 ** -24 * v + 2.0 ** -149)[~beyond])
+    # the step from the moments as they were stored, which carry the loss of small squares
+    under = np.sqrt(got_v / (1 - 0.999 ** t)) + eps
+    with np.errstate(all="ignore"):
+        step = 1e-2 * (got_m / (1 - 0.9 ** t)) / under
+    got = p.double().cpu().numpy()
+    fine = np.isfinite(step)
+    assert np.all(np.abs(got - (p0 - step))[fine] <= (2 * np.abs(p0) + 14 * np.abs(step))[fine] * 2.0 ** -24)
+    assert np.all(np.isfinite(got[fine]))
+    assert np.array_equal(np.isnan(got), np.isnan(step))          # 0 / 0 with eps 0
 
 
 def test_small_roots_do_not_vanish(opt):
