@@ -55,11 +55,15 @@ template <int DT> __device__ __forceinline__ void load8(const void *p, int64_t i
     }
 }
 
-// the first `count` of N, the others 0
-template <int DT, int N> __device__ __forceinline__ void load_part(const void *p, int64_t i, int count, float *v)
+// N elements from i on of a vector of n (n > 0), those past its end 0.  (Every lane loads, the last element where there is none, so that the loads do not
+// wait for one another.)
+template <int DT, int N> __device__ __forceinline__ void load_part(const void *p, int64_t i, int64_t n, float *v)
 {
 #pragma unroll
-    for (int j = 0; j < N; j++) v[j] = j < count ? ElemIO<DT>::load(p, i + j) : 0.0f;
+    for (int j = 0; j < N; j++) v[j] = ElemIO<DT>::load(p, min(i + j, n - 1));
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        if (i + j >= n) v[j] = 0.0f;
 }
 
 template <int DT, bool PASSING = false> __device__ __forceinline__ void store4(void *p, int64_t i, const float *v)

@@ -96,7 +96,7 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
     if (col + 8 <= a.cols)
         load8<DT>(a.x, at, v);
     else
-        load_part<DT, 8>(a.x, at, (int)max((int64_t)0, a.cols - col), v);
+        load_part<DT, 8>(a.x, at, row * a.stride + a.cols, v);
     uniform8<RAND>(a, e, u);
     if (ROTATE) rotate_block(v, a.sign[col >> 5], g);
     uint32_t scale;
@@ -119,10 +119,19 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void 
     const int cols = (int)min((int64_t)8, a.cols - col);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        if (row + j < a.rows && cols == 8)
-            load8<DT>(a.x, (row + j) * a.stride + col, x[j]);
+        const int64_t at = min(row + j, a.rows - 1) * a.stride;
+        if (cols == 8)
+            load8<DT>(a.x, at + col, x[j]);
         else
-            load_part<DT, 8>(a.x, (row + j) * a.stride + col, row + j < a.rows ? cols : 0, x[j]);
+            load_part<DT, 8>(a.x, at + col, at + a.cols, x[j]);
+    }
+    if (row + 8 > a.rows) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (row + j >= a.rows) {
+#pragma unroll
+                for (int c = 0; c < 8; c++) x[j][c] = 0.0f;
+            }
     }
     const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u;
 #pragma unroll

@@ -72,7 +72,12 @@ template <int DT, int TENSORS> __global__ __launch_bounds__(256) void grad_norm_
 #pragma unroll
             for (int j = 0; j < 32 / kPer; j++) {
                 const int64_t i = at + kPer * (256 * j + t);
-                load_part<DT, kPer>(p, i, (int)max((int64_t)0, min((int64_t)kPer, n - i)), v[j]);
+                if (i + kPer > n)
+                    load_part<DT, kPer>(p, i, n, v[j]);
+                else if (DT == DQ_F32)
+                    load4<DT>(p, i, v[j]);
+                else
+                    load8<DT>(p, i, v[j]);
             }
         }
 #pragma unroll
@@ -271,12 +276,12 @@ template <int PD, int GD, int BITS, bool MASTER, int TENSORS, bool PASSING> __gl
         if (mine[h] == 4)
             load4<GD, PASSING>(a.grad[k], e, g + 4 * h);
         else
-            load_part<GD, 4>(a.grad[k], e, mine[h], g + 4 * h);
+            load_part<GD, 4>(a.grad[k], e, n, g + 4 * h);
         if (!MASTER) {
             if (mine[h] == 4)
                 load4<PD, PASSING>(a.param[k], e, p + 4 * h);
             else
-                load_part<PD, 4>(a.param[k], e, mine[h], p + 4 * h);
+                load_part<PD, 4>(a.param[k], e, n, p + 4 * h);
         }
         if (live[h]) {
             if (MASTER) load4<DQ_F32, PASSING>(a.master, s, p + 4 * h);
