@@ -13,6 +13,7 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Generator.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string.h>
@@ -1296,6 +1297,114 @@ PyObject *mx4_product(PyObject *, PyObject *const *v, Py_ssize_t have)
     });
 }
 
+// ---- a linear layer in 4 bits, with its backward pass ----
+
+struct Quantized {
+    at::Tensor held;
+    uint8_t *codes = nullptr, *scales = nullptr;
+    int64_t rows = 0, length = 0;
+};
+
+// x: contiguous.  sign, pool: undefined for none; stochastic without a pool draws from (seed, step)
+Quantized quantized(const at::Tensor &x, bool columns, const at::Tensor &sign, const at::Tensor &pool, bool stochastic, uint64_t seed, uint64_t step)
+{
+    Quantized q;
+    q.rows = x.size(columns ? 1 : 0);
+    q.length = x.size(columns ? 0 : 1);
+    const int64_t supers = (q.length + 255) / 256;
+    need(!sign.defined() || (sign.scalar_type() == at::kInt && sign.is_contiguous() && sign.device() == x.device() && sign.numel() >= 8 * supers),
+         "linear: signs are int32, eight per superchunk of the contraction");
+    need(!pool.defined() || (pool.is_contiguous() && pool.device() == x.device() && pool.numel() == q.rows * 256 * supers),
+         "linear: a rand_pool has one value per element of the quantised gradient, padding included");
+    q.held = at::empty({q.rows * 136 * supers}, at::TensorOptions().dtype(at::kByte).device(x.device()));
+    q.codes = static_cast<uint8_t *>(q.held.data_ptr());
+    q.scales = q.codes + q.rows * 128 * supers;
+    if (q.rows && q.length)
+        check(dq_mx4_quantize(x.data_ptr(), dtype_code(x), x.size(0), x.size(1), x.size(1), columns, sign.defined() ? reinterpret_cast<const uint32_t *>(sign.data_ptr<int32_t>()) : nullptr,
+                              stochastic, pool.defined() ? pool.data_ptr() : nullptr, pool.defined() ? dtype_code(pool) : 0, seed, step, q.codes, q.scales, x.device().index(),
+                              c10::hip::getCurrentHIPStream(x.device().index()).stream()));
+    return q;
+}
+
+at::Tensor product_of(const Quantized &a, const Quantized &b, const at::Tensor &like)
+{
+    const at::Tensor out = at::empty({a.rows, b.rows}, like.options().requires_grad(false));
+    if (a.rows && b.rows && a.length)
+        check(dq_mx4_product(a.codes, a.scales, b.codes, b.scales, out.data_ptr(), dtype_code(out), a.rows, b.rows, a.length, out.device().index(),
+                             c10::hip::getCurrentHIPStream(out.device().index()).stream()));
+    else
+        out.zero_();
+    return out;
+}
+
+struct Linear4 : public torch::autograd::Function<Linear4> {
+    // x [tokens, k] and weight [n, k], contiguous
+    typedef std::optional<at::Tensor> Maybe;
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &sign_out, const Maybe &sign_tokens,
+                              const Maybe &pool_rows, const Maybe &pool_columns, bool seeded, int64_t seed, int64_t step)
+    {
+        ctx->save_for_backward({x, weight, sign_out.value_or(at::Tensor()), sign_tokens.value_or(at::Tensor()), pool_rows.value_or(at::Tensor()), pool_columns.value_or(at::Tensor())});
+        ctx->saved_data["seeded"] = seeded;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["step"] = step;
+        const c10::DeviceGuard on(x.device());
+        const at::Tensor none;
+        return product_of(quantized(x, false, none, none, false, 0, 0), quantized(weight, false, none, none, false, 0, 0), x);
+    }
+    static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
+    {
+        need(!at::GradMode::is_enabled(), "linear: its gradients cannot be differentiated again");
+        const torch::autograd::variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &weight = saved[1], &sign_out = saved[2], &sign_tokens = saved[3], &pool_rows = saved[4], &pool_columns = saved[5], none;
+        const bool seeded = ctx->saved_data["seeded"].toBool();
+        const uint64_t seed = (uint64_t)ctx->saved_data["seed"].toInt(), step = (uint64_t)ctx->saved_data["step"].toInt();
+        torch::autograd::tensor_list out(9);
+        if (!grads[0].defined()) return out;
+        const c10::DeviceGuard on(x.device());
+        const at::Tensor dy = grads[0].contiguous();
+        if (ctx->needs_input_grad(0))
+            out[0] = product_of(quantized(dy, false, sign_out, pool_rows, seeded || pool_rows.defined(), seed, 2 * step), quantized(weight, true, sign_out, none, false, 0, 0), x);
+        if (ctx->needs_input_grad(1))
+            out[1] = product_of(quantized(dy, true, sign_tokens, pool_columns, seeded || pool_columns.defined(), seed, 2 * step + 1),
+                                quantized(x, true, sign_tokens, none, false, 0, 0), weight);
+        return out;
+    }
+};
+
+// x, weight, signs of the outputs and of the tokens, pools of the gradient's rows and columns, seed (None: no random stream), step
+PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 8, [&]() -> PyObject * {
+        for (int k = 0; k < 2; k++)
+            if (!THPVariable_Check(v[k])) refuse(std::string("a tensor argument is required, got ") + Py_TYPE(v[k])->tp_name);
+        const at::Tensor &x = THPVariable_Unpack(v[0]), &weight = THPVariable_Unpack(v[1]);
+        if (!x.is_cuda()) refuse("tensor arguments must live on the GPU (got a " + std::string(c10::DeviceTypeName(x.device().type(), true)) + " tensor)");
+        if (x.device() != weight.device()) refuse("tensor arguments live on different devices");
+        need(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "linear: x [..., k] and weight [n, k] are required");
+        (void)dtype_code(x);
+        (void)dtype_code(weight);
+        std::optional<at::Tensor> extra[4];
+        for (int k = 0; k < 4; k++) {
+            if (v[2 + k] == Py_None) continue;
+            if (!THPVariable_Check(v[2 + k])) refuse(std::string("a tensor argument is required, got ") + Py_TYPE(v[2 + k])->tp_name);
+            extra[k] = THPVariable_Unpack(v[2 + k]);
+        }
+        const bool seeded = v[6] != Py_None;
+        need(!seeded || (!extra[2] && !extra[3]), "linear: rand_pool or seed, not both");
+        const int64_t seed = seeded ? (int64_t)word(v[6], true) : 0, step = (int64_t)word(v[7], true);
+        const int64_t k = weight.size(1), n = weight.size(0), tokens = k ? x.numel() / k : x.numel() == 0 && x.dim() > 1 ? c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)) : 1;
+        // (a matrix that is contiguous takes part as it is: views of it would be nodes of the graph)
+        const at::Tensor flat = x.dim() == 2 && x.is_contiguous() ? x : x.reshape({tokens, k}).contiguous();
+        at::Tensor y = Linear4::apply(flat, weight.is_contiguous() ? weight : weight.contiguous(), extra[0], extra[1], extra[2], extra[3], seeded, seed, step);
+        if (x.dim() != 2) {
+            std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
+            shape.push_back(n);
+            y = y.view(shape);
+        }
+        return THPVariable_Wrap(y);
+    });
+}
+
 PyMethodDef kFunctions[] = {
     {"grad_norm", reinterpret_cast<PyCFunction>(grad_norm), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(adamw_step), METH_FASTCALL, nullptr},
@@ -1303,6 +1412,7 @@ PyMethodDef kFunctions[] = {
     {"mx4_quantize", reinterpret_cast<PyCFunction>(mx4_quantize), METH_FASTCALL, nullptr},
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(mx4_dequantize), METH_FASTCALL, nullptr},
     {"mx4_product", reinterpret_cast<PyCFunction>(mx4_product), METH_FASTCALL, nullptr},
+    {"mx4_linear", reinterpret_cast<PyCFunction>(mx4_linear), METH_FASTCALL, nullptr},
     {"scaling_compress", reinterpret_cast<PyCFunction>(scaling_compress), METH_FASTCALL, nullptr},
     {"scaling_decompress", reinterpret_cast<PyCFunction>(scaling_decompress), METH_FASTCALL, nullptr},
     {"scaling_dec_comp", reinterpret_cast<PyCFunction>(scaling_dec_comp), METH_FASTCALL, nullptr},

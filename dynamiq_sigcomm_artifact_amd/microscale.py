@@ -8,7 +8,6 @@ in-kernel Philox stream.  ``include/dynamiq_eden.h`` (dq_mx4_*) has the format a
 Everything runs on the current stream of the tensors' device, returns new tensors and can be recorded into a graph (a replay draws the
 random numbers of the recording: seed and step are constants of the launch)."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import capi
 
@@ -69,27 +68,6 @@ def product(a, b, dtype=torch.bfloat16):
     return capi.host().mx4_product(a.codes, a.scales, b.codes, b.scales, a.rows, b.rows, a.cols, _like(dtype))
 
 
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, sign_out, sign_tokens, pool_rows, pool_columns, seed, step):
-        ctx.save_for_backward(x, weight, sign_out, sign_tokens, pool_rows, pool_columns)
-        ctx.seed, ctx.step = seed, step
-        return product(quantize(x), quantize(weight), x.dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, sign_out, sign_tokens, pool_rows, pool_columns = ctx.saved_tensors
-        dy = dy.contiguous()
-        seed, step = ctx.seed, ctx.step
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = product(quantize(dy, False, sign_out, pool_rows, seed, 2 * step), quantize(weight, True, sign_out), x.dtype)
-        if ctx.needs_input_grad[1]:
-            dw = product(quantize(dy, True, sign_tokens, pool_columns, seed, 2 * step + 1), quantize(x, True, sign_tokens), weight.dtype)
-        return dx, dw, None, None, None, None, None, None
-
-
 def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0):
     """y = x weight^T for x [..., k] and weight [n, k], all three products of a training step in 4 bits:
 
@@ -101,10 +79,7 @@ def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0):
     the given signs, which spreads outliers over their block and cancels in the product.
 
     sign: (signs of n, signs of the tokens), packed; None leaves R out.  rand_pool: (pool [tokens, n padded to 256], pool [n, tokens padded to
-    256]), or seed and step: then every call needs a step of its own.  With neither the gradients are rounded to nearest, too."""
-    flat = x.reshape(-1, x.shape[-1])
-    if not flat.is_contiguous():
-        flat = flat.contiguous()
+    256]), or seed and step: then every call needs a step of its own.  With neither the gradients are rounded to nearest, too.  The gradients
+    cannot be differentiated again."""
     signs, pools = sign or (None, None), rand_pool or (None, None)
-    y = _Linear.apply(flat, weight.contiguous(), signs[0], signs[1], pools[0], pools[1], seed, step)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    return capi.host().mx4_linear(x, weight, signs[0], signs[1], pools[0], pools[1], seed, step)

@@ -293,6 +293,32 @@ def test_linear_shapes_and_partial_gradients(ms):
     assert ms.linear(x.transpose(0, 1), w).shape == (4, 3, 10)
 
 
+def test_linear_refusals_and_empty(ms):
+    x, w = matrix(6, 64, BF, 1), matrix(10, 64, BF, 2)
+    for args, kw, text in (((x, w[:, :32]), {}, "weight"), ((x, w[0]), {}, "weight"), ((x.double(), w), {}, "unsupported element dtype"), ((x.cpu(), w), {}, "live on the GPU"),
+                           ((x, w.cpu()), {}, "different devices"), ((x, None), {}, "a tensor argument"), ((x, w), dict(rand_pool=(pool(6, 10, BF), pool(10, 6, BF)), seed=1), "not both")):
+        with pytest.raises(RuntimeError, match=text):
+            ms.linear(*args, **kw)
+    xg = x.clone().requires_grad_()
+    for kw, text in ((dict(sign=(torch.zeros(4, dtype=torch.int32, device=DEV), None)), "signs are int32"), (dict(rand_pool=(torch.zeros(6, 10, device=DEV), None)), "rand_pool has one value")):
+        with pytest.raises(RuntimeError, match=text):
+            ms.linear(xg, w, **kw).sum().backward()
+    y = ms.linear(xg, w)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        torch.autograd.grad(y.sum(), xg, create_graph=True)
+    for shape in ((0, 64), (2, 0, 64)):
+        e, v = torch.zeros(shape, dtype=BF, device=DEV, requires_grad=True), w.clone().requires_grad_()
+        y = ms.linear(e, v)
+        assert y.shape == shape[:-1] + (10,)
+        y.sum().backward()
+        assert e.grad.shape == shape and int((v.grad != 0).sum()) == 0
+    assert ms.linear(x[0], w).shape == (10,)
+    y = ms.linear(torch.zeros(3, 0, device=DEV), torch.zeros(5, 0, device=DEV))
+    assert y.shape == (3, 5) and int((y != 0).sum()) == 0
+    big = matrix(6, 128, BF, 3)                              # rows apart, and a transposed weight
+    assert torch.equal(ms.linear(big[:, :64], w.t().contiguous().t()), ms.linear(big[:, :64].contiguous(), w))
+
+
 def test_gradients_against_differences(ms):
     """with operands that 4 bits hold exactly, the layer is the plain product, and its gradients are its differences"""
     rng = np.random.default_rng(0)
