@@ -183,7 +183,7 @@ inline bool dtype_rand_ok(int dtype)
 // rows x length, the length padded to whole superchunks
 inline bool mx4_size_ok(int64_t rows, int64_t length)
 {
-    return rows >= 1 && length >= 1 && rows <= 0x7fffff00 && length <= 0x7fffff00 && rows * ((length + 255) / 256) < dq::kMxMost / 256;
+    return rows >= 1 && length >= 1 && rows <= 0x7fffff00 && length <= 0x7fffff00 && rows * ((length + 255) / 256) <= dq::kMxMost / 256 - 9; // (threads of a grid: below 2^32)
 }
 inline bool mx4_aligned(const void *codes, const void *scales)
 {

@@ -7,6 +7,17 @@
 
 namespace dq {
 
+// n / by for n below 2^27: (n mul) >> shift with mul = ceil(2^shift / by) and shift = 27 + ceil(log2 by), whose excess is less than n 2^-shift
+struct Division {
+    uint32_t by, mul, shift;
+    explicit Division(uint32_t by_) : by(by_), shift(27)
+    {
+        while (((uint64_t)1 << (shift - 27)) < by) shift++;
+        mul = (uint32_t)((((uint64_t)1 << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((uint64_t)n * mul >> shift); }
+};
+
 enum { kNearest = -1, kPhilox = -2 }; // otherwise the element type of the pool
 
 template <int CTRL> __device__ __forceinline__ float quad_f32(float v)
@@ -19,7 +30,8 @@ template <int CTRL> __device__ __forceinline__ float quad_f32(float v)
 __device__ __forceinline__ void rotate_block(float (&v)[8], uint32_t word, int g)
 {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = __uint_as_float(__float_as_uint(v[j]) ^ (word >> (8 * g + j) & 1u) << 31);
+    for (int j = 0; j < 8; j++) // v ^ (its sign bit, shifted up, & the sign's place)
+        v[j] = __uint_as_float(__builtin_amdgcn_bitop3_b32(__float_as_uint(v[j]), (word >> 8 * g) << (31 - j), 0x80000000u, 0x78));
 #pragma unroll
     for (int h = 1; h < 8; h *= 2)
 #pragma unroll
@@ -68,67 +80,82 @@ template <int RAND> __device__ __forceinline__ uint32_t encode_block(const float
         word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4] * down, v[5] * down, 1.0f, 2);
         word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6] * down, v[7] * down, 1.0f, 3);
     } else {
+        // With 2^e the power of two at or below max(y, 1), codes are 2^e / 2 apart and t = 2 y / 2^e counts them from 2 e on (below 1: from 0 on).  The exponent's bits
+        // carry 127 along, twice: 254 in each place of the word, taken off at the end.
+        uint32_t signs = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            // codes 0 .. 3 are halves, 4 and 5 are ones from 2 on, 6 and 7 twos from 4 on
             const float y = __builtin_fabsf(v[j]) * down;
-            const float t = y < 2.0f ? 2.0f * y : y < 4.0f ? y : 0.5f * y;
-            const float low = __builtin_floorf(t);
-            const uint32_t code = (uint32_t)(y < 2.0f ? low : y < 4.0f ? low + 2.0f : low + 4.0f) + (u[j] < t - low ? 1u : 0u);
-            word |= ((code & 7u) | (v[j] < 0.0f ? 8u : 0u)) << (4 * j);
+            const uint32_t power = __float_as_uint(__builtin_fmaxf(y, 1.0f)) & 0x7f800000u;
+            const float t = y * __uint_as_float(0x7f800000u - power);
+            const uint32_t code = (uint32_t)t + (power >> 22) + (u[j] < __builtin_amdgcn_fractf(t) ? 1u : 0u);
+            word += code << 4 * j;
+            signs |= __float_as_uint(v[j]) >> (28 - 4 * j) & (8u << 4 * j);
         }
+        word = (word - 254u * 0x11111111u) | signs;
     }
     return word;
 }
 
 // ---- along the rows ----------------------------------------------------------------------------------------
 
-template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void mx4_rows_kernel(QuantizeArgs a, uint32_t superchunks)
+template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void mx4_rows_kernel(QuantizeArgs a, Division superchunks, uint32_t units)
 {
     const int g = threadIdx.x & 3;
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; // of the result, padding included
-    const int64_t sc = e >> 8;
-    if (sc >= a.rows * superchunks) return;
-    const int64_t row = sc / superchunks;
-    const int64_t col = e - row * superchunks * 256;
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x; // eight elements of the result, padding included
+    if (unit >= units) return;
+    const uint32_t row = superchunks(unit >> 5), col = (unit - row * superchunks.by * 32) * 8;
     float v[8], u[8];
-    const int64_t at = row * a.stride + col;
-    if (col + 8 <= a.cols)
+    const int64_t at = (int64_t)row * a.stride + col;
+    if (col + 8 <= (uint32_t)a.cols)
         load8<DT>(a.x, at, v);
     else
         load_part<DT, 8>(a.x, at, row * a.stride + a.cols, v);
-    uniform8<RAND>(a, e, u);
+    uniform8<RAND>(a, (int64_t)unit * 8, u);
     if (ROTATE) rotate_block(v, a.sign[col >> 5], g);
     uint32_t scale;
-    reinterpret_cast<uint32_t *>(a.codes)[e >> 3] = encode_block<RAND>(v, u, scale);
-    if (g == 0) a.scales[e >> 5] = (uint8_t)scale;
+    reinterpret_cast<uint32_t *>(a.codes)[unit] = encode_block<RAND>(v, u, scale);
+    if (g == 0) a.scales[unit >> 2] = (uint8_t)scale;
 }
 
 // ---- along the columns -------------------------------------------------------------------------------------
 
 // A workgroup takes 256 rows x 128 columns: one superchunk of 128 rows of the result.  A wave takes 32 of the rows, a lane 8 rows x 8 columns, and a
 // column's block lies in a quad as it does above.  The codes leave through LDS, as whole lines.
-template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks)
+template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
 {
     __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __shared__ __attribute__((aligned(8))) uint8_t tile_scales[128 * 8];
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
-    const int64_t col0 = (int64_t)blockIdx.x * 128, col = col0 + 8 * (lane >> 2);
-    const int64_t row0 = (int64_t)blockIdx.y * 256 + 32 * block, row = row0 + 8 * g;
+    const uint32_t superchunk = tiles(blockIdx.x), col0 = (blockIdx.x - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
+    const uint32_t row0 = superchunk * 256 + 32 * block, row = row0 + 8 * g;
     float x[8][8]; // [row][column]
-    const int cols = (int)min((int64_t)8, a.cols - col);
+    if (all_cols >= 8) {
+        // a lane whose eight columns reach past the end loads the last eight, and moves them up
+        const uint32_t from = min(col, all_cols - 8);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const int64_t at = min(row + j, a.rows - 1) * a.stride;
-        if (cols == 8)
-            load8<DT>(a.x, at + col, x[j]);
-        else
-            load_part<DT, 8>(a.x, at + col, at + a.cols, x[j]);
+        for (int j = 0; j < 8; j++) load8<DT>(a.x, (int64_t)min(row + j, last_row) * a.stride + from, x[j]);
+        if (col != from) {
+#pragma unroll
+            for (int k = 1; k < 8; k *= 2)
+                if (col - from & k) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int c = 0; c + k < 8; c++) x[j][c] = x[j][c + k];
+                }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int64_t at = (int64_t)min(row + j, last_row) * a.stride;
+            load_part<DT, 8>(a.x, at + col, at + all_cols, x[j]);
+        }
     }
-    if (row + 8 > a.rows) {
+    if (row + 8 > last_row + 1) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (row + j >= a.rows) {
+            if (row + j > last_row) {
 #pragma unroll
                 for (int c = 0; c < 8; c++) x[j][c] = 0.0f;
             }
@@ -139,7 +166,8 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void 
         float v[8], u[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = x[j][c];
-        if (RAND == kPhilox || c < cols) uniform8<RAND>(a, ((col + c) * superchunks + blockIdx.y) * 256 + 32 * block + 8 * g, u);
+        // (what becomes of columns past the end is not stored)
+        uniform8<RAND>(a, ((int64_t)min(col + c, all_cols - 1) * superchunks + superchunk) * 256 + 32 * block + 8 * g, u);
         if (ROTATE) rotate_block(v, sign, g);
         uint32_t scale;
         const uint32_t word = encode_block<RAND>(v, u, scale);
@@ -151,29 +179,31 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void 
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const int s = threadIdx.x + 512 * k, line = s >> 3, piece = s & 7;
-        if (col0 + line < a.cols)
-            reinterpret_cast<uint4 *>(a.codes)[((col0 + line) * superchunks + blockIdx.y) * 8 + piece] =
+        if (col0 + line < all_cols)
+            reinterpret_cast<uint4 *>(a.codes)[((int64_t)(col0 + line) * superchunks + superchunk) * 8 + piece] =
                 *reinterpret_cast<const uint4 *>(tile + line * 128 + ((piece ^ (line >> 3 & 7)) << 4));
     }
-    if (threadIdx.x < 128 && col0 + threadIdx.x < a.cols)
-        reinterpret_cast<uint2 *>(a.scales)[(col0 + threadIdx.x) * superchunks + blockIdx.y] = reinterpret_cast<const uint2 *>(tile_scales)[threadIdx.x];
+    if (threadIdx.x < 128 && col0 + threadIdx.x < all_cols)
+        reinterpret_cast<uint2 *>(a.scales)[(int64_t)(col0 + threadIdx.x) * superchunks + superchunk] = reinterpret_cast<const uint2 *>(tile_scales)[threadIdx.x];
 }
 
 template <int DT, int RAND> static hipError_t launch_quantize(const QuantizeArgs &a, bool columns, hipStream_t stream)
 {
     const uint32_t superchunks = (uint32_t)(((columns ? a.rows : a.cols) + 255) >> 8);
     if (columns) {
-        const dim3 grid((uint32_t)((a.cols + 127) >> 7), superchunks);
+        const Division tiles((uint32_t)((a.cols + 127) >> 7));
+        const dim3 grid(tiles.by * superchunks);
         if (a.sign)
-            mx4_columns_kernel<DT, RAND, true><<<grid, 512, 0, stream>>>(a, superchunks);
+            mx4_columns_kernel<DT, RAND, true><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
         else
-            mx4_columns_kernel<DT, RAND, false><<<grid, 512, 0, stream>>>(a, superchunks);
+            mx4_columns_kernel<DT, RAND, false><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
     } else {
-        const dim3 grid((uint32_t)((a.rows * superchunks + 7) >> 3));
+        const uint32_t units = (uint32_t)(a.rows * superchunks * 32);
+        const dim3 grid((units + 255) / 256);
         if (a.sign)
-            mx4_rows_kernel<DT, RAND, true><<<grid, 256, 0, stream>>>(a, superchunks);
+            mx4_rows_kernel<DT, RAND, true><<<grid, 256, 0, stream>>>(a, Division(superchunks), units);
         else
-            mx4_rows_kernel<DT, RAND, false><<<grid, 256, 0, stream>>>(a, superchunks);
+            mx4_rows_kernel<DT, RAND, false><<<grid, 256, 0, stream>>>(a, Division(superchunks), units);
     }
     return hipGetLastError();
 }
@@ -196,38 +226,39 @@ hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, b
 // ---- and back ----------------------------------------------------------------------------------------------
 
 template <int DT>
-__global__ __launch_bounds__(256) void mx4_values_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scales, void *__restrict__ out,
-                                                        int64_t rows, int64_t cols, uint32_t superchunks)
+__global__ __launch_bounds__(256) void mx4_values_kernel(const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scales, void *__restrict__ out, uint32_t cols,
+                                                        Division superchunks, uint32_t units)
 {
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8, sc = e >> 8;
-    if (sc >= rows * superchunks) return;
-    const int64_t row = sc / superchunks;
-    const int64_t col = e - row * superchunks * 256;
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
+    if (unit >= units) return;
+    const uint32_t row = superchunks(unit >> 5), col = (unit - row * superchunks.by * 32) * 8;
     if (col >= cols) return;
-    const uint32_t word = codes[e >> 3];
-    const float up = scale_up(scales[e >> 5]);
+    const uint32_t word = codes[unit];
+    const float up = scale_up(scales[unit >> 2]);
     float v[8];
     const f32x2_t p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 1);
     const f32x2_t p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 3);
     v[0] = p0.x * up; v[1] = p0.y * up; v[2] = p1.x * up; v[3] = p1.y * up;
     v[4] = p2.x * up; v[5] = p2.y * up; v[6] = p3.x * up; v[7] = p3.y * up;
+    const int64_t at = (int64_t)row * cols + col;
     if (col + 8 <= cols)
-        store8<DT>(out, row * cols + col, v);
+        store8<DT>(out, at, v);
     else
-        store_part<DT, 8>(out, row * cols + col, (int)(cols - col), v);
+        store_part<DT, 8>(out, at, (int)(cols - col), v);
 }
 
 hipError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int64_t rows, int64_t cols, int dtype, hipStream_t stream)
 {
-    const uint32_t superchunks = (uint32_t)((cols + 255) >> 8);
-    const dim3 grid((uint32_t)((rows * superchunks + 7) >> 3));
+    const Division superchunks((uint32_t)((cols + 255) >> 8));
+    const uint32_t units = (uint32_t)(rows * superchunks.by * 32);
+    const dim3 grid((units + 255) / 256);
     const uint32_t *words = reinterpret_cast<const uint32_t *>(codes);
     if (dtype == DQ_F32)
-        mx4_values_kernel<DQ_F32><<<grid, 256, 0, stream>>>(words, scales, out, rows, cols, superchunks);
+        mx4_values_kernel<DQ_F32><<<grid, 256, 0, stream>>>(words, scales, out, (uint32_t)cols, superchunks, units);
     else if (dtype == DQ_BF16)
-        mx4_values_kernel<DQ_BF16><<<grid, 256, 0, stream>>>(words, scales, out, rows, cols, superchunks);
+        mx4_values_kernel<DQ_BF16><<<grid, 256, 0, stream>>>(words, scales, out, (uint32_t)cols, superchunks, units);
     else
-        mx4_values_kernel<DQ_F16><<<grid, 256, 0, stream>>>(words, scales, out, rows, cols, superchunks);
+        mx4_values_kernel<DQ_F16><<<grid, 256, 0, stream>>>(words, scales, out, (uint32_t)cols, superchunks, units);
     return hipGetLastError();
 }
 
