@@ -55,6 +55,41 @@ template <int DT> __device__ __forceinline__ void load8(const void *p, int64_t i
     }
 }
 
+// the same as words, two elements of a 16-bit type in each, and element j of them
+template <int DT, int WORDS> __device__ __forceinline__ void load_words(const void *p, int64_t i, uint32_t (&x)[WORDS])
+{
+    const char *q = static_cast<const char *>(p) + i * (DT == DQ_F32 ? 4 : 2);
+#pragma unroll
+    for (int k = 0; k < WORDS; k += 4) {
+        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(q + 4 * k);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[k + j] = a[j];
+    }
+}
+template <int DT, int WORDS> __device__ __forceinline__ float word_value(const uint32_t (&x)[WORDS], int j)
+{
+    if (DT == DQ_F32) return __uint_as_float(x[j]);
+    float v[2];
+    unpack2<DT>(x[j / 2], v[0], v[1]);
+    return v[j & 1];
+}
+// ... and the elements i .. of the n that a row of fewer than eight has, those past its end 0
+template <int DT, int WORDS> __device__ __forceinline__ void load_words_part(const void *p, int64_t row, uint32_t i, uint32_t n, uint32_t (&x)[WORDS])
+{
+    constexpr int PER = 8 / WORDS;
+    uint32_t e[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int64_t at = row + min(i + j, n - 1);
+        e[j] = DT == DQ_F32 ? static_cast<const uint32_t *>(p)[at] : static_cast<const uint16_t *>(p)[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (i + j >= n) e[j] = 0u;
+#pragma unroll
+    for (int w = 0; w < WORDS; w++) x[w] = PER == 1 ? e[w] : e[PER * w] | e[PER * w + PER - 1] << 16;
+}
+
 // N elements from i on of a vector of n (n > 0), those past its end 0.  (Every lane loads, the last element where there is none, so that the loads do not
 // wait for one another.)
 template <int DT, int N> __device__ __forceinline__ void load_part(const void *p, int64_t i, int64_t n, float *v)

@@ -122,42 +122,43 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 
 // A workgroup takes 256 rows x 128 columns: one superchunk of 128 rows of the result.  A wave takes 32 of the rows, a lane 8 rows x 8 columns, and a
 // column's block lies in a quad as it does above.  The codes leave through LDS, as whole lines.
-template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
+template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
 {
     __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __shared__ __attribute__((aligned(8))) uint8_t tile_scales[128 * 8];
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
     const uint32_t superchunk = tiles(blockIdx.x), col0 = (blockIdx.x - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
     const uint32_t row0 = superchunk * 256 + 32 * block, row = row0 + 8 * g;
-    float x[8][8]; // [row][column]
+    constexpr int WORDS = DT == DQ_F32 ? 8 : 4;
+    uint32_t x[8][WORDS]; // [row][column], as they are in memory
     if (all_cols >= 8) {
         // a lane whose eight columns reach past the end loads the last eight, and moves them up
-        const uint32_t from = min(col, all_cols - 8);
+        const uint32_t from = min(col, all_cols - 8), up = col - from;
 #pragma unroll
-        for (int j = 0; j < 8; j++) load8<DT>(a.x, (int64_t)min(row + j, last_row) * a.stride + from, x[j]);
-        if (col != from) {
+        for (int j = 0; j < 8; j++) load_words<DT>(a.x, (int64_t)min(row + j, last_row) * a.stride + from, x[j]);
+        if (up) {
 #pragma unroll
-            for (int k = 1; k < 8; k *= 2)
-                if (col - from & k) {
+            for (int j = 0; j < 8; j++) {
+                if (WORDS == 4 && up & 1)
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
+                    for (int w = 0; w < WORDS; w++) x[j][w] = __builtin_amdgcn_alignbit(x[j][min(w + 1, WORDS - 1)], x[j][w], 16);
 #pragma unroll
-                        for (int c = 0; c + k < 8; c++) x[j][c] = x[j][c + k];
-                }
+                for (int k = 1; k < WORDS; k *= 2)
+                    if (up & (8 / WORDS) * k)
+#pragma unroll
+                        for (int w = 0; w + k < WORDS; w++) x[j][w] = x[j][w + k];
+            }
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int64_t at = (int64_t)min(row + j, last_row) * a.stride;
-            load_part<DT, 8>(a.x, at + col, at + all_cols, x[j]);
-        }
+        for (int j = 0; j < 8; j++) load_words_part<DT>(a.x, (int64_t)min(row + j, last_row) * a.stride, col, all_cols, x[j]);
     }
     if (row + 8 > last_row + 1) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (row + j > last_row) {
 #pragma unroll
-                for (int c = 0; c < 8; c++) x[j][c] = 0.0f;
+                for (int w = 0; w < WORDS; w++) x[j][w] = 0u;
             }
     }
     const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u;
@@ -165,7 +166,7 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512) void 
     for (int c = 0; c < 8; c++) {
         float v[8], u[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = x[j][c];
+        for (int j = 0; j < 8; j++) v[j] = word_value<DT>(x[j], c);
         // (what becomes of columns past the end is not stored)
         uniform8<RAND>(a, ((int64_t)min(col + c, all_cols - 1) * superchunks + superchunk) * 256 + 32 * block + 8 * g, u);
         if (ROTATE) rotate_block(v, sign, g);
