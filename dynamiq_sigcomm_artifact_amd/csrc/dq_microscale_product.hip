@@ -374,11 +374,11 @@ template <int DT, int T> static hipError_t launch_tiles(ProductArgs p, hipStream
 // of which two share a CU (2048 x 4096 x 4096, 128 of 256: 33.6 us against 32.3; 4096 x 4096 x 1000, 256: 18.3 against 19.9).  Below 96 tiles of 128 the contraction
 // is shared out among the waves of a workgroup instead (256 x 4096 x 4096, 64 tiles: 16.4 us, split 14.7; 512 x 4096 x 4096, 128 tiles: 17.0, split 28.8), in the
 // largest blocks that leave 192 workgroups: with fewer, CUs have nothing to do (16 x 4096 x 4096, blocks of 16 x 16: 5.4 us, 16 x 64: 9.2), with more the
-// operands are read more often (16 x 14336 x 4096: 13.3 and 9.6 us).
+// operands are read more often (16 x 14336 x 4096: 13.3 and 9.6 us; 1 x 14336 x 4096: 9.3 and 8.4).  No block is twice as high or wide as it need be.
 template <int MF, int NF, int U> static bool try_narrow(const ProductArgs &p, bool last, int dtype, hipStream_t stream, hipError_t &e)
 {
     const int64_t blocks = ((p.m + 16 * MF - 1) / (16 * MF)) * ((p.n + 16 * NF - 1) / (16 * NF));
-    if (!last && (blocks < 192 || 8 * MF >= p.m || 8 * NF >= p.n)) return false;
+    if (!last && (blocks < 192 || (MF > 1 && 8 * MF >= p.m) || (NF > 1 && 8 * NF >= p.n))) return false;
     e = launch_narrow<MF, NF, 8, U>(p, dtype, stream);
     return true;
 }
