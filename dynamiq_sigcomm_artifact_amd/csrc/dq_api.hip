@@ -181,9 +181,12 @@ inline bool dtype_rand_ok(int dtype)
 }
 
 // rows x length, the length padded to whole superchunks
-inline bool mx4_size_ok(int64_t rows, int64_t length)
+static const char kMxSizes[] = "sizes must be positive and at most 2^31 - 256, with at most 2^35 - 4096 elements of every matrix, padding included";
+bool mx4_size_ok(int64_t rows, int64_t length)
 {
-    return rows >= 1 && length >= 1 && rows <= 0x7fffff00 && length <= 0x7fffff00 && rows * ((length + 255) / 256) <= dq::kMxMost / 256 - 9; // (threads of a grid: below 2^32)
+    // (the quantisers' and the products' grids have less than 2^32 threads)
+    constexpr int64_t most = 0x7fffff00;
+    return rows > 0 && length > 0 && rows <= most && length <= most && rows * ((length + 255) / 256) <= dq::kMxMost / 256 - 16;
 }
 inline bool mx4_aligned(const void *codes, const void *scales)
 {
@@ -1180,7 +1183,7 @@ int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, in
 {
     if (!dtype_ok(dtype) || (rand_pool && !dtype_ok(rand_dtype))) return fail(DQ_ERR_DTYPE);
     if (!mx4_size_ok(columns ? x_cols : x_rows, columns ? x_rows : x_cols))
-        return fail(DQ_ERR_SIZE, "rows and columns must be positive, with less than 2^35 elements, padding included");
+        return fail(DQ_ERR_SIZE, kMxSizes);
     if (stride < x_cols || stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
     if (rand_pool && !stochastic) return fail(DQ_ERR_SIZE, "a rand_pool is for stochastic rounding");
     if (!x || !codes || !scales) return fail(DQ_ERR_NULL);
@@ -1194,7 +1197,7 @@ int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, in
 int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows, int64_t cols, int device, dq_stream_t stream)
 {
     if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
-    if (!mx4_size_ok(rows, cols)) return fail(DQ_ERR_SIZE, "rows and columns must be positive, with less than 2^35 elements, padding included");
+    if (!mx4_size_ok(rows, cols)) return fail(DQ_ERR_SIZE, kMxSizes);
     if (!out || !codes || !scales) return fail(DQ_ERR_NULL);
     if (!mx4_aligned(codes, scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
     int rc;
@@ -1207,7 +1210,7 @@ int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_
 {
     if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
     if (!mx4_size_ok(m, k) || !mx4_size_ok(n, k) || !mx4_size_ok(m, n))
-        return fail(DQ_ERR_SIZE, "m, n and k must be positive, with less than 2^35 elements of every matrix, padding included");
+        return fail(DQ_ERR_SIZE, kMxSizes);
     if (k > 1 << 24) return fail(DQ_ERR_SIZE, "k must be at most 2^24");
     if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return fail(DQ_ERR_NULL);
     if (!mx4_aligned(a_codes, a_scales) || !mx4_aligned(b_codes, b_scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");

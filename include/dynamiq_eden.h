@@ -812,8 +812,8 @@ int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double
  * A row is padded with zeros to s = ceil(length / 256) superchunks:
  *   codes  uint8 [rows][128 s], two elements a byte, the first one in the low half
  *   scales uint8 [rows][8 s], k + 127 (255: the block is NaN)
- * codes 16-byte, scales 8-byte aligned.  A matrix has less than 2^35 elements, padding
- * included. */
+ * codes 16-byte, scales 8-byte aligned.  Rows and lengths are at most 2^31 - 256,
+ * and a matrix has at most 2^35 - 4096 elements, padding included. */
 
 /* x: [x_rows][x_cols], row i from element i * stride on.  columns = 0: the rows of
  * the result are those of x; columns = 1: its columns (what the product with the
