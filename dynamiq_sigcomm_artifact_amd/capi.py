@@ -211,7 +211,7 @@ def lib():
         L.dq_adamw_coefficients.restype = i32
         L.dq_adamw_coefficients.argtypes = [vp, c.c_double, vp, c.c_double, c.c_double, c.c_double, vp, vp, i32, vp]
         L.dq_mx4_quantize.restype = i32
-        L.dq_mx4_quantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i32, vp, i32, u64, u64, vp, vp, i32, vp]
+        L.dq_mx4_quantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i32, vp, i32, u64, u64, vp, vp, vp, i32, vp]
         L.dq_mx4_dequantize.restype = i32
         L.dq_mx4_dequantize.argtypes = [vp, vp, vp, i32, i64, i64, i32, vp]
         L.dq_mx4_product.restype = i32

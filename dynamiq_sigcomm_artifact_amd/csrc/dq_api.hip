@@ -1178,19 +1178,20 @@ int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double
 }
 
 int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, int64_t stride, int columns, const uint32_t *sign, int stochastic,
-                    const void *rand_pool, int rand_dtype, uint64_t seed, uint64_t step, uint8_t *codes, uint8_t *scales, int device,
-                    dq_stream_t stream)
+                    const void *rand_pool, int rand_dtype, uint64_t seed, uint64_t step, const uint64_t *step_dev, uint8_t *codes,
+                    uint8_t *scales, int device, dq_stream_t stream)
 {
     if (!dtype_ok(dtype) || (rand_pool && !dtype_ok(rand_dtype))) return fail(DQ_ERR_DTYPE);
     if (!mx4_size_ok(columns ? x_cols : x_rows, columns ? x_rows : x_cols))
         return fail(DQ_ERR_SIZE, kMxSizes);
     if (stride < x_cols || stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
     if (rand_pool && !stochastic) return fail(DQ_ERR_SIZE, "a rand_pool is for stochastic rounding");
+    if (step_dev && (!stochastic || rand_pool)) return fail(DQ_ERR_SIZE, "step_dev is for the in-kernel random stream");
     if (!x || !codes || !scales) return fail(DQ_ERR_NULL);
     if (!mx4_aligned(codes, scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
     int rc;
     if ((rc = select_device(device))) return rc;
-    const dq::QuantizeArgs a = {x, x_rows, x_cols, stride, codes, scales, sign, rand_pool, {seed, step}};
+    const dq::QuantizeArgs a = {x, x_rows, x_cols, stride, codes, scales, sign, rand_pool, {seed, step}, step_dev};
     return finish(dq::launch_mx4_quantize(a, dtype, columns != 0, stochastic != 0, rand_dtype, static_cast<hipStream_t>(stream)));
 }
 

@@ -1223,6 +1223,13 @@ at::Tensor new_matrix(int device, int64_t rows, int64_t cols, at::ScalarType dty
     return at::empty({rows, cols}, at::TensorOptions().dtype(dtype).device(cuda(device)));
 }
 
+// a count of steps in device memory, beside a matrix
+const uint64_t *step_counter(const at::Tensor &step, const at::Tensor &beside)
+{
+    need(step.scalar_type() == at::kLong && step.numel() >= 1 && step.device() == beside.device(), "step: a number, or an int64 tensor [1] beside the matrix");
+    return reinterpret_cast<const uint64_t *>(step.data_ptr<int64_t>());
+}
+
 // x, columns, sign, rand_pool, seed (None: no random stream), step -> (codes, scales)
 PyObject *mx4_quantize(PyObject *, PyObject *const *v, Py_ssize_t have)
 {
@@ -1249,12 +1256,14 @@ PyObject *mx4_quantize(PyObject *, PyObject *const *v, Py_ssize_t have)
             pool = p.data_ptr();
         }
         const bool stochastic = pool || v[4] != Py_None;
-        const uint64_t seed = v[4] == Py_None ? 0 : word(v[4], true), step = word(v[5], true);
+        const uint64_t seed = v[4] == Py_None ? 0 : word(v[4], true);
+        const uint64_t *step_dev = THPVariable_Check(v[5]) ? step_counter(a.tensor(v[5]), x) : nullptr;
+        const uint64_t step = step_dev ? 0 : word(v[5], true);
         const c10::OptionalDeviceGuard on(cuda(a.device));
         const at::Tensor codes = new_matrix(a.device, rows, 128 * supers, at::kByte), scales = new_matrix(a.device, rows, 8 * supers, at::kByte);
         if (rows && length) {
             const dq_stream_t s = c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream();
-            check(dq_mx4_quantize(x.data_ptr(), code, xr, xc, xr > 1 ? x.stride(0) : xc, columns, sign, stochastic, pool, pool_code, seed, step,
+            check(dq_mx4_quantize(x.data_ptr(), code, xr, xc, xr > 1 ? x.stride(0) : xc, columns, sign, stochastic, pool, pool_code, seed, step, stochastic && !pool ? step_dev : nullptr,
                                   static_cast<uint8_t *>(codes.data_ptr()), static_cast<uint8_t *>(scales.data_ptr()), a.device, s));
         }
         return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(codes)).ptr(), py::reinterpret_steal<py::object>(THPVariable_Wrap(scales)).ptr());
@@ -1306,7 +1315,7 @@ struct Quantized {
 };
 
 // x: contiguous.  sign, pool: undefined for none; stochastic without a pool draws from (seed, step)
-Quantized quantized(const at::Tensor &x, bool columns, const at::Tensor &sign, const at::Tensor &pool, bool stochastic, uint64_t seed, uint64_t step)
+Quantized quantized(const at::Tensor &x, bool columns, const at::Tensor &sign, const at::Tensor &pool, bool stochastic, uint64_t seed, uint64_t step, const at::Tensor &step_dev)
 {
     Quantized q;
     q.rows = x.size(columns ? 1 : 0);
@@ -1321,7 +1330,7 @@ Quantized quantized(const at::Tensor &x, bool columns, const at::Tensor &sign, c
     q.scales = q.codes + q.rows * 128 * supers;
     if (q.rows && q.length)
         check(dq_mx4_quantize(x.data_ptr(), dtype_code(x), x.size(0), x.size(1), x.size(1), columns, sign.defined() ? reinterpret_cast<const uint32_t *>(sign.data_ptr<int32_t>()) : nullptr,
-                              stochastic, pool.defined() ? pool.data_ptr() : nullptr, pool.defined() ? dtype_code(pool) : 0, seed, step, q.codes, q.scales, x.device().index(),
+                              stochastic, pool.defined() ? pool.data_ptr() : nullptr, pool.defined() ? dtype_code(pool) : 0, seed, step, step_dev.defined() ? step_counter(step_dev, x) : nullptr, q.codes, q.scales, x.device().index(),
                               c10::hip::getCurrentHIPStream(x.device().index()).stream()));
     return q;
 }
@@ -1337,36 +1346,39 @@ at::Tensor product_of(const Quantized &a, const Quantized &b, const at::Tensor &
     return out;
 }
 
+// what the columns of a gradient add to the step of the random stream that its rows take
+constexpr uint64_t kColumns = (uint64_t)1 << 63;
+
 struct Linear4 : public torch::autograd::Function<Linear4> {
     // x [tokens, k] and weight [n, k], contiguous
     typedef std::optional<at::Tensor> Maybe;
     static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &sign_out, const Maybe &sign_tokens,
-                              const Maybe &pool_rows, const Maybe &pool_columns, bool seeded, int64_t seed, int64_t step)
+                              const Maybe &pool_rows, const Maybe &pool_columns, const Maybe &step_dev, bool seeded, int64_t seed, int64_t step)
     {
-        ctx->save_for_backward({x, weight, sign_out.value_or(at::Tensor()), sign_tokens.value_or(at::Tensor()), pool_rows.value_or(at::Tensor()), pool_columns.value_or(at::Tensor())});
+        ctx->save_for_backward({x, weight, sign_out.value_or(at::Tensor()), sign_tokens.value_or(at::Tensor()), pool_rows.value_or(at::Tensor()), pool_columns.value_or(at::Tensor()), step_dev.value_or(at::Tensor())});
         ctx->saved_data["seeded"] = seeded;
         ctx->saved_data["seed"] = seed;
         ctx->saved_data["step"] = step;
         const c10::DeviceGuard on(x.device());
         const at::Tensor none;
-        return product_of(quantized(x, false, none, none, false, 0, 0), quantized(weight, false, none, none, false, 0, 0), x);
+        return product_of(quantized(x, false, none, none, false, 0, 0, none), quantized(weight, false, none, none, false, 0, 0, none), x);
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
     {
         need(!at::GradMode::is_enabled(), "linear: its gradients cannot be differentiated again");
         const torch::autograd::variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &weight = saved[1], &sign_out = saved[2], &sign_tokens = saved[3], &pool_rows = saved[4], &pool_columns = saved[5], none;
+        const at::Tensor &x = saved[0], &weight = saved[1], &sign_out = saved[2], &sign_tokens = saved[3], &pool_rows = saved[4], &pool_columns = saved[5], &step_dev = saved[6], none;
         const bool seeded = ctx->saved_data["seeded"].toBool();
         const uint64_t seed = (uint64_t)ctx->saved_data["seed"].toInt(), step = (uint64_t)ctx->saved_data["step"].toInt();
-        torch::autograd::tensor_list out(9);
+        torch::autograd::tensor_list out(10);
         if (!grads[0].defined()) return out;
         const c10::DeviceGuard on(x.device());
         const at::Tensor dy = grads[0].contiguous();
         if (ctx->needs_input_grad(0))
-            out[0] = product_of(quantized(dy, false, sign_out, pool_rows, seeded || pool_rows.defined(), seed, 2 * step), quantized(weight, true, sign_out, none, false, 0, 0), x);
+            out[0] = product_of(quantized(dy, false, sign_out, pool_rows, seeded || pool_rows.defined(), seed, step, step_dev), quantized(weight, true, sign_out, none, false, 0, 0, none), x);
         if (ctx->needs_input_grad(1))
-            out[1] = product_of(quantized(dy, true, sign_tokens, pool_columns, seeded || pool_columns.defined(), seed, 2 * step + 1),
-                                quantized(x, true, sign_tokens, none, false, 0, 0), weight);
+            out[1] = product_of(quantized(dy, true, sign_tokens, pool_columns, seeded || pool_columns.defined(), seed, step + kColumns, step_dev),
+                                quantized(x, true, sign_tokens, none, false, 0, 0, none), weight);
         return out;
     }
 };
@@ -1391,11 +1403,17 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
         }
         const bool seeded = v[6] != Py_None;
         need(!seeded || (!extra[2] && !extra[3]), "linear: rand_pool or seed, not both");
-        const int64_t seed = seeded ? (int64_t)word(v[6], true) : 0, step = (int64_t)word(v[7], true);
+        const int64_t seed = seeded ? (int64_t)word(v[6], true) : 0;
+        std::optional<at::Tensor> step_dev;
+        if (THPVariable_Check(v[7])) {
+            (void)step_counter(THPVariable_Unpack(v[7]), x);
+            if (seeded) step_dev = THPVariable_Unpack(v[7]);
+        }
+        const int64_t step = THPVariable_Check(v[7]) ? 0 : (int64_t)word(v[7], true);
         const int64_t k = weight.size(1), n = weight.size(0), tokens = k ? x.numel() / k : x.numel() == 0 && x.dim() > 1 ? c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)) : 1;
         // (a matrix that is contiguous takes part as it is: views of it would be nodes of the graph)
         const at::Tensor flat = x.dim() == 2 && x.is_contiguous() ? x : x.reshape({tokens, k}).contiguous();
-        at::Tensor y = Linear4::apply(flat, weight.is_contiguous() ? weight : weight.contiguous(), extra[0], extra[1], extra[2], extra[3], seeded, seed, step);
+        at::Tensor y = Linear4::apply(flat, weight.is_contiguous() ? weight : weight.contiguous(), extra[0], extra[1], extra[2], extra[3], step_dev, seeded, seed, step);
         if (x.dim() != 2) {
             std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
             shape.push_back(n);

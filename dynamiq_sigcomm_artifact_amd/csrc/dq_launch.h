@@ -399,6 +399,7 @@ struct QuantizeArgs {
     const uint32_t *sign;
     const void *pool;
     RandKey key;
+    const uint64_t *step_dev; // null, or a value in device memory that is added to the step of the random stream
 };
 hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, bool stochastic, int pool_dtype, hipStream_t stream);
 hipError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int64_t rows, int64_t cols, int dtype,

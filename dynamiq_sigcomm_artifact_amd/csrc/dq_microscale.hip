@@ -60,7 +60,8 @@ template <int RAND> __device__ __forceinline__ void uniform8(const QuantizeArgs 
         load8<RAND>(a.pool, e, u);
     } else if constexpr (RAND == kPhilox) {
         uint32_t w[4];
-        chunk_uniform_words(a.key, e >> 4, w);
+        const RandKey key = {a.key.seed, a.key.step + (a.step_dev ? *a.step_dev : 0)};
+        chunk_uniform_words(key, e >> 4, w);
         const uint32_t lo = e & 8 ? w[2] : w[0], hi = e & 8 ? w[3] : w[1];
 #pragma unroll
         for (int j = 0; j < 8; j++) u[j] = (float)(((j < 4 ? lo : hi) >> (8 * (j & 3)) & 0xffu) | 1u) * 0.00390625f;

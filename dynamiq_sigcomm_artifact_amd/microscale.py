@@ -5,8 +5,8 @@ The quantiser is the codec's kind applied to the operands of a product: blocks a
 optional randomized Hadamard transform of each block in front, rounding to nearest or stochastic, from a pool or from the
 in-kernel Philox stream.  ``include/dynamiq_eden.h`` (dq_mx4_*) has the format and the rounding to the bit.
 
-Everything runs on the current stream of the tensors' device, returns new tensors and can be recorded into a graph (a replay draws the
-random numbers of the recording: seed and step are constants of the launch)."""
+Everything runs on the current stream of the tensors' device, returns new tensors and can be recorded into a graph.  A replay draws the random
+numbers of the recording, unless step is an int64 tensor [1] on the device, which is read when the kernel runs."""
 import torch
 
 from . import capi
@@ -40,7 +40,8 @@ def quantize(x, columns=False, sign=None, rand_pool=None, seed=None, step=0):
 
     sign: int32 [>= 8 s], the packed signs of capi.pack_signs or capi.rand_diag_bits, one per element of a vector: every block of 32 is rotated,
     H (s x) / sqrt(32).  The product of two matrices that are rotated with the same signs is that of the matrices.
-    rand_pool: uniform values in [0, 1), [vectors, 256 s], for stochastic rounding; or seed (and step) for the in-kernel stream;
+    rand_pool: uniform values in [0, 1), [vectors, 256 s], for stochastic rounding; or seed (and step, a number or an int64 tensor [1]) for the
+    in-kernel stream;
     neither: to nearest, ties to even."""
     codes, scales = capi.host().mx4_quantize(x, columns, sign, rand_pool, seed, step)
     r, c = x.shape
@@ -79,7 +80,8 @@ def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0):
     the given signs, which spreads outliers over their block and cancels in the product.
 
     sign: (signs of n, signs of the tokens), packed; None leaves R out.  rand_pool: (pool [tokens, n padded to 256], pool [n, tokens padded to
-    256]), or seed and step: then every call needs a step of its own.  With neither the gradients are rounded to nearest, too.  The gradients
+    256]), or seed and step: then every call needs a step of its own, below 2^63 (the gradient's rows draw at step, its columns at step + 2^63).
+    With neither the gradients are rounded to nearest, too.  A step on the device stays as it is until the backward pass has run.  The gradients
     cannot be differentiated again."""
     signs, pools = sign or (None, None), rand_pool or (None, None)
     return capi.host().mx4_linear(x, weight, signs[0], signs[1], pools[0], pools[1], seed, step)

@@ -10,6 +10,8 @@ peak).  ``python evaluate.py --config 1|2|3|4|5``.  A measurement tool beside
   4  Llama-3-8B shaped gradient set in 25 MB buckets: dynamic {2,4,8}-bit allocation
   5  2^30 fp32: compress / decompress / fused sweep, and the blocked transform
 ``--kernels`` times every entry point of the library on one 25 MB bucket.
+``--training-step`` runs whole training steps of one rank: two 4-bit linear layers, their gradients through a dynamic-bitrate bucket,
+the clipping norm, and AdamW.
 ``--reference-benchmark`` prints the table of the reference's own microbenchmark
 (cuda_kernels/tests/benchmark_scaling_quantization.py:60-112: bf16, chunk 16, 268,435,456 elements,
 2/4/8 bits x strategy 2/3, eager launches through the eden_utils module) with the fraction of the HBM peak.
@@ -32,11 +34,11 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 import cpu_baselines                                                                       # noqa: E402
-from dynamiq_sigcomm_artifact_amd import bitrate, capi                                     # noqa: E402
+from dynamiq_sigcomm_artifact_amd import bitrate, capi, microscale, optimizer              # noqa: E402
 from dynamiq_sigcomm_artifact_amd.compressors import Aee_Dynamic_Range_GPU_kern, Mee_Dynamic_Range_GPU_kern   # noqa: E402
 from dynamiq_sigcomm_artifact_amd.dynamiq_pipeline import (dynamic_bitrate_allreduce,     # noqa: E402
                                                            dynamic_bitrate_allreduce_grouped,
-                                                           dynamic_bitrate_allreduce_single_pass, pick_streams)
+                                                           SinglePassBuckets, dynamic_bitrate_allreduce_single_pass, pick_streams)
 from dynamiq_sigcomm_artifact_amd.ring_sim import ring_allreduce, split_chunks             # noqa: E402
 
 HBM_PEAK = 8000.0  # GB/s
@@ -782,6 +784,101 @@ def kernels(dev, n=6553600):
     line("EdenBinsToBits", lambda: capi.bins_to_bits(bins, arr, 5), 4 * d + d // 32 * 5 * 4, n=d, nbits=5)
     line("EdenBitsToBins", lambda: capi.bits_to_bins(bins, arr, 5), 4 * d + d // 32 * 5 * 4, n=d, nbits=5)
     line("quantization_compression", lambda: capi.quantization(y, 0.5, 15.0, 1), 8 * d, n=d)
+    # what follows the all-reduce, and the 4-bit matrices, on the bucket as a matrix of 2560 columns
+    del y, x32, uni, lev, bins, arr
+    rows, cols = n // 2560, 2560
+    n = rows * cols
+    w32, w16 = (torch.randn(n, generator=g, device=dev) * 1e-2 for _ in range(2))
+    g16 = (torch.randn(n, generator=g, device=dev) * 1e-3).bfloat16()
+    w16 = w16.bfloat16()
+    work, norm = optimizer.norm_work(dev), torch.empty(2, dtype=torch.float32, device=dev)
+    line("grad_norm", lambda: optimizer.grad_norm([g16], 1.0, work=work, out=norm), 2 * n, n=n, launches=2)
+    for bits, state_bytes in ((32, 16), (8, 4.125)):
+        state = optimizer.adamw_state([w16], bits)
+        line("adamw_step", lambda: optimizer.adamw_step([w16], [g16], state, 7), (2 + 2 + 2 + state_bytes) * n, n=n, state_bits=bits, elements="bf16")
+        line("adamw_step", lambda: optimizer.adamw_step([w32], [g16], state, 7), (4 + 4 + 2 + state_bytes) * n, n=n, state_bits=bits, elements="fp32")
+        master = optimizer.master_weights([w16])
+        line("adamw_step (master weights)", lambda: optimizer.adamw_step([w16], [g16], state, 7, master=master), (4 + 4 + 2 + 2 + state_bytes) * n, n=n,
+             state_bits=bits, elements="bf16")
+    x = g16.view(rows, cols)
+    bits = [torch.empty(-(-k // 256) * 8, dtype=torch.int32, device=dev) for k in (cols, rows)]
+    for k, b in enumerate(bits):
+        capi.rand_diag_bits(b, b.numel() * 32, k + 1)
+    for columns in (False, True):
+        padded = (cols * -(-rows // 256) if columns else rows * -(-cols // 256)) * 256
+        line("mx4 quantize", lambda: microscale.quantize(x, columns), 2 * n + padded * 17 / 32, n=n, columns=columns)
+        line("mx4 quantize (rotated, stochastic)", lambda: microscale.quantize(x, columns, sign=bits[columns], seed=1), 2 * n + padded * 17 / 32, n=n,
+             columns=columns)
+    q = microscale.quantize(x)
+    line("mx4 dequantize", lambda: microscale.dequantize(q, torch.bfloat16), 2 * n + n * 17 / 32, n=n)
+    for m in (1, 16, 512, 4096):
+        a = microscale.quantize(torch.randn(m, cols, generator=g, device=dev))
+        t = _time_us(lambda: microscale.product(a, q))
+        _emit(kernel="mx4 product", us=round(t, 2), m=m, n=rows, k=cols, TFLOPs=round(2.0 * m * n / t / 1e6, 1))
+
+
+def training_step(dev, tokens=4096, width=1600, hidden=2048, steps=20):
+    """One rank's training steps in whole: two linear layers, width -> hidden -> width, forward and backward in 4 bits (rotated, stochastic gradients);
+    their 6,553,600 gradients, one 25 MB bucket of bf16, through the dynamic-bitrate encoding and back; the norm over them and the factor that clips
+    it; AdamW with 8-bit states and master weights.  The times are those of each part and of the whole step replayed from a graph; beside them the
+    losses of the first and the last of the steps, and what 4 bits and the encoding each change in the gradients."""
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(tokens, width, generator=g, device=dev).bfloat16()
+    true = [torch.randn(r, c, generator=g, device=dev) / math.sqrt(c) for r, c in ((hidden, width), (width, hidden))]
+    aim = (torch.relu(x.float() @ true[0].t()) @ true[1].t()).bfloat16()
+    weights = [(torch.randn(t.shape, generator=g, device=dev) / math.sqrt(t.shape[1])).bfloat16().requires_grad_() for t in true]
+    sizes = [w.numel() for w in weights]
+    bucket, reduced = (torch.zeros(sum(sizes), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    parts, grads = ([v.view_as(w) for v, w in zip(flat.split(sizes), weights)] for flat in (bucket, reduced))
+    signs = {}
+    for k, n in enumerate((tokens, width, hidden)):
+        signs[n] = torch.empty(-(-n // 256) * 8, dtype=torch.int32, device=dev)
+        capi.rand_diag_bits(signs[n], signs[n].numel() * 32, k + 1)
+    count = torch.zeros(1, dtype=torch.int64, device=dev)
+    pipe = SinglePassBuckets(dev, seed=3, u=45.0)
+    opt = optimizer.AdamW(weights, lr=1e-3, bits=8, capturable=True)
+    norm, loss = torch.empty(2, dtype=torch.float32, device=dev), torch.empty((), device=dev)
+
+    def layers():
+        h = torch.relu(microscale.linear(x, weights[0], sign=(signs[hidden], signs[tokens]), seed=1, step=count))
+        off = (microscale.linear(h, weights[1], sign=(signs[width], signs[tokens]), seed=2, step=count) - aim).float()
+        value = off.square().mean()
+        loss.copy_(value.detach())
+        for part, w in zip(parts, torch.autograd.grad(value * tokens, weights)):
+            part.copy_(w)
+        count.add_(1)
+
+    def encode():
+        pipe.begin_step()
+        pipe.run(bucket, reduced)
+
+    def clip():
+        optimizer.grad_norm(grads, 1.0, work=opt.work, out=norm)
+
+    def update():
+        for w, v in zip(weights, grads):
+            w.grad = v
+        opt.step(grad_scale=norm[1:])
+
+    def step():
+        layers()
+        encode()
+        clip()
+        update()
+
+    losses = []
+    for k in range(steps):
+        step()
+        losses.append(float(loss))
+    layers()
+    encode()
+    plain = [w.detach().float().requires_grad_() for w in weights]
+    off = torch.relu(x.float() @ plain[0].t()) @ plain[1].t() - aim.float()
+    exact = torch.cat([v.reshape(-1) for v in torch.autograd.grad(off.square().mean() * tokens, plain)])
+    _emit(training_step="run", tokens=tokens, width=width, hidden=hidden, steps=steps, loss_first=losses[0], loss_last=losses[-1],
+          grad_nmse_of_4_bit_layers=_nmse(exact, bucket), grad_nmse_of_the_encoding=_nmse(bucket, reduced), norm=float(norm[0]))
+    for name, fn in (("layers", layers), ("encode", encode), ("clip", clip), ("update", update), ("step", step)):
+        _emit(training_step=name, us=round(_time_us(fn, warmup=3, iters=10), 2))
 
 
 def quantiser_sizes(dev, nbits=4):
@@ -975,6 +1072,8 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--config", type=int, choices=[1, 2, 3, 4, 5])
     ap.add_argument("--kernels", action="store_true", help="time every entry point of the library on a 25 MB bucket")
+    ap.add_argument("--training-step", action="store_true",
+                    help="whole training steps of one rank: 4-bit linear layers, a dynamic-bitrate bucket, the clipping norm, AdamW")
     ap.add_argument("--quantiser-sizes", action="store_true",
                     help="compress / decompress / fused step of the production quantiser (bf16, 4-bit, AEE and MEE) at 25 MB, at "
                          "the ring-chunk size of the 8-rank configuration and at 2^28 elements")
@@ -995,6 +1094,9 @@ def main():
     torch.cuda.set_device(dev)
     if args.kernels:
         kernels(dev, **({"n": args.n} if args.n else {}))
+        return
+    if args.training_step:
+        training_step(dev)
         return
     if args.quantiser_sizes:
         quantiser_sizes(dev)

@@ -827,11 +827,13 @@ int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double
  * the way from one value to the next: where u is below it, with the least k for
  * which max <= 6 2^k.  u: rand_pool (rand_dtype; [result's rows][256 s], in [0, 1)), or
  * with rand_pool = NULL the in-kernel stream of dq_scaling_compress_philox, keyed by
- * (seed, step, chunk of 16 elements of that layout).
+ * (seed, step, chunk of 16 elements of that layout).  step_dev (may be NULL): one uint64
+ * in device memory that is added to step, so that a recorded call draws anew.
  * A block that holds an infinity or NaN is NaN. */
 int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, int64_t stride, int columns,
                     const uint32_t *sign, int stochastic, const void *rand_pool, int rand_dtype, uint64_t seed,
-                    uint64_t step, uint8_t *codes, uint8_t *scales, int device, dq_stream_t stream);
+                    uint64_t step, const uint64_t *step_dev, uint8_t *codes, uint8_t *scales, int device,
+                    dq_stream_t stream);
 /* out: `dtype` [rows][cols], the values rounded to nearest */
 int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows,
                       int64_t cols, int device, dq_stream_t stream);

@@ -269,8 +269,8 @@ def test_linear(ms, capi, m, n, k, rotate, rounding, dtype):
     y.backward(dy)
     if rounding == "philox":
         pools = tuple(torch.empty(r, -(-c // 256) * 256, device=DEV) for r, c in ((m, n), (n, m)))
-        capi.philox_uniform(pools[0], 77, 6)
-        capi.philox_uniform(pools[1], 77, 7)
+        capi.philox_uniform(pools[0], 77, 3)
+        capi.philox_uniform(pools[1], 77, 3 + (1 << 63))
     want = plain_linear(x.detach(), w.detach(), dy, sn, sm, *(pools or (None, None)))
     for got, t, length in ((y, want[0], k), (x.grad, want[1], n), (w.grad, want[2], m)):
         assert got.dtype == dtype
@@ -393,3 +393,40 @@ def test_layer_in_a_graph(ms, capi):
         a, b = (x0 * (k + 1)).requires_grad_(), w0.clone().requires_grad_()
         e = ms.linear(a, b, seed=1, step=2)
         assert torch.equal(y, e) and all(torch.equal(s, t) for s, t in zip((dx, dw), torch.autograd.grad(e, (a, b), dy)))
+
+
+def test_step_on_the_device(ms):
+    """the random stream of a step in device memory is that of the number, also in a graph that is replayed with another one"""
+    x, w, dy = matrix(40, 96, BF, 1, 1.0).requires_grad_(), matrix(50, 96, BF, 2, 1.0).requires_grad_(), matrix(40, 50, BF, 3, 1.0)
+    step = torch.tensor([7], device=DEV)
+
+    def layer(t):
+        return torch.autograd.grad(ms.linear(x, w, seed=1, step=t), (x, w), dy)
+
+    def same(a, b):
+        return all(torch.equal(s, t) for s, t in zip(a, b))
+    for columns in (False, True):
+        assert torch.equal(ms.quantize(dy, columns, seed=3, step=step).codes, ms.quantize(dy, columns, seed=3, step=7).codes)
+    assert same(layer(step), layer(7)) and not same(layer(7), layer(8))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer(step)
+        step.add_(1)
+    for t in (7, 8, 9):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(got, layer(t))
+    y = ms.linear(x, w, seed=1, step=step)
+    step.add_(1)                                            # the backward pass would draw other numbers than those of its step
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    for bad in (torch.zeros(1, device=DEV), torch.zeros(1, dtype=torch.int64), torch.zeros(0, dtype=torch.int64, device=DEV)):
+        with pytest.raises(RuntimeError):
+            ms.linear(x, w, seed=1, step=bad)
+        with pytest.raises(RuntimeError):
+            ms.quantize(dy, seed=1, step=bad)

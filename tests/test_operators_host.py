@@ -72,12 +72,12 @@ def test_coefficients_refuse(L):
 def test_matrices_refuse(L):
     Z = ctypes.c_uint64(0)
 
-    def quantize(x=P, dtype=1, r=10, c=300, stride=300, columns=0, sign=N, stochastic=0, pool=N, pool_dtype=1, codes=P, scales=P):
-        return L.dq_mx4_quantize(x, dtype, r, c, stride, columns, sign, stochastic, pool, pool_dtype, Z, Z, codes, scales, 0, S)
+    def quantize(x=P, dtype=1, r=10, c=300, stride=300, columns=0, sign=N, stochastic=0, pool=N, pool_dtype=1, counter=N, codes=P, scales=P):
+        return L.dq_mx4_quantize(x, dtype, r, c, stride, columns, sign, stochastic, pool, pool_dtype, Z, Z, counter, codes, scales, 0, S)
     odd, four = ctypes.c_void_p(0x1008), ctypes.c_void_p(0x1004)
     for kw, text in ((dict(dtype=5), "dtype"), (dict(pool=P, stochastic=1, pool_dtype=4), "dtype"), (dict(r=0), "positive"), (dict(c=0), "positive"),
                      (dict(r=1 << 27, c=256), "2^35"), (dict(r=256, c=1 << 27, columns=1, stride=1 << 27), "2^35"),
-                     (dict(r=(1 << 27) - 15, c=256), "2^35"), (dict(r=1 << 31, c=1, columns=1), "2^31"), (dict(r=1, c=1 << 31, stride=1 << 31), "2^31"), (dict(stride=299), "stride"), (dict(pool=P), "stochastic"),
+                     (dict(r=(1 << 27) - 15, c=256), "2^35"), (dict(r=1 << 31, c=1, columns=1), "2^31"), (dict(r=1, c=1 << 31, stride=1 << 31), "2^31"), (dict(stride=299), "stride"), (dict(pool=P), "stochastic"), (dict(counter=P), "step_dev"), (dict(counter=P, pool=P, stochastic=1), "step_dev"),
                      (dict(x=N), "null"), (dict(codes=N), "null"), (dict(scales=N), "null"), (dict(codes=odd), "aligned"), (dict(scales=four), "aligned")):
         refused(L, quantize(**kw), text)
     refused(L, L.dq_mx4_dequantize(P, P, P, 9, 1, 1, 0, S), "dtype")
