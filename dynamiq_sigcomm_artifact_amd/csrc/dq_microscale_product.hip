@@ -147,15 +147,11 @@ template <int MF, int NF, int W, int U> __global__ __launch_bounds__(64 * W) voi
 
 // ---- many rows: tiles through LDS --------------------------------------------------------------------------
 
-// 16 (4) bytes a lane from base + offset to LDS, lane after lane from byte `to` on.  Written out: the compiler takes a read of any part of LDS for one of
+// 16 bytes a lane from base + offset to LDS, lane after lane from byte `to` on.  Written out: the compiler takes a read of any part of LDS for one of
 // what is on its way there, and waits.  Whoever reads waits for vmcnt himself.
 __device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t offset, uint32_t to)
 {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to));
-}
-__device__ __forceinline__ void load_lds4(const uint8_t *base, uint32_t offset, uint32_t to)
-{
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(to));
 }
 
 // Which tile a workgroup takes.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that lie together, four rows of tiles high, so that
@@ -170,23 +166,23 @@ __device__ __forceinline__ uint2 tile_of(uint32_t id, uint32_t tiles, uint32_t t
     return make_uint2(__builtin_amdgcn_readfirstlane(4 * band + in_band % high), __builtin_amdgcn_readfirstlane(in_band / high));
 }
 
-// A workgroup of four waves, 2 x 2, takes a tile of T x T, superchunk by superchunk: rows of 128 bytes of codes and 8 of scales, which lie in LDS twice, one
-// being computed with while the next arrives.  Piece b of row r lies in slot b ^ (r / 2 % 8): the sixteen lanes that read at a time, one piece of sixteen rows,
-// then find sixteen different groups of banks.  The operands of a step are read during the products of the step before; the waves meet before the last step
-// of a superchunk, when everything of it is in registers.
+// A workgroup of four waves, 2 x 2, takes a tile of T x T, superchunk by superchunk: rows of 128 bytes of codes, which lie in LDS twice, one being computed with
+// while the next arrives.  Piece b of row r lies in slot b ^ (r / 2 % 8): the sixteen lanes that read at a time, one piece of sixteen rows, then find sixteen
+// different groups of banks.  The operands of a step are read during the products of the step before; the waves meet before the last step of a superchunk,
+// when everything of it is in registers.  Scales come for four superchunks at a time, 32 bytes a row.
 template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void mx4_tile_kernel(ProductArgs p)
 {
     constexpr int F = T / 64; // 32 x 32 products of a wave, each way
-    constexpr int kCodes = T * 128, kScales = T * 8, kStage = 2 * (kCodes + kScales);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    constexpr int kCodes = T * 128, kStage = 2 * kCodes, kScales = T * 32, kScaleGroup = 2 * kScales;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * (kStage + kScaleGroup)];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
     const uint2 at = tile_of(blockIdx.x, gridDim.x, (uint32_t)((p.m + T - 1) / T), p.tiles_n);
     const int64_t i0 = (int64_t)at.x * T, j0 = (int64_t)at.y * T;
     const uint32_t pitch = p.superchunks * 128u, scale_pitch = p.superchunks * 8u;
 
-    // what this lane fetches: pieces of 16 bytes, eight rows a wave and instruction; scale words, 32 rows likewise.  Rows past the end are the last one's.
-    constexpr int kLoads = T / 32, kScaleLoads = T / 128;
-    uint32_t from_a[kLoads], from_b[kLoads], scale_a[kScaleLoads], scale_b[kScaleLoads];
+    // what this lane fetches: pieces of 16 bytes, eight rows a wave and instruction.  Rows past the end are the last one's.
+    constexpr int kLoads = T / 32, kParts = 2 * kLoads;
+    uint32_t from_a[kLoads], from_b[kLoads];
 #pragma unroll
     for (int k = 0; k < kLoads; k++) {
         const int r = 8 * (4 * k + wave) + (lane >> 3);
@@ -194,44 +190,33 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
         from_a[k] = (uint32_t)min((int64_t)r, p.m - 1 - i0) * pitch + piece;
         from_b[k] = (uint32_t)min((int64_t)r, p.n - 1 - j0) * pitch + piece;
     }
-#pragma unroll
-    for (int k = 0; k < kScaleLoads; k++) {
-        const int r = 32 * (4 * k + wave) + (lane >> 1);
-        scale_a[k] = (uint32_t)min((int64_t)r, p.m - 1 - i0) * scale_pitch + 4 * (lane & 1);
-        scale_b[k] = (uint32_t)min((int64_t)r, p.n - 1 - j0) * scale_pitch + 4 * (lane & 1);
-    }
     const uint8_t *a = p.a_codes + i0 * pitch, *b = p.b_codes + j0 * pitch;
-    const uint8_t *as = p.a_scales + i0 * scale_pitch, *bs = p.b_scales + j0 * scale_pitch;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    constexpr int kParts = 2 * (kLoads + kScaleLoads);
     auto fetch_part = [&](uint32_t stage, int part) {
         const uint32_t to = lds_at + stage;
         const int k = part >> 1;
-        if (k < kLoads) {
-            if (part & 1)
-                load_lds16(b, from_b[k], to + kCodes + 1024 * (4 * k + wave));
-            else
-                load_lds16(a, from_a[k], to + 1024 * (4 * k + wave));
-        } else {
-            if (part & 1)
-                load_lds4(bs, scale_b[k - kLoads], to + 2 * kCodes + kScales + 256 * (4 * (k - kLoads) + wave));
-            else
-                load_lds4(as, scale_a[k - kLoads], to + 2 * kCodes + 256 * (4 * (k - kLoads) + wave));
-        }
+        if (part & 1)
+            load_lds16(b, from_b[k], to + kCodes + 1024 * (4 * k + wave));
+        else
+            load_lds16(a, from_a[k], to + 1024 * (4 * k + wave));
     };
-    auto fetched = [&] { a += 128, b += 128, as += 8, bs += 8; };
-    auto fetch = [&](uint32_t stage) {
-#pragma unroll
-        for (int k = 0; k < kParts; k++) fetch_part(stage, k);
-        fetched();
+    auto fetched = [&] { a += 128, b += 128; };
+    // Part j of the scales of superchunks 4 g .. 4 g + 3: 32 rows a wave and instruction, two lanes a row.  A row's last piece may reach into the next row; the last
+    // row's begins eight bytes earlier instead.
+    constexpr int kScaleParts = T / 64;
+    auto fetch_scales = [&](uint32_t g, uint32_t j) {
+        const bool of_b = j & 1;
+        const uint32_t k = 4 * (j >> 1 & (kScaleParts / 2 - 1)) + wave, last = (uint32_t)(of_b ? p.n : p.m) - 1;
+        const uint32_t row = min((uint32_t)(of_b ? j0 : i0) + 32 * k + (lane >> 1), last);
+        load_lds16(of_b ? p.b_scales : p.a_scales, min(row * scale_pitch + 32 * g + 16 * (lane & 1), (last + 1) * scale_pitch - 16),
+                   lds_at + 2 * kStage + (g & 1) * kScaleGroup + (of_b ? kScales : 0) + 1024 * k);
     };
 
     f32x16 acc[F][F] = {};
     uint4 x[2][F], y[2][F];
     int sa[F], sb[F], next_sa[F], next_sb[F];
     const int ra = (wave >> 1) * (T / 2) + (lane & 31), rb = (wave & 1) * (T / 2) + (lane & 31);
-    const uint8_t *at_a = lds + ra * 128, *at_b = lds + kCodes + rb * 128, *at_sa = lds + 2 * kCodes + ra * 8 + 4 * half,
-                  *at_sb = lds + 2 * kCodes + kScales + rb * 8 + 4 * half;
+    const uint8_t *at_a = lds + ra * 128, *at_b = lds + kCodes + rb * 128, *at_sa = lds + 2 * kStage + ra * 32 + 4 * half, *at_sb = lds + 2 * kStage + kScales + rb * 32 + 4 * half;
     uint32_t slot[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) slot[k] = ((4 * half + k) ^ (lane >> 1 & 7)) * 16;
@@ -242,78 +227,101 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
             y[to][f] = *reinterpret_cast<const uint4 *>(at_b + stage + slot[step] + 4096 * f);
         }
     };
+    // the scales of superchunk s; last: s is the last one, and odd numbers of them end in half a piece
+    auto read_scales = [&](int f, uint32_t s, bool last) {
+        const uint32_t from = (s >> 2 & 1) * kScaleGroup + 8 * (s & 3) + 1024 * f;
+        const bool odd = last && p.superchunks & 1;
+        next_sa[f] = *reinterpret_cast<const int *>(at_sa + from + (odd && i0 + ra + 32 * f >= p.m - 1 ? 8 : 0));
+        next_sb[f] = *reinterpret_cast<const int *>(at_sb + from + (odd && j0 + rb + 32 * f >= p.n - 1 ? 8 : 0));
+    };
     // every wave has what it fetched, and is done with what it read
     auto meet = [] {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
+    // Products of step S from operands FROM, the next step's operands read between them, and parts LOW .. HIGH of what is fetched to stage TO
+#define DQ_STEP(S, FROM, NEXT, STAGE, GO, TO, LOW, HIGH, MORE)                                                                                  \
+    _Pragma("unroll") for (int f = 0; f < F; f++)                                                                                               \
+    {                                                                                                                                           \
+        x[1 - FROM][f] = *reinterpret_cast<const uint4 *>(at_a + STAGE + slot[NEXT] + 4096 * f);                                                \
+        y[1 - FROM][f] = *reinterpret_cast<const uint4 *>(at_b + STAGE + slot[NEXT] + 4096 * f);                                                \
+        MORE;                                                                                                                                   \
+        _Pragma("unroll") for (int h = 0; h < F; h++)                                                                                           \
+        {                                                                                                                                       \
+            acc[f][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(y[FROM][h]), operand(x[FROM][f]), acc[f][h], 4, 4, S, sb[h], S, sa[f]); \
+            if (GO) {                                                                                                                           \
+                _Pragma("unroll") for (int k = (LOW) + (F * f + h) * ((HIGH) - (LOW)) / (F * F); k < (LOW) + (F * f + h + 1) * ((HIGH) - (LOW)) / (F * F); k++) \
+                    fetch_part(TO, k);                                                                                                          \
+            }                                                                                                                                   \
+            __builtin_amdgcn_sched_barrier(0);                                                                                                  \
+        }                                                                                                                                       \
+    }
 #define DQ_PRODUCTS(FROM, S)                                                                                                                    \
     _Pragma("unroll") for (int f = 0; f < F; f++)                                                                                               \
         _Pragma("unroll") for (int h = 0; h < F; h++)                                                                                           \
             acc[f][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(y[FROM][h]), operand(x[FROM][f]), acc[f][h], 4, 4, S, sb[h], S, sa[f]);
     // one read, then as many products as there are to a read
-#define DQ_INTERLEAVE(READS)                                                                                                                    \
+#define DQ_INTERLEAVE                                                                                                                           \
     _Pragma("unroll") for (int k = 0; k < 2 * F; k++) {                                                                                         \
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);                                                                                  \
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                                                                      \
         __builtin_amdgcn_sched_group_barrier(0x008, F / 2, 0);                                                                                  \
     }                                                                                                                                           \
     __builtin_amdgcn_sched_barrier(0);
-    fetch(0);
+    // A fetching instruction keeps a wave for 64 cycles, the time of two products (the four waves share 64 bytes a cycle), and waits for its turn: twenty in one
+    // step, scales among them, took 1280 cycles where its products take 512.  So the fetches for superchunk s + 2 begin behind the meeting of s, in its last
+    // step, and end in the first step of s + 1, and scales, as dear by the row as codes, come once in four superchunks: 4096 x 4096 x 14336 in 110 us instead of 126.
+    constexpr int kFirst = kParts / 2;
+    const int n = p.superchunks;
+#pragma unroll
+    for (int k = 0; k < kParts; k++) fetch_part(0, k);
+    fetched();
+#pragma unroll
+    for (int j = 0; j < kScaleParts; j++) fetch_scales(0, j);
+    fetch_scales(1, 0);
     meet();
-    if (p.superchunks > 1) fetch(kStage);
+    if (n > 1) {
+#pragma unroll
+        for (int k = 0; k < kFirst; k++) fetch_part(kStage, k);
+    }
     read(0, 0, 0);
 #pragma unroll
-    for (int f = 0; f < F; f++) {
-        next_sa[f] = *reinterpret_cast<const int *>(at_sa + 256 * f);
-        next_sb[f] = *reinterpret_cast<const int *>(at_sb + 256 * f);
-    }
+    for (int f = 0; f < F; f++) read_scales(f, 0, n == 1);
     uint32_t stage = 0;
     // (one block of code each, without a branch: products would wander behind it)
-#define DQ_SUPERCHUNK(FETCH)                                                                                                                    \
+#define DQ_SUPERCHUNK(REST, FETCH)                                                                                                              \
     {                                                                                                                                           \
         _Pragma("unroll") for (int f = 0; f < F; f++) sa[f] = next_sa[f], sb[f] = next_sb[f];                                                   \
-        read(1, 1, stage);                                                                                                                      \
-        DQ_PRODUCTS(0, 0)                                                                                                                       \
-        DQ_INTERLEAVE(1)                                                                                                                        \
+        const uint32_t other = kStage - stage;                                                                                                  \
+        DQ_STEP(0, 0, 1, stage, REST, other, kFirst, kParts, )                                                                                  \
+        if (REST) fetched();                                                                                                                    \
         read(0, 2, stage);                                                                                                                      \
         DQ_PRODUCTS(1, 1)                                                                                                                       \
-        DQ_INTERLEAVE(1)                                                                                                                        \
+        DQ_INTERLEAVE                                                                                                                           \
         read(1, 3, stage);                                                                                                                      \
         DQ_PRODUCTS(0, 2)                                                                                                                       \
-        DQ_INTERLEAVE(1)                                                                                                                        \
+        DQ_INTERLEAVE                                                                                                                           \
         meet();                                                                                                                                 \
-        const uint32_t free_stage = stage;                                                                                                      \
-        stage = kStage - stage;                                                                                                                 \
-        /* the first operands of the next superchunk, and what is fetched for the one after it, between the last products of this one */       \
-        _Pragma("unroll") for (int f = 0; f < F; f++)                                                                                           \
-        {                                                                                                                                       \
-            x[0][f] = *reinterpret_cast<const uint4 *>(at_a + stage + slot[0] + 4096 * f);                                                      \
-            y[0][f] = *reinterpret_cast<const uint4 *>(at_b + stage + slot[0] + 4096 * f);                                                      \
-            next_sa[f] = *reinterpret_cast<const int *>(at_sa + stage + 256 * f);                                                               \
-            next_sb[f] = *reinterpret_cast<const int *>(at_sb + stage + 256 * f);                                                               \
-            _Pragma("unroll") for (int h = 0; h < F; h++)                                                                                       \
-            {                                                                                                                                   \
-                acc[f][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(y[1][h]), operand(x[1][f]), acc[f][h], 4, 4, 3, sb[h], 3, sa[f]); \
-                if (FETCH) {                                                                                                                    \
-                    _Pragma("unroll") for (int k = (F * f + h) * kParts / (F * F); k < (F * f + h + 1) * kParts / (F * F); k++) fetch_part(free_stage, k); \
-                }                                                                                                                               \
-                __builtin_amdgcn_sched_barrier(0);                                                                                              \
-            }                                                                                                                                   \
-        }                                                                                                                                       \
-        if (FETCH) fetched();                                                                                                                   \
+        if (FETCH) fetch_scales((s + 1) / 4 + 1, s + 1);                                                                                        \
+        DQ_STEP(3, 1, 0, other, FETCH, stage, 0, kFirst, read_scales(f, s + 1, !(FETCH)))                                                       \
+        stage = other;                                                                                                                          \
     }
-    for (int s = 2; s < p.superchunks; s++) DQ_SUPERCHUNK(true)
-    if (p.superchunks > 1) DQ_SUPERCHUNK(false)
-    DQ_SUPERCHUNK(false) // (what it reads ahead is of the superchunk before, and not used)
+    int s = 0;
+    for (; s < n - 2; s++) DQ_SUPERCHUNK(true, true)
+    if (n > 1) {
+        DQ_SUPERCHUNK(true, false)
+        s++;
+    }
+    DQ_SUPERCHUNK(false, false) // (what it reads ahead is of the superchunk before, and not used)
 #undef DQ_SUPERCHUNK
+#undef DQ_STEP
 #undef DQ_PRODUCTS
 #undef DQ_INTERLEAVE
     // The result leaves through LDS as runs of whole rows: 32 rows x T / 2 columns of a wave at a time.  (All waves have passed the last meeting: what lay there
     // is in registers.)  A lane writes four columns of a row; rows are 16 bytes further apart than long, so that sixteen of them use all banks.
     typedef typename ElemIO<DT>::storage Elem;
     constexpr int kRow = T / 2 * sizeof(Elem), kApart = kRow + 16, kPer = 16 / sizeof(Elem), kLanes = kRow / 16;
-    static_assert(4 * 32 * kApart <= 2 * kStage, "the waves' rows fit");
+    static_assert(4 * 32 * kApart <= 2 * (kStage + kScaleGroup), "the waves' rows fit");
     uint8_t *mine = lds + wave * 32 * kApart;
     const int64_t col0 = j0 + (wave & 1) * (T / 2) + lane % kLanes * kPer;
 #pragma unroll
