@@ -378,11 +378,12 @@ template <int DT, int T> static hipError_t launch_tiles(ProductArgs p, hipStream
     return launch_with(mx4_tile_kernel<DT, T>, dim3((uint32_t)((p.m + T - 1) / T) * p.tiles_n), dim3(256), stream, p);
 }
 
-// Which kernel.  Tiles of 256 x 256 fetch the least per product, but one takes a CU: at 192 of them, three quarters of the CUs, they draw level with tiles of 128,
-// of which two share a CU (2048 x 4096 x 4096, 128 of 256: 33.6 us against 32.3; 4096 x 4096 x 1000, 256: 18.3 against 19.9).  Below 96 tiles of 128 the contraction
-// is shared out among the waves of a workgroup instead (256 x 4096 x 4096, 64 tiles: 16.4 us, split 14.7; 512 x 4096 x 4096, 128 tiles: 17.0, split 28.8), in the
-// largest blocks that leave 192 workgroups: with fewer, CUs have nothing to do (16 x 4096 x 4096, blocks of 16 x 16: 5.4 us, 16 x 64: 9.2), with more the
-// operands are read more often (16 x 14336 x 4096: 13.3 and 9.6 us; 1 x 14336 x 4096: 9.3 and 8.4).  No block is twice as high or wide as it need be.
+// Which kernel.  Two tiles of 128 x 128 share a CU, and 512 of them run at a time; tiles of 256 x 256 fetch half as much per product, but one takes a CU.  Where 512
+// suffice they are the faster (2048 x 4096 x 4096, 512 tiles: 24.0 us, tiles of 256: 29.7), and slower beyond (2304 x 4096 x 4096, 576 tiles: 34.3 and 29.1 us).
+// Below 40 tiles of 128 the contraction is shared out among the waves of a workgroup instead (256 x 3000 x 4096, 48 tiles: 12.6 us, shared out 20.2; 128 x 4096 x 4096,
+// 32 tiles: 10.8 and 11.2; 128 x 2048 x 4096, 16 tiles: 10.7 and 7.9), in the largest blocks that leave 192 workgroups: with fewer, CUs have nothing to do
+// (16 x 4096 x 4096, blocks of 16 x 16: 5.4 us, 16 x 64: 9.2), with more the operands are read more often (16 x 14336 x 4096: 13.3 and 9.6 us; 1 x 14336 x 4096: 9.3 and
+// 8.4).  No block is twice as high or wide as it need be.
 template <int MF, int NF, int U> static bool try_narrow(const ProductArgs &p, bool last, int dtype, hipStream_t stream, hipError_t &e)
 {
     const int64_t blocks = ((p.m + 16 * MF - 1) / (16 * MF)) * ((p.n + 16 * NF - 1) / (16 * NF));
@@ -396,9 +397,9 @@ hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, c
 {
     const ProductArgs p = {a_codes, a_scales, b_codes, b_scales, out, m, n, (int)((k + 255) >> 8), 0};
     const auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    if (m > 64 && n > 64 && tiles(256) >= 192)
+    if (m > 64 && n > 64 && tiles(128) > 512)
         return dtype == DQ_F32 ? launch_tiles<DQ_F32, 256>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 256>(p, stream) : launch_tiles<DQ_F16, 256>(p, stream);
-    if (m > 64 && n > 64 && tiles(128) >= 96)
+    if (m > 64 && n > 64 && tiles(128) >= 40)
         return dtype == DQ_F32 ? launch_tiles<DQ_F32, 128>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 128>(p, stream) : launch_tiles<DQ_F16, 128>(p, stream);
     hipError_t e = hipSuccess;
     (void)(try_narrow<4, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 2, 1>(p, false, dtype, stream, e) ||

@@ -199,7 +199,10 @@ PRODUCTS = [(1, 1, 1), (1, 16, 256), (1, 1000, 4096), (2, 33, 31), (3, 17, 4000)
             (65, 130, 2048), (100, 1, 777), (127, 129, 255), (128, 128, 1024), (129, 257, 2304), (256, 256, 256), (300, 500, 4100), (513, 1030, 1500), (1025, 777, 300),
             # every kernel that sizes choose: few rows and columns of each kind, tiles of 128 and of 256, their last rows and columns
             (5, 3100, 600), (16, 12300, 257), (20, 13000, 300), (33, 5000, 520), (40, 20000, 260), (1000, 40, 300), (3000, 70, 1111), (20000, 9, 300), (129, 12801, 300),
-            (1, 12400, 300), (8, 6200, 520), (9, 3100, 300), (1300, 1281, 900), (2000, 2049, 513), (4097, 3300, 256), (4100, 3200, 1025), (2049, 7000, 100)]
+            (1, 12400, 300), (8, 6200, 520), (9, 3100, 300), (1300, 1281, 900), (2000, 2049, 513), (4097, 3300, 256), (4100, 3200, 1025), (2049, 7000, 100),
+            # scales come for four superchunks at a time, and of odd numbers of them the last row's end early: one to nine of them, in tiles of 128 and of 256
+            (700, 900, 200), (701, 899, 700), (702, 898, 1100), (703, 897, 1281), (640, 1000, 1793), (641, 1001, 2049), (2900, 3000, 250), (2901, 2999, 512), (2817, 3001, 600),
+            (2818, 2990, 1280), (2819, 3011, 1537)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
