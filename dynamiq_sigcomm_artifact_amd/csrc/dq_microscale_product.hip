@@ -42,7 +42,8 @@ struct Rows16 {
 };
 
 // A workgroup takes 16 MF x 16 NF of the result; its waves share the superchunks out, one after the other, and add their sums up in LDS, in the order of the
-// waves.  Bound by memory, or by the time to the first byte: every wave has U superchunks on their way at a time.
+// waves.  Bound by memory, or by the time to the first byte: every wave has U superchunks on their way at a time.  1 x 14336 x 4096: 31 MB of codes and scales in 8.4 us,
+// 3.7 TB/s, some 3 of it the launch and the first load; 1 x 4096 x 4096 in 5.1.
 template <int MF, int NF, int W, int U> __global__ __launch_bounds__(64 * W) void mx4_narrow_kernel(NarrowArgs p)
 {
     __shared__ __attribute__((aligned(16))) float sums[W][MF * NF][64][4];
@@ -170,6 +171,9 @@ __device__ __forceinline__ uint2 tile_of(uint32_t id, uint32_t tiles, uint32_t t
 // while the next arrives.  Piece b of row r lies in slot b ^ (r / 2 % 8): the sixteen lanes that read at a time, one piece of sixteen rows, then find sixteen
 // different groups of banks.  The operands of a step are read during the products of the step before; the waves meet before the last step of a superchunk,
 // when everything of it is in registers.  Scales come for four superchunks at a time, 32 bytes a row.
+// A wave does 16 products of 32 x 32 x 64 per step, 512 cycles, and spends 800, 535, 535 and 800 on the four steps and 120 on the meeting: 4.4 PFLOP/s at 4096 x 4096 x 14336, at
+// the 1.8 to 2.0 GHz that the power limit leaves (products alone, from registers, reach 6.0 to 6.5 on such data).  8192 x 14336 x 4096 in 252 us, 3.8 PFLOP/s: of a tile's
+// 36 us some 2 are its first fetch and 4 its stores.  A workgroup that goes on to the next tile while it stores one gains 2 % there and loses 5 % with short contractions.
 template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void mx4_tile_kernel(ProductArgs p)
 {
     constexpr int F = T / 64; // 32 x 32 products of a wave, each way
@@ -381,7 +385,8 @@ template <int DT, int T> static hipError_t launch_tiles(ProductArgs p, hipStream
 // Which kernel.  Two tiles of 128 x 128 share a CU, and 512 of them run at a time; tiles of 256 x 256 fetch half as much per product, but one takes a CU.  Where 512
 // suffice they are the faster (2048 x 4096 x 4096, 512 tiles: 24.0 us, tiles of 256: 29.7), and slower beyond (2304 x 4096 x 4096, 576 tiles: 34.3 and 29.1 us).
 // Below 40 tiles of 128 the contraction is shared out among the waves of a workgroup instead (256 x 3000 x 4096, 48 tiles: 12.6 us, shared out 20.2; 128 x 4096 x 4096,
-// 32 tiles: 10.8 and 11.2; 128 x 2048 x 4096, 16 tiles: 10.7 and 7.9), in the largest blocks that leave 192 workgroups: with fewer, CUs have nothing to do
+// 32 tiles: 10.8 and 11.2; 128 x 2048 x 4096, 16 tiles: 10.7 and 7.9), with less than four superchunks, which a tile's two barriers and stores outlast, below 96
+// (776 x 1000 x 333, 56 tiles: 6.4 and 4.8; 1024 x 1024 x 1024, 64 tiles: 5.4 and 6.6), in the largest blocks that leave 192 workgroups: with fewer, CUs have nothing to do
 // (16 x 4096 x 4096, blocks of 16 x 16: 5.4 us, 16 x 64: 9.2), with more the operands are read more often (16 x 14336 x 4096: 13.3 and 9.6 us; 1 x 14336 x 4096: 9.3 and
 // 8.4).  No block is twice as high or wide as it need be.
 template <int MF, int NF, int U> static bool try_narrow(const ProductArgs &p, bool last, int dtype, hipStream_t stream, hipError_t &e)
@@ -399,7 +404,7 @@ hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, c
     const auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     if (m > 64 && n > 64 && tiles(128) > 512)
         return dtype == DQ_F32 ? launch_tiles<DQ_F32, 256>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 256>(p, stream) : launch_tiles<DQ_F16, 256>(p, stream);
-    if (m > 64 && n > 64 && tiles(128) >= 40)
+    if (m > 64 && n > 64 && tiles(128) >= (p.superchunks < 4 ? 96 : 40))
         return dtype == DQ_F32 ? launch_tiles<DQ_F32, 128>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 128>(p, stream) : launch_tiles<DQ_F16, 128>(p, stream);
     hipError_t e = hipSuccess;
     (void)(try_narrow<4, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 2, 1>(p, false, dtype, stream, e) ||
