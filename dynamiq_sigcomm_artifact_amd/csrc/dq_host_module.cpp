@@ -1079,12 +1079,12 @@ double number(PyObject *o)
     return v;
 }
 
-// the items of a list or tuple
+// the items of a list or tuple, held: another thread may change the list while a call runs
 struct Items {
     py::object held;
     PyObject **item;
     Py_ssize_t count;
-    explicit Items(PyObject *o) : held(py::reinterpret_steal<py::object>(PySequence_Fast(o, "a list of tensors is required")))
+    explicit Items(PyObject *o) : held(py::reinterpret_steal<py::object>(PySequence_Tuple(o)))
     {
         if (!held) throw py::error_already_set();
         item = PySequence_Fast_ITEMS(held.ptr());

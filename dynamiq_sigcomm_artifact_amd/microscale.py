@@ -42,7 +42,7 @@ def quantize(x, columns=False, sign=None, rand_pool=None, seed=None, step=0):
     H (s x) / sqrt(32).  The product of two matrices that are rotated with the same signs is that of the matrices.
     rand_pool: uniform values in [0, 1), [vectors, 256 s], for stochastic rounding; or seed (and step, a number or an int64 tensor [1]) for the
     in-kernel stream;
-    neither: to nearest, ties to even."""
+    neither: to nearest, ties to even.  Nothing here but linear() is differentiated."""
     codes, scales = capi.host().mx4_quantize(x, columns, sign, rand_pool, seed, step)
     r, c = x.shape
     return Microscaled(codes, scales, c if columns else r, r if columns else c)

@@ -59,7 +59,7 @@ def master_weights(params):
 
 def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master=None, grad_scale=None, coefficients=None):
     """one AdamW step in place.  params, grads: lists of contiguous tensors of the same sizes (fp16, bf16 or fp32 each; a gradient None leaves
-    its parameter as it is); state: of adamw_state; step: the number of this step, from 1; master: of master_weights, for 16-bit
+    its parameter as it is) that share no memory with the parameters; state: of adamw_state; step: the number of this step, from 1; master: of master_weights, for 16-bit
     parameters; grad_scale: float32 tensor [1] that multiplies the gradients (grad_norm's factor, a loss scale's inverse) -- where it is
     infinite or NaN the step changes nothing; coefficients: of adamw_coefficients, in place of step, lr and weight_decay."""
     codes, scales = state if isinstance(state, (tuple, list)) else (state, None)

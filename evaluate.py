@@ -786,7 +786,7 @@ def kernels(dev, n=6553600):
     line("quantization_compression", lambda: capi.quantization(y, 0.5, 15.0, 1), 8 * d, n=d)
     # what follows the all-reduce, and the 4-bit matrices, on the bucket as a matrix of 2560 columns
     del y, x32, uni, lev, bins, arr
-    rows, cols = n // 2560, 2560
+    rows, cols = max(1, n // 2560), 2560
     n = rows * cols
     w32, w16 = (torch.randn(n, generator=g, device=dev) * 1e-2 for _ in range(2))
     g16 = (torch.randn(n, generator=g, device=dev) * 1e-3).bfloat16()

@@ -775,7 +775,8 @@ int dq_grad_norm(const dq_span_t *spans, int count, double max_norm, double *wor
  *            its tensor; r > 0 is stored as no less than the smallest code.
  * master (nullable): float [total], the weights that the step reads and writes;
  * the 16-bit params then only receive them, rounded to nearest.  Without it 16-bit
- * params are read, and rounded to nearest as well. */
+ * params are read, and rounded to nearest as well.  Params, arenas and gradients
+ * share no memory with one another (a gradient may be used twice). */
 typedef struct dq_adamw_tensor {
     void *param;
     const void *grad;
