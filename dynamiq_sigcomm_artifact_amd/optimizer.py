@@ -11,6 +11,13 @@ from . import capi
 _HALF = (torch.float16, torch.bfloat16)
 
 
+def _tensors(of, what):
+    """a list of tensors; one tensor would be taken apart into its rows"""
+    if isinstance(of, torch.Tensor):
+        raise RuntimeError("%s: a list of tensors is required" % what)
+    return list(of)
+
+
 def norm_work(device):
     """the work buffer of grad_norm: kept from call to call, one for every stream (or recorded graph) whose calls may overlap"""
     return torch.empty(int(capi.lib().dq_grad_norm_work_doubles()), dtype=torch.float64, device=device)
@@ -20,7 +27,7 @@ def grad_norm(grads, max_norm=None, work=None, out=None):
     """float32 [2] on the device: the 2-norm of all tensors together, summed in 64 bits, and min(1, max_norm / (norm + 1e-6)), the
     ``grad_scale`` of a step that clips (1 without max_norm).  Where the norm is not finite the factor is NaN, and the step
     changes nothing.  work: from norm_work(); without it the call makes one."""
-    grads = list(grads)
+    grads = _tensors(grads, "grad_norm")
     if not grads:
         raise RuntimeError("grad_norm: no tensors")
     if work is None:
@@ -39,6 +46,9 @@ def padded_elements(params):
 def adamw_state(params, bits=32):
     """fresh states of a list of parameters for adamw_step: float32 [2, total] (the moments m and v), or for 8 bits (codes uint8
     [2, total], scales uint8 [2, total / 32]) of m and sqrt(v).  A parameter's states begin at a multiple of 32 (padded_elements)."""
+    params = _tensors(params, "adamw_state")
+    if not params:
+        raise RuntimeError("adamw_state: no parameters")
     total, device = padded_elements(params), params[0].device
     if bits == 32:
         return torch.zeros((2, total), dtype=torch.float32, device=device)
@@ -49,6 +59,9 @@ def adamw_state(params, bits=32):
 
 def master_weights(params):
     """float32 copies of 16-bit parameters in one arena, laid out as their states are"""
+    params = _tensors(params, "master_weights")
+    if not params:
+        raise RuntimeError("master_weights: no parameters")
     out = torch.zeros(padded_elements(params), dtype=torch.float32, device=params[0].device)
     at = 0
     for p in params:
@@ -62,6 +75,8 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
     its parameter as it is) that share no memory with the parameters; state: of adamw_state; step: the number of this step, from 1; master: of master_weights, for 16-bit
     parameters; grad_scale: float32 tensor [1] that multiplies the gradients (grad_norm's factor, a loss scale's inverse) -- where it is
     infinite or NaN the step changes nothing; coefficients: of adamw_coefficients, in place of step, lr and weight_decay."""
+    if isinstance(params, torch.Tensor) or isinstance(grads, torch.Tensor):
+        raise RuntimeError("adamw_step: lists of tensors are required")
     codes, scales = state if isinstance(state, (tuple, list)) else (state, None)
     capi.host().adamw_step(params, grads, codes, scales, master, grad_scale, coefficients, step, lr, betas[0], betas[1], eps, weight_decay)
 
@@ -88,13 +103,13 @@ class AdamW(object):
     recording.  Replays and other steps of the object follow one another on one stream, or in an order that the caller sees to."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, master=True, capturable=False):
-        params = list(params)
+        params = _tensors(params, "AdamW")
         if not params:
             raise RuntimeError("AdamW: no parameters")
         groups = params if isinstance(params[0], dict) else [{"params": params}]
         defaults = {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay}
         self.bits, self.capturable, self.steps = bits, bool(capturable), 0
-        self.param_groups = [{**defaults, **g, "params": list(g["params"])} for g in groups]
+        self.param_groups = [{**defaults, **g, "params": _tensors(g["params"], "AdamW")} for g in groups]
         every = self.params()
         if len({id(p) for p in every}) < len(every):
             raise RuntimeError("AdamW: a parameter appears twice")

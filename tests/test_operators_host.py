@@ -107,6 +107,14 @@ def test_modules_refuse_host_tensors():
         optimizer.grad_norm([])
     with pytest.raises(RuntimeError, match="32 or in 8"):
         optimizer.adamw_state([x], 16)
+    for call in (lambda: optimizer.grad_norm(x), lambda: optimizer.adamw_state(x), lambda: optimizer.master_weights(x), lambda: optimizer.AdamW(x),
+                 lambda: optimizer.AdamW([{"params": x}]), lambda: optimizer.adamw_step(x, [x], x, 1), lambda: optimizer.adamw_step([x], x, x, 1)):
+        with pytest.raises(RuntimeError, match="of tensors"):
+            call()
+    for call in (lambda: optimizer.adamw_state([]), lambda: optimizer.master_weights([])):
+        with pytest.raises(RuntimeError, match="no parameters"):
+            call()
+    assert optimizer.adamw_state(iter([x, x]), 8)[0].shape == (2, 64)
     a, b = microscale.Microscaled(None, None, 2, 5), microscale.Microscaled(None, None, 2, 6)
     with pytest.raises(RuntimeError, match="vectors of 5 and of 6"):
         microscale.product(a, b)
