@@ -138,15 +138,23 @@ template <int DT, int N> __device__ __forceinline__ void store_part(void *p, int
         if (j < count) ElemIO<DT>::store(p, i + j, v[j]);
 }
 
+// Workgroups go to the eight XCDs in turn: each gets a run of the count units of work that lie together, so that what its 32 CUs work on at a time shares its L2.
+__device__ __forceinline__ uint32_t unit_of(uint32_t id, uint32_t count)
+{
+    const uint32_t xcd = id & 7;
+    return xcd * (count >> 3) + min(xcd, count & 7) + (id >> 3);
+}
+
 // ---- the shared power of two ----
 
 // the largest magnitude of a block, which four neighbouring lanes hold eight elements each of, as a bit pattern: magnitudes are ordered
-// like their patterns, and infinities and NaN lie above every number
+// like their patterns, and infinities and NaN, which the maximum passes on, lie above every number
 __device__ __forceinline__ uint32_t block_max(const float (&v)[8])
 {
-    uint32_t u = 0;
+    float most = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) u = max(u, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; j++) most = __builtin_elementwise_maximum(most, __builtin_fabsf(v[j]));
+    uint32_t u = __float_as_uint(most) & 0x7fffffffu;
     u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0xB1, 0xf, 0xf, true)); // quad_perm [1,0,3,2]
     u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x4E, 0xf, 0xf, true)); // quad_perm [2,3,0,1]
     return u;

@@ -25,7 +25,7 @@ template <int CTRL> __device__ __forceinline__ float quad_f32(float v)
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 
-// H (s x) / sqrt(32) of the quad's 32 elements, in place; word: the sign bits of the block.  Stages of stride 1, 2, 4 lie within a lane, 8 and 16
+// H (s x) of the quad's 32 elements, in place (1 / sqrt(32) is encode_block's); word: the sign bits of the block.  Stages of stride 1, 2, 4 lie within a lane, 8 and 16
 // between lanes.  Every sum is one of two numbers, whichever lane takes it: the result does not depend on the layout.
 __device__ __forceinline__ void rotate_block(float (&v)[8], uint32_t word, int g)
 {
@@ -49,7 +49,7 @@ __device__ __forceinline__ void rotate_block(float (&v)[8], uint32_t word, int g
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float b = quad_f32<0x4E>(v[j]);
-        v[j] = (g & 2 ? b - v[j] : v[j] + b) * 0.17677669529663687f;
+        v[j] = g & 2 ? b - v[j] : v[j] + b;
     }
 }
 
@@ -68,12 +68,15 @@ template <int RAND> __device__ __forceinline__ void uniform8(const QuantizeArgs 
     }
 }
 
-// eight codes in a word, the first in the lowest bits, and the block's scale byte (the same in the quad's lanes)
-template <int RAND> __device__ __forceinline__ uint32_t encode_block(const float (&v)[8], const float (&u)[8], uint32_t &scale)
+// eight codes in a word, the first in the lowest bits, and the block's scale byte (the same in the quad's lanes).  ROTATE: of v / sqrt(32), with one product for an
+// element where there would be two.  (Finite sums are below 2^128, so that down is at least 2^-123 and its product with 1 / sqrt(32) a normal number.)
+template <int RAND, bool ROTATE> __device__ __forceinline__ uint32_t encode_block(const float (&v)[8], const float (&u)[8], uint32_t &scale)
 {
-    const uint32_t largest = block_max(v);
+    constexpr float kUnit = ROTATE ? 0.17677669529663687f : 1.0f;
+    uint32_t largest = block_max(v);
+    if (ROTATE) largest = __float_as_uint(__uint_as_float(largest) * kUnit);
     scale = RAND == kNearest ? block_scale<2, 0x7fffffu>(largest) : block_scale<2, 0x400000u>(largest);
-    const float down = scale_down(scale);
+    const float down = scale_down(scale) * kUnit;
     uint32_t word = 0;
     if constexpr (RAND == kNearest) {
         word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0] * down, v[1] * down, 1.0f, 0);
@@ -83,7 +86,6 @@ template <int RAND> __device__ __forceinline__ uint32_t encode_block(const float
     } else {
         // With 2^e the power of two at or below max(y, 1), codes are 2^e / 2 apart and t = 2 y / 2^e counts them from 2 e on (below 1: from 0 on).  The exponent's bits
         // carry 127 along, twice: 254 in each place of the word, taken off at the end.
-        uint32_t signs = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float y = __builtin_fabsf(v[j]) * down;
@@ -91,9 +93,15 @@ template <int RAND> __device__ __forceinline__ uint32_t encode_block(const float
             const float t = y * __uint_as_float(0x7f800000u - power);
             const uint32_t code = (uint32_t)t + (power >> 22) + (u[j] < __builtin_amdgcn_fractf(t) ? 1u : 0u);
             word += code << 4 * j;
-            signs |= __float_as_uint(v[j]) >> (28 - 4 * j) & (8u << 4 * j);
         }
-        word = (word - 254u * 0x11111111u) | signs;
+        // the signs: the highest bytes of four elements in a word
+        uint32_t even, odd;
+        {
+            const auto top = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0703u); };
+            even = __builtin_amdgcn_perm(top(v[4], v[6]), top(v[0], v[2]), 0x05040100u);
+            odd = __builtin_amdgcn_perm(top(v[5], v[7]), top(v[1], v[3]), 0x05040100u);
+        }
+        word = (word - 254u * 0x11111111u) | (even >> 4 & 0x08080808u) | (odd & 0x80808080u);
     }
     return word;
 }
@@ -117,7 +125,7 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
     uniform8<RAND>(a, (int64_t)unit * 8, u);
     if (ROTATE) rotate_block(v, a.sign[col >> 5], g);
     uint32_t scale;
-    reinterpret_cast<uint32_t *>(a.codes)[unit] = encode_block<RAND>(v, u, scale);
+    reinterpret_cast<uint32_t *>(a.codes)[unit] = encode_block<RAND, ROTATE>(v, u, scale);
     if (g == 0) a.scales[unit >> 2] = (uint8_t)scale;
 }
 
@@ -125,15 +133,15 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 
 // A workgroup takes 256 rows x 128 columns: one superchunk of 128 rows of the result.  A wave takes 32 of the rows, a lane 8 rows x 8 columns, and a
 // column's block lies in a quad as it does above.  The codes leave through LDS, as whole lines.  Elements of 16 bits stay packed until their column's turn: three
-// workgroups on a CU instead of two.  14336 x 4096 bf16, rotated, to the nearest in 32 us (4.7 TB/s; 40 unpacked); 8192 x 14336 with a bf16 pool in 141 us (3.8 TB/s, 157
-// unpacked), where the pool's runs of 64 bytes and some 40 vector instructions for an element's rotation and rounding keep it from more.  Half as wide a tile reads runs of
-// 128 bytes: 147 and 50 us.
+// workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 121 us (4.4 TB/s; 130
+// with the XCDs' workgroups strewn, 8000 x 5000 35 for 40), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
+// instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.
 template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
 {
     __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __shared__ __attribute__((aligned(8))) uint8_t tile_scales[128 * 8];
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
-    const uint32_t superchunk = tiles(blockIdx.x), col0 = (blockIdx.x - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
+    const uint32_t id = unit_of(blockIdx.x, gridDim.x), superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
     const uint32_t row0 = superchunk * 256 + 32 * block, row = row0 + 8 * g;
     constexpr int WORDS = DT == DQ_F32 ? 8 : 4;
     uint32_t x[8][WORDS]; // [row][column], as they are in memory
@@ -167,17 +175,17 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512, DT ==
                 for (int w = 0; w < WORDS; w++) x[j][w] = 0u;
             }
     }
-    const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u;
+    const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u, first = col * superchunks + superchunk, most = (all_cols - 1) * superchunks + superchunk;
 #pragma unroll
     for (int c = 0; c < 8; c++) {
         float v[8], u[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = word_value<DT>(x[j], c);
         // (what becomes of columns past the end is not stored)
-        uniform8<RAND>(a, ((int64_t)min(col + c, all_cols - 1) * superchunks + superchunk) * 256 + 32 * block + 8 * g, u);
+        uniform8<RAND>(a, (int64_t)min(first + c * superchunks, most) * 256 + 32 * block + 8 * g, u);
         if (ROTATE) rotate_block(v, sign, g);
         uint32_t scale;
-        const uint32_t word = encode_block<RAND>(v, u, scale);
+        const uint32_t word = encode_block<RAND, ROTATE>(v, u, scale);
         const int line = 8 * (lane >> 2) + c;
         *reinterpret_cast<uint32_t *>(tile + line * 128 + ((block ^ (line >> 3 & 7)) << 4) + 4 * g) = word;
         if (g == 0) tile_scales[line * 8 + block] = (uint8_t)scale;

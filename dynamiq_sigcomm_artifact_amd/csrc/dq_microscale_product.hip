@@ -155,12 +155,10 @@ __device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t offset,
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to));
 }
 
-// Which tile a workgroup takes.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that lie together, four rows of tiles high, so that
-// what its 32 CUs work on at a time shares operands in its L2.
+// Which tile a workgroup takes: an XCD's run of tiles is four rows of them high.
 __device__ __forceinline__ uint2 tile_of(uint32_t id, uint32_t tiles, uint32_t tiles_m, uint32_t tiles_n)
 {
-    const uint32_t xcd = id & 7, each = tiles >> 3, more = tiles & 7;
-    const uint32_t k = xcd * each + min(xcd, more) + (id >> 3);
+    const uint32_t k = unit_of(id, tiles);
     const uint32_t band = k / (4 * tiles_n), in_band = k - band * 4 * tiles_n;
     const uint32_t high = min(4u, tiles_m - 4 * band);
     // (divided in vector registers, the same in every lane)
