@@ -36,7 +36,7 @@ EXPORTS = [
     "dq_bins_to_bits", "dq_bits_to_bins", "dq_quantization",
     "dq_eden_work_doubles", "dq_eden_quantize", "dq_eden_quantize_static_max_n", "dq_eden_quantize_static", "dq_eden_dequantize", "dq_eden_dequantize_irht", "dq_eden_slice_bytes", "dq_eden_compress", "dq_eden_decompress", "dq_thc_compress", "dq_thc_compress_drawn", "dq_thc_decompress", "dq_thc_quantize", "dq_thc_dequantize", "dq_thc_rht_quantize", "dq_thc_dequantize_irht",
     "dq_grad_norm_work_doubles", "dq_grad_norm", "dq_adamw_step", "dq_adamw_coefficients",
-    "dq_mx4_quantize", "dq_mx4_dequantize", "dq_mx4_product",
+    "dq_mx4_quantize", "dq_mx4_quantize_list", "dq_mx4_dequantize", "dq_mx4_product",
 ]
 
 STAGE_STATS, STAGE_PLAN, STAGE_COMPRESS, STAGE_DECOMPRESS = 1, 2, 4, 8
@@ -59,6 +59,13 @@ class Bucket(ctypes.Structure):
 class Span(ctypes.Structure):
     """dq_span_t of include/dynamiq_eden.h"""
     _fields_ = [("data", ctypes.c_void_p), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class Mx4Matrix(ctypes.Structure):
+    """dq_mx4_matrix_t"""
+    _fields_ = [("x", ctypes.c_void_p), ("x_rows", ctypes.c_int64), ("x_cols", ctypes.c_int64), ("stride", ctypes.c_int64), ("sign", ctypes.c_void_p),
+                ("rand_pool", ctypes.c_void_p), ("seed", ctypes.c_uint64), ("step", ctypes.c_uint64), ("step_dev", ctypes.c_void_p), ("codes", ctypes.c_void_p),
+                ("scales", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("columns", ctypes.c_int32), ("stochastic", ctypes.c_int32), ("rand_dtype", ctypes.c_int32)]
 
 
 class AdamwTensor(ctypes.Structure):
@@ -212,6 +219,8 @@ def lib():
         L.dq_adamw_coefficients.argtypes = [vp, c.c_double, vp, c.c_double, c.c_double, c.c_double, vp, vp, i32, vp]
         L.dq_mx4_quantize.restype = i32
         L.dq_mx4_quantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i32, vp, i32, u64, u64, vp, vp, vp, i32, vp]
+        L.dq_mx4_quantize_list.restype = i32
+        L.dq_mx4_quantize_list.argtypes = [vp, i32, i32, vp]
         L.dq_mx4_dequantize.restype = i32
         L.dq_mx4_dequantize.argtypes = [vp, vp, vp, i32, i64, i64, i32, vp]
         L.dq_mx4_product.restype = i32

@@ -192,6 +192,17 @@ inline bool mx4_aligned(const void *codes, const void *scales)
 {
     return ((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 7)) == 0;
 }
+static int mx4_matrix_ok(const dq_mx4_matrix_t &m)
+{
+    if (!dtype_ok(m.dtype) || (m.rand_pool && !dtype_ok(m.rand_dtype))) return fail(DQ_ERR_DTYPE);
+    if (!mx4_size_ok(m.columns ? m.x_cols : m.x_rows, m.columns ? m.x_rows : m.x_cols)) return fail(DQ_ERR_SIZE, kMxSizes);
+    if (m.stride < m.x_cols || m.stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
+    if (m.rand_pool && !m.stochastic) return fail(DQ_ERR_SIZE, "a rand_pool is for stochastic rounding");
+    if (m.step_dev && (!m.stochastic || m.rand_pool)) return fail(DQ_ERR_SIZE, "step_dev is for the in-kernel random stream");
+    if (!m.x || !m.codes || !m.scales) return fail(DQ_ERR_NULL);
+    if (!mx4_aligned(m.codes, m.scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
+    return 0;
+}
 
 // the production shape: one fused-capable vectorised kernel family
 inline bool hier16_shape(int dtype, int chunk_size, int strategy)
@@ -1181,18 +1192,29 @@ int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, in
                     const void *rand_pool, int rand_dtype, uint64_t seed, uint64_t step, const uint64_t *step_dev, uint8_t *codes,
                     uint8_t *scales, int device, dq_stream_t stream)
 {
-    if (!dtype_ok(dtype) || (rand_pool && !dtype_ok(rand_dtype))) return fail(DQ_ERR_DTYPE);
-    if (!mx4_size_ok(columns ? x_cols : x_rows, columns ? x_rows : x_cols))
-        return fail(DQ_ERR_SIZE, kMxSizes);
-    if (stride < x_cols || stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
-    if (rand_pool && !stochastic) return fail(DQ_ERR_SIZE, "a rand_pool is for stochastic rounding");
-    if (step_dev && (!stochastic || rand_pool)) return fail(DQ_ERR_SIZE, "step_dev is for the in-kernel random stream");
-    if (!x || !codes || !scales) return fail(DQ_ERR_NULL);
-    if (!mx4_aligned(codes, scales)) return fail(DQ_ERR_SIZE, "codes must be 16-byte, scales 8-byte aligned");
+    const dq_mx4_matrix_t m = {x, x_rows, x_cols, stride, sign, rand_pool, seed, step, step_dev, codes, scales, dtype, columns, stochastic, rand_dtype};
+    return dq_mx4_quantize_list(&m, 1, device, stream);
+}
+
+int dq_mx4_quantize_list(const dq_mx4_matrix_t *matrices, int count, int device, dq_stream_t stream)
+{
+    if (count < 0) return fail(DQ_ERR_SIZE, "count must not be negative");
+    if (count && !matrices) return fail(DQ_ERR_NULL);
     int rc;
+    for (int k = 0; k < count; k++)
+        if ((rc = mx4_matrix_ok(matrices[k]))) return rc;
     if ((rc = select_device(device))) return rc;
-    const dq::QuantizeArgs a = {x, x_rows, x_cols, stride, codes, scales, sign, rand_pool, {seed, step}, step_dev};
-    return finish(dq::launch_mx4_quantize(a, dtype, columns != 0, stochastic != 0, rand_dtype, static_cast<hipStream_t>(stream)));
+    hipError_t e = hipSuccess;
+    for (int k = 0; k < count && e == hipSuccess; k += 16) {
+        dq::QuantizeOne list[16];
+        const int n = count - k < 16 ? count - k : 16;
+        for (int i = 0; i < n; i++) {
+            const dq_mx4_matrix_t &m = matrices[k + i];
+            list[i] = {{m.x, m.x_rows, m.x_cols, m.stride, m.codes, m.scales, m.sign, m.rand_pool, {m.seed, m.step}, m.step_dev}, m.dtype, m.rand_dtype, m.columns != 0, m.stochastic != 0};
+        }
+        e = dq::launch_mx4_quantize_list(list, n, static_cast<hipStream_t>(stream));
+    }
+    return finish(e);
 }
 
 int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows, int64_t cols, int device, dq_stream_t stream)

@@ -1309,31 +1309,49 @@ PyObject *mx4_product(PyObject *, PyObject *const *v, Py_ssize_t have)
 // ---- a linear layer in 4 bits, with its backward pass ----
 
 struct Quantized {
-    at::Tensor held;
     uint8_t *codes = nullptr, *scales = nullptr;
     int64_t rows = 0, length = 0;
 };
 
-// x: contiguous.  sign, pool: undefined for none; stochastic without a pool draws from (seed, step)
-Quantized quantized(const at::Tensor &x, bool columns, const at::Tensor &sign, const at::Tensor &pool, bool stochastic, uint64_t seed, uint64_t step, const at::Tensor &step_dev)
-{
-    Quantized q;
-    q.rows = x.size(columns ? 1 : 0);
-    q.length = x.size(columns ? 0 : 1);
-    const int64_t supers = (q.length + 255) / 256;
-    need(!sign.defined() || (sign.scalar_type() == at::kInt && sign.is_contiguous() && sign.device() == x.device() && sign.numel() >= 8 * supers),
-         "linear: signs are int32, eight per superchunk of the contraction");
-    need(!pool.defined() || (pool.is_contiguous() && pool.device() == x.device() && pool.numel() == q.rows * 256 * supers),
-         "linear: a rand_pool has one value per element of the quantised gradient, padding included");
-    q.held = at::empty({q.rows * 136 * supers}, at::TensorOptions().dtype(at::kByte).device(x.device()));
-    q.codes = static_cast<uint8_t *>(q.held.data_ptr());
-    q.scales = q.codes + q.rows * 128 * supers;
-    if (q.rows && q.length)
-        check(dq_mx4_quantize(x.data_ptr(), dtype_code(x), x.size(0), x.size(1), x.size(1), columns, sign.defined() ? reinterpret_cast<const uint32_t *>(sign.data_ptr<int32_t>()) : nullptr,
-                              stochastic, pool.defined() ? pool.data_ptr() : nullptr, pool.defined() ? dtype_code(pool) : 0, seed, step, step_dev.defined() ? step_counter(step_dev, x) : nullptr, q.codes, q.scales, x.device().index(),
-                              c10::hip::getCurrentHIPStream(x.device().index()).stream()));
-    return q;
-}
+// Matrices that are quantised together, in one piece of memory.
+struct Quantizer {
+    std::vector<dq_mx4_matrix_t> list;
+    std::vector<Quantized> made;
+    at::Tensor held;
+    int64_t bytes = 0;
+    // x: contiguous.  sign, pool: undefined for none; stochastic without a pool draws from (seed, step)
+    void add(const at::Tensor &x, bool columns, const at::Tensor &sign, const at::Tensor &pool, bool stochastic, uint64_t seed, uint64_t step, const at::Tensor &step_dev)
+    {
+        Quantized q;
+        q.rows = x.size(columns ? 1 : 0);
+        q.length = x.size(columns ? 0 : 1);
+        const int64_t supers = (q.length + 255) / 256;
+        need(!sign.defined() || (sign.scalar_type() == at::kInt && sign.is_contiguous() && sign.device() == x.device() && sign.numel() >= 8 * supers),
+             "linear: signs are int32, eight per superchunk of the contraction");
+        need(!pool.defined() || (pool.is_contiguous() && pool.device() == x.device() && pool.numel() == q.rows * 256 * supers),
+             "linear: a rand_pool has one value per element of the quantised gradient, padding included");
+        list.push_back({x.data_ptr(), x.size(0), x.size(1), x.size(1), sign.defined() ? reinterpret_cast<const uint32_t *>(sign.data_ptr<int32_t>()) : nullptr,
+                        pool.defined() ? pool.data_ptr() : nullptr, seed, step, step_dev.defined() ? step_counter(step_dev, x) : nullptr, nullptr, nullptr, dtype_code(x),
+                        columns, stochastic, pool.defined() ? dtype_code(pool) : 0});
+        made.push_back(q);
+        bytes += (q.rows * 136 * supers + 15) / 16 * 16;
+    }
+    void run(const c10::Device &device)
+    {
+        held = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(device));
+        uint8_t *at = static_cast<uint8_t *>(held.data_ptr());
+        size_t some = 0; // matrices with elements come first
+        for (size_t k = 0; k < list.size(); k++) {
+            Quantized &q = made[k];
+            const int64_t supers = (q.length + 255) / 256;
+            list[k].codes = q.codes = at;
+            list[k].scales = q.scales = at + q.rows * 128 * supers;
+            at += (q.rows * 136 * supers + 15) / 16 * 16;
+            if (q.rows && q.length) list[some++] = list[k];
+        }
+        if (some) check(dq_mx4_quantize_list(list.data(), (int)some, device.index(), c10::hip::getCurrentHIPStream(device.index()).stream()));
+    }
+};
 
 at::Tensor product_of(const Quantized &a, const Quantized &b, const at::Tensor &like)
 {
@@ -1361,7 +1379,11 @@ struct Linear4 : public torch::autograd::Function<Linear4> {
         ctx->saved_data["step"] = step;
         const c10::DeviceGuard on(x.device());
         const at::Tensor none;
-        return product_of(quantized(x, false, none, none, false, 0, 0, none), quantized(weight, false, none, none, false, 0, 0, none), x);
+        Quantizer q;
+        q.add(x, false, none, none, false, 0, 0, none);
+        q.add(weight, false, none, none, false, 0, 0, none);
+        q.run(x.device());
+        return product_of(q.made[0], q.made[1], x);
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
     {
@@ -1374,11 +1396,19 @@ struct Linear4 : public torch::autograd::Function<Linear4> {
         if (!grads[0].defined()) return out;
         const c10::DeviceGuard on(x.device());
         const at::Tensor dy = grads[0].contiguous();
-        if (ctx->needs_input_grad(0))
-            out[0] = product_of(quantized(dy, false, sign_out, pool_rows, seeded || pool_rows.defined(), seed, step, step_dev), quantized(weight, true, sign_out, none, false, 0, 0, none), x);
-        if (ctx->needs_input_grad(1))
-            out[1] = product_of(quantized(dy, true, sign_tokens, pool_columns, seeded || pool_columns.defined(), seed, step + kColumns, step_dev),
-                                quantized(x, true, sign_tokens, none, false, 0, 0, none), weight);
+        const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1);
+        Quantizer q;
+        if (dx) {
+            q.add(dy, false, sign_out, pool_rows, seeded || pool_rows.defined(), seed, step, step_dev);
+            q.add(weight, true, sign_out, none, false, 0, 0, none);
+        }
+        if (dw) {
+            q.add(dy, true, sign_tokens, pool_columns, seeded || pool_columns.defined(), seed, step + kColumns, step_dev);
+            q.add(x, true, sign_tokens, none, false, 0, 0, none);
+        }
+        q.run(x.device());
+        if (dx) out[0] = product_of(q.made[0], q.made[1], x);
+        if (dw) out[1] = product_of(q.made[dx ? 2 : 0], q.made[dx ? 3 : 1], weight);
         return out;
     }
 };

@@ -402,6 +402,13 @@ struct QuantizeArgs {
     const uint64_t *step_dev; // null, or a value in device memory that is added to the step of the random stream
 };
 hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, bool stochastic, int pool_dtype, hipStream_t stream);
+// one matrix of a list
+struct QuantizeOne {
+    QuantizeArgs a;
+    int dtype, pool_dtype;
+    bool columns, stochastic;
+};
+hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStream_t stream);
 hipError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int64_t rows, int64_t cols, int dtype,
                                  hipStream_t stream);
 hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out,

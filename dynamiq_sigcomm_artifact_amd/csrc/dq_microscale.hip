@@ -10,6 +10,7 @@ namespace dq {
 // n / by for n below 2^27: (n mul) >> shift with mul = ceil(2^shift / by) and shift = 27 + ceil(log2 by), whose excess is less than n 2^-shift
 struct Division {
     uint32_t by, mul, shift;
+    Division() = default;
     explicit Division(uint32_t by_) : by(by_), shift(27)
     {
         while (((uint64_t)1 << (shift - 27)) < by) shift++;
@@ -108,13 +109,10 @@ template <int RAND, bool ROTATE> __device__ __forceinline__ uint32_t encode_bloc
 
 // ---- along the rows ----------------------------------------------------------------------------------------
 
-// Bound by memory: 14336 x 4096 bf16 to the nearest in 28 us (5.3 TB/s), rotated and stochastic with a bf16 pool 4096 x 14336 in 56 (4.8 TB/s).  With the random stream made in
-// the kernel it is the arithmetic of the stream.
-template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void mx4_rows_kernel(QuantizeArgs a, Division superchunks, uint32_t units)
+// unit: eight elements of the result, padding included
+template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void quantize_rows(const QuantizeArgs &a, const Division &superchunks, uint32_t unit)
 {
     const int g = threadIdx.x & 3;
-    const uint32_t unit = blockIdx.x * 256 + threadIdx.x; // eight elements of the result, padding included
-    if (unit >= units) return;
     const uint32_t row = superchunks(unit >> 5), col = (unit - row * superchunks.by * 32) * 8;
     float v[8], u[8];
     const int64_t at = (int64_t)row * a.stride + col;
@@ -129,6 +127,14 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
     if (g == 0) a.scales[unit >> 2] = (uint8_t)scale;
 }
 
+// Bound by memory: 14336 x 4096 bf16 to the nearest in 28 us (5.3 TB/s), rotated and stochastic with a bf16 pool 4096 x 14336 in 56 (4.8 TB/s).  With the random stream made in
+// the kernel it is the arithmetic of the stream.
+template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void mx4_rows_kernel(QuantizeArgs a, Division superchunks, uint32_t units)
+{
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
+    if (unit < units) quantize_rows<DT, RAND, ROTATE>(a, superchunks, unit);
+}
+
 // ---- along the columns -------------------------------------------------------------------------------------
 
 // A workgroup takes 256 rows x 128 columns: one superchunk of 128 rows of the result.  A wave takes 32 of the rows, a lane 8 rows x 8 columns, and a
@@ -136,12 +142,16 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 // workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 121 us (4.4 TB/s; 130
 // with the XCDs' workgroups strewn, 8000 x 5000 35 for 40), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
 // instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.
-template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
+struct ColumnsLds {
+    __attribute__((aligned(16))) uint8_t tile[128 * 128];
+    __attribute__((aligned(8))) uint8_t scales[128 * 8];
+};
+template <int DT, int RAND, bool ROTATE>
+__device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t superchunks, const Division &tiles, uint32_t id, ColumnsLds &lds)
 {
-    __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
-    __shared__ __attribute__((aligned(8))) uint8_t tile_scales[128 * 8];
+    uint8_t *tile = lds.tile, *tile_scales = lds.scales;
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
-    const uint32_t id = unit_of(blockIdx.x, gridDim.x), superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
+    const uint32_t superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
     const uint32_t row0 = superchunk * 256 + 32 * block, row = row0 + 8 * g;
     constexpr int WORDS = DT == DQ_F32 ? 8 : 4;
     uint32_t x[8][WORDS]; // [row][column], as they are in memory
@@ -202,6 +212,13 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(512, DT ==
         reinterpret_cast<uint2 *>(a.scales)[(int64_t)(col0 + threadIdx.x) * superchunks + superchunk] = reinterpret_cast<const uint2 *>(tile_scales)[threadIdx.x];
 }
 
+template <int DT, int RAND, bool ROTATE>
+__global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
+{
+    __shared__ ColumnsLds lds;
+    quantize_columns<DT, RAND, ROTATE>(a, superchunks, tiles, unit_of(blockIdx.x, gridDim.x), lds);
+}
+
 template <int DT, int RAND> static hipError_t launch_quantize(const QuantizeArgs &a, bool columns, hipStream_t stream)
 {
     const uint32_t superchunks = (uint32_t)(((columns ? a.rows : a.cols) + 255) >> 8);
@@ -236,6 +253,95 @@ hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, b
     return dtype == DQ_F32 ? launch_quantize_of<DQ_F32>(a, columns, stochastic, pool_dtype, stream)
          : dtype == DQ_BF16 ? launch_quantize_of<DQ_BF16>(a, columns, stochastic, pool_dtype, stream)
                             : launch_quantize_of<DQ_F16>(a, columns, stochastic, pool_dtype, stream);
+}
+
+// ---- several small matrices at once -------------------------------------------------------------------------
+
+// Up to four matrices of one element type, along either axis and rounded in any way: a workgroup takes 4096 elements along the rows or a tile along the columns.  A small
+// one leaves most CUs without work and costs a launch all the same: a linear layer's step of 333 x 776 x 1000, in a graph, takes 30 us with two such launches where six
+// quantisers of their own made it 46, of 2048 x 2048 x 2048 54 for 66, of 4096 x 4096 x 4096 176 for 193.  Beyond 4096 workgroups they go alone, in kernels that hold less:
+// 4096 x 14336 x 4096 523 us, together 533.
+struct QuantizeJob {
+    QuantizeArgs a;
+    Division by; // superchunks of a row, or tiles of 128 columns
+    uint32_t superchunks, units, first; // first: of its workgroups
+    int32_t kind;
+};
+constexpr int kJobs = 4, kJobBlocks = 4096;
+struct QuantizeJobs {
+    QuantizeJob job[kJobs];
+};
+
+template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void do_job(const QuantizeJob &j, bool columns, uint32_t id, ColumnsLds &lds)
+{
+    if (columns)
+        quantize_columns<DT, RAND, ROTATE>(j.a, j.superchunks, j.by, id, lds);
+    else if (id * 512 + threadIdx.x < j.units)
+        quantize_rows<DT, RAND, ROTATE>(j.a, j.by, id * 512 + threadIdx.x);
+}
+
+template <int DT> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_jobs_kernel(QuantizeJobs jobs)
+{
+    __shared__ ColumnsLds lds;
+    int k = 0;
+#pragma unroll
+    for (int i = 1; i < kJobs; i++) k += blockIdx.x >= jobs.job[i].first ? 1 : 0;
+    const QuantizeJob j = jobs.job[k];
+    const uint32_t id = blockIdx.x - j.first;
+    const bool columns = j.kind & 16;
+    switch (j.kind & 15) {
+    case 0: return do_job<DT, kNearest, false>(j, columns, id, lds);
+    case 1: return do_job<DT, kNearest, true>(j, columns, id, lds);
+    case 2: return do_job<DT, kPhilox, false>(j, columns, id, lds);
+    case 3: return do_job<DT, kPhilox, true>(j, columns, id, lds);
+    case 4: return do_job<DT, DQ_F16, false>(j, columns, id, lds);
+    case 5: return do_job<DT, DQ_F16, true>(j, columns, id, lds);
+    case 6: return do_job<DT, DQ_BF16, false>(j, columns, id, lds);
+    case 7: return do_job<DT, DQ_BF16, true>(j, columns, id, lds);
+    case 8: return do_job<DT, DQ_F32, false>(j, columns, id, lds);
+    default: return do_job<DT, DQ_F32, true>(j, columns, id, lds);
+    }
+}
+
+hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStream_t stream)
+{
+    const auto blocks_of = [](const QuantizeOne &q) {
+        return q.columns ? ((q.a.cols + 127) >> 7) * ((q.a.rows + 255) >> 8) : (q.a.rows * ((q.a.cols + 255) >> 8) + 15) >> 4;
+    };
+    for (int next = 0; next < count;) {
+        int take = 0;
+        int64_t blocks = 0;
+        while (take < kJobs && next + take < count && list[next + take].dtype == list[next].dtype && blocks + blocks_of(list[next + take]) <= kJobBlocks)
+            blocks += blocks_of(list[next + take++]);
+        hipError_t e;
+        if (take < 2) {
+            const QuantizeOne &q = list[next++];
+            e = launch_mx4_quantize(q.a, q.dtype, q.columns, q.stochastic, q.pool_dtype, stream);
+        } else {
+            QuantizeJobs jobs = {};
+            uint32_t first = 0;
+            for (int k = 0; k < kJobs; k++) {
+                QuantizeJob &j = jobs.job[k];
+                j.first = k < take ? first : 0xffffffffu;
+                j.by = Division(1);
+                if (k >= take) continue;
+                const QuantizeOne &q = list[next + k];
+                j.a = q.a;
+                j.superchunks = (uint32_t)(((q.columns ? q.a.rows : q.a.cols) + 255) >> 8);
+                j.by = Division(q.columns ? (uint32_t)((q.a.cols + 127) >> 7) : j.superchunks);
+                j.units = (uint32_t)(q.a.rows * j.superchunks * 32);
+                j.kind = (q.columns ? 16 : 0) + (!q.stochastic ? 0 : !q.a.pool ? 2 : 4 + 2 * q.pool_dtype) + (q.a.sign ? 1 : 0);
+                first += (uint32_t)blocks_of(q);
+            }
+            const dim3 grid((uint32_t)blocks), block(512);
+            e = list[next].dtype == DQ_F32 ? launch_with(mx4_jobs_kernel<DQ_F32>, grid, block, stream, jobs)
+              : list[next].dtype == DQ_BF16 ? launch_with(mx4_jobs_kernel<DQ_BF16>, grid, block, stream, jobs)
+                                            : launch_with(mx4_jobs_kernel<DQ_F16>, grid, block, stream, jobs);
+            next += take;
+        }
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // ---- and back ----------------------------------------------------------------------------------------------

@@ -835,6 +835,19 @@ int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, in
                     const uint32_t *sign, int stochastic, const void *rand_pool, int rand_dtype, uint64_t seed,
                     uint64_t step, const uint64_t *step_dev, uint8_t *codes, uint8_t *scales, int device,
                     dq_stream_t stream);
+/* The same for a list of matrices, which small ones need fewer launches for (up to four
+ * neighbours of one element type share one). */
+typedef struct dq_mx4_matrix {
+    const void *x;
+    int64_t x_rows, x_cols, stride;
+    const uint32_t *sign;
+    const void *rand_pool;
+    uint64_t seed, step;
+    const uint64_t *step_dev;
+    uint8_t *codes, *scales;
+    int32_t dtype, columns, stochastic, rand_dtype;
+} dq_mx4_matrix_t;
+int dq_mx4_quantize_list(const dq_mx4_matrix_t *matrices, int count, int device, dq_stream_t stream);
 /* out: `dtype` [rows][cols], the values rounded to nearest */
 int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, int dtype, int64_t rows,
                       int64_t cols, int device, dq_stream_t stream);

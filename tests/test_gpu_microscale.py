@@ -433,3 +433,31 @@ def test_step_on_the_device(ms):
             ms.linear(x, w, seed=1, step=bad)
         with pytest.raises(RuntimeError):
             ms.quantize(dy, seed=1, step=bad)
+
+
+def test_list_is_one_after_the_other(ms, capi):
+    """every kind of matrix in a list, in runs of one type and alternating, too large to share a launch, and the same matrix twice"""
+    kinds = [(rows, columns, rotate, source) for rows in ((70, 300), (257, 513)) for columns in (False, True) for rotate in (False, True)
+             for source in (None, "philox", FP, BF, HF)]
+    entries = [(matrix(*kinds[k][0], dtype, k),) + kinds[k][1:] for dtype in (BF, FP, HF) for k in range(len(kinds))]
+    entries += [(matrix(9000, 2100, BF, 1), True, False, None), (matrix(30000, 2100, HF, 2), False, False, None), (matrix(50, 40, HF, 3), False, False, None)]
+    entries += [entries[0], entries[-1], entries[0], entries[7], entries[50], entries[3], entries[90]]
+    step = torch.tensor([5], device=DEV)
+    jobs, wants, held = [], [], []
+    codes = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    for k, (x, columns, rotate, source) in enumerate(entries):
+        rows, length = (x.shape[1], x.shape[0]) if columns else x.shape
+        sign = signs(capi, length, k)[0] if rotate else None
+        drawn = pool(rows, length, source, k) if source not in (None, "philox") else None
+        want = ms.quantize(x, columns, sign, drawn, **(dict(seed=k, step=5 + k) if source == "philox" else {}))
+        out = torch.full_like(want.codes, 77), torch.full_like(want.scales, 77)
+        jobs.append(capi.Mx4Matrix(x.data_ptr(), x.shape[0], x.shape[1], x.shape[1], None if sign is None else sign.data_ptr(), None if drawn is None else drawn.data_ptr(), k, k,
+                                   step.data_ptr() if source == "philox" else None, out[0].data_ptr(), out[1].data_ptr(), codes[x.dtype], int(columns),
+                                   int(source is not None), 0 if drawn is None else codes[drawn.dtype]))
+        wants.append((want, out))
+        held.append((x, sign, drawn))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert capi.lib().dq_mx4_quantize_list((capi.Mx4Matrix * len(jobs))(*jobs), len(jobs), 0, stream) == 0
+    for k, (want, out) in enumerate(wants):
+        assert torch.equal(out[0], want.codes) and torch.equal(out[1], want.scales), (k, entries[k][1:], entries[k][0].shape)
+    assert capi.lib().dq_mx4_quantize_list(None, 0, 0, stream) == 0

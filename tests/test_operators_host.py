@@ -80,6 +80,13 @@ def test_matrices_refuse(L):
                      (dict(r=(1 << 27) - 15, c=256), "2^35"), (dict(r=1 << 31, c=1, columns=1), "2^31"), (dict(r=1, c=1 << 31, stride=1 << 31), "2^31"), (dict(stride=299), "stride"), (dict(pool=P), "stochastic"), (dict(counter=P), "step_dev"), (dict(counter=P, pool=P, stochastic=1), "step_dev"),
                      (dict(x=N), "null"), (dict(codes=N), "null"), (dict(scales=N), "null"), (dict(codes=odd), "aligned"), (dict(scales=four), "aligned")):
         refused(L, quantize(**kw), text)
+    from dynamiq_sigcomm_artifact_amd.capi import Mx4Matrix
+    good = dict(x=0x1000, x_rows=10, x_cols=300, stride=300, codes=0x1000, scales=0x1000, dtype=1)
+    for kw, text in ((dict(dtype=5), "dtype"), (dict(x_rows=0), "positive"), (dict(stride=299), "stride"), (dict(rand_pool=0x1000), "stochastic"), (dict(codes=0x1008), "aligned"),
+                     (dict(x=None), "null")):
+        refused(L, L.dq_mx4_quantize_list((Mx4Matrix * 2)(Mx4Matrix(**good), Mx4Matrix(**{**good, **kw})), 2, 0, S), text)
+    refused(L, L.dq_mx4_quantize_list(None, 1, 0, S), "null")
+    refused(L, L.dq_mx4_quantize_list(None, -1, 0, S), "count")
     refused(L, L.dq_mx4_dequantize(P, P, P, 9, 1, 1, 0, S), "dtype")
     refused(L, L.dq_mx4_dequantize(P, P, P, 1, 1, 0, 0, S), "positive")
     refused(L, L.dq_mx4_dequantize(P, P, N, 1, 1, 1, 0, S), "null")
