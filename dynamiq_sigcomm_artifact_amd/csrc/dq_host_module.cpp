@@ -1441,6 +1441,19 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
         }
         const int64_t step = THPVariable_Check(v[7]) ? 0 : (int64_t)word(v[7], true);
         const int64_t k = weight.size(1), n = weight.size(0), tokens = k ? x.numel() / k : x.numel() == 0 && x.dim() > 1 ? c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)) : 1;
+        // The engine hands a leaf's gradient to the stream that the leaf's node was made on.  One made by an eager pass whose graph still lives draws that stream into a
+        // recording, which ends badly there; so it is refused here.
+        if (at::GradMode::is_enabled()) {
+            const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(x.device().index());
+            unsigned long long recording;
+            if (Buckets::capturing(now.stream(), &recording))
+                for (const at::Tensor *t : {&x, &weight}) {
+                    if (!t->requires_grad() || !t->is_leaf()) continue;
+                    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(*t);
+                    const std::optional<c10::Stream> of = node ? node->stream() : std::nullopt;
+                    need(!of || of->id() == now.id(), "linear: an earlier graph of the same leaf, made on another stream, is still alive: let go of its outputs before recording");
+                }
+        }
         // (a matrix that is contiguous takes part as it is: views of it would be nodes of the graph)
         const at::Tensor flat = x.dim() == 2 && x.is_contiguous() ? x : x.reshape({tokens, k}).contiguous();
         at::Tensor y = Linear4::apply(flat, weight.is_contiguous() ? weight : weight.contiguous(), extra[0], extra[1], extra[2], extra[3], step_dev, seeded, seed, step);

@@ -461,3 +461,27 @@ def test_list_is_one_after_the_other(ms, capi):
     for k, (want, out) in enumerate(wants):
         assert torch.equal(out[0], want.codes) and torch.equal(out[1], want.scales), (k, entries[k][1:], entries[k][0].shape)
     assert capi.lib().dq_mx4_quantize_list(None, 0, 0, stream) == 0
+
+
+def test_recording_beside_a_living_graph_is_refused(ms):
+    x, w, dy = matrix(40, 96, BF, 1, 1.0).requires_grad_(), matrix(50, 96, BF, 2, 1.0).requires_grad_(), matrix(40, 50, BF, 3, 1.0)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def record():
+        with torch.cuda.graph(graph, stream=side):
+            return torch.autograd.grad(ms.linear(x, w, seed=1, step=2), (x, w), dy)
+    alive = ms.linear(x, w)
+    with pytest.raises(RuntimeError, match="still alive"):
+        record()
+    torch.cuda.synchronize()
+    with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+        ms.linear(x, w)                                     # no backward pass, nothing to refuse
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    got = record()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.autograd.grad(ms.linear(x, w, seed=1, step=2), (x, w), dy)
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
+        del want
