@@ -11,7 +11,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct ProductArgs {
     const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
     void *out;
-    int64_t m, n;
+    int64_t m, n, out_pitch;
     int superchunks;
     uint32_t tiles_n;
 };
@@ -349,7 +349,7 @@ template <int DT, int T> __global__ __launch_bounds__(256, T == 256 ? 1 : 2) voi
             const int64_t i = i0 + (wave >> 1) * (T / 2) + 32 * f + r;
             const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * kApart + lane % kLanes * 16);
             if (i < p.m) {
-                Elem *to = static_cast<Elem *>(p.out) + i * p.n + col0;
+                Elem *to = static_cast<Elem *>(p.out) + i * p.out_pitch + col0;
                 if (col0 + kPer <= p.n) {
                     const u32x4_any w = {v.x, v.y, v.z, v.w};
                     *reinterpret_cast<u32x4_any *>(to) = w;
@@ -380,6 +380,11 @@ template <int DT, int T> static hipError_t launch_tiles(ProductArgs p, hipStream
     return launch_with(mx4_tile_kernel<DT, T>, dim3((uint32_t)((p.m + T - 1) / T) * p.tiles_n), dim3(256), stream, p);
 }
 
+template <int T> static hipError_t launch_tiles_of(const ProductArgs &p, int dtype, hipStream_t stream)
+{
+    return dtype == DQ_F32 ? launch_tiles<DQ_F32, T>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, T>(p, stream) : launch_tiles<DQ_F16, T>(p, stream);
+}
+
 // Which kernel.  Two tiles of 128 x 128 share a CU, and 512 of them run at a time; tiles of 256 x 256 fetch half as much per product, but one takes a CU.  Where 512
 // suffice they are the faster (2048 x 4096 x 4096, 512 tiles: 24.0 us, tiles of 256: 29.7), and slower beyond (2304 x 4096 x 4096, 576 tiles: 34.3 and 29.1 us).
 // Below 40 tiles of 128 the contraction is shared out among the waves of a workgroup instead (256 x 3000 x 4096, 48 tiles: 12.6 us, shared out 20.2; 128 x 4096 x 4096,
@@ -398,12 +403,38 @@ template <int MF, int NF, int U> static bool try_narrow(const ProductArgs &p, bo
 hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out, int64_t m,
                               int64_t n, int64_t k, int dtype, hipStream_t stream)
 {
-    const ProductArgs p = {a_codes, a_scales, b_codes, b_scales, out, m, n, (int)((k + 255) >> 8), 0};
+    const ProductArgs p = {a_codes, a_scales, b_codes, b_scales, out, m, n, n, (int)((k + 255) >> 8), 0};
     const auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    if (m > 64 && n > 64 && tiles(128) > 512)
-        return dtype == DQ_F32 ? launch_tiles<DQ_F32, 256>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 256>(p, stream) : launch_tiles<DQ_F16, 256>(p, stream);
+    if (m > 64 && n > 64 && tiles(128) > 512) {
+        // A last round of tiles of 256 in which less than half of the CUs have work takes as long as a full one; the same in tiles of 128, two to a CU, two thirds of
+        // that.  So the longer side is cut where whole rounds end, and the rest is a launch of its own (3000 x 6000 x 4096, 288 tiles: 51 us instead of 62; 4352 x 4352 x 8192,
+        // 289: 87 for 100; with half a round left, 4096 x 14336 x 4096, 138 for 140).  Short contractions do not make up for the launch.
+        const bool along_n = n >= m;
+        const int64_t side = ((along_n ? n : m) + 255) / 256, across = ((along_n ? m : n) + 255) / 256, whole = side * across / 256 * 256 / across;
+        if (p.superchunks >= 8 && whole > 0 && (side - whole) * across <= 128 && whole < side) {
+            ProductArgs first = p, rest = p;
+            const int64_t cut = whole * 256;
+            const int64_t row = (int64_t)p.superchunks;
+            if (along_n) {
+                first.n = cut;
+                rest.n = n - cut;
+                rest.b_codes += cut * row * 128;
+                rest.b_scales += cut * row * 8;
+                rest.out = static_cast<char *>(out) + cut * (dtype == DQ_F32 ? 4 : 2);
+            } else {
+                first.m = cut;
+                rest.m = m - cut;
+                rest.a_codes += cut * row * 128;
+                rest.a_scales += cut * row * 8;
+                rest.out = static_cast<char *>(out) + cut * n * (dtype == DQ_F32 ? 4 : 2);
+            }
+            const hipError_t e = launch_tiles_of<256>(first, dtype, stream);
+            return e != hipSuccess ? e : launch_tiles_of<128>(rest, dtype, stream);
+        }
+        return launch_tiles_of<256>(p, dtype, stream);
+    }
     if (m > 64 && n > 64 && tiles(128) >= (p.superchunks < 4 ? 96 : 40))
-        return dtype == DQ_F32 ? launch_tiles<DQ_F32, 128>(p, stream) : dtype == DQ_BF16 ? launch_tiles<DQ_BF16, 128>(p, stream) : launch_tiles<DQ_F16, 128>(p, stream);
+        return launch_tiles_of<128>(p, dtype, stream);
     hipError_t e = hipSuccess;
     (void)(try_narrow<4, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 4, 1>(p, false, dtype, stream, e) || try_narrow<2, 2, 1>(p, false, dtype, stream, e) ||
            try_narrow<1, 4, 1>(p, false, dtype, stream, e) || try_narrow<1, 2, 2>(p, false, dtype, stream, e) || try_narrow<1, 1, 2>(p, true, dtype, stream, e));

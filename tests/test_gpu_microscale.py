@@ -202,7 +202,9 @@ PRODUCTS = [(1, 1, 1), (1, 16, 256), (1, 1000, 4096), (2, 33, 31), (3, 17, 4000)
             (1, 12400, 300), (8, 6200, 520), (9, 3100, 300), (1300, 1281, 900), (2000, 2049, 513), (4097, 3300, 256), (4100, 3200, 1025), (2049, 7000, 100),
             # scales come for four superchunks at a time, and of odd numbers of them the last row's end early: one to nine of them, in tiles of 128 and of 256
             (700, 900, 200), (701, 899, 700), (702, 898, 1100), (703, 897, 1281), (640, 1000, 1793), (641, 1001, 2049), (2900, 3000, 250), (2901, 2999, 512), (2817, 3001, 600),
-            (2818, 2990, 1280), (2819, 3011, 1537)]
+            (2818, 2990, 1280), (2819, 3011, 1537),
+            # a last round that is cut, along either side
+            (4100, 4200, 2049), (4400, 4090, 1900)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
