@@ -128,3 +128,30 @@ def test_command(lib):
         evaluate._emit = emit
     assert [v["training_step"] for v in lines] == ["run", "layers", "encode", "clip", "update", "step"]
     assert math.isfinite(lines[0]["loss_last"]) and all(v["us"] > 0 for v in lines[1:])
+
+
+def test_threads_on_their_own_streams(lib):
+    """models that step at once, a thread and a stream each, come out as one after the other"""
+    import threading
+
+    def run(k, steps, out):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            m = Model(lib, (32, 8)[k % 2], False)
+            m.x.add_(k)
+            for _ in range(steps):
+                m.step()
+            m.pipe.join()
+            stream.synchronize()
+            out[k] = [v.detach().clone() for v in m.weights] + [m.norm.clone()]
+            stream.synchronize()
+    alone, together = {}, {}
+    for k in range(4):
+        run(k, 12, alone)
+    threads = [threading.Thread(target=run, args=(k, 12, together)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(4):
+        assert all(torch.equal(v, w) for v, w in zip(alone[k], together[k])), k
