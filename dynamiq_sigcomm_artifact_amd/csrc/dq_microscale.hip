@@ -71,13 +71,14 @@ template <int RAND> __device__ __forceinline__ void uniform8(const QuantizeArgs 
 
 // eight codes in a word, the first in the lowest bits, and the block's scale byte (the same in the quad's lanes).  ROTATE: of v / sqrt(32), with one product for an
 // element where there would be two.  (Finite sums are below 2^128, so that down is at least 2^-123 and its product with 1 / sqrt(32) a normal number.)
-template <int RAND, bool ROTATE> __device__ __forceinline__ uint32_t encode_block(const float (&v)[8], const float (&u)[8], uint32_t &scale)
+template <int RAND, bool ROTATE, uint32_t LIFT = 0> __device__ __forceinline__ uint32_t encode_block(const float (&v)[8], const float (&u)[8], uint32_t &scale)
 {
     constexpr float kUnit = ROTATE ? 0.17677669529663687f : 1.0f;
     uint32_t largest = block_max(v);
     if (ROTATE) largest = __float_as_uint(__uint_as_float(largest) * kUnit);
     scale = RAND == kNearest ? block_scale<2, 0x7fffffu>(largest) : block_scale<2, 0x400000u>(largest);
     const float down = scale_down(scale) * kUnit;
+    if (LIFT) scale = min(scale + LIFT, 255u); // (255 where it was, and beyond the largest scale)
     uint32_t word = 0;
     if constexpr (RAND == kNearest) {
         word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0] * down, v[1] * down, 1.0f, 0);
@@ -107,6 +108,16 @@ template <int RAND, bool ROTATE> __device__ __forceinline__ uint32_t encode_bloc
     return word;
 }
 
+// Sums of 32 elements from 2^123 on may pass 2^128, and nothing of their block is finite then.  So a rotated block whose scale has become 255 is taken once more, 2^-6 of it, with its
+// scale raised by 6: v are its elements as they were.  It is 255 still if it holds an infinity or NaN, or is beyond the largest scale.  (Half precision never gets there.)
+template <int RAND> __device__ __forceinline__ uint32_t encode_lowered(float (&v)[8], const float (&u)[8], uint32_t sign, int g, uint32_t &scale)
+{
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] *= 0x1p-6f;
+    rotate_block(v, sign, g);
+    return encode_block<RAND, true, 6>(v, u, scale);
+}
+
 // ---- along the rows ----------------------------------------------------------------------------------------
 
 // unit: eight elements of the result, padding included
@@ -116,15 +127,28 @@ template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void quantiz
     const uint32_t row = superchunks(unit >> 5), col = (unit - row * superchunks.by * 32) * 8;
     float v[8], u[8];
     const int64_t at = (int64_t)row * a.stride + col;
-    if (col + 8 <= (uint32_t)a.cols)
-        load8<DT>(a.x, at, v);
-    else
-        load_part<DT, 8>(a.x, at, row * a.stride + a.cols, v);
+    const auto load = [&] {
+        if (col + 8 <= (uint32_t)a.cols)
+            load8<DT>(a.x, at, v);
+        else
+            load_part<DT, 8>(a.x, at, row * a.stride + a.cols, v);
+    };
+    const uint32_t sign = ROTATE ? a.sign[col >> 5] : 0u;
+    load();
     uniform8<RAND>(a, (int64_t)unit * 8, u);
-    if (ROTATE) rotate_block(v, a.sign[col >> 5], g);
+    if (ROTATE) rotate_block(v, sign, g);
+    const auto put = [&](uint32_t word, uint32_t scale) {
+        reinterpret_cast<uint32_t *>(a.codes)[unit] = word;
+        if (g == 0) a.scales[unit >> 2] = (uint8_t)scale;
+    };
     uint32_t scale;
-    reinterpret_cast<uint32_t *>(a.codes)[unit] = encode_block<RAND, ROTATE>(v, u, scale);
-    if (g == 0) a.scales[unit >> 2] = (uint8_t)scale;
+    const uint32_t word = encode_block<RAND, ROTATE>(v, u, scale);
+    put(word, scale);
+    if (ROTATE && DT != DQ_F16 && DQ_UNLIKELY(scale == 255u)) { // (in all four lanes of a block)
+        load();
+        const uint32_t again = encode_lowered<RAND>(v, u, sign, g, scale);
+        put(again, scale);
+    }
 }
 
 // Bound by memory: 14336 x 4096 bf16 to the nearest in 28 us (5.3 TB/s), rotated and stochastic with a bf16 pool 4096 x 14336 in 56 (4.8 TB/s).  With the random stream made in
@@ -141,7 +165,8 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 // column's block lies in a quad as it does above.  The codes leave through LDS, as whole lines.  Elements of 16 bits stay packed until their column's turn: three
 // workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 121 us (4.4 TB/s; 130
 // with the XCDs' workgroups strewn, 8000 x 5000 35 for 40), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
-// instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.
+// instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.  Blocks that have to be lowered are looked for while their columns
+// are encoded and taken behind the loop, where nothing else needs registers (in it: 2 to 6 % for every matrix); to the nearest four workgroups share a CU, which 65 registers would not let them.
 struct ColumnsLds {
     __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __attribute__((aligned(8))) uint8_t scales[128 * 8];
@@ -186,19 +211,48 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
             }
     }
     const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u, first = col * superchunks + superchunk, most = (all_cols - 1) * superchunks + superchunk;
+    // (what becomes of columns past the end is not stored)
+    const auto draw = [&](int c, float (&u)[8]) { uniform8<RAND>(a, (int64_t)min(first + c * superchunks, most) * 256 + 32 * block + 8 * g, u); };
+    const auto put = [&](int c, uint32_t word, uint32_t scale) {
+        const int line = 8 * (lane >> 2) + c;
+        *reinterpret_cast<uint32_t *>(tile + line * 128 + ((block ^ (line >> 3 & 7)) << 4) + 4 * g) = word;
+        if (g == 0) tile_scales[line * 8 + block] = (uint8_t)scale;
+    };
+    bool beyond = false;
 #pragma unroll
     for (int c = 0; c < 8; c++) {
         float v[8], u[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = word_value<DT>(x[j], c);
-        // (what becomes of columns past the end is not stored)
-        uniform8<RAND>(a, (int64_t)min(first + c * superchunks, most) * 256 + 32 * block + 8 * g, u);
+        draw(c, u);
         if (ROTATE) rotate_block(v, sign, g);
         uint32_t scale;
         const uint32_t word = encode_block<RAND, ROTATE>(v, u, scale);
-        const int line = 8 * (lane >> 2) + c;
-        *reinterpret_cast<uint32_t *>(tile + line * 128 + ((block ^ (line >> 3 & 7)) << 4) + 4 * g) = word;
-        if (g == 0) tile_scales[line * 8 + block] = (uint8_t)scale;
+        put(c, word, scale);
+        beyond |= scale == 255u;
+    }
+    if (ROTATE && DT != DQ_F16 && DQ_UNLIKELY(__builtin_amdgcn_ballot_w64(beyond) != 0)) {
+#pragma unroll 1
+        for (int c = 0; c < 8; c++) { // what nobody holds any more, element by element
+            float v[8], u[8];
+            uint32_t scale;
+            const auto load = [&] {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    v[j] = ElemIO<DT>::load(a.x, (int64_t)min(row + j, last_row) * a.stride + min(col + c, all_cols - 1));
+                    if (row + j > last_row) v[j] = 0.0f;
+                }
+            };
+            load();
+            draw(c, u);
+            rotate_block(v, sign, g);
+            (void)encode_block<RAND, true>(v, u, scale);
+            if (scale == 255u) {
+                load();
+                const uint32_t word = encode_lowered<RAND>(v, u, sign, g, scale);
+                put(c, word, scale);
+            }
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -213,7 +267,7 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
 }
 
 template <int DT, int RAND, bool ROTATE>
-__global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
+__global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : RAND == kNearest && ROTATE ? 8 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
 {
     __shared__ ColumnsLds lds;
     quantize_columns<DT, RAND, ROTATE>(a, superchunks, tiles, unit_of(blockIdx.x, gridDim.x), lds);

@@ -830,7 +830,8 @@ int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double
  * with rand_pool = NULL the in-kernel stream of dq_scaling_compress_philox, keyed by
  * (seed, step, chunk of 16 elements of that layout).  step_dev (may be NULL): one uint64
  * in device memory that is added to step, so that a recorded call draws anew.
- * A block that holds an infinity or NaN is NaN. */
+ * A block that holds an infinity or NaN is NaN, and so is one whose rotation is beyond
+ * what the largest scale, 2^127, holds (its elements alone never are). */
 int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, int64_t stride, int columns,
                     const uint32_t *sign, int stochastic, const void *rand_pool, int rand_dtype, uint64_t seed,
                     uint64_t step, const uint64_t *step_dev, uint8_t *codes, uint8_t *scales, int device,

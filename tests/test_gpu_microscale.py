@@ -487,3 +487,53 @@ def test_recording_beside_a_living_graph_is_refused(ms):
         want = torch.autograd.grad(ms.linear(x, w, seed=1, step=2), (x, w), dy)
         assert all(torch.equal(s, t) for s, t in zip(got, want))
         del want
+
+
+# ---- what lies at the ends of a rotation, of a draw and of the layer's arguments ----
+
+@pytest.mark.parametrize("columns", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP], ids=str)
+@pytest.mark.parametrize("rounding", ["nearest", "pool", "philox"])
+def test_rotation_of_the_largest_numbers(ms, capi, columns, dtype, rounding):
+    """a power of two in front of a matrix is one in its scales, also where the sums of 32 pass binary32's range; only beyond the largest scale is a block NaN"""
+    top = 1.9921875 * 2.0 ** 9                            # the largest number of bf16, over 2^118
+    x = matrix(70, 300, dtype, 5, spread=1.0).clamp(-top, top)
+    x[:, 64:96] *= 2.0 ** -3
+    x[:8] = torch.where(x[:8] < 0, -top, top).to(dtype)
+    x[32:64, 128:160] = 0
+    x[64:, 0:2] = 0
+    rows, n = (300, 70) if columns else (70, 300)
+    bits, s = signs(capi, n, 4)
+    at = x.t() if columns else x
+    at[0, :64] = torch.from_numpy(s[:64]).to(DEV).to(dtype) * top                             # 32 top / sqrt(32) is above 2^130 over 2^118: more than the largest scale holds
+    at[1, :32] = torch.from_numpy(s[:32]).to(DEV).to(dtype) * 2.0 ** 9
+    kw = dict(rand_pool=pool(rows, n, BF)) if rounding == "pool" else dict(seed=3, step=4) if rounding == "philox" else {}
+    small, far = ms.quantize(x, columns, bits, **kw), ms.quantize(x * 2.0 ** 118, columns, bits, **kw)
+    assert torch.isfinite(x * 2.0 ** 118).all()
+    want = small.scales.int() + 118
+    empty = ms.quantize(x, columns, bits).scales == 0
+    want = torch.where(empty, 0, torch.where(want > 254, 255, want))
+    assert (want[0, :2] == 255).all() and int(want[1, 0]) == 254
+    assert torch.equal(far.scales.int(), want)
+    live = (want != 255).repeat_interleave(16, 1)
+    assert torch.equal(far.codes[live], small.codes[live])
+    # and what a product makes of them: the same sums, 2^118 times
+    one = ms.quantize(torch.full((3, n), 2.0 ** -100, device=DEV))
+    a, b = ms.product(small, one, FP), ms.product(far, one, FP)
+    gone = (want == 255).any(1)
+    assert torch.equal(b[~gone], a[~gone] * 2.0 ** 118) and torch.isnan(b[gone]).all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_rotation_beside_what_is_not_finite(ms, capi, bad):
+    """in one row: a block with an infinity or NaN, a block of the largest numbers and ordinary ones"""
+    x = matrix(6, 256, BF, 2, 1.0)
+    bits, _ = signs(capi, 256, 4)
+    want = ms.quantize(x, sign=bits)
+    x[2, 40] = bad
+    x[2, 64:96] *= 2.0 ** 100
+    x[2, 70] = -2.0 ** 126
+    got = ms.quantize(x, sign=bits)
+    same_block = torch.ones(6, 8, dtype=torch.bool, device=DEV)
+    same_block[2, 1:3] = False
+    assert torch.equal(got.scales[same_block], want.scales[same_block]) and int(got.scales[2, 1]) == 255 and 245 <= int(got.scales[2, 2]) <= 254
