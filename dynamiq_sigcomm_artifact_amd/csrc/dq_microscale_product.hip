@@ -152,7 +152,7 @@ template <int MF, int NF, int W, int U> __global__ __launch_bounds__(64 * W) voi
 // what is on its way there, and waits.  Whoever reads waits for vmcnt himself.
 __device__ __forceinline__ void load_lds16(const uint8_t *base, uint32_t offset, uint32_t to)
 {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "m0");
 }
 
 // Which tile a workgroup takes: an XCD's run of tiles is four rows of them high.

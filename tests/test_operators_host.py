@@ -159,3 +159,18 @@ def test_reference_codes_and_dither():
         c, s = R.encode8(x, R.dither(32, t), False)
         mean += R.decode8(c, s) / 4096
     assert np.all(np.abs(mean - x) <= 2.0 ** -8 * 2 ** -3 * 16 / 4096)
+
+
+def test_inline_assembly_names_what_it_writes():
+    """an assembly statement that writes a register of its own choosing says so, or the compiler may keep a value there"""
+    import glob
+    import os
+    import re
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dynamiq_sigcomm_artifact_amd", "csrc")
+    seen = 0
+    for path in sorted(glob.glob(os.path.join(root, "*.hip")) + glob.glob(os.path.join(root, "*.cuh"))):
+        for text in re.findall(r"asm volatile\((.*?)\);", open(path).read(), re.S):
+            if re.search(r"s_mov_b32 m0\b", text):
+                seen += 1
+                assert re.search(r':\s*"m0"|,\s*"m0"', text), (os.path.basename(path), text)
+    assert seen >= 1
