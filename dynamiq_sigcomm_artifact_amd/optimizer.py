@@ -96,9 +96,11 @@ class AdamW(object):
         opt.step(grad_scale=clip[1:])
 
     bits: of the states.  master: float32 master weights beside 16-bit parameters.  ``param_groups`` may be changed between steps (a
-    learning rate's schedule).  A parameter without a gradient is left as it is; the steps are counted for all parameters together.
+    learning rate's schedule).  A parameter without a gradient is left as it is; the steps are counted for all parameters together, those that
+    grad_scale makes do nothing excepted.  What grad_scale is the device alone knows: from the first step that is given one the count lives
+    there, and advancing it is a launch more for each group.
 
-    capturable: the count of the steps lives on the device (a step that grad_scale makes do nothing is not counted), and lr may be a float32
+    capturable: the count lives there from the beginning, and lr may be a float32
     tensor [1] that is read when a step runs: step() may then be recorded into a graph and replayed, with gradients at the addresses of the
     recording.  Replays and other steps of the object follow one another on one stream, or in an order that the caller sees to."""
 
@@ -108,7 +110,7 @@ class AdamW(object):
             raise RuntimeError("AdamW: no parameters")
         groups = params if isinstance(params[0], dict) else [{"params": params}]
         defaults = {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay}
-        self.bits, self.capturable, self.steps = bits, bool(capturable), 0
+        self.bits, self.capturable = bits, bool(capturable)
         self.param_groups = [{**defaults, **g, "params": _tensors(g["params"], "AdamW")} for g in groups]
         every = self.params()
         if len({id(p) for p in every}) < len(every):
@@ -124,6 +126,8 @@ class AdamW(object):
                 if chosen:
                     self._parts.append({"group": g, "params": chosen, "state": adamw_state(chosen, bits),
                                         "master": master_weights(chosen) if with_master else None})
+        # the steps done: a number, or None and a count per group on the device, all of them the same
+        self._count = None if self.capturable else 0
         self._steps = torch.zeros(len(self.param_groups), dtype=torch.int64, device=self.device)
         self._coefficients = torch.zeros((len(self.param_groups), 4), dtype=torch.float32, device=self.device)
         self._work = None
@@ -134,6 +138,17 @@ class AdamW(object):
         if self._work is None:
             self._work = norm_work(self.device)
         return self._work
+
+    @property
+    def steps(self):
+        """the steps done (waits for the device where it counts them)"""
+        return int(self._steps[0]) if self._count is None else self._count
+
+    @steps.setter
+    def steps(self, done):
+        self._steps.fill_(done)
+        if self._count is not None:
+            self._count = int(done)
 
     def params(self):
         return [p for group in self.param_groups for p in group["params"]]
@@ -147,24 +162,29 @@ class AdamW(object):
 
     @torch.no_grad()
     def step(self, grad_scale=None):
-        if self.capturable:
+        if grad_scale is not None and self._count is not None and not torch.cuda.is_current_stream_capturing():
+            self._steps.fill_(self._count)
+            self._count = None
+        counted = self._count is None
+        if counted:
             for g, group in enumerate(self.param_groups):
-                adamw_coefficients(self._steps[g:g + 1], self._coefficients[g], group["lr"], group["betas"], group["weight_decay"], grad_scale)
+                lr = group["lr"] if self.capturable else float(group["lr"])
+                adamw_coefficients(self._steps[g:g + 1], self._coefficients[g], lr, group["betas"], group["weight_decay"], grad_scale)
         else:
-            self.steps += 1
+            self._count += 1
         for part in self._parts:
             group = self.param_groups[part["group"]]
             grads = [p.grad if p.grad is None or p.grad.is_contiguous() else p.grad.contiguous() for p in part["params"]]
             if all(g is None for g in grads):
                 continue
-            adamw_step(part["params"], grads, part["state"], max(1, self.steps), 0.0 if self.capturable else group["lr"], group["betas"], group["eps"],
-                       group["weight_decay"], part["master"], grad_scale, self._coefficients[part["group"]] if self.capturable else None)
+            adamw_step(part["params"], grads, part["state"], 1 if counted else self._count, 0.0 if counted else group["lr"], group["betas"], group["eps"],
+                       group["weight_decay"], part["master"], grad_scale, self._coefficients[part["group"]] if counted else None)
 
     def state_dict(self):
         """copies of the states: a step after load_state_dict() is the step that would have followed"""
         def copy(x):
             return None if x is None else tuple(t.clone() for t in x) if isinstance(x, tuple) else x.clone()
-        return {"bits": self.bits, "steps": self._steps.tolist() if self.capturable else [self.steps] * len(self.param_groups),
+        return {"bits": self.bits, "steps": self._steps.tolist() if self._count is None else [self._count] * len(self.param_groups),
                 "groups": [{k: copy(v) if isinstance(v, torch.Tensor) else v for k, v in group.items() if k != "params"} for group in self.param_groups],
                 "parts": [{"state": copy(part["state"]), "master": copy(part["master"])} for part in self._parts]}
 
@@ -183,5 +203,6 @@ class AdamW(object):
                     group[k].copy_(v)
                 else:
                     group[k] = v
-        self.steps = saved["steps"][0]
+        if self._count is not None:
+            self._count = saved["steps"][0]
         self._steps.copy_(torch.tensor(saved["steps"], dtype=torch.int64))

@@ -399,3 +399,40 @@ def test_other_streams(opt):
     torch.cuda.synchronize()
     opt.adamw_step(want, [new], state2, 1, grad_scale=opt.grad_norm([new], 1.0)[1:])
     assert torch.equal(params[0], want[0]) and torch.equal(state, state2)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_skipped_steps_are_not_counted(opt, bits):
+    """a step that its factor makes do nothing leaves the count where it is, recorded or not, with or without factors before it, and across load_state_dict()"""
+    def model(**kw):
+        params = [p.clone() for p in views([1000, 77], FP, 1) + views([300], BF, 2)]
+        return params, opt.AdamW([{"params": params[:2]}, {"params": params[2:], "lr": 1e-2}], lr=1e-3, bits=bits, **kw)
+    fine, bad = torch.full((1,), 0.5, device=DEV), torch.full((1,), float("nan"), device=DEV)
+    scales = [None, bad, fine, bad, torch.full((1,), float("inf"), device=DEV), None, fine]
+    (p, eager), (q, device), (r, only) = model(), model(capturable=True), model()
+    done = 0
+    for t, scale in enumerate(scales):
+        grads = [torch.randn_like(v) for v in p]
+        for params in (p, q, r):
+            for v, g in zip(params, grads):
+                v.grad = g.clone()
+        if t == 4:                                    # the count goes with the state
+            saved = eager.state_dict()
+            again = model()
+            for v, u in zip(again[0], p):
+                v.copy_(u)
+            again[1].load_state_dict(saved)
+            for v, g in zip(again[0], grads):
+                v.grad = g.clone()
+            p, eager = again
+        eager.step(grad_scale=scale)
+        device.step(grad_scale=scale)
+        if scale is None or bool(torch.isfinite(scale)):
+            only.step(grad_scale=scale)               # the steps that count, alone
+            done += 1
+        assert eager.steps == device.steps == only.steps == done
+        for a, b, c in zip(p, q, r):
+            assert torch.equal(a, c) and torch.equal(b, c)
+        for x, y, z in zip(eager._parts, device._parts, only._parts):
+            for a, b, c in zip(*((s["state"] if bits == 8 else [s["state"]]) for s in (x, y, z))):
+                assert torch.equal(a, c) and torch.equal(b, c)
