@@ -18,6 +18,10 @@ def _tensors(of, what):
     return list(of)
 
 
+def _contiguous(grad):
+    return grad if grad is None or grad.is_contiguous() else grad.contiguous()
+
+
 def norm_work(device):
     """the work buffer of grad_norm: kept from call to call, one for every stream (or recorded graph) whose calls may overlap"""
     return torch.empty(int(capi.lib().dq_grad_norm_work_doubles()), dtype=torch.float64, device=device)
@@ -26,14 +30,17 @@ def norm_work(device):
 def grad_norm(grads, max_norm=None, work=None, out=None):
     """float32 [2] on the device: the 2-norm of all tensors together, summed in 64 bits, and min(1, max_norm / (norm + 1e-6)), the
     ``grad_scale`` of a step that clips (1 without max_norm).  Where the norm is not finite the factor is NaN, and the step
-    changes nothing.  work: from norm_work(); without it the call makes one."""
-    grads = _tensors(grads, "grad_norm")
-    if not grads:
+    changes nothing.  grads: contiguous tensors; None among them takes no part (where all are, work or out names the device).
+    work: from norm_work(); without it the call makes one."""
+    listed = _tensors(grads, "grad_norm")
+    grads = [g for g in listed if g is not None]
+    beside = grads[0] if grads else out if work is None else work
+    if not listed or beside is None:
         raise RuntimeError("grad_norm: no tensors")
     if work is None:
-        work = norm_work(grads[0].device)
+        work = norm_work(beside.device)
     if out is None:
-        out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
+        out = torch.empty(2, dtype=torch.float32, device=beside.device)
     capi.host().grad_norm(grads, float("inf") if max_norm is None else max_norm, work, out)
     return out
 
@@ -92,7 +99,7 @@ class AdamW(object):
 
         opt = AdamW(model.parameters(), lr=3e-4, bits=8)
         loss.backward()
-        clip = grad_norm([p.grad for p in opt.params()], 1.0, work=opt.work)
+        clip = grad_norm(opt.grads(), 1.0, work=opt.work)
         opt.step(grad_scale=clip[1:])
 
     bits: of the states.  master: float32 master weights beside 16-bit parameters.  ``param_groups`` may be changed between steps (a
@@ -153,6 +160,10 @@ class AdamW(object):
     def params(self):
         return [p for group in self.param_groups for p in group["params"]]
 
+    def grads(self):
+        """the parameters' gradients as step() takes them: contiguous (copies of those that are not), None where there is none"""
+        return [_contiguous(p.grad) for p in self.params()]
+
     def zero_grad(self, set_to_none=True):
         for p in self.params():
             if set_to_none:
@@ -174,7 +185,7 @@ class AdamW(object):
             self._count += 1
         for part in self._parts:
             group = self.param_groups[part["group"]]
-            grads = [p.grad if p.grad is None or p.grad.is_contiguous() else p.grad.contiguous() for p in part["params"]]
+            grads = [_contiguous(p.grad) for p in part["params"]]
             if all(g is None for g in grads):
                 continue
             adamw_step(part["params"], grads, part["state"], 1 if counted else self._count, 0.0 if counted else group["lr"], group["betas"], group["eps"],

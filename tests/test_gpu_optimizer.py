@@ -436,3 +436,23 @@ def test_skipped_steps_are_not_counted(opt, bits):
         for x, y, z in zip(eager._parts, device._parts, only._parts):
             for a, b, c in zip(*((s["state"] if bits == 8 else [s["state"]]) for s in (x, y, z))):
                 assert torch.equal(a, c) and torch.equal(b, c)
+
+
+def test_norm_of_gradients_that_are_missing(opt):
+    """None takes no part, and what AdamW.step() takes grad_norm(AdamW.grads()) takes"""
+    params = [torch.ones(40, 30, device=DEV), torch.ones(7, device=DEV), torch.ones(64, device=DEV), torch.ones(3, device=DEV)]
+    a = opt.AdamW(params, lr=1e-2)
+    params[0].grad = torch.randn(30, 40, device=DEV).t()
+    params[2].grad = torch.randn(64, device=DEV)
+    norm = math.sqrt(float(params[0].grad.double().square().sum() + params[2].grad.double().square().sum()))
+    got = opt.grad_norm([None, params[2].grad, None, params[0].grad.contiguous()], 1.0)
+    assert abs(float(got[0]) - norm) <= norm * 2.0 ** -23
+    clip = opt.grad_norm(a.grads(), 1.0, work=a.work)
+    assert abs(float(clip[0]) - norm) <= norm * 2.0 ** -23
+    was = [p.clone() for p in params]
+    a.step(grad_scale=clip[1:])
+    assert [torch.equal(p, w) for p, w in zip(params, was)] == [False, True, False, True]
+    a.zero_grad()
+    assert opt.grad_norm(a.grads(), 1.0, work=a.work).tolist() == [0.0, 1.0]
+    with pytest.raises(RuntimeError, match="no tensors"):
+        opt.grad_norm(a.grads(), 1.0)

@@ -174,3 +174,18 @@ def test_inline_assembly_names_what_it_writes():
                 seen += 1
                 assert re.search(r':\s*"m0"|,\s*"m0"', text), (os.path.basename(path), text)
     assert seen >= 1
+
+
+def test_norm_of_nothing_is_refused():
+    """None takes no part; a list of nothing else needs a buffer that says where"""
+    from dynamiq_sigcomm_artifact_amd import optimizer
+    for grads in ([None], [None, None], iter([None])):
+        with pytest.raises(RuntimeError, match="no tensors"):
+            optimizer.grad_norm(grads)
+    with pytest.raises(RuntimeError, match="must live on the GPU"):
+        optimizer.grad_norm([None], out=torch.zeros(2))
+    p = torch.zeros(4, 6)
+    opt = optimizer.AdamW([p, torch.zeros(3)])
+    p.grad = torch.ones(6, 4).t()
+    got = opt.grads()
+    assert got[1] is None and got[0].is_contiguous() and torch.equal(got[0], p.grad)
