@@ -212,6 +212,8 @@ class AdamW(object):
             for k, v in was.items():
                 if isinstance(v, torch.Tensor) and isinstance(group.get(k), torch.Tensor):
                     group[k].copy_(v)
+                elif isinstance(v, torch.Tensor): # (a step on the device reads it there)
+                    group[k] = v.detach().to(self.device if self.capturable else v.device, copy=True)
                 else:
                     group[k] = v
         if self._count is not None:

@@ -456,3 +456,20 @@ def test_norm_of_gradients_that_are_missing(opt):
     assert opt.grad_norm(a.grads(), 1.0, work=a.work).tolist() == [0.0, 1.0]
     with pytest.raises(RuntimeError, match="no tensors"):
         opt.grad_norm(a.grads(), 1.0)
+
+
+def test_loaded_learning_rates_are_ones_own(opt):
+    """a learning rate on the device that load_state_dict() brings is a copy, on the parameters' device"""
+    def model(lr):
+        p = torch.ones(10, device=DEV)
+        p.grad = torch.ones(10, device=DEV)
+        return opt.AdamW([p], lr=lr, capturable=True)
+    a = model(torch.full((1,), 0.25, device=DEV))
+    saved = a.state_dict()
+    for state in (saved, {**saved, "groups": [{**saved["groups"][0], "lr": saved["groups"][0]["lr"].cpu()}]}):
+        b, c = model(0.1), model(0.1)
+        b.load_state_dict(state)
+        c.load_state_dict(state)
+        b.param_groups[0]["lr"].fill_(7.0)
+        c.step()
+        assert float(c.param_groups[0]["lr"]) == 0.25 and float(state["groups"][0]["lr"]) == 0.25

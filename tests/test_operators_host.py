@@ -189,3 +189,14 @@ def test_norm_of_nothing_is_refused():
     p.grad = torch.ones(6, 4).t()
     got = opt.grads()
     assert got[1] is None and got[0].is_contiguous() and torch.equal(got[0], p.grad)
+
+
+def test_loaded_hyperparameters_are_copies():
+    """what one object does to a value that it has loaded changes neither the saved state nor another object"""
+    from dynamiq_sigcomm_artifact_amd import optimizer
+    saved = optimizer.AdamW([torch.zeros(5)], lr=torch.full((1,), 0.25)).state_dict()
+    a, b = optimizer.AdamW([torch.zeros(5)], lr=0.1), optimizer.AdamW([torch.zeros(5)], lr=0.1)
+    a.load_state_dict(saved)
+    b.load_state_dict(saved)
+    a.param_groups[0]["lr"].fill_(7.0)
+    assert float(b.param_groups[0]["lr"]) == 0.25 and float(saved["groups"][0]["lr"]) == 0.25
