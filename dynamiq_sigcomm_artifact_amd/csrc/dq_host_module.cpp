@@ -1313,6 +1313,17 @@ struct Quantized {
     int64_t rows = 0, length = 0;
 };
 
+// what a gradient of rows x length elements is rotated and rounded with
+void linear_takes(const at::Tensor &sign, const at::Tensor &pool, int64_t rows, int64_t length, const c10::Device &device)
+{
+    const int64_t supers = (length + 255) / 256;
+    need(!sign.defined() || (sign.scalar_type() == at::kInt && sign.is_contiguous() && sign.device() == device && sign.numel() >= 8 * supers),
+         "linear: signs are int32, eight per superchunk of the contraction");
+    need(!pool.defined() || (pool.is_contiguous() && pool.device() == device && pool.numel() == rows * 256 * supers),
+         "linear: a rand_pool has one value per element of the quantised gradient, padding included");
+    if (pool.defined()) (void)dtype_code(pool);
+}
+
 // Matrices that are quantised together, in one piece of memory.
 struct Quantizer {
     std::vector<dq_mx4_matrix_t> list;
@@ -1326,10 +1337,7 @@ struct Quantizer {
         q.rows = x.size(columns ? 1 : 0);
         q.length = x.size(columns ? 0 : 1);
         const int64_t supers = (q.length + 255) / 256;
-        need(!sign.defined() || (sign.scalar_type() == at::kInt && sign.is_contiguous() && sign.device() == x.device() && sign.numel() >= 8 * supers),
-             "linear: signs are int32, eight per superchunk of the contraction");
-        need(!pool.defined() || (pool.is_contiguous() && pool.device() == x.device() && pool.numel() == q.rows * 256 * supers),
-             "linear: a rand_pool has one value per element of the quantised gradient, padding included");
+        linear_takes(sign, pool, q.rows, q.length, x.device());
         list.push_back({x.data_ptr(), x.size(0), x.size(1), x.size(1), sign.defined() ? reinterpret_cast<const uint32_t *>(sign.data_ptr<int32_t>()) : nullptr,
                         pool.defined() ? pool.data_ptr() : nullptr, seed, step, step_dev.defined() ? step_counter(step_dev, x) : nullptr, nullptr, nullptr, dtype_code(x),
                         columns, stochastic, pool.defined() ? dtype_code(pool) : 0});
@@ -1441,6 +1449,10 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
         }
         const int64_t step = THPVariable_Check(v[7]) ? 0 : (int64_t)word(v[7], true);
         const int64_t k = weight.size(1), n = weight.size(0), tokens = k ? x.numel() / k : x.numel() == 0 && x.dim() > 1 ? c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)) : 1;
+        if (at::GradMode::is_enabled()) { // what the backward pass will want is refused here, where the mistake is
+            if (x.requires_grad()) linear_takes(extra[0].value_or(at::Tensor()), extra[2].value_or(at::Tensor()), tokens, n, x.device());
+            if (weight.requires_grad()) linear_takes(extra[1].value_or(at::Tensor()), extra[3].value_or(at::Tensor()), n, tokens, x.device());
+        }
         // The engine hands a leaf's gradient to the stream that the leaf's node was made on.  One made by an eager pass whose graph still lives draws that stream into a
         // recording, which ends badly there; so it is refused here.
         if (at::GradMode::is_enabled()) {

@@ -537,3 +537,28 @@ def test_rotation_beside_what_is_not_finite(ms, capi, bad):
     same_block = torch.ones(6, 8, dtype=torch.bool, device=DEV)
     same_block[2, 1:3] = False
     assert torch.equal(got.scales[same_block], want.scales[same_block]) and int(got.scales[2, 1]) == 255 and 245 <= int(got.scales[2, 2]) <= 254
+
+
+def test_linear_refuses_before_its_backward_pass(ms):
+    """what the backward pass would refuse is refused with the call, and only what it would take"""
+    x, w = matrix(6, 64, BF, 1), matrix(10, 64, BF, 2)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    short, good = torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(8, dtype=torch.int32, device=DEV)
+    rows, columns = torch.zeros(6, 256, device=DEV), torch.zeros(10, 256, device=DEV)
+    for kw, text in ((dict(sign=(short, None)), "signs are int32"), (dict(sign=(good.float(), None)), "signs are int32"), (dict(sign=(good.cpu(), None)), "signs are int32"),
+                     (dict(rand_pool=(rows[:, :10].contiguous(), None)), "rand_pool has one value"), (dict(rand_pool=(rows.cpu(), None)), "rand_pool has one value"),
+                     (dict(rand_pool=(rows.double(), None)), "unsupported element dtype")):
+        with pytest.raises(RuntimeError, match=text):
+            ms.linear(xg, w, **kw)
+        flip = {k: v[::-1] for k, v in kw.items()}
+        if "rand_pool" in kw:
+            flip = dict(rand_pool=(None, columns.cpu() if kw["rand_pool"][0].device.type == "cpu" else columns.double() if kw["rand_pool"][0].dtype == torch.float64 else rows))
+        with pytest.raises(RuntimeError, match=text):
+            ms.linear(x, wg, **flip)
+        # the other operand's gradient does not take them, nor does a call without gradients
+        ms.linear(x, wg, **kw).sum().backward()
+        ms.linear(xg, w, **flip).sum().backward()
+        with torch.no_grad():
+            ms.linear(xg, wg, **kw)
+        ms.linear(x, w, **kw)
+    ms.linear(xg, wg, sign=(good, good), rand_pool=(rows, columns)).sum().backward()
