@@ -1453,8 +1453,9 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
             if (x.requires_grad()) linear_takes(extra[0].value_or(at::Tensor()), extra[2].value_or(at::Tensor()), tokens, n, x.device());
             if (weight.requires_grad()) linear_takes(extra[1].value_or(at::Tensor()), extra[3].value_or(at::Tensor()), n, tokens, x.device());
         }
-        // The engine hands a leaf's gradient to the stream that the leaf's node was made on.  One made by an eager pass whose graph still lives draws that stream into a
-        // recording, which ends badly there; so it is refused here.
+        // The engine hands a leaf's gradient to the stream that the leaf's node was made on.  That node is alive as long as an earlier graph of the leaf is, or a reducer or hook
+        // that holds it.  A stream of one's own joins a recording by the engine's events and leaves it again; the default stream cannot take part in one, and to draw it in ends
+        // badly; so that is refused here.
         if (at::GradMode::is_enabled()) {
             const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(x.device().index());
             unsigned long long recording;
@@ -1463,7 +1464,9 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
                     if (!t->requires_grad() || !t->is_leaf()) continue;
                     const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(*t);
                     const std::optional<c10::Stream> of = node ? node->stream() : std::nullopt;
-                    need(!of || of->id() == now.id(), "linear: an earlier graph of the same leaf, made on another stream, is still alive: let go of its outputs before recording");
+                    need(!of || of->id() != c10::hip::getDefaultHIPStream(x.device().index()).id(),
+                         "linear: the node of a leaf's gradient was made on the default stream, which cannot be recorded, and is still alive: let go of the outputs (or the reducer, "
+                         "or hook) that hold it before recording, or make them on another stream");
                 }
         }
         // (a matrix that is contiguous takes part as it is: views of it would be nodes of the graph)

@@ -562,3 +562,52 @@ def test_linear_refuses_before_its_backward_pass(ms):
             ms.linear(xg, wg, **kw)
         ms.linear(x, w, **kw)
     ms.linear(xg, wg, sign=(good, good), rand_pool=(rows, columns)).sum().backward()
+
+
+def accumulator(t):
+    """the node that a leaf's gradient goes through, as a reducer or a hook holds it"""
+    return t.view_as(t).grad_fn.next_functions[0][0]
+
+
+def test_recording_beside_held_accumulators(ms):
+    """nodes that were made on a stream which can take part in a recording do not keep a layer from being recorded; nodes of the default stream, which cannot, do"""
+    x, w, dy = matrix(40, 96, BF, 1, 1.0).requires_grad_(), matrix(50, 96, BF, 2, 1.0).requires_grad_(), matrix(40, 50, BF, 3, 1.0)
+    made, recorder = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def record():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=recorder):
+            return graph, torch.autograd.grad(ms.linear(x, w, seed=1, step=2), (x, w), dy)
+    held = [accumulator(t) for t in (x, w)]
+    with pytest.raises(RuntimeError, match="default stream"):
+        record()
+    torch.cuda.synchronize()
+    del held
+    made.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(made):
+        held = [accumulator(t) for t in (x, w)]
+        eager = torch.autograd.grad(ms.linear(x, w, seed=1, step=2), (x, w), dy)
+    torch.cuda.current_stream().wait_stream(made)
+    torch.cuda.synchronize()
+    graph, got = record()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(s, t) for s, t in zip(got, eager))
+    # gradients that are added up where they lie, as a reducer's are
+    x.grad, w.grad = torch.zeros_like(x), torch.zeros_like(w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=recorder):
+        ms.linear(x, w, seed=1, step=2).backward(dy)
+    for t in (x, w):
+        t.grad.zero_()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, eager[0]) and torch.equal(w.grad, eager[1])
+        for t in (x, w):
+            t.grad.zero_()
+    assert len(held) == 2
