@@ -41,7 +41,8 @@ def quantize(x, columns=False, sign=None, rand_pool=None, seed=None, step=0):
     sign: int32 [>= 8 s], the packed signs of capi.pack_signs or capi.rand_diag_bits, one per element of a vector: every block of 32 is rotated,
     H (s x) / sqrt(32).  The product of two matrices that are rotated with the same signs is that of the matrices.
     rand_pool: uniform values in [0, 1), [vectors, 256 s], for stochastic rounding; or seed (and step, a number or an int64 tensor [1]) for the
-    in-kernel stream;
+    in-kernel stream, the codec's, whose values are the 128 odd multiples of 1/256: elements up to 2^k / 512, k of their block, become 0 in every draw,
+    and the mean of the draws of another is off by up to 1/256 of the distance between its neighbours (a float32 pool has 24 bits);
     neither: to nearest, ties to even.  Nothing here but linear() is differentiated."""
     codes, scales = capi.host().mx4_quantize(x, columns, sign, rand_pool, seed, step)
     r, c = x.shape
@@ -76,11 +77,11 @@ def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0):
       dx = S(dy R) (Q(weight^T R))^T    along n
       dw = S(dy^T R) (Q(x^T R))^T       along the tokens
 
-    Q rounds to nearest and S stochastically, so that the gradients' rounding has no bias, R is the rotation of every block of 32 with
-    the given signs, which spreads outliers over their block and cancels in the product.
+    Q rounds to nearest (and what it makes of x and weight is off by that), S stochastically, so that the rounding of dy has no bias but for the resolution
+    of the random numbers (quantize), R is the rotation of every block of 32 with the given signs, which spreads outliers over their block and cancels in the product.
 
     sign: (signs of n, signs of the tokens), packed; None leaves R out.  rand_pool: (pool [tokens, n padded to 256], pool [n, tokens padded to
-    256]), or seed and step: then every call needs a step of its own, below 2^63 (the gradient's rows draw at step, its columns at step + 2^63).
+    256]), checked here where their gradient is wanted, or seed and step: then every call needs a step of its own, below 2^63 (the gradient's rows draw at step, its columns at step + 2^63).
     With neither the gradients are rounded to nearest, too.  A step on the device stays as it is until the backward pass has run.  The gradients
     cannot be differentiated again."""
     signs, pools = sign or (None, None), rand_pool or (None, None)

@@ -828,7 +828,10 @@ int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double
  * the way from one value to the next: where u is below it, with the least k for
  * which max <= 6 2^k.  u: rand_pool (rand_dtype; [result's rows][256 s], in [0, 1)), or
  * with rand_pool = NULL the in-kernel stream of dq_scaling_compress_philox, keyed by
- * (seed, step, chunk of 16 elements of that layout).  step_dev (may be NULL): one uint64
+ * (seed, step, chunk of 16 elements of that layout).  That stream's values are the 128 odd
+ * multiples of 1/256: the probability is the share's to 1/256, and a share of 1/256 or less
+ * never goes up (elements up to 2^k / 512 become 0), one above 255/256 always does.  A pool
+ * resolves as many bits as its values have.  step_dev (may be NULL): one uint64
  * in device memory that is added to step, so that a recorded call draws anew.
  * A block that holds an infinity or NaN is NaN, and so is one whose rotation is beyond
  * what the largest scale, 2^127, holds (its elements alone never are). */

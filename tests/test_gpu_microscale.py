@@ -611,3 +611,33 @@ def test_recording_beside_held_accumulators(ms):
         for t in (x, w):
             t.grad.zero_()
     assert len(held) == 2
+
+
+@pytest.mark.parametrize("columns", [False, True])
+def test_resolution_of_the_draws(ms, columns):
+    """The in-kernel stream's uniform values are the 128 odd multiples of 1/256: a draw goes up with the nearest probability that they have, and never from a share of the way of
+    1/256 or less (always from 255/256); a pool of float32 has no such limits."""
+    share = torch.tensor([1 / 4096, 1 / 512, 1 / 256, 3 / 512, 1 / 64, 0.1, 0.25, 1 / 3, 0.5, 0.7, 254.9 / 256, 255.5 / 256], device=DEV)
+    low = torch.tensor([0.0, 0.5, 1.0, 2.0, 4.0], device=DEV)
+    step = torch.tensor([0.5, 0.5, 0.5, 1.0, 2.0], device=DEV)
+    values = (low[:, None] + step[:, None] * share).flatten()                      # 60 values, in two blocks whose largest is 6
+    x = torch.zeros(64, device=DEV)
+    x[:30], x[32:62], x[31], x[63] = values[:30], values[30:], 6.0, 6.0
+    draws = 16384
+    many = x.repeat(draws, 1)
+    many = many.t().contiguous() if columns else many
+
+    def ups(**kw):
+        v = ms.dequantize(ms.quantize(many, columns, **kw)).double()
+        v = torch.cat([v[:, :30], v[:, 32:62]], 1)
+        up = (v - low.double().repeat_interleave(12)) / step.double().repeat_interleave(12)
+        assert torch.all((up == 0) | (up == 1))
+        return up.mean(0).view(5, 12)
+    p = share.double().expand(5, 12)
+    # odd multiples of 1/256 below the share; six standard deviations of a mean of 16384 draws.  (low + step * share is rounded, by 2^-22 of a step at most, and no share lies that near
+    # to a multiple that it is not.)
+    q = torch.ceil((256 * p - 1) / 2) / 128
+    assert torch.all((q - p).abs() <= 1 / 256) and torch.all(q[:, share <= 1 / 256] == 0) and torch.all(q[:, share > 255 / 256] == 1)
+    assert torch.all((ups(seed=11, step=2) - q).abs() <= 6 * (q * (1 - q) / draws).sqrt())
+    fine = ups(rand_pool=torch.rand(draws, 256, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV))
+    assert torch.all((fine - p).abs() <= 6 * (p * (1 - p) / draws).sqrt() + 2.0 ** -21)
