@@ -101,3 +101,26 @@ def test_norm_and_step(ops):
             lo = n - 1000
             assert torch.equal(state[:, lo:lo + 1000], small[:, :1000])
         del state
+
+
+def test_states_in_8_bits(ops):
+    """What the last elements' states become, and what the next step makes of them.  The dither of element i at step t is a function of i C + t D mod 2^32 with D odd: it is that
+    of element i - lo at the step t + lo C / D, which a small call is given.  (The moments do not depend on the step's number otherwise; the weights do.)"""
+    opt = ops[1]
+    n = (1 << 31) + 1234
+    lo = (n - 1000) // 32 * 32
+    shift = lo * 0x9E3779B9 * pow(0xB504F333, -1, 1 << 32) % (1 << 32)
+    p = torch.full((n,), 0.5, dtype=torch.float32, device=DEV)
+    state = opt.adamw_state([p], 8)
+    tail, small = p[lo:].clone(), opt.adamw_state([p[lo:]], 8)
+    g = torch.empty(n, dtype=BF, device=DEV)
+    for t in (1, 2, 3):
+        g.copy_(big(1, 1 << 20, 10 + t).view(-1).repeat(n // (1 << 20) + 1)[:n])
+        now = tuple(s.clone() for s in small)
+        opt.adamw_step([p], [g], state, t)
+        opt.adamw_step([tail], [g[lo:]], now, t)                               # the weights, from the states before
+        opt.adamw_step([torch.zeros_like(tail)], [g[lo:]], small, t + shift)   # the states behind
+        assert torch.equal(p[lo:], tail)
+        for whole, part, unit in zip(state, small, (1, 32)):
+            assert torch.equal(whole[:, lo // unit:], part)
+        assert int((state[0][:, lo:] != 0).sum()) > 1900                       # (both moments of nearly all 1000 elements)

@@ -155,3 +155,40 @@ def test_threads_on_their_own_streams(lib):
         t.join()
     for k in range(4):
         assert all(torch.equal(v, w) for v, w in zip(alone[k], together[k])), k
+
+
+def test_gradients_are_the_layers(lib):
+    """the gradients in the bucket are those of the two layers, each against its definition in 64 bits on what it was given"""
+    from test_gpu_microscale import plain_linear
+    capi, _, ms, _ = lib
+    m = Model(lib, 32, False)
+
+    def plus_or_minus(bits, n):
+        return 1.0 - 2.0 * ((bits.cpu().numpy().view(np.uint32)[:, None] >> np.arange(32)) & 1).reshape(-1)
+
+    def drawn(seed, step, rows, length):
+        out = torch.empty(rows, 256 * -(-length // 256), device=DEV)
+        capi.philox_uniform(out, seed, step)
+        return out
+    for step in range(2):
+        w = [v.detach().clone().requires_grad_() for v in m.weights]
+        z = ms.linear(m.x, w[0], sign=(m.signs[HIDDEN], m.signs[TOKENS]), seed=1, step=step)
+        h = torch.relu(z)
+        y = ms.linear(h, w[1], sign=(m.signs[WIDTH], m.signs[TOKENS]), seed=2, step=step)
+        dy, dh, dz, dw0, dw1 = torch.autograd.grad((y - m.aim).float().square().mean(), (y, h, z, w[0], w[1]))
+        m.step()
+        assert torch.equal(m.parts[0], dw0) and torch.equal(m.parts[1], dw1)
+        # the loss's gradient: a difference rounded to bf16, then 2 / n of it rounded once more (and a product in binary32)
+        want = 2.0 / y.numel() * (y.detach().double() - m.aim.double())
+        assert float(((dy.double() - want).abs() - want.abs() * (2 * 2.0 ** -8 + 2.0 ** -15)).max()) <= 0
+        assert torch.equal(dz, torch.where(z > 0, dh, torch.zeros_like(dh)))
+        for x, weight, out, grad, seed, (dx, dw) in ((m.x, w[0], z, dz, 1, (None, dw0)), (h, w[1], y, dy, 2, (dh, dw1))):
+            tokens, n, k = x.shape[0], weight.shape[0], x.shape[1]
+            plain = plain_linear(x.detach(), weight.detach(), grad, plus_or_minus(m.signs[n], n)[:256 * -(-n // 256)], plus_or_minus(m.signs[tokens], tokens),
+                                 drawn(seed, step, tokens, n), drawn(seed, step + (1 << 63), n, tokens))
+            for got, t, length in ((out, plain[0], k), (dx, plain[1], n), (dw, plain[2], tokens)):
+                if got is None:
+                    continue
+                # one rounding to bf16 and `length` additions in binary32, of products up to `size`
+                g, size = got.detach().double().cpu().numpy(), np.abs(t).max() * 4 + 1e-30
+                assert np.all(np.abs(g - t) <= 2.0 ** -8 * np.abs(t) + length * 2.0 ** -23 * size * 8)
