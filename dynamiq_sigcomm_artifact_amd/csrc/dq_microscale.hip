@@ -151,8 +151,9 @@ template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void quantiz
     }
 }
 
-// Bound by memory: 14336 x 4096 bf16 to the nearest in 28 us (5.3 TB/s), rotated and stochastic with a bf16 pool 4096 x 14336 in 56 (4.8 TB/s).  With the random stream made in
-// the kernel it is the arithmetic of the stream.
+// Bound by memory: 14336 x 4096 bf16 to the nearest in 27 us (5.5 TB/s), rotated and stochastic with a bf16 pool 4096 x 14336 in 47 to 56 (up to 5.7 TB/s).  With the random stream
+// made in the kernel it is the arithmetic of the stream: 40 us for the latter's 149 MB, rotated 46 (30 at a copy's rate); along the columns, rotated, 50.  A lane takes half of the
+// sixteen numbers that a call of the stream gives.
 template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void mx4_rows_kernel(QuantizeArgs a, Division superchunks, uint32_t units)
 {
     const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
@@ -163,8 +164,8 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 
 // A workgroup takes 256 rows x 128 columns: one superchunk of 128 rows of the result.  A wave takes 32 of the rows, a lane 8 rows x 8 columns, and a
 // column's block lies in a quad as it does above.  The codes leave through LDS, as whole lines.  Elements of 16 bits stay packed until their column's turn: three
-// workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 121 us (4.4 TB/s; 130
-// with the XCDs' workgroups strewn, 8000 x 5000 35 for 40), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
+// workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 116 us (4.6 TB/s, 132
+// under a trace; 130 to 121 by then with the XCDs' workgroups strewn, 8000 x 5000 35 for 40), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
 // instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.  Blocks that have to be lowered are looked for while their columns
 // are encoded and taken behind the loop, where nothing else needs registers (in it: 2 to 6 % for every matrix); to the nearest four workgroups share a CU, which 65 registers would not let them.
 struct ColumnsLds {
@@ -312,9 +313,10 @@ hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, b
 // ---- several small matrices at once -------------------------------------------------------------------------
 
 // Up to four matrices of one element type, along either axis and rounded in any way: a workgroup takes 4096 elements along the rows or a tile along the columns.  A small
-// one leaves most CUs without work and costs a launch all the same: a linear layer's step of 333 x 776 x 1000, in a graph, takes 30 us with two such launches where six
-// quantisers of their own made it 46, of 2048 x 2048 x 2048 54 for 66, of 4096 x 4096 x 4096 176 for 193.  Beyond 4096 workgroups they go alone, in kernels that hold less:
-// 4096 x 14336 x 4096 523 us, together 533.
+// one leaves most CUs without work and costs a launch all the same: a linear layer's step of 333 x 776 x 1000, in a graph, takes 28 us with two such launches where six
+// quantisers of their own made it 44, of 2048 x 2048 x 2048 56 for 66, of 4096 x 4096 x 4096 171 for 177.  What shares a launch has 4096 workgroups at most: 4096 x 14336 x 4096,
+// whose last three matrices have just those, takes 534 us for 542 alone, 6000 x 6000 x 6000 500 for 512.  Without that limit, with the largest ones in kernels that hold
+// less than they could, they are back at 541 and 513, and 8192 x 14336 x 4096 takes 980 us for 973.
 struct QuantizeJob {
     QuantizeArgs a;
     Division by; // superchunks of a row, or tiles of 128 columns
