@@ -164,8 +164,8 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 
 // A workgroup takes 256 rows x 128 columns: one superchunk of 128 rows of the result.  A wave takes 32 of the rows, a lane 8 rows x 8 columns, and a
 // column's block lies in a quad as it does above.  The codes leave through LDS, as whole lines.  Elements of 16 bits stay packed until their column's turn: three
-// workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 116 us (4.6 TB/s, 132
-// under a trace; 130 to 121 by then with the XCDs' workgroups strewn, 8000 x 5000 35 for 40), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
+// workgroups on a CU instead of two (14336 x 4096 bf16, rotated, to the nearest in 28 us, 5.3 TB/s; unpacked 33).  8192 x 14336 with a bf16 pool takes 116 us behind its like
+// (4.6 TB/s), 132 behind other work (with the XCDs' workgroups strewn 8 % more, 8000 x 5000 40 for 35), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
 // instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.  Blocks that have to be lowered are looked for while their columns
 // are encoded and taken behind the loop, where nothing else needs registers (in it: 2 to 6 % for every matrix); to the nearest four workgroups share a CU, which 65 registers would not let them.
 struct ColumnsLds {

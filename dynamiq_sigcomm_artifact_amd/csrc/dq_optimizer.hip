@@ -245,7 +245,8 @@ __device__ __forceinline__ void roots8(const float (&v)[8], float (&r)[8])
     }
 }
 
-// PASSING: more than the 256 MB of cache in front of the memory hold, so that nothing of it is there at the next step.  With the hint that says so on every load and
+// PASSING: a launch moves more than the 256 MB of cache in front of the memory hold, so that nothing of it is there at the next step.  (That goes by the launch: a step of several,
+// each below that, runs without the hint even if together they are beyond it.)  With the hint that says so on every load and
 // store 124,439,808 binary32 weights take 593 us with 32-bit states and 328 with 8-bit ones where they take 667 and 385 without it (5.9 and 6.1 TB/s for 5.2; in 148
 // tensors at odd addresses 622 and 358 for 671 and 376; on the loads or the stores alone it gains little or loses).  A bucket of 6,553,600, whose 183 MB stay, takes
 // 32 us without the hint and 39 with it.  Bound by memory, also with 8-bit states, since roots, quotients and the cut to E4M3 take few instructions (above; before, 375 us

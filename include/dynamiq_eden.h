@@ -761,7 +761,9 @@ int dq_grad_norm(const dq_span_t *spans, int count, double max_norm, double *wor
  * *grad_scale and t the number of the step, counted from 1:
  *   m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in binary32.  The states of all tensors lie in arenas of `total` elements, a
+ * in binary32: every operation rounded to nearest (the root but for one in millions) but the
+ * last quotient, which a reciprocal good to a unit in the last place makes and which moves
+ * the weight only.  The states of all tensors lie in arenas of `total` elements, a
  * tensor's from element `start` on, a multiple of 32; the gap up to the next
  * multiple of 32 is set to zero.
  *   bits 32: state = float [2][total], m and v; scales unused.
