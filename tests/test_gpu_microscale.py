@@ -641,3 +641,16 @@ def test_resolution_of_the_draws(ms, columns):
     assert torch.all((ups(seed=11, step=2) - q).abs() <= 6 * (q * (1 - q) / draws).sqrt())
     fine = ups(rand_pool=torch.rand(draws, 256, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV))
     assert torch.all((fine - p).abs() <= 6 * (p * (1 - p) / draws).sqrt() + 2.0 ** -21)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=str)
+def test_gradients_of_the_largest_numbers(ms, capi, dtype):
+    """a power of two in front of a layer's gradient is one in front of what it makes of it, also where a rotation's sums pass binary32's range: 2^127 is the largest here"""
+    x, w = ((matrix(r, 96, dtype, r, 1.0) * 2.0 ** -20).requires_grad_() for r in (70, 300))
+    dy = matrix(70, 300, dtype, 3, 1.0).clamp(-2.0 ** 9, 2.0 ** 9)
+    dy[:20] = torch.where(dy[:20] < 0, -2.0 ** 9, 2.0 ** 9).to(dtype)
+    (bn, _), (bm, _) = signs(capi, 300, 5), signs(capi, 70, 6)
+    for kw in (dict(seed=1, step=2), dict(rand_pool=(pool(70, 300, BF), pool(300, 70, BF))), dict()):
+        small, far = (torch.autograd.grad(ms.linear(x, w, sign=(bn, bm), **kw), (x, w), dy * f) for f in (1.0, 2.0 ** 118))
+        for a, b in zip(small, far):
+            assert torch.isfinite(b).all() and torch.equal(b, a * 2.0 ** 118)
