@@ -41,6 +41,7 @@ HIP_SOURCES = [
     "dq_io_floor.hip",
     "dq_optimizer.hip",
     "dq_microscale.hip", "dq_microscale_product.hip",
+    "dq_activations.hip",
 ]
 
 HIPCC_FLAGS = [

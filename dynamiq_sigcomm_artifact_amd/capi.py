@@ -15,7 +15,7 @@ import os
 
 import torch
 
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, E4M3 = 0, 1, 2, 3
 RAND_BF16 = 0x10
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libdynamiq_eden.so")
@@ -37,6 +37,7 @@ EXPORTS = [
     "dq_eden_work_doubles", "dq_eden_quantize", "dq_eden_quantize_static_max_n", "dq_eden_quantize_static", "dq_eden_dequantize", "dq_eden_dequantize_irht", "dq_eden_slice_bytes", "dq_eden_compress", "dq_eden_decompress", "dq_thc_compress", "dq_thc_compress_drawn", "dq_thc_decompress", "dq_thc_quantize", "dq_thc_dequantize", "dq_thc_rht_quantize", "dq_thc_dequantize_irht",
     "dq_grad_norm_work_doubles", "dq_grad_norm", "dq_adamw_step", "dq_adamw_coefficients",
     "dq_mx4_quantize", "dq_mx4_quantize_list", "dq_mx4_dequantize", "dq_mx4_product",
+    "dq_checkpoint_bytes", "dq_checkpoint_compress", "dq_checkpoint_restore",
 ]
 
 STAGE_STATS, STAGE_PLAN, STAGE_COMPRESS, STAGE_DECOMPRESS = 1, 2, 4, 8
@@ -225,6 +226,12 @@ def lib():
         L.dq_mx4_dequantize.argtypes = [vp, vp, vp, i32, i64, i64, i32, vp]
         L.dq_mx4_product.restype = i32
         L.dq_mx4_product.argtypes = [vp, vp, vp, vp, vp, i32, i64, i64, i64, i32, vp]
+        L.dq_checkpoint_bytes.restype = i64
+        L.dq_checkpoint_bytes.argtypes = [i64, i64]
+        L.dq_checkpoint_compress.restype = i32
+        L.dq_checkpoint_compress.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp]
+        L.dq_checkpoint_restore.restype = i32
+        L.dq_checkpoint_restore.argtypes = [vp, vp, i32, i64, i64, i32, vp]
         _lib = L
     return _lib
 

@@ -192,9 +192,21 @@ inline bool mx4_aligned(const void *codes, const void *scales)
 {
     return ((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 7)) == 0;
 }
+// a checkpoint of rows x cols
+bool checkpoint_size_ok(int64_t rows, int64_t cols)
+{
+    constexpr int64_t most = 0x7fffff00;
+    return rows > 0 && cols > 0 && rows <= most && cols <= most && rows * ((cols + 31) / 32) <= (dq::kMxMost - 4096) / 32;
+}
+static const char kCheckpointSizes[] = "rows and cols must be positive and at most 2^31 - 256, with at most 2^35 - 4096 elements, padding included";
 static int mx4_matrix_ok(const dq_mx4_matrix_t &m)
 {
-    if (!dtype_ok(m.dtype) || (m.rand_pool && !dtype_ok(m.rand_dtype))) return fail(DQ_ERR_DTYPE);
+    if (!(dtype_ok(m.dtype) || m.dtype == DQ_E4M3) || (m.rand_pool && !dtype_ok(m.rand_dtype))) return fail(DQ_ERR_DTYPE);
+    if (m.dtype == DQ_E4M3) {
+        if (!checkpoint_size_ok(m.x_rows, m.x_cols)) return fail(DQ_ERR_SIZE, kCheckpointSizes);
+        if (m.stochastic) return fail(DQ_ERR_SIZE, "a checkpoint is rounded to nearest");
+        if (m.stride != (m.x_cols + 31) / 32 * 32 || (reinterpret_cast<uintptr_t>(m.x) & 15)) return fail(DQ_ERR_SIZE, "a checkpoint's stride is its padded columns, and it is 16-byte aligned");
+    }
     if (!mx4_size_ok(m.columns ? m.x_cols : m.x_rows, m.columns ? m.x_rows : m.x_cols)) return fail(DQ_ERR_SIZE, kMxSizes);
     if (m.stride < m.x_cols || m.stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
     if (m.rand_pool && !m.stochastic) return fail(DQ_ERR_SIZE, "a rand_pool is for stochastic rounding");
@@ -1210,7 +1222,8 @@ int dq_mx4_quantize_list(const dq_mx4_matrix_t *matrices, int count, int device,
         const int n = count - k < 16 ? count - k : 16;
         for (int i = 0; i < n; i++) {
             const dq_mx4_matrix_t &m = matrices[k + i];
-            list[i] = {{m.x, m.x_rows, m.x_cols, m.stride, m.codes, m.scales, m.sign, m.rand_pool, {m.seed, m.step}, m.step_dev}, m.dtype, m.rand_dtype, m.columns != 0, m.stochastic != 0};
+            list[i] = {{m.x, m.x_rows, m.x_cols, m.stride, m.codes, m.scales, m.sign, m.rand_pool, {m.seed, m.step}, m.step_dev,
+                        m.dtype == DQ_E4M3 ? static_cast<const uint8_t *>(m.x) + m.x_rows * m.stride : nullptr}, m.dtype, m.rand_dtype, m.columns != 0, m.stochastic != 0};
         }
         e = dq::launch_mx4_quantize_list(list, n, static_cast<hipStream_t>(stream));
     }
@@ -1240,6 +1253,32 @@ int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_
     int rc;
     if ((rc = select_device(device))) return rc;
     return finish(dq::launch_mx4_product(a_codes, a_scales, b_codes, b_scales, out, m, n, k, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int64_t dq_checkpoint_bytes(int64_t rows, int64_t cols) { return checkpoint_size_ok(rows, cols) ? rows * ((cols + 31) / 32) * 33 : 0; }
+
+int dq_checkpoint_compress(const void *x, int dtype, int64_t rows, int64_t cols, int64_t stride, uint8_t *data, int device, dq_stream_t stream)
+{
+    if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
+    if (!checkpoint_size_ok(rows, cols)) return fail(DQ_ERR_SIZE, kCheckpointSizes);
+    if (stride < cols || stride >= (int64_t)1 << 40) return fail(DQ_ERR_SIZE, "stride must be at least the columns");
+    if (!x || !data) return fail(DQ_ERR_NULL);
+    if (reinterpret_cast<uintptr_t>(data) & 15) return fail(DQ_ERR_SIZE, "data must be 16-byte aligned");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    const dq::CheckpointArgs a = {x, data, rows, stride, (uint32_t)cols};
+    return finish(dq::launch_checkpoint_compress(a, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int dq_checkpoint_restore(const uint8_t *data, void *out, int dtype, int64_t rows, int64_t cols, int device, dq_stream_t stream)
+{
+    if (!dtype_ok(dtype)) return fail(DQ_ERR_DTYPE);
+    if (!checkpoint_size_ok(rows, cols)) return fail(DQ_ERR_SIZE, kCheckpointSizes);
+    if (!data || !out) return fail(DQ_ERR_NULL);
+    if (reinterpret_cast<uintptr_t>(data) & 15) return fail(DQ_ERR_SIZE, "data must be 16-byte aligned");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    return finish(dq::launch_checkpoint_restore(data, out, rows, cols, dtype, static_cast<hipStream_t>(stream)));
 }
 
 } // extern "C"

@@ -1270,6 +1270,95 @@ PyObject *mx4_quantize(PyObject *, PyObject *const *v, Py_ssize_t have)
     });
 }
 
+// ---- 8-bit activation checkpoints (activations.py) ----
+
+int64_t checkpoint_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 31) / 32) * 33; }
+
+// a checkpoint's buffer, of rows x cols
+const uint8_t *checkpoint_of(const at::Tensor &data, int64_t rows, int64_t cols)
+{
+    need(data.scalar_type() == at::kByte && data.is_contiguous() && rows >= 0 && cols >= 0 && data.numel() == checkpoint_bytes(rows, cols),
+         "the data does not belong to a checkpoint of this size");
+    return static_cast<const uint8_t *>(data.data_ptr());
+}
+
+// x as rows of consecutive elements (a matrix whose rows are apart is taken as it is)
+at::Tensor as_rows(const at::Tensor &x)
+{
+    if (x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1) && (x.stride(0) >= x.size(1) || x.size(0) <= 1)) return x;
+    const int64_t cols = x.size(-1);
+    return x.reshape({c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)), cols}).contiguous();
+}
+int64_t row_stride(const at::Tensor &x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+at::Tensor new_bytes(const c10::Device &device, int64_t bytes) { return at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(device)); }
+
+void compress_into(const at::Tensor &x, uint8_t *data)
+{
+    if (x.numel())
+        check(dq_checkpoint_compress(x.data_ptr(), dtype_code(x), x.size(0), x.size(1), row_stride(x), data, x.device().index(), c10::hip::getCurrentHIPStream(x.device().index()).stream()));
+}
+
+// a tensor on the GPU, in any layout
+const at::Tensor &gpu_tensor(PyObject *o)
+{
+    if (!THPVariable_Check(o)) refuse(std::string("a tensor argument is required, got ") + Py_TYPE(o)->tp_name);
+    const at::Tensor &x = THPVariable_Unpack(o);
+    if (!x.is_cuda()) refuse("tensor arguments must live on the GPU (got a " + std::string(c10::DeviceTypeName(x.device().type(), true)) + " tensor)");
+    return x;
+}
+
+// x [..., cols] -> data
+PyObject *checkpoint_compress(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 1, [&]() -> PyObject * {
+        const at::Tensor &x = gpu_tensor(v[0]);
+        need(x.dim() >= 1, "compress: rows are required");
+        (void)dtype_code(x);
+        const c10::DeviceGuard on(x.device());
+        const at::NoGradGuard constant;
+        const at::Tensor rows = as_rows(x), data = new_bytes(x.device(), checkpoint_bytes(rows.size(0), rows.size(1)));
+        compress_into(rows, static_cast<uint8_t *>(data.data_ptr()));
+        return THPVariable_Wrap(data);
+    });
+}
+
+// data, rows, cols, a tensor of the element type asked for
+PyObject *checkpoint_restore(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 4, [&]() -> PyObject * {
+        Args a;
+        const at::Tensor &data = a.tensor(v[0]);
+        const int64_t rows = integer(v[1]), cols = integer(v[2]);
+        const uint8_t *from = checkpoint_of(data, rows, cols);
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const at::Tensor out = new_matrix(a.device, rows, cols, THPVariable_Unpack(v[3]).scalar_type());
+        if (rows && cols)
+            check(dq_checkpoint_restore(from, out.data_ptr(), dtype_code(out), rows, cols, a.device, c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream()));
+        return THPVariable_Wrap(out);
+    });
+}
+
+// data, rows, cols, columns, sign -> (codes, scales)
+PyObject *mx4_quantize_checkpoint(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 5, [&]() -> PyObject * {
+        Args a;
+        const at::Tensor &data = a.tensor(v[0]);
+        const int64_t rows = integer(v[1]), cols = integer(v[2]);
+        const uint8_t *from = checkpoint_of(data, rows, cols);
+        const bool columns = PyObject_IsTrue(v[3]);
+        const int64_t vectors = columns ? cols : rows, supers = ((columns ? rows : cols) + 255) / 256;
+        const uint32_t *sign = v[4] == Py_None ? nullptr : reinterpret_cast<const uint32_t *>(a.typed(v[4], at::kInt, 8 * supers, "sign").data_ptr<int32_t>());
+        const c10::OptionalDeviceGuard on(cuda(a.device));
+        const at::Tensor codes = new_matrix(a.device, vectors, 128 * supers, at::kByte), scales = new_matrix(a.device, vectors, 8 * supers, at::kByte);
+        if (rows && cols)
+            check(dq_mx4_quantize(from, DQ_E4M3, rows, cols, (cols + 31) / 32 * 32, columns, sign, 0, nullptr, 0, 0, 0, nullptr, static_cast<uint8_t *>(codes.data_ptr()),
+                                  static_cast<uint8_t *>(scales.data_ptr()), a.device, c10::hip::getCurrentHIPStream((c10::DeviceIndex)a.device).stream()));
+        return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(codes)).ptr(), py::reinterpret_steal<py::object>(THPVariable_Wrap(scales)).ptr());
+    });
+}
+
 // codes, scales, rows, cols, a tensor of the element type asked for
 PyObject *mx4_dequantize(PyObject *, PyObject *const *v, Py_ssize_t have)
 {
@@ -1344,6 +1433,19 @@ struct Quantizer {
         made.push_back(q);
         bytes += (q.rows * 136 * supers + 15) / 16 * 16;
     }
+    // the columns of a checkpoint of rows x cols
+    void add_checkpoint(const at::Tensor &data, int64_t rows, int64_t cols, const at::Tensor &sign)
+    {
+        Quantized q;
+        q.rows = cols;
+        q.length = rows;
+        const int64_t supers = (q.length + 255) / 256;
+        linear_takes(sign, at::Tensor(), q.rows, q.length, data.device());
+        list.push_back({checkpoint_of(data, rows, cols), rows, cols, (cols + 31) / 32 * 32, sign.defined() ? reinterpret_cast<const uint32_t *>(sign.data_ptr<int32_t>()) : nullptr,
+                        nullptr, 0, 0, nullptr, nullptr, nullptr, DQ_E4M3, true, false, 0});
+        made.push_back(q);
+        bytes += (q.rows * 136 * supers + 15) / 16 * 16;
+    }
     void run(const c10::Device &device)
     {
         held = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(device));
@@ -1361,9 +1463,9 @@ struct Quantizer {
     }
 };
 
-at::Tensor product_of(const Quantized &a, const Quantized &b, const at::Tensor &like)
+at::Tensor product_of(const Quantized &a, const Quantized &b, const c10::Device &device, at::ScalarType dtype)
 {
-    const at::Tensor out = at::empty({a.rows, b.rows}, like.options().requires_grad(false));
+    const at::Tensor out = at::empty({a.rows, b.rows}, at::TensorOptions().dtype(dtype).device(device));
     if (a.rows && b.rows && a.length)
         check(dq_mx4_product(a.codes, a.scales, b.codes, b.scales, out.data_ptr(), dtype_code(out), a.rows, b.rows, a.length, out.device().index(),
                              c10::hip::getCurrentHIPStream(out.device().index()).stream()));
@@ -1376,22 +1478,34 @@ at::Tensor product_of(const Quantized &a, const Quantized &b, const at::Tensor &
 constexpr uint64_t kColumns = (uint64_t)1 << 63;
 
 struct Linear4 : public torch::autograd::Function<Linear4> {
-    // x [tokens, k] and weight [n, k], contiguous
+    // x [tokens, k] and weight [n, k], contiguous.  kept: the checkpoint of x that the backward pass takes in its place; eight without one: x is cut to one here
     typedef std::optional<at::Tensor> Maybe;
     static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &sign_out, const Maybe &sign_tokens,
-                              const Maybe &pool_rows, const Maybe &pool_columns, const Maybe &step_dev, bool seeded, int64_t seed, int64_t step)
+                              const Maybe &pool_rows, const Maybe &pool_columns, const Maybe &step_dev, bool seeded, int64_t seed, int64_t step,
+                              bool eight, const Maybe &kept)
     {
-        ctx->save_for_backward({x, weight, sign_out.value_or(at::Tensor()), sign_tokens.value_or(at::Tensor()), pool_rows.value_or(at::Tensor()), pool_columns.value_or(at::Tensor()), step_dev.value_or(at::Tensor())});
+        const c10::DeviceGuard on(x.device());
+        at::Tensor keep = x;
+        if (eight) {
+            keep = kept.value_or(at::Tensor());
+            if (!keep.defined() && weight.requires_grad()) {
+                keep = new_bytes(x.device(), checkpoint_bytes(x.size(0), x.size(1)));
+                compress_into(x, static_cast<uint8_t *>(keep.data_ptr()));
+            }
+        }
+        ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
+        ctx->saved_data["tokens"] = x.size(0);
+        ctx->saved_data["eight"] = eight;
+        ctx->save_for_backward({keep, weight, sign_out.value_or(at::Tensor()), sign_tokens.value_or(at::Tensor()), pool_rows.value_or(at::Tensor()), pool_columns.value_or(at::Tensor()), step_dev.value_or(at::Tensor())});
         ctx->saved_data["seeded"] = seeded;
         ctx->saved_data["seed"] = seed;
         ctx->saved_data["step"] = step;
-        const c10::DeviceGuard on(x.device());
         const at::Tensor none;
         Quantizer q;
         q.add(x, false, none, none, false, 0, 0, none);
         q.add(weight, false, none, none, false, 0, 0, none);
         q.run(x.device());
-        return product_of(q.made[0], q.made[1], x);
+        return product_of(q.made[0], q.made[1], x.device(), x.scalar_type());
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
     {
@@ -1400,9 +1514,10 @@ struct Linear4 : public torch::autograd::Function<Linear4> {
         const at::Tensor &x = saved[0], &weight = saved[1], &sign_out = saved[2], &sign_tokens = saved[3], &pool_rows = saved[4], &pool_columns = saved[5], &step_dev = saved[6], none;
         const bool seeded = ctx->saved_data["seeded"].toBool();
         const uint64_t seed = (uint64_t)ctx->saved_data["seed"].toInt(), step = (uint64_t)ctx->saved_data["step"].toInt();
-        torch::autograd::tensor_list out(10);
+        torch::autograd::tensor_list out(12);
         if (!grads[0].defined()) return out;
-        const c10::DeviceGuard on(x.device());
+        const c10::Device device = weight.device();
+        const c10::DeviceGuard on(device);
         const at::Tensor dy = grads[0].contiguous();
         const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1);
         Quantizer q;
@@ -1412,19 +1527,41 @@ struct Linear4 : public torch::autograd::Function<Linear4> {
         }
         if (dw) {
             q.add(dy, true, sign_tokens, pool_columns, seeded || pool_columns.defined(), seed, step + kColumns, step_dev);
-            q.add(x, true, sign_tokens, none, false, 0, 0, none);
+            if (ctx->saved_data["eight"].toBool())
+                q.add_checkpoint(x, ctx->saved_data["tokens"].toInt(), weight.size(1), sign_tokens);
+            else
+                q.add(x, true, sign_tokens, none, false, 0, 0, none);
         }
-        q.run(x.device());
-        if (dx) out[0] = product_of(q.made[0], q.made[1], x);
-        if (dw) out[1] = product_of(q.made[dx ? 2 : 0], q.made[dx ? 3 : 1], weight);
+        q.run(device);
+        if (dx) out[0] = product_of(q.made[0], q.made[1], device, (at::ScalarType)ctx->saved_data["dtype"].toInt());
+        if (dw) out[1] = product_of(q.made[dx ? 2 : 0], q.made[dx ? 3 : 1], device, weight.scalar_type());
         return out;
     }
 };
 
-// x, weight, signs of the outputs and of the tokens, pools of the gradient's rows and columns, seed (None: no random stream), step
+// The engine hands a leaf's gradient to the stream that the leaf's node was made on.  That node is alive as long as an earlier graph of the leaf is, or a reducer or hook
+// that holds it.  A stream of one's own joins a recording by the engine's events and leaves it again; the default stream cannot take part in one, and to draw it in ends
+// badly; so that is refused.
+void leaves_can_be_recorded(const char *what, const c10::Device &device, std::initializer_list<const at::Tensor *> tensors)
+{
+    if (!at::GradMode::is_enabled()) return;
+    const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(device.index());
+    unsigned long long recording;
+    if (!Buckets::capturing(now.stream(), &recording)) return;
+    for (const at::Tensor *t : tensors) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const std::optional<c10::Stream> of = node ? node->stream() : std::nullopt;
+        if (of && of->id() == c10::hip::getDefaultHIPStream(device.index()).id())
+            refuse(std::string(what) + ": the node of a leaf's gradient was made on the default stream, which cannot be recorded, and is still alive: let go of the outputs (or the reducer, "
+                   "or hook) that hold it before recording, or make them on another stream");
+    }
+}
+
+// x, weight, signs of the outputs and of the tokens, pools of the gradient's rows and columns, seed (None: no random stream), step, checkpoint (None, True or the data of one)
 PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
 {
-    return answering(have, 8, [&]() -> PyObject * {
+    return answering(have, 9, [&]() -> PyObject * {
         for (int k = 0; k < 2; k++)
             if (!THPVariable_Check(v[k])) refuse(std::string("a tensor argument is required, got ") + Py_TYPE(v[k])->tp_name);
         const at::Tensor &x = THPVariable_Unpack(v[0]), &weight = THPVariable_Unpack(v[1]);
@@ -1453,25 +1590,17 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
             if (x.requires_grad()) linear_takes(extra[0].value_or(at::Tensor()), extra[2].value_or(at::Tensor()), tokens, n, x.device());
             if (weight.requires_grad()) linear_takes(extra[1].value_or(at::Tensor()), extra[3].value_or(at::Tensor()), n, tokens, x.device());
         }
-        // The engine hands a leaf's gradient to the stream that the leaf's node was made on.  That node is alive as long as an earlier graph of the leaf is, or a reducer or hook
-        // that holds it.  A stream of one's own joins a recording by the engine's events and leaves it again; the default stream cannot take part in one, and to draw it in ends
-        // badly; so that is refused here.
-        if (at::GradMode::is_enabled()) {
-            const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(x.device().index());
-            unsigned long long recording;
-            if (Buckets::capturing(now.stream(), &recording))
-                for (const at::Tensor *t : {&x, &weight}) {
-                    if (!t->requires_grad() || !t->is_leaf()) continue;
-                    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(*t);
-                    const std::optional<c10::Stream> of = node ? node->stream() : std::nullopt;
-                    need(!of || of->id() != c10::hip::getDefaultHIPStream(x.device().index()).id(),
-                         "linear: the node of a leaf's gradient was made on the default stream, which cannot be recorded, and is still alive: let go of the outputs (or the reducer, "
-                         "or hook) that hold it before recording, or make them on another stream");
-                }
+        leaves_can_be_recorded("linear", x.device(), {&x, &weight});
+        const bool eight = v[8] != Py_None && at::GradMode::is_enabled();
+        std::optional<at::Tensor> kept;
+        if (v[8] != Py_None && v[8] != Py_True) {
+            kept = gpu_tensor(v[8]);
+            need(kept->device() == x.device(), "tensor arguments live on different devices");
+            (void)checkpoint_of(*kept, tokens, k);
         }
         // (a matrix that is contiguous takes part as it is: views of it would be nodes of the graph)
         const at::Tensor flat = x.dim() == 2 && x.is_contiguous() ? x : x.reshape({tokens, k}).contiguous();
-        at::Tensor y = Linear4::apply(flat, weight.is_contiguous() ? weight : weight.contiguous(), extra[0], extra[1], extra[2], extra[3], step_dev, seeded, seed, step);
+        at::Tensor y = Linear4::apply(flat, weight.is_contiguous() ? weight : weight.contiguous(), extra[0], extra[1], extra[2], extra[3], step_dev, seeded, seed, step, eight, kept);
         if (x.dim() != 2) {
             std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
             shape.push_back(n);
@@ -1488,6 +1617,9 @@ PyMethodDef kFunctions[] = {
     {"mx4_quantize", reinterpret_cast<PyCFunction>(mx4_quantize), METH_FASTCALL, nullptr},
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(mx4_dequantize), METH_FASTCALL, nullptr},
     {"mx4_product", reinterpret_cast<PyCFunction>(mx4_product), METH_FASTCALL, nullptr},
+    {"mx4_quantize_checkpoint", reinterpret_cast<PyCFunction>(mx4_quantize_checkpoint), METH_FASTCALL, nullptr},
+    {"checkpoint_compress", reinterpret_cast<PyCFunction>(checkpoint_compress), METH_FASTCALL, nullptr},
+    {"checkpoint_restore", reinterpret_cast<PyCFunction>(checkpoint_restore), METH_FASTCALL, nullptr},
     {"mx4_linear", reinterpret_cast<PyCFunction>(mx4_linear), METH_FASTCALL, nullptr},
     {"scaling_compress", reinterpret_cast<PyCFunction>(scaling_compress), METH_FASTCALL, nullptr},
     {"scaling_decompress", reinterpret_cast<PyCFunction>(scaling_decompress), METH_FASTCALL, nullptr},

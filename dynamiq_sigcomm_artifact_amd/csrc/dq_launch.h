@@ -400,6 +400,7 @@ struct QuantizeArgs {
     const void *pool;
     RandKey key;
     const uint64_t *step_dev; // null, or a value in device memory that is added to the step of the random stream
+    const uint8_t *x_scales;  // of a checkpoint, whose codes are x
 };
 hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, bool stochastic, int pool_dtype, hipStream_t stream);
 // one matrix of a list
@@ -413,5 +414,15 @@ hipError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, vo
                                  hipStream_t stream);
 hipError_t launch_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales, void *out,
                               int64_t m, int64_t n, int64_t k, int dtype, hipStream_t stream);
+
+// activation checkpoints (dq_activations.hip)
+struct CheckpointArgs {
+    const void *x;
+    uint8_t *data;
+    int64_t rows, stride;
+    uint32_t cols;
+};
+hipError_t launch_checkpoint_compress(const CheckpointArgs &a, int dtype, hipStream_t stream);
+hipError_t launch_checkpoint_restore(const uint8_t *data, void *out, int64_t rows, int64_t cols, int dtype, hipStream_t stream);
 
 } // namespace dq

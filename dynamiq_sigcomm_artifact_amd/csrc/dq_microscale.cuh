@@ -1,10 +1,22 @@
 // Microscaled blocks: 32 consecutive elements share a power of two 2^k, stored as the byte k + 127 (255: the block is not a number).
-// What the 4-bit operands of products and the 8-bit optimizer states have in common.
+// What the 4-bit operands of products, the 8-bit optimizer states and the 8-bit activation checkpoints have in common.
 #pragma once
 
 #include "dq_device.cuh"
 
 namespace dq {
+
+// n / by for n below 2^bits (at most 30): (n mul) >> shift with mul = ceil(2^shift / by) and shift = bits + ceil(log2 by), whose excess is less than n 2^-shift
+struct Division {
+    uint32_t by, mul, shift;
+    Division() = default;
+    explicit Division(uint32_t by_, uint32_t bits = 27) : by(by_), shift(bits)
+    {
+        while (((uint64_t)1 << (shift - bits)) < by) shift++;
+        mul = (uint32_t)((((uint64_t)1 << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((uint64_t)n * mul >> shift); }
+};
 
 // ---- four or eight consecutive elements of a vector that may lie anywhere: a view into a gradient bucket is aligned to its elements only, and
 // gfx950 loads and stores 16 bytes from any address.  PASSING: with the hint that nothing of it is wanted again soon ----
@@ -175,5 +187,42 @@ __device__ __forceinline__ float scale_up(uint32_t byte)
     const uint32_t bits = byte << 23;
     return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : bits);
 }
+
+
+// ---- activation checkpoints: eight E4M3 codes of a lane in two words, four neighbouring lanes hold a block ----
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// Rounded to nearest, ties to even, with the least k for which the block's largest is at most 448 2^k.  At the largest k that a type needs, 240 2^k is the last multiple within its
+// range, and magnitudes beyond become that: what is finite stays so in its own type.  The scale is the same in the block's lanes; of a block that is not a number the codes mean nothing.
+template <int DT> __device__ __forceinline__ u32x2_t encode_e4m3(const float (&v)[8], uint32_t &scale)
+{
+    constexpr uint32_t kLast = DT == DQ_F16 ? 127 + 8 : 127 + 120;
+    scale = block_scale<8, 0x600000u>(block_max(v));
+    const float down = scale_down(scale), most = scale == kLast ? 240.0f : 448.0f;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = __builtin_amdgcn_fmed3f(v[j] * down, -most, most);
+    u32x2_t w;
+    w[0] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+    w[1] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false), true);
+    return w;
+}
+__device__ __forceinline__ void decode_e4m3(u32x2_t w, uint32_t scale, float (&v)[8])
+{
+    const float up = scale_up(scale);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(w[k], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w[k], true);
+        v[4 * k] = a.x * up; v[4 * k + 1] = a.y * up; v[4 * k + 2] = b.x * up; v[4 * k + 3] = b.y * up;
+    }
+}
+
+// a checkpoint's buffer: codes [rows][32 blocks], scales [rows][blocks]
+template <class BYTE> struct CheckpointOf {
+    BYTE *codes, *scales;
+    uint32_t blocks;
+    __host__ __device__ __forceinline__ CheckpointOf(BYTE *data, int64_t rows, uint32_t cols) : codes(data), scales(data + rows * ((cols + 31) >> 5) * 32), blocks((cols + 31) >> 5) {}
+};
 
 } // namespace dq

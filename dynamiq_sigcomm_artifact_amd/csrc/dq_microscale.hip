@@ -1,23 +1,13 @@
 // 4-bit microscaled matrices: quantised along the rows or the columns, and their values.
 //
+// x may also be an activation checkpoint (DQ_E4M3), whose values are taken as they are: what a weight's gradient reads of it is a byte an element.
+//
 // Both quantisers give a block of 32 elements to four neighbouring lanes, eight each: its largest magnitude and the last two stages of its
 // rotation are two exchanges within the quad, and a lane's eight codes are one word.
 #include "dq_launch.h"
 #include "dq_microscale.cuh"
 
 namespace dq {
-
-// n / by for n below 2^27: (n mul) >> shift with mul = ceil(2^shift / by) and shift = 27 + ceil(log2 by), whose excess is less than n 2^-shift
-struct Division {
-    uint32_t by, mul, shift;
-    Division() = default;
-    explicit Division(uint32_t by_) : by(by_), shift(27)
-    {
-        while (((uint64_t)1 << (shift - 27)) < by) shift++;
-        mul = (uint32_t)((((uint64_t)1 << shift) + by - 1) / by);
-    }
-    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((uint64_t)n * mul >> shift); }
-};
 
 enum { kNearest = -1, kPhilox = -2 }; // otherwise the element type of the pool
 
@@ -126,9 +116,16 @@ template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void quantiz
     const int g = threadIdx.x & 3;
     const uint32_t row = superchunks(unit >> 5), col = (unit - row * superchunks.by * 32) * 8;
     float v[8], u[8];
-    const int64_t at = (int64_t)row * a.stride + col;
+    [[maybe_unused]] const int64_t at = (int64_t)row * a.stride + col;
     const auto load = [&] {
-        if (col + 8 <= (uint32_t)a.cols)
+        if constexpr (DT == DQ_E4M3) {
+            const uint32_t from = min(col, (uint32_t)a.stride - 8); // (the stride is a multiple of 32)
+            decode_e4m3(*reinterpret_cast<const u32x2_t *>(static_cast<const uint8_t *>(a.x) + (int64_t)row * a.stride + from),
+                        a.x_scales[(int64_t)row * (a.stride >> 5) + (from >> 5)], v);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (col + j >= (uint32_t)a.cols) v[j] = 0.0f;
+        } else if (col + 8 <= (uint32_t)a.cols)
             load8<DT>(a.x, at, v);
         else
             load_part<DT, 8>(a.x, at, row * a.stride + a.cols, v);
@@ -172,6 +169,13 @@ struct ColumnsLds {
     __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __attribute__((aligned(8))) uint8_t scales[128 * 8];
 };
+// element j of eight E4M3 codes (j a constant once the loop around it is unrolled)
+__device__ __forceinline__ float byte_value(const uint32_t (&x)[2], int j)
+{
+    const f32x2_t v = j & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(x[j >> 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8(x[j >> 2], false);
+    return j & 1 ? v.y : v.x;
+}
+
 template <int DT, int RAND, bool ROTATE>
 __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t superchunks, const Division &tiles, uint32_t id, ColumnsLds &lds)
 {
@@ -179,9 +183,20 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
     const uint32_t superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
     const uint32_t row0 = superchunk * 256 + 32 * block, row = row0 + 8 * g;
-    constexpr int WORDS = DT == DQ_F32 ? 8 : 4;
+    constexpr int WORDS = DT == DQ_F32 ? 8 : DT == DQ_E4M3 ? 2 : 4;
     uint32_t x[8][WORDS]; // [row][column], as they are in memory
-    if (all_cols >= 8) {
+    float up[8];          // of a checkpoint's rows
+    if constexpr (DT == DQ_E4M3) {
+        const uint32_t from = min(col, (uint32_t)a.stride - 8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int64_t r = min(row + j, last_row);
+            const u32x2_t w = *reinterpret_cast<const u32x2_t *>(static_cast<const uint8_t *>(a.x) + r * a.stride + from);
+            x[j][0] = w[0];
+            x[j][1] = w[1];
+            up[j] = scale_up(a.x_scales[r * (a.stride >> 5) + (from >> 5)]);
+        }
+    } else if (all_cols >= 8) {
         // a lane whose eight columns reach past the end loads the last eight, and moves them up
         const uint32_t from = min(col, all_cols - 8), up = col - from;
 #pragma unroll
@@ -209,6 +224,7 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
             if (row + j > last_row) {
 #pragma unroll
                 for (int w = 0; w < WORDS; w++) x[j][w] = 0u;
+                up[j] = 0.0f;
             }
     }
     const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u, first = col * superchunks + superchunk, most = (all_cols - 1) * superchunks + superchunk;
@@ -224,7 +240,12 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
     for (int c = 0; c < 8; c++) {
         float v[8], u[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = word_value<DT>(x[j], c);
+        for (int j = 0; j < 8; j++) {
+            if constexpr (DT == DQ_E4M3)
+                v[j] = byte_value(x[j], c) * up[j];
+            else
+                v[j] = word_value<DT>(x[j], c);
+        }
         draw(c, u);
         if (ROTATE) rotate_block(v, sign, g);
         uint32_t scale;
@@ -240,7 +261,12 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
             const auto load = [&] {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    v[j] = ElemIO<DT>::load(a.x, (int64_t)min(row + j, last_row) * a.stride + min(col + c, all_cols - 1));
+                    const int64_t r = min(row + j, last_row);
+                    const uint32_t at = min(col + c, all_cols - 1);
+                    if constexpr (DT == DQ_E4M3)
+                        v[j] = __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t *>(a.x)[r * a.stride + at], 0) * scale_up(a.x_scales[r * (a.stride >> 5) + (at >> 5)]);
+                    else
+                        v[j] = ElemIO<DT>::load(a.x, r * a.stride + at);
                     if (row + j > last_row) v[j] = 0.0f;
                 }
             };
@@ -305,6 +331,7 @@ template <int DT> static hipError_t launch_quantize_of(const QuantizeArgs &a, bo
 
 hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, bool stochastic, int pool_dtype, hipStream_t stream)
 {
+    if (dtype == DQ_E4M3) return launch_quantize<DQ_E4M3, kNearest>(a, columns, stream); // (a checkpoint is rounded to the nearest)
     return dtype == DQ_F32 ? launch_quantize_of<DQ_F32>(a, columns, stochastic, pool_dtype, stream)
          : dtype == DQ_BF16 ? launch_quantize_of<DQ_BF16>(a, columns, stochastic, pool_dtype, stream)
                             : launch_quantize_of<DQ_F16>(a, columns, stochastic, pool_dtype, stream);
@@ -312,7 +339,7 @@ hipError_t launch_mx4_quantize(const QuantizeArgs &a, int dtype, bool columns, b
 
 // ---- several small matrices at once -------------------------------------------------------------------------
 
-// Up to four matrices of one element type, along either axis and rounded in any way: a workgroup takes 4096 elements along the rows or a tile along the columns.  A small
+// Up to four matrices of one element type, and checkpoints, along either axis and rounded in any way: a workgroup takes 4096 elements along the rows or a tile along the columns.  A small
 // one leaves most CUs without work and costs a launch all the same: a linear layer's step of 333 x 776 x 1000, in a graph, takes 28 us with two such launches where six
 // quantisers of their own made it 44, of 2048 x 2048 x 2048 56 for 66, of 4096 x 4096 x 4096 171 for 177.  What shares a launch has 4096 workgroups at most: 4096 x 14336 x 4096,
 // whose last three matrices have just those, takes 534 us for 542 alone, 6000 x 6000 x 6000 500 for 512.  Without that limit, with the largest ones in kernels that hold
@@ -355,7 +382,9 @@ template <int DT> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void m
     case 6: return do_job<DT, DQ_BF16, false>(j, columns, id, lds);
     case 7: return do_job<DT, DQ_BF16, true>(j, columns, id, lds);
     case 8: return do_job<DT, DQ_F32, false>(j, columns, id, lds);
-    default: return do_job<DT, DQ_F32, true>(j, columns, id, lds);
+    case 9: return do_job<DT, DQ_F32, true>(j, columns, id, lds);
+    case 10: return do_job<DQ_E4M3, kNearest, false>(j, columns, id, lds);
+    default: return do_job<DQ_E4M3, kNearest, true>(j, columns, id, lds);
     }
 }
 
@@ -365,10 +394,14 @@ hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStrea
         return q.columns ? ((q.a.cols + 127) >> 7) * ((q.a.rows + 255) >> 8) : (q.a.rows * ((q.a.cols + 255) >> 8) + 15) >> 4;
     };
     for (int next = 0; next < count;) {
-        int take = 0;
+        int take = 0, dtype = DQ_E4M3; // the type of what is no checkpoint
         int64_t blocks = 0;
-        while (take < kJobs && next + take < count && list[next + take].dtype == list[next].dtype && blocks + blocks_of(list[next + take]) <= kJobBlocks)
+        while (take < kJobs && next + take < count && blocks + blocks_of(list[next + take]) <= kJobBlocks) {
+            const int of = list[next + take].dtype;
+            if (of != DQ_E4M3 && dtype != DQ_E4M3 && of != dtype) break;
+            if (of != DQ_E4M3) dtype = of;
             blocks += blocks_of(list[next + take++]);
+        }
         hipError_t e;
         if (take < 2) {
             const QuantizeOne &q = list[next++];
@@ -386,13 +419,13 @@ hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStrea
                 j.superchunks = (uint32_t)(((q.columns ? q.a.rows : q.a.cols) + 255) >> 8);
                 j.by = Division(q.columns ? (uint32_t)((q.a.cols + 127) >> 7) : j.superchunks);
                 j.units = (uint32_t)(q.a.rows * j.superchunks * 32);
-                j.kind = (q.columns ? 16 : 0) + (!q.stochastic ? 0 : !q.a.pool ? 2 : 4 + 2 * q.pool_dtype) + (q.a.sign ? 1 : 0);
+                j.kind = (q.columns ? 16 : 0) + (q.dtype == DQ_E4M3 ? 10 : !q.stochastic ? 0 : !q.a.pool ? 2 : 4 + 2 * q.pool_dtype) + (q.a.sign ? 1 : 0);
                 first += (uint32_t)blocks_of(q);
             }
             const dim3 grid((uint32_t)blocks), block(512);
-            e = list[next].dtype == DQ_F32 ? launch_with(mx4_jobs_kernel<DQ_F32>, grid, block, stream, jobs)
-              : list[next].dtype == DQ_BF16 ? launch_with(mx4_jobs_kernel<DQ_BF16>, grid, block, stream, jobs)
-                                            : launch_with(mx4_jobs_kernel<DQ_F16>, grid, block, stream, jobs);
+            e = dtype == DQ_F32 ? launch_with(mx4_jobs_kernel<DQ_F32>, grid, block, stream, jobs)
+              : dtype == DQ_F16 ? launch_with(mx4_jobs_kernel<DQ_F16>, grid, block, stream, jobs)
+                                : launch_with(mx4_jobs_kernel<DQ_BF16>, grid, block, stream, jobs);
             next += take;
         }
         if (e != hipSuccess) return e;

@@ -10,6 +10,7 @@ numbers of the recording, unless step is an int64 tensor [1] on the device, whic
 import torch
 
 from . import capi
+from .activations import Checkpoint
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -37,6 +38,7 @@ class Microscaled(object):
 
 def quantize(x, columns=False, sign=None, rand_pool=None, seed=None, step=0):
     """x [r, c] (fp16, bf16 or fp32; the elements of a row consecutive) -> Microscaled: its rows, or with ``columns`` its columns, as vectors.
+    x may be an activations.Checkpoint, whose values are rounded to nearest.
 
     sign: int32 [>= 8 s], the packed signs of capi.pack_signs or capi.rand_diag_bits, one per element of a vector: every block of 32 is rotated,
     H (s x) / sqrt(32).  The product of two matrices that are rotated with the same signs is that of the matrices.
@@ -44,6 +46,11 @@ def quantize(x, columns=False, sign=None, rand_pool=None, seed=None, step=0):
     in-kernel stream, the codec's, whose values are the 128 odd multiples of 1/256: elements up to 2^k / 512, k of their block, become 0 in every draw,
     and the mean of the draws of another is off by up to 1/256 of the distance between its neighbours (a float32 pool has 24 bits);
     neither: to nearest, ties to even.  Nothing here but linear() is differentiated."""
+    if isinstance(x, Checkpoint):
+        if rand_pool is not None or seed is not None:
+            raise RuntimeError("quantize: a checkpoint is rounded to nearest")
+        codes, scales = capi.host().mx4_quantize_checkpoint(x.data, x.rows, x.cols, columns, sign)
+        return Microscaled(codes, scales, x.cols if columns else x.rows, x.rows if columns else x.cols)
     codes, scales = capi.host().mx4_quantize(x, columns, sign, rand_pool, seed, step)
     r, c = x.shape
     return Microscaled(codes, scales, c if columns else r, r if columns else c)
@@ -70,7 +77,7 @@ def product(a, b, dtype=torch.bfloat16):
     return capi.host().mx4_product(a.codes, a.scales, b.codes, b.scales, a.rows, b.rows, a.cols, _like(dtype))
 
 
-def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0):
+def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0, checkpoint=None):
     """y = x weight^T for x [..., k] and weight [n, k], all three products of a training step in 4 bits:
 
       y  = Q(x) Q(weight)^T             along k, to nearest
@@ -83,6 +90,15 @@ def linear(x, weight, sign=None, rand_pool=None, seed=None, step=0):
     sign: (signs of n, signs of the tokens), packed; None leaves R out.  rand_pool: (pool [tokens, n padded to 256], pool [n, tokens padded to
     256]), checked here where their gradient is wanted, or seed and step: then every call needs a step of its own, below 2^63 (the gradient's rows draw at step, its columns at step + 2^63).
     With neither the gradients are rounded to nearest, too.  A step on the device stays as it is until the backward pass has run.  The gradients
-    cannot be differentiated again."""
+    cannot be differentiated again.
+
+    checkpoint: the backward pass keeps c(x), x in 8 bits (activations.compress), in place of x, and dw takes its columns from there.  True: made here, where weight wants a
+    gradient; or the Checkpoint of x that activations.residual_norm or gated has made, which several layers may share."""
     signs, pools = sign or (None, None), rand_pool or (None, None)
-    return capi.host().mx4_linear(x, weight, signs[0], signs[1], pools[0], pools[1], seed, step)
+    if isinstance(checkpoint, Checkpoint):
+        if checkpoint.cols != x.shape[-1]:
+            raise RuntimeError("linear: the checkpoint is of %d columns, x of %d" % (checkpoint.cols, x.shape[-1]))
+        kept = checkpoint.data
+    else:
+        kept = True if checkpoint else None
+    return capi.host().mx4_linear(x, weight, signs[0], signs[1], pools[0], pools[1], seed, step, kept)

@@ -35,7 +35,8 @@ typedef void *dq_stream_t; /* hipStream_t */
 enum dq_dtype {
     DQ_F16 = 0,  /* reference __half path: every intermediate in binary16   */
     DQ_BF16 = 1, /* reference __nv_bfloat16 path: fp32 math, bf16 storage   */
-    DQ_F32 = 2   /* extension: the bf16 path's math on fp32 storage         */
+    DQ_F32 = 2,  /* extension: the bf16 path's math on fp32 storage         */
+    DQ_E4M3 = 3  /* an 8-bit activation checkpoint, where that is said      */
 };
 /* OR-ed into the dtype argument of dq_scaling_compress / dq_scaling_dec_comp:
  * rand_pool holds bfloat16 values although the gradient elements are DQ_F32
@@ -836,7 +837,9 @@ int dq_adamw_coefficients(int64_t *steps, double lr, const float *lr_dev, double
  * resolves as many bits as its values have.  step_dev (may be NULL): one uint64
  * in device memory that is added to step, so that a recorded call draws anew.
  * A block that holds an infinity or NaN is NaN, and so is one whose rotation is beyond
- * what the largest scale, 2^127, holds (its elements alone never are). */
+ * what the largest scale, 2^127, holds (its elements alone never are).
+ * dtype DQ_E4M3: x is a checkpoint of x_rows x x_cols (dq_checkpoint_compress), 16-byte aligned,
+ * stride 32 ceil(x_cols / 32), rounded to nearest only. */
 int dq_mx4_quantize(const void *x, int dtype, int64_t x_rows, int64_t x_cols, int64_t stride, int columns,
                     const uint32_t *sign, int stochastic, const void *rand_pool, int rand_dtype, uint64_t seed,
                     uint64_t step, const uint64_t *step_dev, uint8_t *codes, uint8_t *scales, int device,
@@ -862,6 +865,25 @@ int dq_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, in
 int dq_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes,
                    const uint8_t *b_scales, void *out, int dtype, int64_t m, int64_t n, int64_t k, int device,
                    dq_stream_t stream);
+
+/* ---- 8-bit activation checkpoints -------------------------------------
+ *
+ * No counterpart in the reference.  What a backward pass keeps of an activation, a matrix of
+ * rows x cols, in one buffer: with b = ceil(cols / 32)
+ *   codes  uint8 [rows][32 b], E4M3, zero behind the cols-th
+ *   scales uint8 [rows][b], the byte k + 127 of a block of 32: its values are the codes' times
+ *          2^k, k >= -127 the least with max <= 448 2^k (255: the block holds an infinity or
+ *          NaN, and is NaN; its codes mean nothing)
+ * rounded to nearest, ties to even.  At the largest k of the matrix' type, 8 for binary16 and 120 for
+ * the others, magnitudes beyond 240 2^k become that: finite values stay finite in their type.
+ * data 16-byte aligned; rows and cols at most 2^31 - 256, and 32 b rows at most 2^35 - 4096. */
+int64_t dq_checkpoint_bytes(int64_t rows, int64_t cols);
+/* x: row i from element i * stride on */
+int dq_checkpoint_compress(const void *x, int dtype, int64_t rows, int64_t cols, int64_t stride, uint8_t *data,
+                           int device, dq_stream_t stream);
+/* out: `dtype` [rows][cols], the values rounded to nearest */
+int dq_checkpoint_restore(const uint8_t *data, void *out, int dtype, int64_t rows, int64_t cols, int device,
+                          dq_stream_t stream);
 
 #ifdef __cplusplus
 }
