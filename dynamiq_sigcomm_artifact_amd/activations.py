@@ -56,3 +56,43 @@ def restore(c, dtype=torch.float32):
     if dtype not in _EMPTY:
         raise RuntimeError("unsupported element dtype %s" % dtype)
     return capi.host().checkpoint_restore(c.data, c.rows, c.cols, _EMPTY[dtype])
+
+
+def residual_norm(y, residual=None, weight=None, bias=None, gate=None, residual_scale=1.0, block_scale=1.0, after=False, after_weight=None, after_bias=None, before=True,
+                  center=False, eps=1e-6, checkpoint=False):
+    """what lies between a block's last linear layer and the next block's first, in one pass over y [..., cols], the block's output:
+
+      z = norm(y) * after_weight + after_bias     the norm after the block, with ``after``; otherwise y
+      r = residual_scale * residual + block_scale * gate * z
+      h = norm(r) * weight + bias                 the norm before the next block, unless ``before`` is False
+
+    norm(x) = x / sqrt(mean(x^2) + eps), or with ``center`` (x - mean(x)) / sqrt(variance(x) + eps).  Everything but y may be missing.
+
+    residual: of y's shape; its type, y's or float32, is r's.  gate: [cols], or of y's shape with ones in place of the last dimensions that share it: [batch, 1, cols] is a gate
+    for each sequence.  weights, biases, gate: of y's type or float32, and so are their gradients.  cols: 8 to 32768.
+
+    -> (h, r), r being y itself where nothing is added to it or done with it; r alone without ``before``.
+    checkpoint: (h, r, c) with c the Checkpoint of h, for the layers that take it, and the backward pass keeps r and y in 8 bits.
+    What is not contiguous is copied.  The gradients cannot be differentiated again."""
+    h, r, data = capi.host().residual_norm(y, residual, weight, bias, gate, after_weight, after_bias, residual_scale, block_scale, eps, after, before, center, checkpoint)
+    if not before:
+        return r
+    if r is None:
+        r = y
+    return (h, r, Checkpoint(data, _rows(h), h.shape[-1])) if checkpoint else (h, r)
+
+
+_KINDS = {"silu": 0, "gelu_tanh": 1}
+
+
+def gated(x, up=None, kind="silu", checkpoint=False):
+    """act(gate) * up, [..., cols]: gate and up are the halves of x [..., 2 cols], side by side as a linear layer with both weights gives them, or x and up, of one shape.
+    Views whose elements of a row are consecutive are read in place, others are copied.
+
+    kind: "silu", g sigmoid(g), or "gelu_tanh", g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3)) = g / 2 (1 + tanh(...)).
+    checkpoint: also the Checkpoint of the result, for the layers that take it -- the answer is (out, Checkpoint) -- and the backward pass keeps gate and up in 8 bits.
+    The gradients cannot be differentiated again."""
+    if kind not in _KINDS:
+        raise RuntimeError("gated: unknown activation %r" % (kind,))
+    out, data = capi.host().gated(x, up, _KINDS[kind], checkpoint)
+    return (out, Checkpoint(data, _rows(out), out.shape[-1])) if checkpoint else out

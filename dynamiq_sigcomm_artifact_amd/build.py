@@ -42,6 +42,7 @@ HIP_SOURCES = [
     "dq_optimizer.hip",
     "dq_microscale.hip", "dq_microscale_product.hip",
     "dq_activations.hip",
+    "dq_residual_norm.hip", "dq_residual_norm_f16.hip", "dq_residual_norm_bf16.hip", "dq_residual_norm_f32.hip",
 ]
 
 HIPCC_FLAGS = [

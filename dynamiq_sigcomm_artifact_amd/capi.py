@@ -37,7 +37,8 @@ EXPORTS = [
     "dq_eden_work_doubles", "dq_eden_quantize", "dq_eden_quantize_static_max_n", "dq_eden_quantize_static", "dq_eden_dequantize", "dq_eden_dequantize_irht", "dq_eden_slice_bytes", "dq_eden_compress", "dq_eden_decompress", "dq_thc_compress", "dq_thc_compress_drawn", "dq_thc_decompress", "dq_thc_quantize", "dq_thc_dequantize", "dq_thc_rht_quantize", "dq_thc_dequantize_irht",
     "dq_grad_norm_work_doubles", "dq_grad_norm", "dq_adamw_step", "dq_adamw_coefficients",
     "dq_mx4_quantize", "dq_mx4_quantize_list", "dq_mx4_dequantize", "dq_mx4_product",
-    "dq_checkpoint_bytes", "dq_checkpoint_compress", "dq_checkpoint_restore",
+    "dq_checkpoint_bytes", "dq_checkpoint_compress", "dq_checkpoint_restore", "dq_gated_forward", "dq_gated_backward",
+    "dq_residual_norm_forward", "dq_residual_norm_work_floats", "dq_residual_norm_backward",
 ]
 
 STAGE_STATS, STAGE_PLAN, STAGE_COMPRESS, STAGE_DECOMPRESS = 1, 2, 4, 8
@@ -81,6 +82,22 @@ class Adamw(ctypes.Structure):
                 ("bits", ctypes.c_int32), ("reserved", ctypes.c_int32), ("lr", ctypes.c_double), ("beta1", ctypes.c_double),
                 ("beta2", ctypes.c_double), ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64),
                 ("grad_scale", ctypes.c_void_p), ("coefficients", ctypes.c_void_p)]
+
+
+class Gated(ctypes.Structure):
+    """dq_gated_t"""
+    _fields_ = [("gate", ctypes.c_void_p), ("up", ctypes.c_void_p), ("gate_stride", ctypes.c_int64), ("up_stride", ctypes.c_int64), ("out", ctypes.c_void_p),
+                ("out8", ctypes.c_void_p), ("gate8", ctypes.c_void_p), ("up8", ctypes.c_void_p), ("dgate", ctypes.c_void_p), ("dup", ctypes.c_void_p),
+                ("dgate_stride", ctypes.c_int64), ("dup_stride", ctypes.c_int64), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("kind", ctypes.c_int32)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """dq_residual_norm_t"""
+    _fields_ = [(k, ctypes.c_void_p) for k in ("y", "residual", "gate", "weight", "bias", "after_weight", "after_bias", "h", "r", "h8", "kept", "stats", "dh", "dr", "dy",
+                                               "dresidual", "dgate", "dweight", "dbias", "dafter_weight", "dafter_bias", "work")] + \
+               [(k, ctypes.c_int64) for k in ("work_floats", "rows", "cols", "rows_per_gate")] + [(k, ctypes.c_double) for k in ("eps", "residual_scale", "block_scale")] + \
+               [(k, ctypes.c_int32) for k in ("dtype", "stream_dtype", "center", "after", "before", "keep_r", "keep_y", "float32")]
 
 
 _lib = None
@@ -232,6 +249,14 @@ def lib():
         L.dq_checkpoint_compress.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp]
         L.dq_checkpoint_restore.restype = i32
         L.dq_checkpoint_restore.argtypes = [vp, vp, i32, i64, i64, i32, vp]
+        for call in (L.dq_gated_forward, L.dq_gated_backward):
+            call.restype = i32
+            call.argtypes = [c.POINTER(Gated), i32, vp]
+        for call in (L.dq_residual_norm_forward, L.dq_residual_norm_backward):
+            call.restype = i32
+            call.argtypes = [c.POINTER(ResidualNorm), i32, vp]
+        L.dq_residual_norm_work_floats.restype = i64
+        L.dq_residual_norm_work_floats.argtypes = [c.POINTER(ResidualNorm)]
         _lib = L
     return _lib
 

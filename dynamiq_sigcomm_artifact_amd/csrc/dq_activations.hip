@@ -69,4 +69,141 @@ hipError_t launch_checkpoint_restore(const uint8_t *data, void *out, int64_t row
     return hipGetLastError();
 }
 
+// ---- the gated activation -----------------------------------------------------------------------------------
+
+// sigmoid(q) and 1 - sigmoid(q), both to their own precision: with e = exp(-|q|) they are 1 / (1 + e) and e / (1 + e)
+template <int DT> __device__ __forceinline__ void sigmoids(float q, float &s, float &rest)
+{
+    const float e = DT == DQ_F32 ? expf(-__builtin_fabsf(q)) : __expf(-__builtin_fabsf(q));
+    const float big = DT == DQ_F32 ? 1.0f / (1.0f + e) : __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+    s = q >= 0.0f ? big : small;
+    rest = q >= 0.0f ? small : big;
+}
+// act(g) = g sigmoid(q(g)): q = g, or for the hyperbolic tangent's form of gelu q = 2 sqrt(2 / pi) (g + 0.044715 g^3), of which from 20 on nothing changes the sigmoid any more
+template <int KIND> __device__ __forceinline__ float exponent_of(float g, float &slope)
+{
+    if (KIND == DQ_SILU) {
+        slope = 1.0f;
+        return g;
+    }
+    constexpr float c = 1.5957691216057308f;
+    const float x = __builtin_amdgcn_fmed3f(g, -20.0f, 20.0f), square = x * x;
+    slope = c + 3 * 0.044715f * c * square;
+    return x * (c + 0.044715f * c * square);
+}
+
+// A lane takes eight elements, four of them a block of 32, padding included: the last block of a row may be a part.
+template <int DT, int KIND, bool EIGHT> __global__ __launch_bounds__(256) void gated_kernel(GatedArgs a, Division blocks, uint32_t units)
+{
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
+    if (unit >= units) return;
+    const uint32_t row = blocks(unit >> 2), col = (unit - row * blocks.by * 4) * 8;
+    if (!EIGHT && col >= a.cols) return;
+    const bool whole = col + 8 <= a.cols;
+    const int64_t at_gate = row * a.gate_stride + col, at_up = row * a.up_stride + col, at = (int64_t)row * a.cols + col;
+    float g[8], u[8], v[8];
+    if (whole) {
+        load8<DT>(a.gate, at_gate, g);
+        load8<DT>(a.up, at_up, u);
+    } else {
+        load_part<DT, 8>(a.gate, at_gate, row * a.gate_stride + a.cols, g);
+        load_part<DT, 8>(a.up, at_up, row * a.up_stride + a.cols, u);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        float slope, s, rest;
+        sigmoids<DT>(exponent_of<KIND>(g[j], slope), s, rest);
+        v[j] = ElemIO<DT>::round(g[j] * s * u[j]);
+    }
+    if (whole)
+        store8<DT>(a.out, at, v);
+    else if (col < a.cols)
+        store_part<DT, 8>(a.out, at, (int)(a.cols - col), v);
+    if (EIGHT) {
+        const int64_t scales = (int64_t)units * 8 + (unit >> 2);
+        const auto put = [&](uint8_t *data, const float (&x)[8]) {
+            if (!data) return; // (the same for every lane)
+            uint32_t scale;
+            const u32x2_t w = encode_e4m3<DT>(x, scale);
+            reinterpret_cast<u32x2_t *>(data)[unit] = w;
+            if ((threadIdx.x & 3) == 0) data[scales] = (uint8_t)scale;
+        };
+        put(a.out8, v);
+        put(a.gate8, g);
+        put(a.up8, u);
+    }
+}
+
+template <int DT, int KIND, bool EIGHT> __global__ __launch_bounds__(256) void gated_backward_kernel(GatedArgs a, Division blocks, uint32_t units)
+{
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
+    if (unit >= units) return;
+    const uint32_t row = blocks(unit >> 2), col = (unit - row * blocks.by * 4) * 8;
+    if (col >= a.cols) return;
+    const bool whole = col + 8 <= a.cols;
+    const int64_t at = (int64_t)row * a.cols + col;
+    float g[8], u[8], d[8];
+    if (whole)
+        load8<DT>(a.out, at, d);
+    else
+        load_part<DT, 8>(a.out, at, (int64_t)(row + 1) * a.cols, d);
+    if (EIGHT) {
+        const int64_t scales = (int64_t)units * 8 + (unit >> 2);
+        decode_e4m3(reinterpret_cast<const u32x2_t *>(a.gate8)[unit], a.gate8[scales], g);
+        decode_e4m3(reinterpret_cast<const u32x2_t *>(a.up8)[unit], a.up8[scales], u);
+    } else if (whole) {
+        load8<DT>(a.gate, row * a.gate_stride + col, g);
+        load8<DT>(a.up, row * a.up_stride + col, u);
+    } else {
+        load_part<DT, 8>(a.gate, row * a.gate_stride + col, row * a.gate_stride + a.cols, g);
+        load_part<DT, 8>(a.up, row * a.up_stride + col, row * a.up_stride + a.cols, u);
+    }
+    // act' = s + g s (1 - s) q'
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        float slope, s, rest;
+        sigmoids<DT>(exponent_of<KIND>(g[j], slope), s, rest);
+        const float value = g[j] * s;
+        g[j] = d[j] * u[j] * (s + value * (rest * slope));
+        u[j] = d[j] * value;
+    }
+    const int64_t to_gate = row * a.dgate_stride + col, to_up = row * a.dup_stride + col;
+    if (a.dgate) {
+        if (whole)
+            store8<DT>(a.dgate, to_gate, g);
+        else
+            store_part<DT, 8>(a.dgate, to_gate, (int)(a.cols - col), g);
+    }
+    if (a.dup) {
+        if (whole)
+            store8<DT>(a.dup, to_up, u);
+        else
+            store_part<DT, 8>(a.dup, to_up, (int)(a.cols - col), u);
+    }
+}
+
+template <int DT, int KIND, bool EIGHT> static hipError_t launch_gated_of(const GatedArgs &a, bool backward, hipStream_t stream)
+{
+    const Division blocks((a.cols + 31) >> 5, 30);
+    const uint32_t units = (uint32_t)(a.rows * blocks.by * 4);
+    const dim3 grid((units + 255) / 256);
+    if (backward)
+        gated_backward_kernel<DT, KIND, EIGHT><<<grid, 256, 0, stream>>>(a, blocks, units);
+    else
+        gated_kernel<DT, KIND, EIGHT><<<grid, 256, 0, stream>>>(a, blocks, units);
+    return hipGetLastError();
+}
+template <int DT> static hipError_t launch_gated_with(const GatedArgs &a, int kind, bool backward, hipStream_t stream)
+{
+    const bool eight = backward ? a.gate8 != nullptr : a.out8 || a.gate8 || a.up8;
+    if (kind == DQ_SILU) return eight ? launch_gated_of<DT, DQ_SILU, true>(a, backward, stream) : launch_gated_of<DT, DQ_SILU, false>(a, backward, stream);
+    return eight ? launch_gated_of<DT, DQ_GELU_TANH, true>(a, backward, stream) : launch_gated_of<DT, DQ_GELU_TANH, false>(a, backward, stream);
+}
+
+hipError_t launch_gated(const GatedArgs &a, int dtype, int kind, bool backward, hipStream_t stream)
+{
+    return dtype == DQ_F32 ? launch_gated_with<DQ_F32>(a, kind, backward, stream)
+         : dtype == DQ_BF16 ? launch_gated_with<DQ_BF16>(a, kind, backward, stream) : launch_gated_with<DQ_F16>(a, kind, backward, stream);
+}
+
 } // namespace dq

@@ -1281,4 +1281,96 @@ int dq_checkpoint_restore(const uint8_t *data, void *out, int dtype, int64_t row
     return finish(dq::launch_checkpoint_restore(data, out, rows, cols, dtype, static_cast<hipStream_t>(stream)));
 }
 
+static int gated(const dq_gated_t *o, bool backward, int device, dq_stream_t stream)
+{
+    if (!o) return fail(DQ_ERR_NULL);
+    if (!dtype_ok(o->dtype)) return fail(DQ_ERR_DTYPE);
+    if (o->kind != DQ_SILU && o->kind != DQ_GELU_TANH) return fail(DQ_ERR_SIZE, "unknown activation");
+    if (!checkpoint_size_ok(o->rows, o->cols)) return fail(DQ_ERR_SIZE, kCheckpointSizes);
+    const bool eight = backward && o->gate8;
+    if (backward && !o->gate8 != !o->up8) return fail(DQ_ERR_NULL, "the checkpoints of gate and up, or neither");
+    if (!o->out || (!eight && (!o->gate || !o->up))) return fail(DQ_ERR_NULL);
+    const auto apart = [&](const void *p, int64_t stride) { return !p || (stride >= o->cols && stride < (int64_t)1 << 40); };
+    if ((!eight && !(apart(o->gate, o->gate_stride) && apart(o->up, o->up_stride))) || (backward && !(apart(o->dgate, o->dgate_stride) && apart(o->dup, o->dup_stride))))
+        return fail(DQ_ERR_SIZE, "stride must be at least the columns");
+    if ((reinterpret_cast<uintptr_t>(o->gate8) | reinterpret_cast<uintptr_t>(o->up8) | (backward ? 0 : reinterpret_cast<uintptr_t>(o->out8))) & 15)
+        return fail(DQ_ERR_SIZE, "checkpoints must be 16-byte aligned");
+    int rc;
+    if ((rc = select_device(device))) return rc;
+    const dq::GatedArgs a = {o->gate, o->up, o->out, backward ? nullptr : o->out8, o->gate8, o->up8, o->dgate, o->dup, o->gate_stride, o->up_stride, o->dgate_stride, o->dup_stride, o->rows,
+                             (uint32_t)o->cols};
+    return finish(dq::launch_gated(a, o->dtype, o->kind, backward, static_cast<hipStream_t>(stream)));
+}
+int dq_gated_forward(const dq_gated_t *o, int device, dq_stream_t stream) { return gated(o, false, device, stream); }
+int dq_gated_backward(const dq_gated_t *o, int device, dq_stream_t stream) { return gated(o, true, device, stream); }
+
+// what both passes ask of it
+static int norm_ok(const dq_residual_norm_t *o)
+{
+    if (!o) return fail(DQ_ERR_NULL);
+    if (!dtype_ok(o->dtype) || (o->stream_dtype != o->dtype && o->stream_dtype != DQ_F32)) return fail(DQ_ERR_DTYPE);
+    if (o->rows <= 0 || o->rows > 0x7fffff00 || o->cols < 8 || o->cols > dq::kNormCols) return fail(DQ_ERR_SIZE, "rows must be in [1, 2^31 - 256], cols in [8, 32768]");
+    if (o->gate && (o->rows_per_gate <= 0 || o->rows % o->rows_per_gate)) return fail(DQ_ERR_SIZE, "rows_per_gate must divide the rows");
+    if (!(o->eps >= 0) || !__builtin_isfinite(o->eps) || !__builtin_isfinite(o->residual_scale) || !__builtin_isfinite(o->block_scale))
+        return fail(DQ_ERR_SIZE, "eps must be a number and not negative, the scales numbers");
+    if ((o->keep_r || o->keep_y) && !o->kept) return fail(DQ_ERR_NULL);
+    if ((reinterpret_cast<uintptr_t>(o->h8) | reinterpret_cast<uintptr_t>(o->kept) | reinterpret_cast<uintptr_t>(o->stats)) & 15)
+        return fail(DQ_ERR_SIZE, "checkpoints and stats must be 16-byte aligned");
+    return 0;
+}
+static uint32_t norm_flags(const dq_residual_norm_t *o)
+{
+    return (o->center ? dq::kNormCenter : 0) | (o->after ? dq::kNormAfter : 0) | (o->before ? dq::kNormBefore : 0) | ((uint32_t)o->float32 & 31) * dq::kNormWeight32;
+}
+// r is y itself
+static bool norm_plain(const dq_residual_norm_t *o) { return !o->residual && !o->gate && !o->after && o->block_scale == 1.0; }
+
+int dq_residual_norm_forward(const dq_residual_norm_t *o, int device, dq_stream_t stream)
+{
+    int rc;
+    if ((rc = norm_ok(o))) return rc;
+    if (!o->residual && o->stream_dtype != o->dtype) return fail(DQ_ERR_DTYPE, "without a residual the stream is of y's type");
+    if (!o->y || (o->before && !o->h) || (!o->r && !norm_plain(o))) return fail(DQ_ERR_NULL);
+    if (!o->before && (o->h || o->h8 || !o->r)) return fail(DQ_ERR_SIZE, "h and its checkpoint are for `before`, and without it r is the result");
+    if ((reinterpret_cast<uintptr_t>(o->stats) & 15)) return fail(DQ_ERR_SIZE, "stats must be 16-byte aligned");
+    if ((rc = select_device(device))) return rc;
+    dq::BlockNormArgs a = {o->y, o->residual, o->weight, o->bias, o->gate, o->after_weight, o->after_bias, o->h, o->r, o->stats, o->h8, o->kept, (uint32_t)o->rows, (uint32_t)o->cols,
+                      o->gate ? (uint32_t)o->rows_per_gate : 1, norm_flags(o) | (o->keep_r ? dq::kNormKeepR : 0) | (o->keep_y ? dq::kNormKeepY : 0), 0,
+                      (float)o->residual_scale, (float)o->block_scale, (float)o->eps};
+    return finish(dq::launch_norm(a, o->dtype, o->stream_dtype == DQ_F32, static_cast<hipStream_t>(stream)));
+}
+
+int64_t dq_residual_norm_work_floats(const dq_residual_norm_t *o)
+{
+    if (norm_ok(o)) return -1;
+    const dq::NormShares s = dq::norm_shares(o->rows, o->gate ? o->rows_per_gate : 0, (uint32_t)o->cols);
+    const int sums = !!o->dweight + !!o->dbias + (o->dgate && s.parts > 1) + !!o->dafter_weight + !!o->dafter_bias;
+    return (int64_t)sums * s.grid * o->cols;
+}
+
+int dq_residual_norm_backward(const dq_residual_norm_t *o, int device, dq_stream_t stream)
+{
+    int rc;
+    if ((rc = norm_ok(o))) return rc;
+    if (!o->stats || (!o->dh && !o->dr)) return fail(DQ_ERR_NULL);
+    if (o->dh && !o->before) return fail(DQ_ERR_SIZE, "dh is for `before`");
+    if (((o->dweight || o->dbias) && !o->dh) || (o->dgate && !o->gate) || ((o->dafter_weight || o->dafter_bias) && !o->after))
+        return fail(DQ_ERR_SIZE, "a gradient is asked for of what took no part");
+    const bool plain = norm_plain(o);
+    const bool wants_r = o->dh, wants_y = !plain && (o->dgate || (o->after && (o->dy || o->dafter_weight || o->dafter_bias)));
+    if ((wants_r && !o->keep_r && !(plain && o->y) && !o->r) || (wants_y && !o->keep_y && !o->y)) return fail(DQ_ERR_NULL, "r, y or their checkpoints");
+    if (wants_r && wants_y && !o->keep_r != !o->keep_y) return fail(DQ_ERR_SIZE, "r and y are both in 8 bits, or neither");
+    if (!o->work && dq_residual_norm_work_floats(o)) return fail(DQ_ERR_NULL);
+    if (o->work_floats < dq_residual_norm_work_floats(o)) return fail(DQ_ERR_SIZE, "work buffer is too small (dq_residual_norm_work_floats)");
+    if ((rc = select_device(device))) return rc;
+    const uint8_t *kept_y = o->kept ? o->kept + (o->keep_r ? (dq_checkpoint_bytes(o->rows, o->cols) + 15) / 16 * 16 : 0) : nullptr;
+    const bool eight = (wants_r && o->keep_r) || (wants_y && o->keep_y);
+    dq::BlockNormBackArgs a = {o->dh, o->dr, wants_r ? (o->keep_r ? o->kept : o->r ? o->r : o->y) : nullptr, wants_y ? (o->keep_y ? kept_y : o->y) : nullptr, o->weight, o->gate, o->after_weight,
+                          o->after_bias, o->stats, o->dy, o->dresidual, nullptr, o->work, (uint32_t)o->rows, (uint32_t)o->cols, o->gate ? (uint32_t)o->rows_per_gate : 1,
+                          norm_flags(o) | (eight ? dq::kNormEight : 0), 0, 0, 0, 0, (float)o->residual_scale, (float)o->block_scale};
+    const auto sum = [&](void *out, int bit) { return dq::NormSum{out, o->float32 & bit ? DQ_F32 : o->dtype}; };
+    const dq::NormSum sums[5] = {sum(o->dweight, 1), sum(o->dbias, 2), sum(o->dgate, 4), sum(o->dafter_weight, 8), sum(o->dafter_bias, 16)};
+    return finish(dq::launch_norm_backward(a, sums, o->dtype, o->stream_dtype == DQ_F32, static_cast<hipStream_t>(stream)));
+}
+
 } // extern "C"

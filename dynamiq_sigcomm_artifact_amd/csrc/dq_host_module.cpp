@@ -1610,7 +1610,331 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
     });
 }
 
+// ---- the gated activation, with its backward pass (activations.py) ----
+
+struct GatedOf : public torch::autograd::Function<GatedOf> {
+    typedef std::optional<at::Tensor> Maybe;
+    // gate and up as rows; without up gate holds both, side by side
+    static void fill(dq_gated_t &o, const at::Tensor &x, const Maybe &up)
+    {
+        const int64_t cols = up ? x.size(1) : x.size(1) / 2;
+        o.gate = x.data_ptr();
+        o.gate_stride = std::max(row_stride(x), cols);
+        o.up = up ? up->data_ptr() : static_cast<char *>(x.data_ptr()) + cols * (int64_t)x.element_size();
+        o.up_stride = up ? std::max(row_stride(*up), cols) : o.gate_stride;
+    }
+    // kept: what the backward pass will want is kept (in 8 bits, if eight)
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const Maybe &up, int64_t kind, bool eight, bool kept)
+    {
+        const c10::DeviceGuard on(x.device());
+        const at::Tensor a = as_rows(x);
+        const Maybe b = up ? Maybe(as_rows(*up)) : Maybe();
+        dq_gated_t o;
+        memset(&o, 0, sizeof(o));
+        fill(o, a, b);
+        o.rows = a.size(0);
+        o.cols = up ? a.size(1) : a.size(1) / 2;
+        o.dtype = dtype_code(x);
+        o.kind = (int32_t)kind;
+        std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = o.cols;
+        const at::Tensor out = at::empty(shape, at::TensorOptions().dtype(x.scalar_type()).device(x.device()));
+        const int64_t bytes = checkpoint_bytes(o.rows, o.cols), room = (bytes + 15) / 16 * 16;
+        at::Tensor data, keep;
+        if (eight) {
+            data = new_bytes(x.device(), bytes);
+            o.out8 = static_cast<uint8_t *>(data.data_ptr());
+            if (kept) {
+                keep = new_bytes(x.device(), 2 * room);
+                o.gate8 = static_cast<uint8_t *>(keep.data_ptr());
+                o.up8 = o.gate8 + room;
+            }
+        }
+        o.out = out.data_ptr();
+        if (o.rows && o.cols) check(dq_gated_forward(&o, x.device().index(), c10::hip::getCurrentHIPStream(x.device().index()).stream()));
+        if (kept) {
+            if (eight)
+                ctx->save_for_backward({keep});
+            else if (up)
+                ctx->save_for_backward({x, *up});
+            else
+                ctx->save_for_backward({x});
+        }
+        ctx->saved_data["kind"] = kind;
+        ctx->saved_data["eight"] = eight;
+        ctx->saved_data["packed"] = !up;
+        ctx->saved_data["shape"] = x.sizes();
+        if (!eight) return {out};
+        ctx->mark_non_differentiable({data});
+        return {out, data};
+    }
+    static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
+    {
+        need(!at::GradMode::is_enabled(), "gated: its gradients cannot be differentiated again");
+        torch::autograd::tensor_list out(5);
+        const torch::autograd::variable_list saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return out;
+        const c10::Device device = grads[0].device();
+        const c10::DeviceGuard on(device);
+        const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+        const bool packed = ctx->saved_data["packed"].toBool();
+        const at::Tensor d = grads[0].contiguous();
+        const int64_t size = (int64_t)d.element_size();
+        dq_gated_t o;
+        memset(&o, 0, sizeof(o));
+        o.cols = packed ? shape.back() / 2 : shape.back();
+        o.rows = c10::multiply_integers(shape.begin(), shape.end() - 1);
+        o.dtype = dtype_code(d);
+        o.kind = (int32_t)ctx->saved_data["kind"].toInt();
+        o.out = d.data_ptr();
+        at::Tensor a, b;
+        if (ctx->saved_data["eight"].toBool()) {
+            o.gate8 = static_cast<uint8_t *>(saved[0].data_ptr());
+            o.up8 = o.gate8 + (checkpoint_bytes(o.rows, o.cols) + 15) / 16 * 16;
+        } else {
+            a = as_rows(saved[0]);
+            if (!packed) b = as_rows(saved[1]);
+            fill(o, a, packed ? Maybe() : Maybe(b));
+        }
+        const at::TensorOptions of = at::TensorOptions().dtype(d.scalar_type()).device(device);
+        o.dgate_stride = o.dup_stride = shape.back();
+        if (packed) {
+            out[0] = at::empty(shape, of);
+            o.dgate = out[0].data_ptr();
+            o.dup = static_cast<char *>(o.dgate) + o.cols * size;
+        } else {
+            if (ctx->needs_input_grad(0)) o.dgate = (out[0] = at::empty(shape, of)).data_ptr();
+            if (ctx->needs_input_grad(1)) o.dup = (out[1] = at::empty(shape, of)).data_ptr();
+        }
+        if (o.rows && o.cols) check(dq_gated_backward(&o, device.index(), c10::hip::getCurrentHIPStream(device.index()).stream()));
+        return out;
+    }
+};
+
+// x, up (None: x holds both), kind, checkpoint -> (out, data or None)
+PyObject *gated(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 4, [&]() -> PyObject * {
+        const at::Tensor &x = gpu_tensor(v[0]);
+        (void)dtype_code(x);
+        std::optional<at::Tensor> up;
+        if (v[1] != Py_None) {
+            up = gpu_tensor(v[1]);
+            need(up->device() == x.device(), "tensor arguments live on different devices");
+            need(up->sizes() == x.sizes() && up->scalar_type() == x.scalar_type(), "gated: the two halves have one shape and one type");
+        }
+        need(x.dim() >= 1 && (up || x.size(-1) % 2 == 0), "gated: x [..., 2 cols], or two tensors, are required");
+        const bool eight = PyObject_IsTrue(v[3]), kept = at::GradMode::is_enabled() && (x.requires_grad() || (up && up->requires_grad()));
+        leaves_can_be_recorded("gated", x.device(), {&x, up ? &*up : &x});
+        const torch::autograd::variable_list out = GatedOf::apply(x, up, integer(v[2]), eight, kept);
+        const py::object a = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[0]));
+        return PyTuple_Pack(2, a.ptr(), eight ? py::reinterpret_steal<py::object>(THPVariable_Wrap(out[1])).ptr() : Py_None);
+    });
+}
+
+// ---- the norms around a block, with their backward pass (activations.py) ----
+
+struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+    typedef std::optional<at::Tensor> Maybe;
+    struct Settings {
+        double residual_scale, block_scale, eps;
+        bool after, before, center, eight, kept;
+        int64_t per; // rows of a gate
+    };
+    enum { Y, RESIDUAL, WEIGHT, BIAS, GATE, AFTER_WEIGHT, AFTER_BIAS, INPUTS };
+    static const void *data_of(const Maybe &t) { return t ? t->data_ptr() : nullptr; }
+
+    // what both passes fill in; vectors: weight, bias, gate, after_weight, after_bias
+    static dq_residual_norm_t begin(int64_t rows, int64_t cols, at::ScalarType dtype, at::ScalarType stream, const Settings &s, const at::Tensor *const (&vectors)[5])
+    {
+        const auto code = [](at::ScalarType t) { return t == at::kHalf ? DQ_F16 : t == at::kBFloat16 ? DQ_BF16 : DQ_F32; };
+        dq_residual_norm_t o;
+        memset(&o, 0, sizeof(o));
+        const void **at[5] = {&o.weight, &o.bias, &o.gate, &o.after_weight, &o.after_bias};
+        for (int k = 0; k < 5; k++) {
+            if (!vectors[k] || !vectors[k]->defined()) continue;
+            *at[k] = vectors[k]->data_ptr();
+            if (vectors[k]->scalar_type() == at::kFloat) o.float32 |= 1 << k;
+        }
+        o.rows = rows;
+        o.cols = cols;
+        o.rows_per_gate = s.per;
+        o.eps = s.eps;
+        o.residual_scale = s.residual_scale;
+        o.block_scale = s.block_scale;
+        o.dtype = code(dtype);
+        o.stream_dtype = code(stream);
+        o.center = s.center;
+        o.after = s.after;
+        o.before = s.before;
+        return o;
+    }
+
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &y_, const Maybe &residual_, const Maybe &weight_, const Maybe &bias_,
+                                                  const Maybe &gate_, const Maybe &after_weight_, const Maybe &after_bias_, const Settings &s)
+    {
+        const c10::Device device = y_.device();
+        const c10::DeviceGuard on(device);
+        const auto whole = [](const Maybe &t) { return t ? t->contiguous() : at::Tensor(); };
+        const at::Tensor y = y_.contiguous(), residual = whole(residual_), weight = whole(weight_), bias = whole(bias_), gate = whole(gate_), after_weight = whole(after_weight_),
+                         after_bias = whole(after_bias_);
+        const int64_t cols = y.size(-1), rows = y.numel() / cols;
+        const at::ScalarType dtype = y.scalar_type(), stream = residual.defined() ? residual.scalar_type() : dtype;
+        const bool plain = !residual.defined() && !gate.defined() && !s.after && s.block_scale == 1.0;
+        const bool keep_r = s.kept && s.before, keep_y = s.kept && (s.after || (gate.defined() && gate_->requires_grad()));
+        dq_residual_norm_t o = begin(rows, cols, dtype, stream, s, {&weight, &bias, &gate, &after_weight, &after_bias});
+        const int64_t bytes = checkpoint_bytes(rows, cols), room = (bytes + 15) / 16 * 16;
+        at::Tensor h, r, data, kept, stats;
+        if (s.before) o.h = (h = at::empty(y.sizes(), at::TensorOptions().dtype(dtype).device(device))).data_ptr();
+        if (!plain || !s.before) o.r = (r = at::empty(y.sizes(), at::TensorOptions().dtype(stream).device(device))).data_ptr();
+        if (s.eight && s.before) o.h8 = static_cast<uint8_t *>((data = new_bytes(device, bytes)).data_ptr());
+        if (s.kept) o.stats = (stats = at::empty({rows, 4}, at::TensorOptions().dtype(at::kFloat).device(device))).data_ptr<float>();
+        if (s.eight && (keep_r || keep_y)) {
+            kept = new_bytes(device, room * ((int)keep_r + (int)keep_y));
+            o.kept = static_cast<uint8_t *>(kept.data_ptr());
+            o.keep_r = keep_r;
+            o.keep_y = keep_y;
+        }
+        o.y = y.data_ptr();
+        if (residual.defined()) o.residual = residual.data_ptr();
+        if (rows) check(dq_residual_norm_forward(&o, device.index(), c10::hip::getCurrentHIPStream(device.index()).stream()));
+        if (s.kept) {
+            const at::Tensor none;
+            const bool sixteen = !s.eight;
+            ctx->set_materialize_grads(false);
+            ctx->save_for_backward({sixteen && keep_r ? (plain ? y : r) : none, sixteen && keep_y ? y : none, weight, gate, after_weight, after_bias, stats, kept});
+            ctx->saved_data["scales"] = std::vector<double>{s.residual_scale, s.block_scale, s.eps};
+            ctx->saved_data["flags"] = std::vector<int64_t>{s.after, s.before, s.center, s.eight, s.per, keep_r, keep_y, plain, (int64_t)dtype, (int64_t)stream,
+                                                            residual.defined(), bias.defined() ? (int64_t)bias.scalar_type() : -1};
+            ctx->saved_data["shape"] = y.sizes();
+        }
+        torch::autograd::variable_list out;
+        if (h.defined()) out.push_back(h);
+        if (r.defined()) out.push_back(r);
+        if (data.defined()) {
+            ctx->mark_non_differentiable({data});
+            out.push_back(data);
+        }
+        return out;
+    }
+
+    static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
+    {
+        need(!at::GradMode::is_enabled(), "residual_norm: its gradients cannot be differentiated again");
+        torch::autograd::tensor_list out(INPUTS + 1);
+        const torch::autograd::variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &r = saved[0], &y = saved[1], &weight = saved[2], &gate = saved[3], &after_weight = saved[4], &after_bias = saved[5], &stats = saved[6], &kept = saved[7];
+        const std::vector<int64_t> flags = ctx->saved_data["flags"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
+        const std::vector<double> scales = ctx->saved_data["scales"].toDoubleVector();
+        const Settings s = {scales[0], scales[1], scales[2], flags[0] != 0, flags[1] != 0, flags[2] != 0, flags[3] != 0, true, flags[4]};
+        const bool plain = flags[7], has_residual = flags[10];
+        const at::ScalarType dtype = (at::ScalarType)flags[8], stream = (at::ScalarType)flags[9];
+        const c10::Device device = stats.device();
+        const c10::DeviceGuard on(device);
+        const int64_t cols = shape.back(), rows = c10::multiply_integers(shape.begin(), shape.end() - 1);
+        const at::Tensor none;
+        const at::Tensor dh = s.before && grads[0].defined() ? grads[0].contiguous() : none;
+        const at::Tensor dr = !plain || !s.before ? grads[s.before ? 1 : 0].defined() ? grads[s.before ? 1 : 0].contiguous() : none : none;
+        if (!dh.defined() && !dr.defined()) return out;
+        // which of the inputs that took part want a gradient
+        const bool part[INPUTS] = {true, has_residual, weight.defined(), flags[11] >= 0, gate.defined(), after_weight.defined(), after_bias.defined()};
+        bool wanted[INPUTS];
+        size_t edge = 0;
+        for (int k = 0; k < INPUTS; k++) wanted[k] = part[k] && ctx->needs_input_grad(edge++);
+        if (!dh.defined()) wanted[WEIGHT] = wanted[BIAS] = false;
+        dq_residual_norm_t o = begin(rows, cols, dtype, stream, s, {&weight, nullptr, &gate, &after_weight, &after_bias});
+        if (flags[11] == (int64_t)at::kFloat) o.float32 |= 2;
+        const auto make = [&](int k, at::IntArrayRef of, at::ScalarType type) {
+            out[k] = rows ? at::empty(of, at::TensorOptions().dtype(type).device(device)) : at::zeros(of, at::TensorOptions().dtype(type).device(device));
+            return out[k].data_ptr();
+        };
+        // with nothing between them, both gradients are one
+        const bool same = wanted[Y] && wanted[RESIDUAL] && !gate.defined() && !s.after && s.block_scale == s.residual_scale && dtype == stream;
+        if (wanted[RESIDUAL]) o.dresidual = make(RESIDUAL, shape, stream);
+        if (wanted[Y] && !same) o.dy = make(Y, shape, dtype);
+        if (wanted[WEIGHT]) o.dweight = make(WEIGHT, weight.sizes(), weight.scalar_type());
+        if (wanted[BIAS]) o.dbias = make(BIAS, {cols}, (at::ScalarType)flags[11]);
+        if (wanted[GATE]) o.dgate = make(GATE, gate.sizes(), gate.scalar_type());
+        if (wanted[AFTER_WEIGHT]) o.dafter_weight = make(AFTER_WEIGHT, after_weight.sizes(), after_weight.scalar_type());
+        if (wanted[AFTER_BIAS]) o.dafter_bias = make(AFTER_BIAS, after_bias.sizes(), after_bias.scalar_type());
+        if (same) out[Y] = out[RESIDUAL];
+        if (!rows) return out;
+        if (r.defined()) o.r = r.data_ptr();
+        if (y.defined()) o.y = y.data_ptr();
+        if (kept.defined()) {
+            o.kept = static_cast<uint8_t *>(kept.data_ptr());
+            o.keep_r = (int32_t)flags[5];
+            o.keep_y = (int32_t)flags[6];
+        }
+        if (has_residual) o.residual = stats.data_ptr(); // (that there is one; it is not read)
+        o.stats = stats.data_ptr<float>();
+        if (dh.defined()) o.dh = dh.data_ptr();
+        if (dr.defined()) o.dr = dr.data_ptr();
+        o.work_floats = dq_residual_norm_work_floats(&o);
+        need(o.work_floats >= 0, dq_last_error());
+        const at::Tensor work = at::empty({o.work_floats}, at::TensorOptions().dtype(at::kFloat).device(device));
+        o.work = o.work_floats ? work.data_ptr<float>() : nullptr;
+        check(dq_residual_norm_backward(&o, device.index(), c10::hip::getCurrentHIPStream(device.index()).stream()));
+        return out;
+    }
+};
+
+// y, residual, weight, bias, gate, after_weight, after_bias, residual_scale, block_scale, eps, after, before, center, checkpoint -> (h, r, data), None for what there is not
+PyObject *residual_norm(PyObject *, PyObject *const *v, Py_ssize_t have)
+{
+    return answering(have, 14, [&]() -> PyObject * {
+        typedef ResidualNorm F;
+        const at::Tensor &y = gpu_tensor(v[0]);
+        (void)dtype_code(y);
+        need(y.dim() >= 1 && y.size(-1) > 0, "residual_norm: y [..., cols] is required");
+        const int64_t cols = y.size(-1), rows = y.numel() / cols;
+        std::optional<at::Tensor> in[F::INPUTS];
+        bool any = at::GradMode::is_enabled() && y.requires_grad();
+        for (int k = 1; k < F::INPUTS; k++) {
+            if (v[k] == Py_None) continue;
+            in[k] = gpu_tensor(v[k]);
+            need(in[k]->device() == y.device(), "tensor arguments live on different devices");
+            need(in[k]->scalar_type() == y.scalar_type() || in[k]->scalar_type() == at::kFloat, "residual_norm: what comes beside y is of its type or float32");
+            need(k == F::RESIDUAL ? in[k]->sizes() == y.sizes() : k == F::GATE || (in[k]->dim() == 1 && in[k]->size(0) == cols),
+                 k == F::RESIDUAL ? "residual_norm: the residual has y's shape" : "residual_norm: weights and biases are [cols]");
+            any = any || (at::GradMode::is_enabled() && in[k]->requires_grad());
+        }
+        F::Settings s;
+        s.residual_scale = number(v[7]);
+        s.block_scale = number(v[8]);
+        s.eps = number(v[9]);
+        s.after = PyObject_IsTrue(v[10]);
+        s.before = PyObject_IsTrue(v[11]);
+        s.center = PyObject_IsTrue(v[12]);
+        s.eight = PyObject_IsTrue(v[13]);
+        s.kept = any;
+        s.per = 1;
+        need(s.after || (!in[F::AFTER_WEIGHT] && !in[F::AFTER_BIAS]), "residual_norm: after_weight and after_bias are for after=True");
+        need(s.before || (!in[F::WEIGHT] && !in[F::BIAS]), "residual_norm: weight and bias are for before=True");
+        if (in[F::GATE]) {
+            const at::Tensor &gate = *in[F::GATE];
+            bool fits = gate.dim() >= 1 && gate.size(-1) == cols && (gate.dim() == 1 || gate.dim() == y.dim());
+            if (fits && gate.dim() > 1) {
+                int64_t k = 0;
+                while (k < y.dim() - 1 && gate.size(k) == y.size(k)) k++;
+                for (; k < y.dim() - 1; k++) fits = fits && gate.size(k) == 1;
+            }
+            need(fits, "residual_norm: a gate is [cols], or of y's shape with ones in place of the dimensions, the last of them before cols, that share it");
+            s.per = rows ? rows / (gate.numel() / cols) : 1;
+        }
+        leaves_can_be_recorded("residual_norm", y.device(), {&y, in[1] ? &*in[1] : &y, in[2] ? &*in[2] : &y, in[3] ? &*in[3] : &y, in[4] ? &*in[4] : &y, in[5] ? &*in[5] : &y, in[6] ? &*in[6] : &y});
+        const torch::autograd::variable_list out = F::apply(y, in[1], in[2], in[3], in[4], in[5], in[6], s);
+        const bool plain = !in[F::RESIDUAL] && !in[F::GATE] && !s.after && s.block_scale == 1.0;
+        size_t next = 0;
+        const auto take = [&](bool there) { return there ? py::reinterpret_steal<py::object>(THPVariable_Wrap(out[next++])) : py::reinterpret_borrow<py::object>(Py_None); };
+        const py::object h = take(s.before), r = take(!plain || !s.before), data = take(s.eight && s.before);
+        return PyTuple_Pack(3, h.ptr(), r.ptr(), data.ptr());
+    });
+}
+
 PyMethodDef kFunctions[] = {
+    {"residual_norm", reinterpret_cast<PyCFunction>(residual_norm), METH_FASTCALL, nullptr},
+    {"gated", reinterpret_cast<PyCFunction>(gated), METH_FASTCALL, nullptr},
     {"grad_norm", reinterpret_cast<PyCFunction>(grad_norm), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(adamw_step), METH_FASTCALL, nullptr},
     {"adamw_coefficients", reinterpret_cast<PyCFunction>(adamw_coefficients), METH_FASTCALL, nullptr},

@@ -425,4 +425,56 @@ struct CheckpointArgs {
 hipError_t launch_checkpoint_compress(const CheckpointArgs &a, int dtype, hipStream_t stream);
 hipError_t launch_checkpoint_restore(const uint8_t *data, void *out, int64_t rows, int64_t cols, int dtype, hipStream_t stream);
 
+// the gated activation: forward out = act(gate) up and the checkpoints that are asked for, backward dgate and dup of out's gradient, from gate and up or their checkpoints
+struct GatedArgs {
+    const void *gate, *up;
+    void *out;
+    uint8_t *out8, *gate8, *up8;
+    void *dgate, *dup;
+    int64_t gate_stride, up_stride, dgate_stride, dup_stride, rows;
+    uint32_t cols;
+};
+hipError_t launch_gated(const GatedArgs &a, int dtype, int kind, bool backward, hipStream_t stream);
+
+// the norms around a block (dq_residual_norm*.hip): the flags of a row's kernels, its threads above them
+enum : uint32_t {
+    kNormCenter = 1, kNormAfter = 2, kNormBefore = 4, kNormKeepR = 8, kNormKeepY = 16, kNormEight = 32, // kNormEight: r and y are checkpoints
+    kNormWeight32 = 64, kNormBias32 = 128, kNormGate32 = 256, kNormAfterWeight32 = 512, kNormAfterBias32 = 1024
+};
+struct BlockNormArgs {
+    const void *y, *residual, *weight, *bias, *gate, *after_weight, *after_bias;
+    void *h, *r;
+    float *stats;        // [rows][4]: mean and 1 / deviation of r, and of y
+    uint8_t *h8, *kept;  // kept: the checkpoint of r, and 16-byte aligned behind it that of y
+    uint32_t rows, cols, per, flags, grid;
+    float residual_scale, block_scale, eps;
+};
+static_assert(sizeof(BlockNormArgs) <= 128, "a launch whose arguments are longer takes longer");
+struct BlockNormBackArgs {
+    const void *dh, *dr, *r, *y, *weight, *gate, *after_weight, *after_bias;
+    const float *stats;
+    void *dy, *dresidual, *dgate;
+    float *work; // [sums][grid][cols]
+    uint32_t rows, cols, per, flags, grid, run, parts, sums;
+    float residual_scale, block_scale;
+};
+struct NormShares {
+    uint32_t grid, run, parts;
+};
+struct NormSum {
+    void *out;
+    int dtype;
+};
+constexpr int64_t kNormCols = 32768;
+NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols);
+hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t stream);
+hipError_t launch_norm_f16(const BlockNormArgs &a, bool stream32, hipStream_t stream);
+hipError_t launch_norm_bf16(const BlockNormArgs &a, bool stream32, hipStream_t stream);
+hipError_t launch_norm_f32(const BlockNormArgs &a, bool stream32, hipStream_t stream);
+// sums: of weight, bias, gate, after_weight, after_bias, those without out are not wanted
+hipError_t launch_norm_backward(BlockNormBackArgs a, const NormSum (&sums)[5], int dtype, bool stream32, hipStream_t stream);
+hipError_t launch_norm_backward_f16(const BlockNormBackArgs &a, bool stream32, hipStream_t stream);
+hipError_t launch_norm_backward_bf16(const BlockNormBackArgs &a, bool stream32, hipStream_t stream);
+hipError_t launch_norm_backward_f32(const BlockNormBackArgs &a, bool stream32, hipStream_t stream);
+
 } // namespace dq

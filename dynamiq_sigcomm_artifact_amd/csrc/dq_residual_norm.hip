@@ -1,0 +1,109 @@
+// The norms around a block: launches, and the sums over rows that end a backward pass.
+#include "dq_launch.h"
+#include "dq_microscale.cuh"
+
+namespace dq {
+
+// Threads of a row: eight elements each as far as 1024 of them go, then twice and four times eight.
+static uint32_t norm_threads(uint32_t cols)
+{
+    const uint32_t vectors = (cols + 7) >> 3;
+    const uint32_t each = vectors <= 1024 ? 1 : vectors <= 2048 ? 2 : 4;
+    return ((vectors + each - 1) / each + 63) & ~63u;
+}
+
+hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t stream)
+{
+    a.flags |= norm_threads(a.cols) << 16;
+    a.grid = std::min(a.rows, 1u << 20); // (beyond that a workgroup takes several rows)
+    return dtype == DQ_F32 ? launch_norm_f32(a, stream32, stream) : dtype == DQ_BF16 ? launch_norm_bf16(a, stream32, stream) : launch_norm_f16(a, stream32, stream);
+}
+
+// How a backward pass shares its rows out: runs of `run` rows, `parts` of them (the last one shorter) to the rows of a gate, or one of whole gates.
+NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols)
+{
+    const int64_t groups = norm_threads(cols) <= 256 ? 1024 : 512;
+    int64_t run = (rows + groups - 1) / groups;
+    NormShares s;
+    if (per == 0 || per <= run) {
+        if (per) run = run / per * per;
+        s.parts = 1;
+        s.grid = (uint32_t)((rows + run - 1) / run);
+    } else {
+        s.parts = (uint32_t)((per + run - 1) / run);
+        run = (per + s.parts - 1) / s.parts;
+        s.parts = (uint32_t)((per + run - 1) / run);
+        s.grid = (uint32_t)(rows / per * s.parts);
+    }
+    s.run = (uint32_t)run;
+    return s;
+}
+
+struct ColumnSums {
+    const float *work;
+    uint32_t grid, cols, count, tiles;
+    struct One {
+        void *out;
+        uint32_t segments, parts, dtype;
+    } one[5];
+};
+
+// out[s][c]: the sum of `parts` rows of work, which lie one behind the other.  Four threads share a column's rows, in an order that does not change.
+__global__ __launch_bounds__(256) void column_sums_kernel(ColumnSums a)
+{
+    __shared__ float part[4][64];
+    uint32_t id = blockIdx.x / a.tiles, k = 0;
+    const uint32_t col = (blockIdx.x - id * a.tiles) * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6, at = min(col, a.cols - 1);
+    while (id >= a.one[k].segments) id -= a.one[k++].segments;
+    const ColumnSums::One o = a.one[k];
+    const float *from = a.work + ((int64_t)k * a.grid + (int64_t)id * o.parts) * a.cols + at;
+    float sum = 0.0f;
+    uint32_t p = slice;
+    for (; p + 28 < o.parts; p += 32) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = from[(int64_t)(p + 4 * j) * a.cols];
+        sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    for (; p < o.parts; p += 4) sum += from[(int64_t)p * a.cols];
+    part[slice][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (slice || col >= a.cols) return;
+    sum = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    const int64_t to = (int64_t)id * a.cols + col;
+    if (o.dtype == DQ_F32)
+        ElemIO<DQ_F32>::store(o.out, to, sum);
+    else if (o.dtype == DQ_BF16)
+        ElemIO<DQ_BF16>::store(o.out, to, sum);
+    else
+        ElemIO<DQ_F16>::store(o.out, to, sum);
+}
+
+hipError_t launch_norm_backward(BlockNormBackArgs a, const NormSum (&sums)[5], int dtype, bool stream32, hipStream_t stream)
+{
+    const NormShares s = norm_shares(a.rows, a.gate ? a.per : 0, a.cols);
+    a.flags |= norm_threads(a.cols) << 16;
+    a.grid = s.grid;
+    a.run = s.run;
+    a.parts = s.parts;
+    a.sums = 0;
+    a.dgate = nullptr;
+    ColumnSums c = {a.work, s.grid, a.cols, 0, (a.cols + 63) / 64, {}};
+    uint32_t segments = 0;
+    for (int k = 0; k < 5; k++) {
+        if (!sums[k].out) continue;
+        a.sums |= 1u << k;
+        if (k == 2 && s.parts == 1) { // a gate's rows lie within one workgroup
+            a.dgate = sums[k].out;
+            continue;
+        }
+        c.one[c.count++] = {sums[k].out, k == 2 ? a.rows / a.per : 1, k == 2 ? s.parts : s.grid, (uint32_t)sums[k].dtype};
+        segments += c.one[c.count - 1].segments;
+    }
+    const hipError_t e = dtype == DQ_F32 ? launch_norm_backward_f32(a, stream32, stream)
+                       : dtype == DQ_BF16 ? launch_norm_backward_bf16(a, stream32, stream) : launch_norm_backward_f16(a, stream32, stream);
+    if (e != hipSuccess || !segments) return e;
+    return launch_with(column_sums_kernel, dim3(segments * c.tiles), dim3(256), stream, c);
+}
+
+} // namespace dq

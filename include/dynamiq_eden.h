@@ -885,6 +885,72 @@ int dq_checkpoint_compress(const void *x, int dtype, int64_t rows, int64_t cols,
 int dq_checkpoint_restore(const uint8_t *data, void *out, int dtype, int64_t rows, int64_t cols, int device,
                           dq_stream_t stream);
 
+/* ---- the gated activation ----------------------------------------------
+ *
+ * No counterpart in the reference.  out = act(gate) up with act(g) = g s(q), s the sigmoid:
+ *   DQ_SILU       q = g
+ *   DQ_GELU_TANH  q = 2 sqrt(2 / pi) (g + 0.044715 g^3)
+ * and backward, of d = the gradient of out:  dgate = d up (s + g s (1 - s) q'),  dup = d act(gate).
+ * In binary32, rounded once. */
+enum dq_activation { DQ_SILU = 0, DQ_GELU_TANH = 1 };
+typedef struct dq_gated {
+    const void *gate, *up;           /* `dtype` [rows][cols], row i from element i * stride on (halves of one matrix, for one) */
+    int64_t gate_stride, up_stride;
+    void *out;                       /* `dtype` [rows][cols]: written forward; backward its gradient, read */
+    uint8_t *out8;                   /* forward, each nullable: the checkpoints of out as it is stored, of gate and of up; */
+    uint8_t *gate8, *up8;            /* backward: both, to be read in place of gate and up, or neither */
+    void *dgate, *dup;               /* backward, each nullable */
+    int64_t dgate_stride, dup_stride;
+    int64_t rows, cols;
+    int32_t dtype, kind;
+} dq_gated_t;
+int dq_gated_forward(const dq_gated_t *gated, int device, dq_stream_t stream);
+int dq_gated_backward(const dq_gated_t *gated, int device, dq_stream_t stream);
+
+/* ---- the norms around a block, its gate and the residual -----------------
+ *
+ * No counterpart in the reference.  For every row, of a block's output y and the residual stream:
+ *   z = norm(y) with after_weight and after_bias where `after` is set, y otherwise
+ *   r = residual_scale residual + block_scale gate z
+ *   h = norm(r) with weight and bias, where `before` (the next block) is set
+ * norm(x) = x / sqrt(mean(x^2) + eps) w + b, or with `center` (x - mean) / sqrt(variance + eps) w + b.
+ * In binary32: r is rounded once where it is stored, h once, from the unrounded r.  Backward, with the mean and
+ * 1 / sqrt(..) that the forward pass has left in stats:
+ *   dr' = dr + the norm's part of dh,  dresidual = residual_scale dr',  t = block_scale dr',  dgate = sum t z,
+ *   dy = t gate, or the norm's part of that; the weights' gradients are the sums over the rows, in binary32 and in
+ *   an order that does not change.
+ * Pointers without need are NULL: residual, gate, weight (1) and bias (0) each; r where it is y itself (no residual,
+ * gate or after, block_scale 1), h without `before`; stats and kept for no backward pass; dh or dr where there is no such
+ * gradient; every result that is not wanted.
+ * 8 bits: h8 takes the checkpoint of h as it is stored, kept those of r as it is stored (keep_r) and, at the next
+ * multiple of 16 bytes, of y (keep_y): the backward pass reads them where keep_r or keep_y is set, in place of r
+ * and y.  It needs r with `before`, y with `after` and for dgate.
+ * Where r is y, the backward pass takes it as r. */
+typedef struct dq_residual_norm {
+    const void *y, *residual;                               /* [rows][cols]: dtype, stream_dtype */
+    const void *gate;                                       /* [rows / rows_per_gate][cols] */
+    const void *weight, *bias, *after_weight, *after_bias;  /* [cols] */
+    void *h, *r;                                            /* dtype, stream_dtype */
+    uint8_t *h8, *kept;                                     /* 16-byte aligned */
+    float *stats;                                           /* [rows][4], 16-byte aligned */
+    const void *dh, *dr;                                    /* dtype, stream_dtype */
+    void *dy, *dresidual;                                   /* dtype, stream_dtype */
+    void *dgate, *dweight, *dbias, *dafter_weight, *dafter_bias;
+    float *work;
+    int64_t work_floats;      /* dq_residual_norm_work_floats */
+    int64_t rows, cols;       /* cols in [8, 32768] */
+    int64_t rows_per_gate;    /* divides rows; with gate only */
+    double eps, residual_scale, block_scale;
+    int32_t dtype;            /* of the block's activations */
+    int32_t stream_dtype;     /* of the residual stream: dtype or DQ_F32 */
+    int32_t center, after, before, keep_r, keep_y;
+    int32_t float32;          /* which of weight 1, bias 2, gate 4, after_weight 8, after_bias 16 (and their gradients) are float32; the others are of dtype */
+} dq_residual_norm_t;
+int dq_residual_norm_forward(const dq_residual_norm_t *norm, int device, dq_stream_t stream);
+/* floats of the backward pass' work buffer for the gradients that are asked for; -1: wrong arguments */
+int64_t dq_residual_norm_work_floats(const dq_residual_norm_t *norm);
+int dq_residual_norm_backward(const dq_residual_norm_t *norm, int device, dq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,11 +81,9 @@ def block_gradients(kept_y, kept_r, st_r, st_y, gate, s, dh, dr_in):
 
 
 def act(g, kind):
-    """the activation and its derivative"""
+    """the activation and its derivative (the sigmoid as a quotient: from the hyperbolic tangent, 1 + tanh cancels where the sigmoid is small)"""
     with np.errstate(over="ignore"):
-        if kind == "silu":
-            t = np.tanh(g / 2)
-            return g * (1 + t) / 2, (1 + t) / 2 + g * (1 - t * t) / 4
-        k = np.sqrt(2 / np.pi)
-        t = np.tanh(k * (g + 0.044715 * g ** 3))
-        return g * (1 + t) / 2, (1 + t) / 2 + g * (1 - t * t) / 2 * k * (1 + 3 * 0.044715 * g ** 2)
+        q = g if kind == "silu" else 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)
+        s, rest = 1 / (1 + np.exp(-q)), 1 / (1 + np.exp(q))
+        dq = 1.0 if kind == "silu" else 2 * np.sqrt(2 / np.pi) * (1 + 3 * 0.044715 * g ** 2)
+        return g * s, s + g * s * rest * dq

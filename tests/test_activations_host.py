@@ -73,3 +73,86 @@ def test_definition_against_the_cast():
     y = torch.from_numpy(padded.reshape(40, 4, 32) / 2.0 ** (scales.astype(np.float64) - 127)[:, :, None]).float()
     assert float(y.abs().max()) <= 448 and np.array_equal(y.to(torch.float8_e4m3fn).view(torch.uint8).reshape(40, 128).numpy(), codes)
     assert np.abs(values[:, :100] - x).max() <= np.abs(x).max() * 2.0 ** -4
+
+
+def test_gated_refuses(L):
+    from dynamiq_sigcomm_artifact_amd import capi
+    good = dict(gate=0x1000, up=0x1000, gate_stride=20, up_stride=20, out=0x1000, rows=4, cols=10, dtype=1, kind=0)
+    back = dict(good, dgate=0x1000, dup=0x1000, dgate_stride=20, dup_stride=20)
+    for fn, base in ((L.dq_gated_forward, good), (L.dq_gated_backward, back)):
+        refused(L, fn(None, 0, S), "null")
+        for kw, text in ((dict(dtype=3), "dtype"), (dict(kind=2), "activation"), (dict(rows=0), "positive"), (dict(cols=-1), "positive"), (dict(rows=1 << 31), "2^31"),
+                         (dict(rows=1 << 30, cols=32, gate_stride=32, up_stride=32, dgate_stride=32, dup_stride=32), "2^35"), (dict(gate=None), "null"), (dict(up=None), "null"),
+                         (dict(out=None), "null"), (dict(gate_stride=9), "stride"), (dict(up_stride=1 << 40), "stride"), (dict(gate8=0x1004, up8=0x1000), "aligned")):
+            refused(L, fn(ctypes.byref(capi.Gated(**{**base, **kw})), 0, S), text)
+    refused(L, L.dq_gated_forward(ctypes.byref(capi.Gated(**good, out8=0x1008)), 0, S), "aligned")
+    refused(L, L.dq_gated_backward(ctypes.byref(capi.Gated(**back, gate8=0x1000)), 0, S), "or neither")
+    refused(L, L.dq_gated_backward(ctypes.byref(capi.Gated(**{**back, "dup_stride": 5})), 0, S), "stride")
+
+
+def test_gradients_of_the_definitions_against_differences():
+    """the formulas of the reference itself, in 64 bits: central differences with a step of 1e-5 are off by some 1e-10 of the third derivative and 1e-11 of the value"""
+    rng = np.random.default_rng(3)
+    step = 1e-5
+    for kind in ("silu", "gelu_tanh"):
+        g = rng.standard_normal(200) * 3
+        slope = (A.act(g + step, kind)[0] - A.act(g - step, kind)[0]) / (2 * step)
+        assert np.abs(slope - A.act(g, kind)[1]).max() < 1e-8
+    rows, cols = 3, 11
+    for case in range(24):
+        center, after, gated, residual, before = case & 1, case >> 1 & 1, case >> 2 & 1, case >> 3 & 1, case < 16
+        v = {k: rng.standard_normal((rows, cols)) for k in ("y", "residual", "gate")}
+        p = {k: rng.standard_normal(cols) for k in ("weight", "bias", "after_weight", "after_bias")}
+        dh, dr = rng.standard_normal((rows, cols)), rng.standard_normal((rows, cols))
+
+        def settings(p):
+            return {**p, "center": center, "after": after, "before": before, "eps": 1e-3, "residual_scale": 0.7, "block_scale": 1.3,
+                    **({} if before else {"weight": None, "bias": None}), **({} if after else {"after_weight": None, "after_bias": None})}
+
+        def loss(v, p):
+            h, r, _, _ = A.block(v["y"], v["residual"] if residual else None, v["gate"] if gated else None, settings(p))
+            return (r * dr).sum() + ((h * dh).sum() if before else 0.0)
+        _, r, st_r, st_y = A.block(v["y"], v["residual"] if residual else None, v["gate"] if gated else None, settings(p))
+        got = A.block_gradients(v["y"], r, st_r, st_y, v["gate"] if gated else None, settings(p), dh if before else None, dr)
+        names = ["y"] + ["residual"] * residual + ["gate"] * gated + ["weight", "bias"] * before + ["after_weight", "after_bias"] * after
+        for name in names:
+            where = v if name in v else p
+            direction = rng.standard_normal(where[name].shape)
+            ends = [loss(*[{**d, name: d[name] + sign * step * direction} if d is where else d for d in (v, p)]) for sign in (1, -1)]
+            want = (ends[0] - ends[1]) / (2 * step)
+            mine = (got[name] * direction).sum()
+            assert abs(want - mine) <= 1e-6 * max(1.0, abs(want)), (case, name, want, mine)
+
+
+def test_residual_norm_refuses(L):
+    from dynamiq_sigcomm_artifact_amd import capi
+    inf = float("inf")
+    forward = dict(y=0x1000, residual=0x1000, h=0x1000, r=0x1000, rows=6, cols=40, eps=1e-5, residual_scale=1.0, block_scale=1.0, dtype=1, stream_dtype=1, before=1)
+    backward = dict(forward, stats=0x1000, dh=0x1000, dr=0x1000, dy=0x1000, dweight=0x1000, work=0x1000, work_floats=1 << 20)
+
+    def call(fn, base, **kw):
+        return fn(ctypes.byref(capi.ResidualNorm(**{**base, **kw})), 0, S)
+    for fn, base in ((L.dq_residual_norm_forward, forward), (L.dq_residual_norm_backward, backward)):
+        refused(L, fn(None, 0, S), "null")
+        for kw, text in ((dict(dtype=3), "dtype"), (dict(stream_dtype=0), "dtype"), (dict(rows=0), "rows must"), (dict(rows=1 << 31), "rows must"), (dict(cols=7), "cols"), (dict(cols=32769), "cols"),
+                         (dict(gate=0x1000, rows_per_gate=4), "divide"), (dict(gate=0x1000, rows_per_gate=0), "divide"), (dict(eps=-1.0), "eps"), (dict(eps=inf), "eps"),
+                         (dict(residual_scale=inf), "scales"), (dict(block_scale=float("nan")), "scales"), (dict(keep_r=1), "null"), (dict(kept=0x1008), "aligned"), (dict(stats=0x1008), "aligned"),
+                         (dict(h8=0x1004), "aligned")):
+            refused(L, call(fn, base, **kw), text)
+    for kw, text in ((dict(y=None), "null"), (dict(h=None), "null"), (dict(r=None), "null"), (dict(before=0), "before"), (dict(residual=None, stream_dtype=2), "stream")):
+        refused(L, call(L.dq_residual_norm_forward, forward, **kw), text)
+    for kw, text in ((dict(stats=None), "null"), (dict(dh=None, dr=None), "null"), (dict(before=0), "before"), (dict(dh=None), "took no part"), (dict(dgate=0x1000), "took no part"),
+                     (dict(dafter_weight=0x1000), "took no part"), (dict(r=None), "checkpoints"), (dict(after=1, y=None), "checkpoints"), (dict(work=None), "null"), (dict(work_floats=6 * 40 - 1), "too small"),
+                     (dict(after=1, keep_y=1, kept=0x1000), "both in 8 bits")):
+        refused(L, call(L.dq_residual_norm_backward, backward, **kw), text)
+
+    def room(**kw):
+        return L.dq_residual_norm_work_floats(ctypes.byref(capi.ResidualNorm(**{**backward, **kw})))
+    assert room() == 6 * 40 and room(dweight=None) == 0 and room(dbias=0x1000) == 2 * 6 * 40 and room(cols=7) == -1
+    assert room(gate=0x1000, dgate=0x1000, rows_per_gate=1) == 6 * 40
+    # runs of rows: as many partial sums as workgroups, and a gate's rows with none but their own
+    assert room(rows=1 << 20, dbias=0x1000) % (2 * 40) == 0 and room(rows=1 << 20) // 40 <= 2048
+    assert room(rows=1 << 20, gate=0x1000, dgate=0x1000, rows_per_gate=1 << 19) // 40 <= 4096
+    for rows in (1, 2, 1000, 4097, 100003):
+        for per in (1, rows):
+            assert 0 < room(rows=rows, gate=0x1000, dgate=0x1000, rows_per_gate=per) <= 2 * 40 * min(rows, 2048)
