@@ -1367,7 +1367,7 @@ int dq_residual_norm_backward(const dq_residual_norm_t *o, int device, dq_stream
     const bool eight = (wants_r && o->keep_r) || (wants_y && o->keep_y);
     dq::BlockNormBackArgs a = {o->dh, o->dr, wants_r ? (o->keep_r ? o->kept : o->r ? o->r : o->y) : nullptr, wants_y ? (o->keep_y ? kept_y : o->y) : nullptr, o->weight, o->gate, o->after_weight,
                           o->after_bias, o->stats, o->dy, o->dresidual, nullptr, o->work, (uint32_t)o->rows, (uint32_t)o->cols, o->gate ? (uint32_t)o->rows_per_gate : 1,
-                          norm_flags(o) | (eight ? dq::kNormEight : 0), 0, 0, 0, 0, (float)o->residual_scale, (float)o->block_scale};
+                          norm_flags(o) | (eight ? dq::kNormEight : 0), 0, 0, 0, 0, 0, (float)o->residual_scale, (float)o->block_scale};
     const auto sum = [&](void *out, int bit) { return dq::NormSum{out, o->float32 & bit ? DQ_F32 : o->dtype}; };
     const dq::NormSum sums[5] = {sum(o->dweight, 1), sum(o->dbias, 2), sum(o->dgate, 4), sum(o->dafter_weight, 8), sum(o->dafter_bias, 16)};
     return finish(dq::launch_norm_backward(a, sums, o->dtype, o->stream_dtype == DQ_F32, static_cast<hipStream_t>(stream)));

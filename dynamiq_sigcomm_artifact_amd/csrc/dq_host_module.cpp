@@ -1612,8 +1612,22 @@ PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
 
 // ---- the gated activation, with its backward pass (activations.py) ----
 
+// what a node's two passes hand on besides tensors: as one object, since a dictionary's entries cost a pass microseconds
+template <class T> struct Noted : torch::CustomClassHolder {
+    T value;
+    explicit Noted(T t) : value(std::move(t)) {}
+    static void keep(torch::autograd::AutogradContext *ctx, T t) { ctx->saved_data["noted"] = c10::IValue::make_capsule(c10::make_intrusive<Noted>(std::move(t))); }
+    // (the context holds it as long as the pass runs)
+    static const T &of(torch::autograd::AutogradContext *ctx) { return static_cast<const Noted *>(ctx->saved_data["noted"].toCapsule().get())->value; }
+};
+
 struct GatedOf : public torch::autograd::Function<GatedOf> {
     typedef std::optional<at::Tensor> Maybe;
+    struct Notes {
+        int64_t kind;
+        bool eight, packed;
+        std::vector<int64_t> shape;
+    };
     // gate and up as rows; without up gate holds both, side by side
     static void fill(dq_gated_t &o, const at::Tensor &x, const Maybe &up)
     {
@@ -1660,10 +1674,7 @@ struct GatedOf : public torch::autograd::Function<GatedOf> {
             else
                 ctx->save_for_backward({x});
         }
-        ctx->saved_data["kind"] = kind;
-        ctx->saved_data["eight"] = eight;
-        ctx->saved_data["packed"] = !up;
-        ctx->saved_data["shape"] = x.sizes();
+        if (kept) Noted<Notes>::keep(ctx, {kind, eight, !up, x.sizes().vec()});
         if (!eight) return {out};
         ctx->mark_non_differentiable({data});
         return {out, data};
@@ -1676,8 +1687,9 @@ struct GatedOf : public torch::autograd::Function<GatedOf> {
         if (!grads[0].defined()) return out;
         const c10::Device device = grads[0].device();
         const c10::DeviceGuard on(device);
-        const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-        const bool packed = ctx->saved_data["packed"].toBool();
+        const Notes &notes = Noted<Notes>::of(ctx);
+        const std::vector<int64_t> &shape = notes.shape;
+        const bool packed = notes.packed;
         const at::Tensor d = grads[0].contiguous();
         const int64_t size = (int64_t)d.element_size();
         dq_gated_t o;
@@ -1685,10 +1697,10 @@ struct GatedOf : public torch::autograd::Function<GatedOf> {
         o.cols = packed ? shape.back() / 2 : shape.back();
         o.rows = c10::multiply_integers(shape.begin(), shape.end() - 1);
         o.dtype = dtype_code(d);
-        o.kind = (int32_t)ctx->saved_data["kind"].toInt();
+        o.kind = (int32_t)notes.kind;
         o.out = d.data_ptr();
         at::Tensor a, b;
-        if (ctx->saved_data["eight"].toBool()) {
+        if (notes.eight) {
             o.gate8 = static_cast<uint8_t *>(saved[0].data_ptr());
             o.up8 = o.gate8 + (checkpoint_bytes(o.rows, o.cols) + 15) / 16 * 16;
         } else {
@@ -1742,6 +1754,12 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         int64_t per; // rows of a gate
     };
     enum { Y, RESIDUAL, WEIGHT, BIAS, GATE, AFTER_WEIGHT, AFTER_BIAS, INPUTS };
+    struct Notes {
+        Settings s;
+        bool keep_r, keep_y, plain, residual, bias;
+        at::ScalarType dtype, stream, bias_dtype;
+        std::vector<int64_t> shape;
+    };
     static const void *data_of(const Maybe &t) { return t ? t->data_ptr() : nullptr; }
 
     // what both passes fill in; vectors: weight, bias, gate, after_weight, after_bias
@@ -1803,10 +1821,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
             const bool sixteen = !s.eight;
             ctx->set_materialize_grads(false);
             ctx->save_for_backward({sixteen && keep_r ? (plain ? y : r) : none, sixteen && keep_y ? y : none, weight, gate, after_weight, after_bias, stats, kept});
-            ctx->saved_data["scales"] = std::vector<double>{s.residual_scale, s.block_scale, s.eps};
-            ctx->saved_data["flags"] = std::vector<int64_t>{s.after, s.before, s.center, s.eight, s.per, keep_r, keep_y, plain, (int64_t)dtype, (int64_t)stream,
-                                                            residual.defined(), bias.defined() ? (int64_t)bias.scalar_type() : -1};
-            ctx->saved_data["shape"] = y.sizes();
+            Noted<Notes>::keep(ctx, {s, keep_r, keep_y, plain, residual.defined(), bias.defined(), dtype, stream, bias.defined() ? bias.scalar_type() : dtype, y.sizes().vec()});
         }
         torch::autograd::variable_list out;
         if (h.defined()) out.push_back(h);
@@ -1824,11 +1839,11 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         torch::autograd::tensor_list out(INPUTS + 1);
         const torch::autograd::variable_list saved = ctx->get_saved_variables();
         const at::Tensor &r = saved[0], &y = saved[1], &weight = saved[2], &gate = saved[3], &after_weight = saved[4], &after_bias = saved[5], &stats = saved[6], &kept = saved[7];
-        const std::vector<int64_t> flags = ctx->saved_data["flags"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
-        const std::vector<double> scales = ctx->saved_data["scales"].toDoubleVector();
-        const Settings s = {scales[0], scales[1], scales[2], flags[0] != 0, flags[1] != 0, flags[2] != 0, flags[3] != 0, true, flags[4]};
-        const bool plain = flags[7], has_residual = flags[10];
-        const at::ScalarType dtype = (at::ScalarType)flags[8], stream = (at::ScalarType)flags[9];
+        const Notes &notes = Noted<Notes>::of(ctx);
+        const Settings &s = notes.s;
+        const std::vector<int64_t> &shape = notes.shape;
+        const bool plain = notes.plain, has_residual = notes.residual;
+        const at::ScalarType dtype = notes.dtype, stream = notes.stream;
         const c10::Device device = stats.device();
         const c10::DeviceGuard on(device);
         const int64_t cols = shape.back(), rows = c10::multiply_integers(shape.begin(), shape.end() - 1);
@@ -1837,13 +1852,13 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         const at::Tensor dr = !plain || !s.before ? grads[s.before ? 1 : 0].defined() ? grads[s.before ? 1 : 0].contiguous() : none : none;
         if (!dh.defined() && !dr.defined()) return out;
         // which of the inputs that took part want a gradient
-        const bool part[INPUTS] = {true, has_residual, weight.defined(), flags[11] >= 0, gate.defined(), after_weight.defined(), after_bias.defined()};
+        const bool part[INPUTS] = {true, has_residual, weight.defined(), notes.bias, gate.defined(), after_weight.defined(), after_bias.defined()};
         bool wanted[INPUTS];
         size_t edge = 0;
         for (int k = 0; k < INPUTS; k++) wanted[k] = part[k] && ctx->needs_input_grad(edge++);
         if (!dh.defined()) wanted[WEIGHT] = wanted[BIAS] = false;
         dq_residual_norm_t o = begin(rows, cols, dtype, stream, s, {&weight, nullptr, &gate, &after_weight, &after_bias});
-        if (flags[11] == (int64_t)at::kFloat) o.float32 |= 2;
+        if (notes.bias && notes.bias_dtype == at::kFloat) o.float32 |= 2;
         const auto make = [&](int k, at::IntArrayRef of, at::ScalarType type) {
             out[k] = rows ? at::empty(of, at::TensorOptions().dtype(type).device(device)) : at::zeros(of, at::TensorOptions().dtype(type).device(device));
             return out[k].data_ptr();
@@ -1853,7 +1868,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         if (wanted[RESIDUAL]) o.dresidual = make(RESIDUAL, shape, stream);
         if (wanted[Y] && !same) o.dy = make(Y, shape, dtype);
         if (wanted[WEIGHT]) o.dweight = make(WEIGHT, weight.sizes(), weight.scalar_type());
-        if (wanted[BIAS]) o.dbias = make(BIAS, {cols}, (at::ScalarType)flags[11]);
+        if (wanted[BIAS]) o.dbias = make(BIAS, {cols}, notes.bias_dtype);
         if (wanted[GATE]) o.dgate = make(GATE, gate.sizes(), gate.scalar_type());
         if (wanted[AFTER_WEIGHT]) o.dafter_weight = make(AFTER_WEIGHT, after_weight.sizes(), after_weight.scalar_type());
         if (wanted[AFTER_BIAS]) o.dafter_bias = make(AFTER_BIAS, after_bias.sizes(), after_bias.scalar_type());
@@ -1863,8 +1878,8 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         if (y.defined()) o.y = y.data_ptr();
         if (kept.defined()) {
             o.kept = static_cast<uint8_t *>(kept.data_ptr());
-            o.keep_r = (int32_t)flags[5];
-            o.keep_y = (int32_t)flags[6];
+            o.keep_r = notes.keep_r;
+            o.keep_y = notes.keep_y;
         }
         if (has_residual) o.residual = stats.data_ptr(); // (that there is one; it is not read)
         o.stats = stats.data_ptr<float>();

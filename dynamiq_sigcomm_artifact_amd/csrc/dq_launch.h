@@ -439,7 +439,8 @@ hipError_t launch_gated(const GatedArgs &a, int dtype, int kind, bool backward, 
 // the norms around a block (dq_residual_norm*.hip): the flags of a row's kernels, its threads above them
 enum : uint32_t {
     kNormCenter = 1, kNormAfter = 2, kNormBefore = 4, kNormKeepR = 8, kNormKeepY = 16, kNormEight = 32, // kNormEight: r and y are checkpoints
-    kNormWeight32 = 64, kNormBias32 = 128, kNormGate32 = 256, kNormAfterWeight32 = 512, kNormAfterBias32 = 1024
+    kNormWeight32 = 64, kNormBias32 = 128, kNormGate32 = 256, kNormAfterWeight32 = 512, kNormAfterBias32 = 1024,
+    kNormPassing = 2048
 };
 struct BlockNormArgs {
     const void *y, *residual, *weight, *bias, *gate, *after_weight, *after_bias;
@@ -455,11 +456,11 @@ struct BlockNormBackArgs {
     const float *stats;
     void *dy, *dresidual, *dgate;
     float *work; // [sums][grid][cols]
-    uint32_t rows, cols, per, flags, grid, run, parts, sums;
+    uint32_t rows, cols, per, flags, grid, teams, run, parts, sums;
     float residual_scale, block_scale;
 };
 struct NormShares {
-    uint32_t grid, run, parts;
+    uint32_t grid, teams, run, parts;
 };
 struct NormSum {
     void *out;

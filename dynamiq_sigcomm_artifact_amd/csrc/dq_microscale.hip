@@ -18,11 +18,14 @@ template <int CTRL> __device__ __forceinline__ float quad_f32(float v)
 
 // H (s x) of the quad's 32 elements, in place (1 / sqrt(32) is encode_block's); word: the sign bits of the block.  Stages of stride 1, 2, 4 lie within a lane, 8 and 16
 // between lanes.  Every sum is one of two numbers, whichever lane takes it: the result does not depend on the layout.
-__device__ __forceinline__ void rotate_block(float (&v)[8], uint32_t word, int g)
+// (SIGNED: v has its signs already.)
+template <bool SIGNED = false> __device__ __forceinline__ void rotate_block(float (&v)[8], uint32_t word, int g)
 {
+    if (!SIGNED) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) // v ^ (its sign bit, shifted up, & the sign's place)
-        v[j] = __uint_as_float(__builtin_amdgcn_bitop3_b32(__float_as_uint(v[j]), (word >> 8 * g) << (31 - j), 0x80000000u, 0x78));
+        for (int j = 0; j < 8; j++) // v ^ (its sign bit, shifted up, & the sign's place)
+            v[j] = __uint_as_float(__builtin_amdgcn_bitop3_b32(__float_as_uint(v[j]), (word >> 8 * g) << (31 - j), 0x80000000u, 0x78));
+    }
 #pragma unroll
     for (int h = 1; h < 8; h *= 2)
 #pragma unroll
@@ -32,16 +35,11 @@ __device__ __forceinline__ void rotate_block(float (&v)[8], uint32_t word, int g
                 v[j] = a + b;
                 v[j + h] = a - b;
             }
+    const uint32_t first = (uint32_t)g << 31, second = (uint32_t)(g & 2) << 30; // the lane that takes the difference turns its own sign round
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float b = quad_f32<0xB1>(v[j]);
-        v[j] = g & 1 ? b - v[j] : v[j] + b;
-    }
+    for (int j = 0; j < 8; j++) v[j] = quad_f32<0xB1>(v[j]) + __uint_as_float(__float_as_uint(v[j]) ^ first);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float b = quad_f32<0x4E>(v[j]);
-        v[j] = g & 2 ? b - v[j] : v[j] + b;
-    }
+    for (int j = 0; j < 8; j++) v[j] = quad_f32<0x4E>(v[j]) + __uint_as_float(__float_as_uint(v[j]) ^ second);
 }
 
 // the eight uniform values of elements e .. e + 7 of the result (e a multiple of 8)
@@ -165,35 +163,41 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 // (4.6 TB/s), 132 behind other work (with the XCDs' workgroups strewn 8 % more, 8000 x 5000 40 for 35), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
 // instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.  Blocks that have to be lowered are looked for while their columns
 // are encoded and taken behind the loop, where nothing else needs registers (in it: 2 to 6 % for every matrix); to the nearest four workgroups share a CU, which 65 registers would not let them.
-struct ColumnsLds {
-    __attribute__((aligned(16))) uint8_t tile[128 * 128];
-    __attribute__((aligned(8))) uint8_t scales[128 * 8];
+// A checkpoint's tile is twice as wide, 16 columns a lane: runs of 256 bytes of it as of a 16-bit matrix.
+template <int DT> constexpr uint32_t kColumns = DT == DQ_E4M3 ? 16 : 8; // of a lane
+inline uint32_t columns_tiles(int64_t cols, int dtype) { return dtype == DQ_E4M3 ? (uint32_t)((cols + 255) >> 8) : (uint32_t)((cols + 127) >> 7); }
+template <uint32_t LINES> struct ColumnsLds {
+    __attribute__((aligned(16))) uint8_t tile[LINES * 128];
+    __attribute__((aligned(8))) uint8_t scales[LINES * 8];
 };
-// element j of eight E4M3 codes (j a constant once the loop around it is unrolled)
-__device__ __forceinline__ float byte_value(const uint32_t (&x)[2], int j)
+// element j of E4M3 codes (j a constant once the loop around it is unrolled)
+__device__ __forceinline__ float byte_value(const uint32_t (&x)[4], int j)
 {
     const f32x2_t v = j & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(x[j >> 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8(x[j >> 2], false);
     return j & 1 ? v.y : v.x;
 }
 
-template <int DT, int RAND, bool ROTATE>
-__device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t superchunks, const Division &tiles, uint32_t id, ColumnsLds &lds)
+template <int DT, int RAND, bool ROTATE, class LDS>
+__device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t superchunks, const Division &tiles, uint32_t id, LDS &lds)
 {
+    constexpr uint32_t EACH = kColumns<DT>, LINES = 16 * EACH, TURN = EACH == 16 ? 4 : 3; // TURN: neighbouring lanes' lines lie in turned pieces
     uint8_t *tile = lds.tile, *tile_scales = lds.scales;
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
-    const uint32_t superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * 128, col = col0 + 8 * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
+    const uint32_t superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * LINES, col = col0 + EACH * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
     const uint32_t row0 = superchunk * 256 + 32 * block, row = row0 + 8 * g;
-    constexpr int WORDS = DT == DQ_F32 ? 8 : DT == DQ_E4M3 ? 2 : 4;
+    constexpr int WORDS = DT == DQ_F32 ? 8 : 4;
     uint32_t x[8][WORDS]; // [row][column], as they are in memory
     float up[8];          // of a checkpoint's rows
     if constexpr (DT == DQ_E4M3) {
-        const uint32_t from = min(col, (uint32_t)a.stride - 8);
+        const uint32_t from = min(col, (uint32_t)a.stride - 16);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int64_t r = min(row + j, last_row);
-            const u32x2_t w = *reinterpret_cast<const u32x2_t *>(static_cast<const uint8_t *>(a.x) + r * a.stride + from);
-            x[j][0] = w[0];
-            x[j][1] = w[1];
+            const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.x) + r * a.stride + from);
+            x[j][0] = w.x;
+            x[j][1] = w.y;
+            x[j][2] = w.z;
+            x[j][3] = w.w;
             up[j] = scale_up(a.x_scales[r * (a.stride >> 5) + (from >> 5)]);
         }
     } else if (all_cols >= 8) {
@@ -227,17 +231,22 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
                 up[j] = 0.0f;
             }
     }
-    const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u, first = col * superchunks + superchunk, most = (all_cols - 1) * superchunks + superchunk;
+    const uint32_t sign = ROTATE ? a.sign[row0 >> 5] : 0u;
+    if constexpr (DT == DQ_E4M3 && ROTATE) { // a row's sign goes with its scale
+#pragma unroll
+        for (int j = 0; j < 8; j++) up[j] = __uint_as_float(__float_as_uint(up[j]) ^ (sign >> (8 * g + j)) << 31);
+    }
+    const uint32_t first = col * superchunks + superchunk, most = (all_cols - 1) * superchunks + superchunk;
     // (what becomes of columns past the end is not stored)
     const auto draw = [&](int c, float (&u)[8]) { uniform8<RAND>(a, (int64_t)min(first + c * superchunks, most) * 256 + 32 * block + 8 * g, u); };
     const auto put = [&](int c, uint32_t word, uint32_t scale) {
-        const int line = 8 * (lane >> 2) + c;
-        *reinterpret_cast<uint32_t *>(tile + line * 128 + ((block ^ (line >> 3 & 7)) << 4) + 4 * g) = word;
+        const int line = EACH * (lane >> 2) + c;
+        *reinterpret_cast<uint32_t *>(tile + line * 128 + ((block ^ (line >> TURN & 7)) << 4) + 4 * g) = word;
         if (g == 0) tile_scales[line * 8 + block] = (uint8_t)scale;
     };
     bool beyond = false;
 #pragma unroll
-    for (int c = 0; c < 8; c++) {
+    for (int c = 0; c < (int)EACH; c++) {
         float v[8], u[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -247,27 +256,30 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
                 v[j] = word_value<DT>(x[j], c);
         }
         draw(c, u);
-        if (ROTATE) rotate_block(v, sign, g);
+        if (ROTATE) rotate_block<DT == DQ_E4M3>(v, sign, g);
         uint32_t scale;
         const uint32_t word = encode_block<RAND, ROTATE>(v, u, scale);
         put(c, word, scale);
         beyond |= scale == 255u;
+        if (DT == DQ_E4M3 && c & 1) __builtin_amdgcn_sched_barrier(0); // (16 columns at once would need registers that there are not)
     }
     if (ROTATE && DT != DQ_F16 && DQ_UNLIKELY(__builtin_amdgcn_ballot_w64(beyond) != 0)) {
+        uint32_t at_row = row, at_col = col; // (as values of their own: what was worked out from the others for the first loads is not held until here)
+        asm("" : "+v"(at_row), "+v"(at_col));
 #pragma unroll 1
-        for (int c = 0; c < 8; c++) { // what nobody holds any more, element by element
+        for (int c = 0; c < (int)EACH; c++) { // what nobody holds any more, element by element
             float v[8], u[8];
             uint32_t scale;
             const auto load = [&] {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int64_t r = min(row + j, last_row);
-                    const uint32_t at = min(col + c, all_cols - 1);
+                    const int64_t r = min(at_row + j, last_row);
+                    const uint32_t at = min(at_col + c, all_cols - 1);
                     if constexpr (DT == DQ_E4M3)
                         v[j] = __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t *>(a.x)[r * a.stride + at], 0) * scale_up(a.x_scales[r * (a.stride >> 5) + (at >> 5)]);
                     else
                         v[j] = ElemIO<DT>::load(a.x, r * a.stride + at);
-                    if (row + j > last_row) v[j] = 0.0f;
+                    if (at_row + j > last_row) v[j] = 0.0f;
                 }
             };
             load();
@@ -283,20 +295,20 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
+    for (int k = 0; k < (int)LINES / 64; k++) {
         const int s = threadIdx.x + 512 * k, line = s >> 3, piece = s & 7;
         if (col0 + line < all_cols)
             reinterpret_cast<uint4 *>(a.codes)[((int64_t)(col0 + line) * superchunks + superchunk) * 8 + piece] =
-                *reinterpret_cast<const uint4 *>(tile + line * 128 + ((piece ^ (line >> 3 & 7)) << 4));
+                *reinterpret_cast<const uint4 *>(tile + line * 128 + ((piece ^ (line >> TURN & 7)) << 4));
     }
-    if (threadIdx.x < 128 && col0 + threadIdx.x < all_cols)
+    if (threadIdx.x < LINES && col0 + threadIdx.x < all_cols)
         reinterpret_cast<uint2 *>(a.scales)[(int64_t)(col0 + threadIdx.x) * superchunks + superchunk] = reinterpret_cast<const uint2 *>(tile_scales)[threadIdx.x];
 }
 
 template <int DT, int RAND, bool ROTATE>
-__global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : RAND == kNearest && ROTATE ? 8 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
+__global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : RAND == kNearest && ROTATE && DT != DQ_E4M3 ? 8 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
 {
-    __shared__ ColumnsLds lds;
+    __shared__ ColumnsLds<16 * kColumns<DT>> lds;
     quantize_columns<DT, RAND, ROTATE>(a, superchunks, tiles, unit_of(blockIdx.x, gridDim.x), lds);
 }
 
@@ -304,7 +316,7 @@ template <int DT, int RAND> static hipError_t launch_quantize(const QuantizeArgs
 {
     const uint32_t superchunks = (uint32_t)(((columns ? a.rows : a.cols) + 255) >> 8);
     if (columns) {
-        const Division tiles((uint32_t)((a.cols + 127) >> 7));
+        const Division tiles(columns_tiles(a.cols, DT));
         const dim3 grid(tiles.by * superchunks);
         if (a.sign)
             mx4_columns_kernel<DT, RAND, true><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
@@ -355,7 +367,7 @@ struct QuantizeJobs {
     QuantizeJob job[kJobs];
 };
 
-template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void do_job(const QuantizeJob &j, bool columns, uint32_t id, ColumnsLds &lds)
+template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void do_job(const QuantizeJob &j, bool columns, uint32_t id, ColumnsLds<256> &lds)
 {
     if (columns)
         quantize_columns<DT, RAND, ROTATE>(j.a, j.superchunks, j.by, id, lds);
@@ -365,7 +377,7 @@ template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void do_job(
 
 template <int DT> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_jobs_kernel(QuantizeJobs jobs)
 {
-    __shared__ ColumnsLds lds;
+    __shared__ ColumnsLds<256> lds;
     int k = 0;
 #pragma unroll
     for (int i = 1; i < kJobs; i++) k += blockIdx.x >= jobs.job[i].first ? 1 : 0;
@@ -391,7 +403,7 @@ template <int DT> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void m
 hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStream_t stream)
 {
     const auto blocks_of = [](const QuantizeOne &q) {
-        return q.columns ? ((q.a.cols + 127) >> 7) * ((q.a.rows + 255) >> 8) : (q.a.rows * ((q.a.cols + 255) >> 8) + 15) >> 4;
+        return q.columns ? columns_tiles(q.a.cols, q.dtype) * ((q.a.rows + 255) >> 8) : (q.a.rows * ((q.a.cols + 255) >> 8) + 15) >> 4;
     };
     for (int next = 0; next < count;) {
         int take = 0, dtype = DQ_E4M3; // the type of what is no checkpoint
@@ -417,7 +429,7 @@ hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStrea
                 const QuantizeOne &q = list[next + k];
                 j.a = q.a;
                 j.superchunks = (uint32_t)(((q.columns ? q.a.rows : q.a.cols) + 255) >> 8);
-                j.by = Division(q.columns ? (uint32_t)((q.a.cols + 127) >> 7) : j.superchunks);
+                j.by = Division(q.columns ? columns_tiles(q.a.cols, q.dtype) : j.superchunks);
                 j.units = (uint32_t)(q.a.rows * j.superchunks * 32);
                 j.kind = (q.columns ? 16 : 0) + (q.dtype == DQ_E4M3 ? 10 : !q.stochastic ? 0 : !q.a.pool ? 2 : 4 + 2 * q.pool_dtype) + (q.a.sign ? 1 : 0);
                 first += (uint32_t)blocks_of(q);

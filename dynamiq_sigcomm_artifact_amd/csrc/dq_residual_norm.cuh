@@ -34,7 +34,7 @@ __device__ __forceinline__ float wave_sum_f32(float v)
 // met, in the sum between, everybody who still read it.
 struct GroupSums {
     f32x2_t (*part)[16];
-    uint32_t waves;
+    uint32_t waves, first; // of those that share a row
     int turn = 0;
     __device__ __forceinline__ void operator()(float &a, float &b)
     {
@@ -46,7 +46,7 @@ struct GroupSums {
         if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = f32x2_t{a, b};
         __syncthreads();
         const uint32_t w = threadIdx.x & 15;
-        const f32x2_t v = at[min(w, waves - 1)];
+        const f32x2_t v = at[first + min(w, waves - 1)];
         a = row16_sum(w < waves ? v.x : 0.0f);
         b = row16_sum(w < waves ? v.y : 0.0f);
     }
@@ -59,15 +59,30 @@ __device__ __forceinline__ float inverse_root(float x)
     return (float)(y + 0.5 * y * rest);
 }
 
-// Eight elements of a row as words, 0 behind the last column.  A lane whose eight reach past the end loads the last eight of the row and moves them up: no lane loads less or
-// apart (columns are eight at least).
-template <int DT> __device__ __forceinline__ void load_row(const void *p, int64_t base, uint32_t col, uint32_t cols, uint32_t (&x)[kWords<DT>])
+// where a row of elements begins, the same for every lane
+template <int DT> __device__ __forceinline__ const char *row_of(const void *p, int64_t element) { return static_cast<const char *>(p) + element * (DT == DQ_F32 ? 4 : 2); }
+template <int DT> __device__ __forceinline__ char *row_of(void *p, int64_t element) { return static_cast<char *>(p) + element * (DT == DQ_F32 ? 4 : 2); }
+
+// Eight elements of a row as words.  A lane whose eight reach past the end loads the last eight of the row, and moves them up when they are used (settle), with zeros behind the
+// last column: no lane loads less or apart (columns are eight at least), and no load is waited for before the next is on its way.
+template <int DT, bool PASSING = false> __device__ __forceinline__ void load_row(const char *row, uint32_t col, uint32_t cols, uint32_t (&x)[kWords<DT>])
 {
+    constexpr int N = kWords<DT>;
     const uint32_t from = min(col, cols - 8);
-    load_words<DT>(p, base + from, x);
-    const uint32_t up = min(col - from, 8u);
+    const char *q = row + from * (uint32_t)(DT == DQ_F32 ? 4 : 2);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+        const u32x4_any *at = reinterpret_cast<const u32x4_any *>(q + 4 * k);
+        const u32x4_any w = PASSING ? __builtin_nontemporal_load(at) : *at;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[k + j] = w[j];
+    }
+}
+template <int DT> __device__ __forceinline__ void settle(uint32_t col, uint32_t cols, uint32_t (&x)[kWords<DT>])
+{
+    constexpr int N = kWords<DT>;
+    const uint32_t up = min(col - min(col, cols - 8), 8u);
     if (up) {
-        constexpr int N = kWords<DT>;
         if (N == 4 && up & 1) {
 #pragma unroll
             for (int w = 0; w < N; w++) x[w] = w + 1 < N ? __builtin_amdgcn_alignbit(x[(w + 1) % N], x[w], 16) : x[w] >> 16;
@@ -89,8 +104,9 @@ __device__ __forceinline__ void clip(float (&v)[8], int own)
         for (int j = 0; j < 8; j++) v[j] = j < own ? v[j] : 0.0f;
     }
 }
-template <int DT> __device__ __forceinline__ void row_values(const uint32_t (&x)[kWords<DT>], float (&v)[8])
+template <int DT> __device__ __forceinline__ void row_values(uint32_t (&x)[kWords<DT>], uint32_t col, uint32_t cols, float (&v)[8])
 {
+    settle<DT>(col, cols, x);
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = word_value<DT>(x, j);
 }
@@ -99,20 +115,22 @@ template <int DT> __device__ __forceinline__ void load_columns(const void *p, bo
 {
     if (DT == DQ_F32 || in32) {
         uint32_t x[8];
-        load_row<DQ_F32>(p, base, col, cols, x);
-        row_values<DQ_F32>(x, v);
+        load_row<DQ_F32>(row_of<DQ_F32>(p, base), col, cols, x);
+        row_values<DQ_F32>(x, col, cols, v);
     } else {
         uint32_t x[kWords<DT>];
-        load_row<DT>(p, base, col, cols, x);
-        row_values<DT>(x, v);
+        load_row<DT>(row_of<DT>(p, base), col, cols, x);
+        row_values<DT>(x, col, cols, v);
     }
 }
-template <int DT> __device__ __forceinline__ void store_row(void *p, int64_t base, uint32_t col, uint32_t cols, const float (&v)[8])
+template <int DT, bool PASSING = false> __device__ __forceinline__ void store_row(char *row, uint32_t col, uint32_t cols, const float (&v)[8])
 {
-    if (col + 8 <= cols)
-        store8<DT>(p, base + col, v);
-    else if (col < cols)
-        store_part<DT, 8>(p, base + col, (int)(cols - col), v);
+    if (col + 8 <= cols) {
+        store4<DT, PASSING>(row, col, v);
+        store4<DT, PASSING>(row, col + 4, v + 4);
+    } else if (col < cols) {
+        store_part<DT, 8>(row, col, (int)(cols - col), v);
+    }
 }
 
 // eight elements of a row into a checkpoint (four neighbouring lanes together; those past the last column are 0)
@@ -126,12 +144,48 @@ template <int DT> __device__ __forceinline__ void keep_row(uint8_t *data, int64_
     if ((threadIdx.x & 3) == 0) c.scales[(int64_t)row * c.blocks + (col >> 5)] = (uint8_t)scale;
 }
 
-template <int DT, int RT, int V, int THREADS> __global__ __launch_bounds__(THREADS) void residual_norm_kernel(BlockNormArgs a)
+// What the columns are multiplied by, or added to them: words, and when they have all been asked for values (`none` where there is no such vector, 0 behind the last column).
+template <int DT> struct Columns {
+    uint32_t x[8];
+    float v[8];
+    __device__ __forceinline__ void ask(const void *p, bool in32, int64_t base, uint32_t col, uint32_t cols)
+    {
+        if (!p) return;
+        if (DT == DQ_F32 || in32) {
+            load_row<DQ_F32>(row_of<DQ_F32>(p, base), col, cols, x);
+        } else {
+            uint32_t y[kWords<DT>];
+            load_row<DT>(row_of<DT>(p, base), col, cols, y);
+#pragma unroll
+            for (int w = 0; w < kWords<DT>; w++) x[w] = y[w];
+        }
+    }
+    __device__ __forceinline__ void take(const void *p, bool in32, uint32_t col, uint32_t cols, float none)
+    {
+        if (!p) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = none;
+            clip(v, lanes_own(col, cols));
+        } else if (DT == DQ_F32 || in32) {
+            row_values<DQ_F32>(x, col, cols, v);
+        } else {
+            uint32_t y[kWords<DT>];
+#pragma unroll
+            for (int w = 0; w < kWords<DT>; w++) y[w] = x[w];
+            row_values<DT>(y, col, cols, v);
+        }
+    }
+};
+
+// FULL: there is a norm after the block, or a gate.  Rows up to 8192 wide are taken in turn by as many workgroups as the chip holds, which keep the vectors and ask for a row
+// before they work on the one in front of it.
+template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global__ __launch_bounds__(THREADS, 4) void residual_norm_kernel(BlockNormArgs a)
 {
+    constexpr bool HELD = V == 1;
     __shared__ f32x2_t part[2][16];
     const uint32_t threads = a.flags >> 16, cols = a.cols;
-    const bool center = a.flags & kNormCenter, after = a.flags & kNormAfter, before = a.flags & kNormBefore;
-    GroupSums sums = {part, threads >> 6};
+    const bool center = a.flags & kNormCenter, after = FULL && a.flags & kNormAfter, before = a.flags & kNormBefore;
+    GroupSums sums = {part, threads >> 6, 0};
     // mean and 1 / sqrt(var + eps) of a row, whose elements past the last column are 0
     const auto statistics = [&](const float (&x)[V][8], float &mean, float &rs) {
         float s = 0.0f, none = 0.0f;
@@ -157,61 +211,84 @@ template <int DT, int RT, int V, int THREADS> __global__ __launch_bounds__(THREA
         sums(s, none);
         rs = inverse_root(s / (float)cols + a.eps);
     };
-    const auto normalise = [&](float (&x)[8], float mean, float rs, const void *weight, bool weight32, const void *bias, bool bias32, uint32_t col) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = (x[j] - mean) * rs;
-        if (weight) {
-            load_columns<DT>(weight, weight32, 0, col, cols, v);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] *= v[j];
-        }
-        if (bias) {
-            load_columns<DT>(bias, bias32, 0, col, cols, v);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] += v[j];
-        }
-        clip(x, lanes_own(col, cols));
+    Columns<DT> weight, bias, after_weight, after_bias, gate;
+    const auto ask_gate = [&](uint32_t row, uint32_t col) { gate.ask(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols); };
+    const auto take_gate = [&](uint32_t col) { gate.take(a.gate, a.flags & kNormGate32, col, cols, 1.0f); };
+    const auto ask_after = [&](uint32_t col) {
+        after_weight.ask(a.after_weight, a.flags & kNormAfterWeight32, 0, col, cols);
+        after_bias.ask(a.after_bias, a.flags & kNormAfterBias32, 0, col, cols);
     };
-    for (uint32_t row = blockIdx.x; row < a.rows; row += a.grid) {
+    const auto take_after = [&](uint32_t col) {
+        after_weight.take(a.after_weight, a.flags & kNormAfterWeight32, col, cols, 1.0f);
+        after_bias.take(a.after_bias, a.flags & kNormAfterBias32, col, cols, 0.0f);
+    };
+    const auto ask_before = [&](uint32_t col) {
+        weight.ask(a.weight, a.flags & kNormWeight32, 0, col, cols);
+        bias.ask(a.bias, a.flags & kNormBias32, 0, col, cols);
+    };
+    const auto take_before = [&](uint32_t col) {
+        weight.take(a.weight, a.flags & kNormWeight32, col, cols, 1.0f);
+        bias.take(a.bias, a.flags & kNormBias32, col, cols, 0.0f);
+    };
+    struct Raw {
+        uint32_t y[V][kWords<DT>], residual[V][kWords<RT>];
+    };
+    const auto load = [&](Raw &raw, uint32_t row) {
         const int64_t base = (int64_t)row * cols;
-        uint32_t yw[V][kWords<DT>], rw[V][kWords<RT>];
 #pragma unroll
-        for (int k = 0; k < V; k++) load_row<DT>(a.y, base, 8 * (threadIdx.x + k * threads), cols, yw[k]);
+        for (int k = 0; k < V; k++) load_row<DT, PASSING>(row_of<DT>(a.y, base), 8 * (threadIdx.x + k * threads), cols, raw.y[k]);
         if (a.residual) {
 #pragma unroll
-            for (int k = 0; k < V; k++) load_row<RT>(a.residual, base, 8 * (threadIdx.x + k * threads), cols, rw[k]);
+            for (int k = 0; k < V; k++) load_row<RT, PASSING>(row_of<RT>(a.residual, base), 8 * (threadIdx.x + k * threads), cols, raw.residual[k]);
         }
+    };
+    uint32_t gated = blockIdx.x / a.per; // the gate that is held
+    const auto step = [&](Raw &now, Raw &next, uint32_t row) {
+        const int64_t base = (int64_t)row * cols;
+        if (HELD && row + a.grid < a.rows) load(next, row + a.grid);
+        if (!HELD) load(now, row);
         float x[V][8], mean_y = 0.0f, rs_y = 1.0f;
 #pragma unroll
-        for (int k = 0; k < V; k++) row_values<DT>(yw[k], x[k]);
+        for (int k = 0; k < V; k++) row_values<DT>(now.y[k], 8 * (threadIdx.x + k * threads), cols, x[k]);
         if (a.flags & kNormKeepY) {
             uint8_t *data = a.kept + (a.flags & kNormKeepR ? (((int64_t)a.rows * ((cols + 31) >> 5) * 33 + 15) & ~(int64_t)15) : 0);
 #pragma unroll
             for (int k = 0; k < V; k++) keep_row<DT>(data, a.rows, row, 8 * (threadIdx.x + k * threads), cols, x[k]);
         }
         if (after) statistics(x, mean_y, rs_y);
+        if (FULL && HELD && a.gate && row / a.per != gated) {
+            gated = row / a.per;
+            ask_gate(row, 8 * threadIdx.x);
+            take_gate(8 * threadIdx.x);
+        }
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const uint32_t col = 8 * (threadIdx.x + k * threads);
             if (after) {
-                normalise(x[k], mean_y, rs_y, a.after_weight, a.flags & kNormAfterWeight32, a.after_bias, a.flags & kNormAfterBias32, col);
-            }
-            if (a.gate) {
-                float g[8];
-                load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols, g);
+                if (!HELD) {
+                    ask_after(col);
+                    take_after(col);
+                }
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[k][j] *= g[j];
+                for (int j = 0; j < 8; j++) x[k][j] = (x[k][j] - mean_y) * rs_y * after_weight.v[j] + after_bias.v[j];
+            }
+            if (FULL && a.gate) {
+                if (!HELD) {
+                    ask_gate(row, col);
+                    take_gate(col);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[k][j] *= gate.v[j];
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) x[k][j] *= a.block_scale;
             if (a.residual) {
                 float v[8];
-                row_values<RT>(rw[k], v);
+                row_values<RT>(now.residual[k], col, cols, v);
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[k][j] = v[j] * a.residual_scale + x[k][j];
             }
-            if (a.r) store_row<RT>(a.r, base, col, cols, x[k]);
+            if (a.r) store_row<RT>(row_of<RT>(a.r, base), col, cols, x[k]);
             if (a.flags & kNormKeepR) { // of r as it is stored
                 float v[8];
 #pragma unroll
@@ -225,14 +302,38 @@ template <int DT, int RT, int V, int THREADS> __global__ __launch_bounds__(THREA
 #pragma unroll
             for (int k = 0; k < V; k++) {
                 const uint32_t col = 8 * (threadIdx.x + k * threads);
-                normalise(x[k], mean, rs, a.weight, a.flags & kNormWeight32, a.bias, a.flags & kNormBias32, col);
+                if (!HELD) {
+                    ask_before(col);
+                    take_before(col);
+                }
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[k][j] = ElemIO<DT>::round(x[k][j]);
-                store_row<DT>(a.h, base, col, cols, x[k]);
+                for (int j = 0; j < 8; j++) x[k][j] = ElemIO<DT>::round((x[k][j] - mean) * rs * weight.v[j] + bias.v[j]);
+                store_row<DT>(row_of<DT>(a.h, base), col, cols, x[k]);
                 if (a.h8) keep_row<DT>(a.h8, a.rows, row, col, cols, x[k]);
             }
         }
         if (a.stats && threadIdx.x == 0) reinterpret_cast<float4 *>(a.stats)[row] = make_float4(mean, rs, mean_y, rs_y);
+    };
+    Raw one, other;
+    if (HELD) {
+        const uint32_t col = 8 * threadIdx.x;
+        load(one, blockIdx.x);
+        if (FULL) {
+            ask_after(col);
+            ask_gate(blockIdx.x, col);
+        }
+        ask_before(col);
+        if (FULL) {
+            take_after(col);
+            take_gate(col);
+        }
+        take_before(col);
+        for (uint32_t row = blockIdx.x; row < a.rows; row += 2 * a.grid) {
+            step(one, other, row);
+            if (row + a.grid < a.rows) step(other, one, row + a.grid);
+        }
+    } else {
+        for (uint32_t row = blockIdx.x; row < a.rows; row += a.grid) step(one, one, row);
     }
 }
 
@@ -242,15 +343,19 @@ template <int DT, int RT, int V, int THREADS> __global__ __launch_bounds__(THREA
 //   dresidual = residual_scale dr, t = block_scale dr, dgate = sum t z, t gate through the norm of y likewise: dy
 //   dweight = sum dh xhat, dbias = sum dh, and of the norm of y with t gate in dh's place
 //
-// SUMS: which of them registers are kept for, at least those that are wanted.
+// SUMS: which of them registers are kept for, at least those that are wanted.  Narrow rows are shared by fewer threads than a workgroup has: those that share one, a team, have a
+// run of rows each, and add up what they have of the columns before it leaves.
 enum { kSumWeight = 1, kSumBias = 2, kSumGate = 4, kSumAfterWeight = 8, kSumAfterBias = 16 };
 
-template <int DT, int RT, int V, int THREADS, int SUMS> __global__ __launch_bounds__(THREADS) void residual_norm_backward_kernel(BlockNormBackArgs a)
+template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING> __global__ __launch_bounds__(THREADS, 4) void residual_norm_backward_kernel(BlockNormBackArgs a)
 {
+    constexpr bool AHEAD = V == 1 && !(SUMS & ~(kSumWeight | kSumBias));
+    constexpr bool AFTER = SUMS & (kSumAfterWeight | kSumAfterBias), BETWEEN = SUMS & ~(kSumWeight | kSumBias);
     __shared__ f32x2_t part[2][16];
-    const uint32_t threads = a.flags >> 16, cols = a.cols, sums_wanted = a.sums;
-    const bool center = a.flags & kNormCenter, after = a.flags & kNormAfter, eight = a.flags & kNormEight;
-    GroupSums sums = {part, threads >> 6};
+    const uint32_t threads = a.flags >> 16, cols = a.cols;
+    const bool center = a.flags & kNormCenter, after = AFTER && a.flags & kNormAfter;
+    const uint32_t team = V == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / threads) : 0, lane = threadIdx.x - team * threads;
+    GroupSums sums = {part, threads >> 6, team * (threads >> 6)};
     const float share = 1.0f / (float)cols;
     float acc[5][V][8];
     const auto clear = [&](int s) {
@@ -262,71 +367,106 @@ template <int DT, int RT, int V, int THREADS, int SUMS> __global__ __launch_boun
 #pragma unroll
     for (int s = 0; s < 5; s++)
         if (SUMS >> s & 1) clear(s);
-    // the workgroup's rows: of one gate, or of whole ones
-    const uint32_t of = a.parts > 1 ? blockIdx.x / a.parts : 0;
-    const uint32_t start = a.parts > 1 ? of * a.per + (blockIdx.x - of * a.parts) * a.run : blockIdx.x * a.run;
+    // a team's rows: of one gate, or of whole ones
+    const uint32_t id = blockIdx.x * a.teams + team, of = a.parts > 1 ? id / a.parts : 0;
+    const uint32_t start = a.parts > 1 ? of * a.per + (id - of * a.parts) * a.run : id * a.run;
     const uint32_t end = min(start + a.run, a.parts > 1 ? (of + 1) * a.per : a.rows);
     uint32_t left = a.per;
-    const auto load_kept = [&](const void *p, auto &x, int64_t row, uint32_t col, auto type) {
-        constexpr int T = decltype(type)::value;
-        if (eight) {
-            const CheckpointOf<const uint8_t> c(static_cast<const uint8_t *>(p), a.rows, cols);
-            const uint32_t from = min(col, 32 * c.blocks - 8);
-            const u32x2_t w = *reinterpret_cast<const u32x2_t *>(c.codes + row * 32 * c.blocks + from);
-            x[0] = w[0];
-            x[1] = w[1];
-            x[2] = c.scales[row * c.blocks + (from >> 5)];
+    // What the columns are multiplied by, in registers where they hold it all along (1 where there is no weight; 0 behind the last column, where nothing else need be).
+    constexpr bool HELD = V == 1;
+    float weight[HELD ? 1 : V][8], after_weight[HELD ? 1 : V][8], gate[HELD ? 1 : V][8];
+    const auto load_weight = [&](const void *p, bool in32, int64_t base, uint32_t col, float (&v)[8]) {
+        if (p) {
+            load_columns<DT>(p, in32, base, col, cols, v);
         } else {
-            load_row<T>(p, row * cols, col, cols, x);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = 1.0f;
+            clip(v, lanes_own(col, cols));
         }
     };
-    const auto kept_values = [&](const auto &x, float (&v)[8], auto type) {
+    if (HELD) {
+        load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * lane, weight[0]);
+        if (AFTER) load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, 8 * lane, after_weight[0]);
+        if (BETWEEN && a.gate) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(min(start, a.rows - 1) / a.per) * cols, 8 * lane, cols, gate[0]); // (a team may have no rows)
+    }
+    const auto load_kept = [&](const void *p, auto &x, uint32_t row, uint32_t col, auto type) {
         constexpr int T = decltype(type)::value;
-        if (eight) {
+        if (EIGHT) {
+            const CheckpointOf<const uint8_t> c(static_cast<const uint8_t *>(p), a.rows, cols);
+            const uint32_t from = min(col, 32 * c.blocks - 8);
+            const u32x2_t *at = reinterpret_cast<const u32x2_t *>(c.codes + (int64_t)row * 32 * c.blocks + from), w = PASSING ? __builtin_nontemporal_load(at) : *at;
+            x[0] = w[0];
+            x[1] = w[1];
+            x[2] = (c.scales + (int64_t)row * c.blocks)[from >> 5];
+        } else {
+            load_row<T, PASSING>(row_of<T>(p, (int64_t)row * cols), col, cols, x);
+        }
+    };
+    const auto kept_values = [&](auto &x, uint32_t col, float (&v)[8], auto type) {
+        constexpr int T = decltype(type)::value;
+        if (EIGHT) {
             const u32x2_t w = {x[0], x[1]};
             decode_e4m3(w, x[2], v);
         } else {
-            row_values<T>(x, v);
+            row_values<T>(x, col, cols, v);
         }
     };
     typedef std::integral_constant<int, DT> Y;
     typedef std::integral_constant<int, RT> R;
-    for (uint32_t row = start; row < end; row++) {
+    // a row as it comes from memory
+    struct Raw {
+        uint32_t dh[V][kWords<DT>], dr[V][kWords<RT>], r[V][kWords<RT>], y[V][kWords<DT>];
+        float4 stats;
+    };
+    const auto load = [&](Raw &x, uint32_t row) {
         const int64_t base = (int64_t)row * cols;
-        uint32_t dhw[V][kWords<DT>], drw[V][kWords<RT>], rw[V][kWords<RT>], yw[V][kWords<DT>];
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const uint32_t col = 8 * (threadIdx.x + k * threads);
+            const uint32_t col = 8 * (lane + k * threads);
             if (a.dh) {
-                load_row<DT>(a.dh, base, col, cols, dhw[k]);
-                load_kept(a.r, rw[k], row, col, R());
+                load_row<DT, PASSING>(row_of<DT>(a.dh, base), col, cols, x.dh[k]);
+                load_kept(a.r, x.r[k], row, col, R());
             }
-            if (a.dr) load_row<RT>(a.dr, base, col, cols, drw[k]);
-            if (a.y) load_kept(a.y, yw[k], row, col, Y());
+            if (a.dr) load_row<RT, PASSING>(row_of<RT>(a.dr, base), col, cols, x.dr[k]);
+            if (BETWEEN && a.y) load_kept(a.y, x.y[k], row, col, Y());
         }
-        const float4 stats = reinterpret_cast<const float4 *>(a.stats)[row];
+        x.stats = reinterpret_cast<const float4 *>(a.stats)[row];
+    };
+    // what becomes of row start + i (as many for every team: they meet), while `next` is on its way
+    const auto step = [&](Raw &now, Raw &next, uint32_t i) {
+        const uint32_t row = start + i;
+        const bool there = row < end;
+        const int64_t base = (int64_t)row * cols;
+        if (AHEAD) {
+            if (row + 1 < end) load(next, row + 1);
+        } else if (there) {
+            load(now, row);
+        }
+        if (!there) { // a row of zeros, which adds nothing
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+#pragma unroll
+                for (int w = 0; w < kWords<DT>; w++) now.dh[k][w] = now.y[k][w] = 0u;
+#pragma unroll
+                for (int w = 0; w < kWords<RT>; w++) now.dr[k][w] = now.r[k][w] = 0u;
+            }
+            now.stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        const float4 stats = now.stats;
         float t[V][8];
         if (a.dh) {
             float xhat[V][8], first = 0.0f, second = 0.0f;
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                const uint32_t col = 8 * (threadIdx.x + k * threads);
-                float w[8], v[8];
-                kept_values(rw[k], v, R());
-                row_values<DT>(dhw[k], t[k]);
+                kept_values(now.r[k], 8 * (lane + k * threads), xhat[k], R());
+                row_values<DT>(now.dh[k], 8 * (lane + k * threads), cols, t[k]);
+                if (!HELD) load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * (lane + k * threads), weight[k]);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    xhat[k][j] = (v[j] - stats.x) * stats.y;
+                    xhat[k][j] = (xhat[k][j] - stats.x) * stats.y;
                     if (SUMS & kSumWeight) acc[0][k][j] += t[k][j] * xhat[k][j];
                     if (SUMS & kSumBias) acc[1][k][j] += t[k][j];
-                }
-                if (a.weight) {
-                    load_columns<DT>(a.weight, a.flags & kNormWeight32, 0, col, cols, w);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) t[k][j] *= w[j];
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
+                    t[k][j] *= weight[k][j];
                     first += t[k][j];
                     second += t[k][j] * xhat[k][j];
                 }
@@ -346,109 +486,129 @@ template <int DT, int RT, int V, int THREADS, int SUMS> __global__ __launch_boun
         }
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const uint32_t col = 8 * (threadIdx.x + k * threads);
+            const uint32_t col = 8 * (lane + k * threads);
             float v[8];
             if (a.dr) {
-                row_values<RT>(drw[k], v);
+                row_values<RT>(now.dr[k], col, cols, v);
 #pragma unroll
                 for (int j = 0; j < 8; j++) t[k][j] += v[j];
             }
-            if (a.dresidual) {
+            if (a.dresidual && there) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[j] = t[k][j] * a.residual_scale;
-                store_row<RT>(a.dresidual, base, col, cols, v);
+                store_row<RT>(row_of<RT>(a.dresidual, base), col, cols, v);
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) t[k][j] *= a.block_scale;
         }
-        if (SUMS & (kSumGate | kSumAfterWeight | kSumAfterBias)) {
-            if (a.y) {
-                float yhat[V][8], first = 0.0f, second = 0.0f;
-#pragma unroll
-                for (int k = 0; k < V; k++) {
-                    const uint32_t col = 8 * (threadIdx.x + k * threads);
-                    float w[8], v[8];
-                    kept_values(yw[k], yhat[k], Y());
-                    if (after) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) yhat[k][j] = (yhat[k][j] - stats.z) * stats.w;
-                        clip(t[k], lanes_own(col, cols));
-                    }
-                    if (after && a.after_weight) {
-                        load_columns<DT>(a.after_weight, a.flags & kNormAfterWeight32, 0, col, cols, w);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) w[j] = 1.0f;
-                    }
-                    if (SUMS & kSumGate && sums_wanted & kSumGate) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) acc[2][k][j] += t[k][j] * (yhat[k][j] * w[j]);
-                        if (a.after_bias) {
-                            load_columns<DT>(a.after_bias, a.flags & kNormAfterBias32, 0, col, cols, v);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) acc[2][k][j] += t[k][j] * v[j];
-                        }
-                    }
-                    if (a.gate) {
-                        load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols, v);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) t[k][j] *= v[j];
-                    }
-                    if (after) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            if (SUMS & kSumAfterWeight) acc[3][k][j] += t[k][j] * yhat[k][j];
-                            if (SUMS & kSumAfterBias) acc[4][k][j] += t[k][j];
-                            t[k][j] *= w[j];
-                            first += t[k][j];
-                            second += t[k][j] * yhat[k][j];
-                        }
-                    }
-                }
-                if (after) {
-                    sums(first, second);
-                    first = center ? first * share : 0.0f;
-                    second *= share;
-#pragma unroll
-                    for (int k = 0; k < V; k++)
-#pragma unroll
-                        for (int j = 0; j < 8; j++) t[k][j] = (t[k][j] - first - yhat[k][j] * second) * stats.w;
-                }
-            } else if (a.gate) {
-#pragma unroll
-                for (int k = 0; k < V; k++) {
-                    float g[8];
-                    load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, 8 * (threadIdx.x + k * threads), cols, g);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) t[k][j] *= g[j];
-                }
-            }
-        }
-        if (a.dy) {
-#pragma unroll
-            for (int k = 0; k < V; k++) store_row<DT>(a.dy, base, 8 * (threadIdx.x + k * threads), cols, t[k]);
-        }
-        if (SUMS & kSumGate && a.dgate && --left == 0) { // the last row of a gate that no other workgroup has rows of
-            left = a.per;
-            const int64_t to = (int64_t)(row / a.per) * cols;
+        if (BETWEEN) {
+            float yhat[V][8], first = 0.0f, second = 0.0f;
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                const uint32_t col = 8 * (threadIdx.x + k * threads);
-                if (DT == DQ_F32 || a.flags & kNormGate32)
-                    store_row<DQ_F32>(a.dgate, to, col, cols, acc[2][k]);
-                else
-                    store_row<DT>(a.dgate, to, col, cols, acc[2][k]);
+                const uint32_t col = 8 * (lane + k * threads);
+                if (a.y) {
+                    kept_values(now.y[k], col, yhat[k], Y());
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) yhat[k][j] = 0.0f;
+                }
+                if (after) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) yhat[k][j] = (yhat[k][j] - stats.z) * stats.w;
+                    if (!HELD) load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, col, after_weight[k]);
+                }
+                if (SUMS & kSumGate) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) acc[2][k][j] += t[k][j] * (after ? yhat[k][j] * after_weight[k][j] : yhat[k][j]);
+                    if (after && a.after_bias) {
+                        float v[8];
+                        load_columns<DT>(a.after_bias, a.flags & kNormAfterBias32, 0, col, cols, v);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) acc[2][k][j] += t[k][j] * v[j];
+                    }
+                }
+                if (a.gate) {
+                    if (!HELD) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(min(row, a.rows - 1) / a.per) * cols, col, cols, gate[k]);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) t[k][j] *= gate[k][j];
+                }
+                if (after) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        if (SUMS & kSumAfterWeight) acc[3][k][j] += t[k][j] * yhat[k][j];
+                        if (SUMS & kSumAfterBias) acc[4][k][j] += t[k][j];
+                        t[k][j] *= after_weight[k][j];
+                        first += t[k][j];
+                        second += t[k][j] * yhat[k][j];
+                    }
+                }
             }
-            clear(2);
+            if (after) {
+                sums(first, second);
+                first = center ? first * share : 0.0f;
+                second *= share;
+#pragma unroll
+                for (int k = 0; k < V; k++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) t[k][j] = (t[k][j] - first - yhat[k][j] * second) * stats.w;
+            }
         }
+        if (a.dy && there) {
+#pragma unroll
+            for (int k = 0; k < V; k++) store_row<DT>(row_of<DT>(a.dy, base), 8 * (lane + k * threads), cols, t[k]);
+        }
+        if (SUMS & kSumGate && a.gate && --left == 0) { // the last row of a gate; where all of its rows are this team's, its gradient is whole
+            left = a.per;
+            if (a.dgate && there) {
+                const int64_t to = (int64_t)(row / a.per) * cols;
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    const uint32_t col = 8 * (lane + k * threads);
+                    if (DT == DQ_F32 || a.flags & kNormGate32)
+                        store_row<DQ_F32>(row_of<DQ_F32>(a.dgate, to), col, cols, acc[2][k]);
+                    else
+                        store_row<DT>(row_of<DT>(a.dgate, to), col, cols, acc[2][k]);
+                }
+                clear(2);
+            }
+            if (HELD && row + 1 < end) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)((row + 1) / a.per) * cols, 8 * lane, cols, gate[0]);
+        }
+    };
+    Raw one, other;
+    if (AHEAD) {
+        if (start < end) load(one, start);
+        for (uint32_t i = 0; i < a.run; i += 2) {
+            step(one, other, i);
+            if (i + 1 < a.run) step(other, one, i + 1);
+        }
+    } else {
+        for (uint32_t i = 0; i < a.run; i++) step(one, one, i);
     }
     uint32_t slot = 0;
 #pragma unroll
     for (int s = 0; s < 5; s++) {
-        if (!(SUMS >> s & 1) || !(sums_wanted >> s & 1) || (s == 2 && a.dgate)) continue;
-        const int64_t to = ((int64_t)slot++ * a.grid + blockIdx.x) * cols;
+        if (!(SUMS >> s & 1) || !(a.sums >> s & 1) || (s == 2 && a.dgate)) continue;
+        char *to = row_of<DQ_F32>(a.work, ((int64_t)slot++ * a.grid + blockIdx.x) * cols);
+        if constexpr (V == 1 && THREADS == 512) {
+            if (a.teams > 1) {
+                __shared__ float4 both[2][512];
+                __syncthreads();
+                both[0][threadIdx.x] = make_float4(acc[s][0][0], acc[s][0][1], acc[s][0][2], acc[s][0][3]);
+                both[1][threadIdx.x] = make_float4(acc[s][0][4], acc[s][0][5], acc[s][0][6], acc[s][0][7]);
+                __syncthreads();
+                if (team == 0) {
+                    for (uint32_t m = 1; m < a.teams; m++) {
+                        const float4 x = both[0][m * threads + lane], y = both[1][m * threads + lane];
+                        acc[s][0][0] += x.x; acc[s][0][1] += x.y; acc[s][0][2] += x.z; acc[s][0][3] += x.w;
+                        acc[s][0][4] += y.x; acc[s][0][5] += y.y; acc[s][0][6] += y.z; acc[s][0][7] += y.w;
+                    }
+                }
+            }
+        }
+        if (team == 0) {
 #pragma unroll
-        for (int k = 0; k < V; k++) store_row<DQ_F32>(a.work, to, 8 * (threadIdx.x + k * threads), cols, acc[s][k]);
+            for (int k = 0; k < V; k++) store_row<DQ_F32>(to, 8 * (lane + k * threads), cols, acc[s][k]);
+        }
     }
 }
 
@@ -458,29 +618,42 @@ template <int DT, int RT> static hipError_t launch_norm_of(const BlockNormArgs &
 {
     const uint32_t threads = a.flags >> 16;
     const dim3 grid(a.grid), block(threads);
-    return a.cols > 16384 ? launch_with(residual_norm_kernel<DT, RT, 4, 1024>, grid, block, stream, a)
-         : a.cols > 8192 ? launch_with(residual_norm_kernel<DT, RT, 2, 1024>, grid, block, stream, a)
-         : threads > 256 ? launch_with(residual_norm_kernel<DT, RT, 1, 1024>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 256>, grid, block, stream, a);
+    const bool full = a.gate || a.flags & kNormAfter, passing = a.flags & kNormPassing;
+    if (a.cols > 16384) return launch_with(residual_norm_kernel<DT, RT, 4, 1024, true, false>, grid, block, stream, a);
+    if (a.cols > 8192) return launch_with(residual_norm_kernel<DT, RT, 2, 1024, true, false>, grid, block, stream, a);
+    if (threads > 512)
+        return full ? passing ? launch_with(residual_norm_kernel<DT, RT, 1, 1024, true, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 1024, true, false>, grid, block, stream, a)
+                    : passing ? launch_with(residual_norm_kernel<DT, RT, 1, 1024, false, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 1024, false, false>, grid, block, stream, a);
+    return full ? passing ? launch_with(residual_norm_kernel<DT, RT, 1, 512, true, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 512, true, false>, grid, block, stream, a)
+                : passing ? launch_with(residual_norm_kernel<DT, RT, 1, 512, false, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 512, false, false>, grid, block, stream, a);
 }
 
-template <int DT, int RT, int SUMS> static hipError_t launch_norm_backward_with(const BlockNormBackArgs &a, hipStream_t stream)
+template <int DT, int RT, int V, int THREADS, int SUMS> static hipError_t launch_norm_backward_with(const BlockNormBackArgs &a, hipStream_t stream)
 {
-    const uint32_t threads = a.flags >> 16;
-    const dim3 grid(a.grid), block(threads);
-    return a.cols > 16384 ? launch_with(residual_norm_backward_kernel<DT, RT, 4, 1024, SUMS>, grid, block, stream, a)
-         : a.cols > 8192 ? launch_with(residual_norm_backward_kernel<DT, RT, 2, 1024, SUMS>, grid, block, stream, a)
-         : threads > 512 ? launch_with(residual_norm_backward_kernel<DT, RT, 1, 1024, SUMS>, grid, block, stream, a)
-                         : launch_with(residual_norm_backward_kernel<DT, RT, 1, 512, SUMS>, grid, block, stream, a);
+    const dim3 grid(a.grid), block((a.flags >> 16) * a.teams);
+    if constexpr (V == 1) {
+        if (a.flags & kNormPassing)
+            return a.flags & kNormEight ? launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, true, true>, grid, block, stream, a)
+                                        : launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, false, true>, grid, block, stream, a);
+    }
+    return a.flags & kNormEight ? launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, true, false>, grid, block, stream, a)
+                                : launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, false, false>, grid, block, stream, a);
 }
 template <int DT, int RT> static hipError_t launch_norm_backward_of(const BlockNormBackArgs &a, hipStream_t stream)
 {
     // the block between r and y takes part only in kernels that keep sums of it
     const uint32_t want = a.sums | (a.gate ? kSumGate : 0) | (a.flags & kNormAfter ? kSumAfterWeight : 0);
-    if (!(want & ~kSumWeight)) return launch_norm_backward_with<DT, RT, kSumWeight>(a, stream);
-    if (!(want & ~(kSumWeight | kSumBias))) return launch_norm_backward_with<DT, RT, kSumWeight | kSumBias>(a, stream);
-    if (!(want & ~(kSumWeight | kSumGate))) return launch_norm_backward_with<DT, RT, kSumWeight | kSumGate>(a, stream);
-    if (!(want & ~(kSumWeight | kSumGate | kSumAfterWeight))) return launch_norm_backward_with<DT, RT, kSumWeight | kSumGate | kSumAfterWeight>(a, stream);
-    return launch_norm_backward_with<DT, RT, 31>(a, stream);
+    const auto within = [&](uint32_t of) { return !(want & ~of); };
+    if (a.cols > 16384) return within(3) ? launch_norm_backward_with<DT, RT, 4, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 4, 1024, 31>(a, stream);
+    if (a.cols > 8192) return within(3) ? launch_norm_backward_with<DT, RT, 2, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 2, 1024, 31>(a, stream);
+    if (a.cols > 4096)
+        return within(3) ? launch_norm_backward_with<DT, RT, 1, 1024, 3>(a, stream)
+             : within(13) ? launch_norm_backward_with<DT, RT, 1, 1024, 13>(a, stream) : launch_norm_backward_with<DT, RT, 1, 1024, 31>(a, stream);
+    if (within(1)) return launch_norm_backward_with<DT, RT, 1, 512, 1>(a, stream);
+    if (within(3)) return launch_norm_backward_with<DT, RT, 1, 512, 3>(a, stream);
+    if (within(7)) return launch_norm_backward_with<DT, RT, 1, 512, 7>(a, stream);
+    if (within(13)) return launch_norm_backward_with<DT, RT, 1, 512, 13>(a, stream);
+    return launch_norm_backward_with<DT, RT, 1, 512, 31>(a, stream);
 }
 
 template <int DT> static hipError_t launch_norm_in(const BlockNormArgs &a, bool stream32, hipStream_t stream)

@@ -12,28 +12,35 @@ static uint32_t norm_threads(uint32_t cols)
     return ((vectors + each - 1) / each + 63) & ~63u;
 }
 
+// Whether a pass' arrays, four or so, are more than half of the 256 MB cache: then its loads carry the hint that nothing of them is wanted again soon.
+static bool norm_passing(int64_t rows, uint32_t cols, int dtype) { return rows * cols * 4 * (dtype == DQ_F32 ? 4 : 2) > (int64_t)128 << 20; }
+
 hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t stream)
 {
     a.flags |= norm_threads(a.cols) << 16;
-    a.grid = std::min(a.rows, 1u << 20); // (beyond that a workgroup takes several rows)
+    if (norm_passing(a.rows, a.cols, dtype)) a.flags |= kNormPassing;
+    a.grid = std::min(a.rows, 4096 * 64 / norm_threads(a.cols)); // sixteen waves for each CU
     return dtype == DQ_F32 ? launch_norm_f32(a, stream32, stream) : dtype == DQ_BF16 ? launch_norm_bf16(a, stream32, stream) : launch_norm_f16(a, stream32, stream);
 }
 
-// How a backward pass shares its rows out: runs of `run` rows, `parts` of them (the last one shorter) to the rows of a gate, or one of whole gates.
+// How a backward pass shares its rows out: teams of as many threads as a row takes, up to 512 together in a workgroup, have runs of `run` rows -- `parts` of them (the last ones
+// shorter) to the rows of a gate, all of a workgroup's of the same one, or one of whole gates.
 NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols)
 {
-    const int64_t groups = norm_threads(cols) <= 256 ? 1024 : 512;
-    int64_t run = (rows + groups - 1) / groups;
     NormShares s;
+    const uint32_t threads = norm_threads(cols);
+    s.teams = std::max(1u, 512 / threads);
+    const int64_t runs = 512 * (int64_t)s.teams;
+    int64_t run = (rows + runs - 1) / runs;
     if (per == 0 || per <= run) {
         if (per) run = run / per * per;
         s.parts = 1;
-        s.grid = (uint32_t)((rows + run - 1) / run);
+        s.grid = (uint32_t)((rows + run * s.teams - 1) / (run * s.teams));
     } else {
         s.parts = (uint32_t)((per + run - 1) / run);
+        s.parts = (s.parts + s.teams - 1) / s.teams * s.teams;
         run = (per + s.parts - 1) / s.parts;
-        s.parts = (uint32_t)((per + run - 1) / run);
-        s.grid = (uint32_t)(rows / per * s.parts);
+        s.grid = (uint32_t)(rows / per * (s.parts / s.teams));
     }
     s.run = (uint32_t)run;
     return s;
@@ -48,10 +55,10 @@ struct ColumnSums {
     } one[5];
 };
 
-// out[s][c]: the sum of `parts` rows of work, which lie one behind the other.  Four threads share a column's rows, in an order that does not change.
-__global__ __launch_bounds__(256) void column_sums_kernel(ColumnSums a)
+// out[s][c]: the sum of `parts` rows of work, which lie one behind the other.  Sixteen threads share a column's rows, in an order that does not change.
+__global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSums a)
 {
-    __shared__ float part[4][64];
+    __shared__ float part[16][64];
     uint32_t id = blockIdx.x / a.tiles, k = 0;
     const uint32_t col = (blockIdx.x - id * a.tiles) * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6, at = min(col, a.cols - 1);
     while (id >= a.one[k].segments) id -= a.one[k++].segments;
@@ -59,17 +66,19 @@ __global__ __launch_bounds__(256) void column_sums_kernel(ColumnSums a)
     const float *from = a.work + ((int64_t)k * a.grid + (int64_t)id * o.parts) * a.cols + at;
     float sum = 0.0f;
     uint32_t p = slice;
-    for (; p + 28 < o.parts; p += 32) {
+    for (; p + 112 < o.parts; p += 128) {
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = from[(int64_t)(p + 4 * j) * a.cols];
+        for (int j = 0; j < 8; j++) v[j] = from[(int64_t)(p + 16 * j) * a.cols];
         sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     }
-    for (; p < o.parts; p += 4) sum += from[(int64_t)p * a.cols];
+    for (; p < o.parts; p += 16) sum += from[(int64_t)p * a.cols];
     part[slice][threadIdx.x & 63] = sum;
     __syncthreads();
     if (slice || col >= a.cols) return;
-    sum = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) sum += (part[j][threadIdx.x] + part[j + 1][threadIdx.x]) + (part[j + 2][threadIdx.x] + part[j + 3][threadIdx.x]);
     const int64_t to = (int64_t)id * a.cols + col;
     if (o.dtype == DQ_F32)
         ElemIO<DQ_F32>::store(o.out, to, sum);
@@ -83,7 +92,9 @@ hipError_t launch_norm_backward(BlockNormBackArgs a, const NormSum (&sums)[5], i
 {
     const NormShares s = norm_shares(a.rows, a.gate ? a.per : 0, a.cols);
     a.flags |= norm_threads(a.cols) << 16;
+    if (norm_passing(a.rows, a.cols, dtype)) a.flags |= kNormPassing;
     a.grid = s.grid;
+    a.teams = s.teams;
     a.run = s.run;
     a.parts = s.parts;
     a.sums = 0;
@@ -97,13 +108,13 @@ hipError_t launch_norm_backward(BlockNormBackArgs a, const NormSum (&sums)[5], i
             a.dgate = sums[k].out;
             continue;
         }
-        c.one[c.count++] = {sums[k].out, k == 2 ? a.rows / a.per : 1, k == 2 ? s.parts : s.grid, (uint32_t)sums[k].dtype};
+        c.one[c.count++] = {sums[k].out, k == 2 ? a.rows / a.per : 1, k == 2 ? s.parts / s.teams : s.grid, (uint32_t)sums[k].dtype};
         segments += c.one[c.count - 1].segments;
     }
     const hipError_t e = dtype == DQ_F32 ? launch_norm_backward_f32(a, stream32, stream)
                        : dtype == DQ_BF16 ? launch_norm_backward_bf16(a, stream32, stream) : launch_norm_backward_f16(a, stream32, stream);
     if (e != hipSuccess || !segments) return e;
-    return launch_with(column_sums_kernel, dim3(segments * c.tiles), dim3(256), stream, c);
+    return launch_with(column_sums_kernel, dim3(segments * c.tiles), dim3(1024), stream, c);
 }
 
 } // namespace dq
