@@ -26,12 +26,14 @@ class Checkpoint(object):
     @property
     def codes(self):
         """uint8 [rows, 32 b], E4M3"""
-        return self.data[:self.data.numel() // 33 * 32].view(self.rows, -(-self.cols // 32) * 32)
+        b = -(-self.cols // 32)
+        return self.data.as_strided((self.rows, 32 * b), (32 * b, 1), self.data.storage_offset())
 
     @property
     def scales(self):
         """uint8 [rows, b]"""
-        return self.data[self.data.numel() // 33 * 32:].view(self.rows, -(-self.cols // 32))
+        b = -(-self.cols // 32)
+        return self.data.as_strided((self.rows, b), (b, 1), self.data.storage_offset() + self.rows * 32 * b)
 
     def __repr__(self):
         return "Checkpoint(%d x %d)" % (self.rows, self.cols)

@@ -55,13 +55,14 @@ template <int DT, bool PASSING = false> __device__ __forceinline__ void load4(co
     }
 }
 
-template <int DT> __device__ __forceinline__ void load8(const void *p, int64_t i, float (&v)[8])
+template <int DT, bool PASSING = false> __device__ __forceinline__ void load8(const void *p, int64_t i, float (&v)[8])
 {
     if (DT == DQ_F32) {
-        load4<DT>(p, i, v);
-        load4<DT>(p, i + 4, v + 4);
+        load4<DT, PASSING>(p, i, v);
+        load4<DT, PASSING>(p, i + 4, v + 4);
     } else {
-        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p) + i);
+        const u32x4_any *q = reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p) + i);
+        const u32x4_any a = PASSING ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
         for (int j = 0; j < 4; j++) unpack2<DT>(a[j], v[2 * j], v[2 * j + 1]);
     }
@@ -132,14 +133,18 @@ template <int DT, bool PASSING = false> __device__ __forceinline__ void store4(v
     }
 }
 
-template <int DT> __device__ __forceinline__ void store8(void *p, int64_t i, const float (&v)[8])
+template <int DT, bool PASSING = false> __device__ __forceinline__ void store8(void *p, int64_t i, const float (&v)[8])
 {
     if (DT == DQ_F32) {
-        store4<DT>(p, i, v);
-        store4<DT>(p, i + 4, v + 4);
+        store4<DT, PASSING>(p, i, v);
+        store4<DT, PASSING>(p, i + 4, v + 4);
     } else {
         const u32x4_any a = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])};
-        *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(p) + i) = a;
+        u32x4_any *q = reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(p) + i);
+        if (PASSING)
+            __builtin_nontemporal_store(a, q);
+        else
+            *q = a;
     }
 }
 

@@ -125,12 +125,10 @@ template <int DT> __device__ __forceinline__ void load_columns(const void *p, bo
 }
 template <int DT, bool PASSING = false> __device__ __forceinline__ void store_row(char *row, uint32_t col, uint32_t cols, const float (&v)[8])
 {
-    if (col + 8 <= cols) {
-        store4<DT, PASSING>(row, col, v);
-        store4<DT, PASSING>(row, col + 4, v + 4);
-    } else if (col < cols) {
+    if (col + 8 <= cols)
+        store8<DT, PASSING>(row, col, v);
+    else if (col < cols)
         store_part<DT, 8>(row, col, (int)(cols - col), v);
-    }
 }
 
 // eight elements of a row into a checkpoint (four neighbouring lanes together; those past the last column are 0)
@@ -177,11 +175,11 @@ template <int DT> struct Columns {
     }
 };
 
-// FULL: there is a norm after the block, or a gate.  Rows up to 8192 wide are taken in turn by as many workgroups as the chip holds, which keep the vectors and ask for a row
+// FULL: there is a norm after the block, or a gate.  Rows up to 8192 wide, without these up to 16384, are taken in turn by as many workgroups as the chip holds, which keep the vectors and ask for a row
 // before they work on the one in front of it.
 template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global__ __launch_bounds__(THREADS, 4) void residual_norm_kernel(BlockNormArgs a)
 {
-    constexpr bool HELD = V == 1;
+    constexpr bool HELD = V == 1 || (V == 2 && !FULL);
     __shared__ f32x2_t part[2][16];
     const uint32_t threads = a.flags >> 16, cols = a.cols;
     const bool center = a.flags & kNormCenter, after = FULL && a.flags & kNormAfter, before = a.flags & kNormBefore;
@@ -211,7 +209,7 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
         sums(s, none);
         rs = inverse_root(s / (float)cols + a.eps);
     };
-    Columns<DT> weight, bias, after_weight, after_bias, gate;
+    Columns<DT> weight[HELD ? V : 1], bias[HELD ? V : 1], after_weight, after_bias, gate;
     const auto ask_gate = [&](uint32_t row, uint32_t col) { gate.ask(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols); };
     const auto take_gate = [&](uint32_t col) { gate.take(a.gate, a.flags & kNormGate32, col, cols, 1.0f); };
     const auto ask_after = [&](uint32_t col) {
@@ -222,13 +220,13 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
         after_weight.take(a.after_weight, a.flags & kNormAfterWeight32, col, cols, 1.0f);
         after_bias.take(a.after_bias, a.flags & kNormAfterBias32, col, cols, 0.0f);
     };
-    const auto ask_before = [&](uint32_t col) {
-        weight.ask(a.weight, a.flags & kNormWeight32, 0, col, cols);
-        bias.ask(a.bias, a.flags & kNormBias32, 0, col, cols);
+    const auto ask_before = [&](int k, uint32_t col) {
+        weight[k].ask(a.weight, a.flags & kNormWeight32, 0, col, cols);
+        bias[k].ask(a.bias, a.flags & kNormBias32, 0, col, cols);
     };
-    const auto take_before = [&](uint32_t col) {
-        weight.take(a.weight, a.flags & kNormWeight32, col, cols, 1.0f);
-        bias.take(a.bias, a.flags & kNormBias32, col, cols, 0.0f);
+    const auto take_before = [&](int k, uint32_t col) {
+        weight[k].take(a.weight, a.flags & kNormWeight32, col, cols, 1.0f);
+        bias[k].take(a.bias, a.flags & kNormBias32, col, cols, 0.0f);
     };
     struct Raw {
         uint32_t y[V][kWords<DT>], residual[V][kWords<RT>];
@@ -303,11 +301,11 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
             for (int k = 0; k < V; k++) {
                 const uint32_t col = 8 * (threadIdx.x + k * threads);
                 if (!HELD) {
-                    ask_before(col);
-                    take_before(col);
+                    ask_before(0, col);
+                    take_before(0, col);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[k][j] = ElemIO<DT>::round((x[k][j] - mean) * rs * weight.v[j] + bias.v[j]);
+                for (int j = 0; j < 8; j++) x[k][j] = ElemIO<DT>::round((x[k][j] - mean) * rs * weight[HELD ? k : 0].v[j] + bias[HELD ? k : 0].v[j]);
                 store_row<DT>(row_of<DT>(a.h, base), col, cols, x[k]);
                 if (a.h8) keep_row<DT>(a.h8, a.rows, row, col, cols, x[k]);
             }
@@ -322,12 +320,14 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
             ask_after(col);
             ask_gate(blockIdx.x, col);
         }
-        ask_before(col);
+#pragma unroll
+        for (int k = 0; k < V; k++) ask_before(k, col + 8 * k * threads);
         if (FULL) {
             take_after(col);
             take_gate(col);
         }
-        take_before(col);
+#pragma unroll
+        for (int k = 0; k < V; k++) take_before(k, col + 8 * k * threads);
         for (uint32_t row = blockIdx.x; row < a.rows; row += 2 * a.grid) {
             step(one, other, row);
             if (row + a.grid < a.rows) step(other, one, row + a.grid);
@@ -373,8 +373,8 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
     const uint32_t end = min(start + a.run, a.parts > 1 ? (of + 1) * a.per : a.rows);
     uint32_t left = a.per;
     // What the columns are multiplied by, in registers where they hold it all along (1 where there is no weight; 0 behind the last column, where nothing else need be).
-    constexpr bool HELD = V == 1;
-    float weight[HELD ? 1 : V][8], after_weight[HELD ? 1 : V][8], gate[HELD ? 1 : V][8];
+    constexpr bool HELD = V == 1 || (V == 2 && !BETWEEN);
+    float weight[V][8], after_weight[V][8], gate[V][8];
     const auto load_weight = [&](const void *p, bool in32, int64_t base, uint32_t col, float (&v)[8]) {
         if (p) {
             load_columns<DT>(p, in32, base, col, cols, v);
@@ -385,7 +385,8 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
         }
     };
     if (HELD) {
-        load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * lane, weight[0]);
+#pragma unroll
+        for (int k = 0; k < V; k++) load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * (lane + k * threads), weight[k]);
         if (AFTER) load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, 8 * lane, after_weight[0]);
         if (BETWEEN && a.gate) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(min(start, a.rows - 1) / a.per) * cols, 8 * lane, cols, gate[0]); // (a team may have no rows)
     }
@@ -620,7 +621,8 @@ template <int DT, int RT> static hipError_t launch_norm_of(const BlockNormArgs &
     const dim3 grid(a.grid), block(threads);
     const bool full = a.gate || a.flags & kNormAfter, passing = a.flags & kNormPassing;
     if (a.cols > 16384) return launch_with(residual_norm_kernel<DT, RT, 4, 1024, true, false>, grid, block, stream, a);
-    if (a.cols > 8192) return launch_with(residual_norm_kernel<DT, RT, 2, 1024, true, false>, grid, block, stream, a);
+    if (a.cols > 8192)
+        return full ? launch_with(residual_norm_kernel<DT, RT, 2, 1024, true, false>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 2, 1024, false, true>, grid, block, stream, a);
     if (threads > 512)
         return full ? passing ? launch_with(residual_norm_kernel<DT, RT, 1, 1024, true, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 1024, true, false>, grid, block, stream, a)
                     : passing ? launch_with(residual_norm_kernel<DT, RT, 1, 1024, false, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 1024, false, false>, grid, block, stream, a);
@@ -645,7 +647,9 @@ template <int DT, int RT> static hipError_t launch_norm_backward_of(const BlockN
     const uint32_t want = a.sums | (a.gate ? kSumGate : 0) | (a.flags & kNormAfter ? kSumAfterWeight : 0);
     const auto within = [&](uint32_t of) { return !(want & ~of); };
     if (a.cols > 16384) return within(3) ? launch_norm_backward_with<DT, RT, 4, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 4, 1024, 31>(a, stream);
-    if (a.cols > 8192) return within(3) ? launch_norm_backward_with<DT, RT, 2, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 2, 1024, 31>(a, stream);
+    if (a.cols > 8192)
+        return within(1) ? launch_norm_backward_with<DT, RT, 2, 1024, 1>(a, stream)
+             : within(3) ? launch_norm_backward_with<DT, RT, 2, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 2, 1024, 31>(a, stream);
     if (a.cols > 4096)
         return within(3) ? launch_norm_backward_with<DT, RT, 1, 1024, 3>(a, stream)
              : within(13) ? launch_norm_backward_with<DT, RT, 1, 1024, 13>(a, stream) : launch_norm_backward_with<DT, RT, 1, 1024, 31>(a, stream);

@@ -23,14 +23,15 @@ hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t st
     return dtype == DQ_F32 ? launch_norm_f32(a, stream32, stream) : dtype == DQ_BF16 ? launch_norm_bf16(a, stream32, stream) : launch_norm_f16(a, stream32, stream);
 }
 
-// How a backward pass shares its rows out: teams of as many threads as a row takes, up to 512 together in a workgroup, have runs of `run` rows -- `parts` of them (the last ones
+// How a backward pass shares its rows out.  As many workgroups as the chip holds at once, two a CU, or one of a thousand threads (1024 x 8192 in 20 us, with two in turn 26); more
+// would leave more sums to add up, fewer take longer than what that saves (with at least 4, 8 or 16 rows each 1024 x 4096 takes 1 % less, 7 and 60 % more).  Teams of as many threads as a row takes, up to 512 together in a workgroup, have runs of `run` rows -- `parts` of them (the last ones
 // shorter) to the rows of a gate, all of a workgroup's of the same one, or one of whole gates.
 NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols)
 {
     NormShares s;
     const uint32_t threads = norm_threads(cols);
     s.teams = std::max(1u, 512 / threads);
-    const int64_t runs = 512 * (int64_t)s.teams;
+    const int64_t runs = (threads > 512 ? 256 : 512) * (int64_t)s.teams;
     int64_t run = (rows + runs - 1) / runs;
     if (per == 0 || per <= run) {
         if (per) run = run / per * per;
