@@ -11,10 +11,17 @@ namespace dq {
 // What is beyond the 256 MB cache is loaded with the hint that nothing of it is wanted again soon: 8192 x 14336 bf16 in 59 us, 6.0 TB/s (65 without).
 inline bool passes(int64_t rows, uint32_t cols, int arrays, int dtype) { return rows * cols * arrays * (dtype == DQ_F32 ? 4 : 2) > (int64_t)128 << 20; }
 
-template <int DT, bool PASSING> __global__ __launch_bounds__(256) void checkpoint_compress_kernel(CheckpointArgs a, Division blocks, uint32_t units)
+struct CompressCall {
+    CheckpointArgs a;
+    Division blocks;
+    uint32_t units;
+};
+template <int DT, bool PASSING> __global__ __launch_bounds__(256) void checkpoint_compress_kernel(CompressCall call)
 {
+    const CheckpointArgs &a = call.a;
+    const Division &blocks = call.blocks;
     const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
-    if (unit >= units) return;
+    if (unit >= call.units) return;
     const uint32_t row = blocks(unit >> 2), col = (unit - row * blocks.by * 4) * 8;
     float v[8];
     const int64_t at = (int64_t)row * a.stride + col;
@@ -31,46 +38,43 @@ template <int DT, bool PASSING> __global__ __launch_bounds__(256) void checkpoin
 hipError_t launch_checkpoint_compress(const CheckpointArgs &a, int dtype, hipStream_t stream)
 {
     const Division blocks((a.cols + 31) >> 5, 30);
-    const uint32_t units = (uint32_t)(a.rows * blocks.by * 4);
-    const dim3 grid((units + 255) / 256);
-    const auto launch = [&](auto passing, auto whole) {
-        passes(a.rows, a.cols, 1, dtype) ? passing<<<grid, 256, 0, stream>>>(a, blocks, units) : whole<<<grid, 256, 0, stream>>>(a, blocks, units);
-        return hipGetLastError();
-    };
+    const CompressCall call = {a, blocks, (uint32_t)(a.rows * blocks.by * 4)};
+    const auto launch = [&](auto passing, auto whole) { return launch_with(passes(a.rows, a.cols, 1, dtype) ? passing : whole, dim3((call.units + 255) / 256), dim3(256), stream, call); };
     return dtype == DQ_F32 ? launch(checkpoint_compress_kernel<DQ_F32, true>, checkpoint_compress_kernel<DQ_F32, false>)
          : dtype == DQ_BF16 ? launch(checkpoint_compress_kernel<DQ_BF16, true>, checkpoint_compress_kernel<DQ_BF16, false>)
                             : launch(checkpoint_compress_kernel<DQ_F16, true>, checkpoint_compress_kernel<DQ_F16, false>);
 }
 
 // 8192 x 14336 to bf16 in 55 us, 6.5 TB/s
-template <int DT> __global__ __launch_bounds__(256) void checkpoint_restore_kernel(const uint8_t *__restrict__ data, void *__restrict__ out, int64_t scales, uint32_t cols, Division blocks, uint32_t units)
+struct RestoreCall {
+    const uint8_t *data;
+    void *out;
+    int64_t scales;
+    uint32_t cols, units;
+    Division blocks;
+};
+template <int DT> __global__ __launch_bounds__(256) void checkpoint_restore_kernel(RestoreCall a)
 {
     const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
-    if (unit >= units) return;
-    const uint32_t row = blocks(unit >> 2), col = (unit - row * blocks.by * 4) * 8;
-    if (col >= cols) return;
+    if (unit >= a.units) return;
+    const uint32_t row = a.blocks(unit >> 2), col = (unit - row * a.blocks.by * 4) * 8;
+    if (col >= a.cols) return;
     float v[8];
-    decode_e4m3(reinterpret_cast<const u32x2_t *>(data)[unit], data[scales + (unit >> 2)], v);
-    const int64_t at = (int64_t)row * cols + col;
-    if (col + 8 <= cols)
-        store8<DT>(out, at, v);
+    decode_e4m3(reinterpret_cast<const u32x2_t *>(a.data)[unit], a.data[a.scales + (unit >> 2)], v);
+    const int64_t at = (int64_t)row * a.cols + col;
+    if (col + 8 <= a.cols)
+        store8<DT>(a.out, at, v);
     else
-        store_part<DT, 8>(out, at, (int)(cols - col), v);
+        store_part<DT, 8>(a.out, at, (int)(a.cols - col), v);
 }
 
 hipError_t launch_checkpoint_restore(const uint8_t *data, void *out, int64_t rows, int64_t cols, int dtype, hipStream_t stream)
 {
     const Division blocks((uint32_t)((cols + 31) >> 5), 30);
-    const uint32_t units = (uint32_t)(rows * blocks.by * 4);
-    const int64_t scales = rows * 32 * blocks.by;
-    const dim3 grid((units + 255) / 256);
-    if (dtype == DQ_F32)
-        checkpoint_restore_kernel<DQ_F32><<<grid, 256, 0, stream>>>(data, out, scales, (uint32_t)cols, blocks, units);
-    else if (dtype == DQ_BF16)
-        checkpoint_restore_kernel<DQ_BF16><<<grid, 256, 0, stream>>>(data, out, scales, (uint32_t)cols, blocks, units);
-    else
-        checkpoint_restore_kernel<DQ_F16><<<grid, 256, 0, stream>>>(data, out, scales, (uint32_t)cols, blocks, units);
-    return hipGetLastError();
+    const RestoreCall call = {data, out, rows * 32 * blocks.by, (uint32_t)cols, (uint32_t)(rows * blocks.by * 4), blocks};
+    const dim3 grid((call.units + 255) / 256), block(256);
+    return dtype == DQ_F32 ? launch_with(checkpoint_restore_kernel<DQ_F32>, grid, block, stream, call)
+         : dtype == DQ_BF16 ? launch_with(checkpoint_restore_kernel<DQ_BF16>, grid, block, stream, call) : launch_with(checkpoint_restore_kernel<DQ_F16>, grid, block, stream, call);
 }
 
 // ---- the gated activation -----------------------------------------------------------------------------------
@@ -96,12 +100,22 @@ template <int KIND> __device__ __forceinline__ float exponent_of(float g, float 
     return x * (c + 0.044715f * c * square);
 }
 
+struct GatedCall {
+    GatedArgs a;
+    Division blocks;
+    uint32_t units;
+};
+static_assert(sizeof(GatedCall) <= 128, "a launch whose arguments are longer takes longer");
+
 // A lane takes eight elements, four of them a block of 32, padding included: the last block of a row may be a part.  Bound by memory: 8192 x 14336 bf16 with all three checkpoints
 // in 158 to 170 us by the box (6.3 to 6.8 TB/s, where loads and the result carry the hint; 178 without, and 175 with it on the checkpoints too), backward from them in 165 to 174
 // (5.4 to 5.7 TB/s): half of that is stores, in two streams.  The hint on its stores takes 161 on one box and 190 on another, on its loads 173 and 170; two units a lane 8 % more,
 // workgroups of 1024 5 %.
-template <int DT, int KIND, bool EIGHT, bool PASSING> __global__ __launch_bounds__(256) void gated_kernel(GatedArgs a, Division blocks, uint32_t units)
+template <int DT, int KIND, bool EIGHT, bool PASSING> __global__ __launch_bounds__(256) void gated_kernel(GatedCall call)
 {
+    const GatedArgs &a = call.a;
+    const Division &blocks = call.blocks;
+    const uint32_t units = call.units;
     const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
     if (unit >= units) return;
     const uint32_t row = blocks(unit >> 2), col = (unit - row * blocks.by * 4) * 8;
@@ -141,8 +155,11 @@ template <int DT, int KIND, bool EIGHT, bool PASSING> __global__ __launch_bounds
     }
 }
 
-template <int DT, int KIND, bool EIGHT> __global__ __launch_bounds__(256) void gated_backward_kernel(GatedArgs a, Division blocks, uint32_t units)
+template <int DT, int KIND, bool EIGHT> __global__ __launch_bounds__(256) void gated_backward_kernel(GatedCall call)
 {
+    const GatedArgs &a = call.a;
+    const Division &blocks = call.blocks;
+    const uint32_t units = call.units;
     const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
     if (unit >= units) return;
     const uint32_t row = blocks(unit >> 2), col = (unit - row * blocks.by * 4) * 8;
@@ -192,14 +209,10 @@ template <int DT, int KIND, bool EIGHT> __global__ __launch_bounds__(256) void g
 template <int DT, int KIND, bool EIGHT> static hipError_t launch_gated_of(const GatedArgs &a, bool backward, hipStream_t stream)
 {
     const Division blocks((a.cols + 31) >> 5, 30);
-    const uint32_t units = (uint32_t)(a.rows * blocks.by * 4);
-    const dim3 grid((units + 255) / 256);
-    const bool passing = passes(a.rows, a.cols, 4, DT);
-    if (backward)
-        gated_backward_kernel<DT, KIND, EIGHT><<<grid, 256, 0, stream>>>(a, blocks, units);
-    else
-        passing ? gated_kernel<DT, KIND, EIGHT, true><<<grid, 256, 0, stream>>>(a, blocks, units) : gated_kernel<DT, KIND, EIGHT, false><<<grid, 256, 0, stream>>>(a, blocks, units);
-    return hipGetLastError();
+    const GatedCall call = {a, blocks, (uint32_t)(a.rows * blocks.by * 4)};
+    const dim3 grid((call.units + 255) / 256), block(256);
+    if (backward) return launch_with(gated_backward_kernel<DT, KIND, EIGHT>, grid, block, stream, call);
+    return passes(a.rows, a.cols, 4, DT) ? launch_with(gated_kernel<DT, KIND, EIGHT, true>, grid, block, stream, call) : launch_with(gated_kernel<DT, KIND, EIGHT, false>, grid, block, stream, call);
 }
 template <int DT> static hipError_t launch_gated_with(const GatedArgs &a, int kind, bool backward, hipStream_t stream)
 {

@@ -1637,7 +1637,7 @@ struct GatedOf : public torch::autograd::Function<GatedOf> {
         o.up = up ? up->data_ptr() : static_cast<char *>(x.data_ptr()) + cols * (int64_t)x.element_size();
         o.up_stride = up ? std::max(row_stride(*up), cols) : o.gate_stride;
     }
-    // kept: what the backward pass will want is kept (in 8 bits, if eight)
+    // kept: what the backward pass will want is kept (in 8 bits, if eight); otherwise there need be no context
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const Maybe &up, int64_t kind, bool eight, bool kept)
     {
         const c10::DeviceGuard on(x.device());
@@ -1676,7 +1676,7 @@ struct GatedOf : public torch::autograd::Function<GatedOf> {
         }
         if (kept) Noted<Notes>::keep(ctx, {kind, eight, !up, x.sizes().vec()});
         if (!eight) return {out};
-        ctx->mark_non_differentiable({data});
+        if (ctx) ctx->mark_non_differentiable({data});
         return {out, data};
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::tensor_list grads)
@@ -1738,7 +1738,7 @@ PyObject *gated(PyObject *, PyObject *const *v, Py_ssize_t have)
         need(x.dim() >= 1 && (up || x.size(-1) % 2 == 0), "gated: x [..., 2 cols], or two tensors, are required");
         const bool eight = PyObject_IsTrue(v[3]), kept = at::GradMode::is_enabled() && (x.requires_grad() || (up && up->requires_grad()));
         leaves_can_be_recorded("gated", x.device(), {&x, up ? &*up : &x});
-        const torch::autograd::variable_list out = GatedOf::apply(x, up, integer(v[2]), eight, kept);
+        const torch::autograd::variable_list out = kept ? GatedOf::apply(x, up, integer(v[2]), eight, true) : GatedOf::forward(nullptr, x, up, integer(v[2]), eight, false);
         const py::object a = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[0]));
         return PyTuple_Pack(2, a.ptr(), eight ? py::reinterpret_steal<py::object>(THPVariable_Wrap(out[1])).ptr() : Py_None);
     });
@@ -1788,6 +1788,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         return o;
     }
 
+    // (without s.kept there need be no context)
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &y_, const Maybe &residual_, const Maybe &weight_, const Maybe &bias_,
                                                   const Maybe &gate_, const Maybe &after_weight_, const Maybe &after_bias_, const Settings &s)
     {
@@ -1827,7 +1828,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         if (h.defined()) out.push_back(h);
         if (r.defined()) out.push_back(r);
         if (data.defined()) {
-            ctx->mark_non_differentiable({data});
+            if (ctx) ctx->mark_non_differentiable({data});
             out.push_back(data);
         }
         return out;
@@ -1938,7 +1939,7 @@ PyObject *residual_norm(PyObject *, PyObject *const *v, Py_ssize_t have)
             s.per = rows ? rows / (gate.numel() / cols) : 1;
         }
         leaves_can_be_recorded("residual_norm", y.device(), {&y, in[1] ? &*in[1] : &y, in[2] ? &*in[2] : &y, in[3] ? &*in[3] : &y, in[4] ? &*in[4] : &y, in[5] ? &*in[5] : &y, in[6] ? &*in[6] : &y});
-        const torch::autograd::variable_list out = F::apply(y, in[1], in[2], in[3], in[4], in[5], in[6], s);
+        const torch::autograd::variable_list out = any ? F::apply(y, in[1], in[2], in[3], in[4], in[5], in[6], s) : F::forward(nullptr, y, in[1], in[2], in[3], in[4], in[5], in[6], s);
         const bool plain = !in[F::RESIDUAL] && !in[F::GATE] && !s.after && s.block_scale == 1.0;
         size_t next = 0;
         const auto take = [&](bool there) { return there ? py::reinterpret_steal<py::object>(THPVariable_Wrap(out[next++])) : py::reinterpret_borrow<py::object>(Py_None); };

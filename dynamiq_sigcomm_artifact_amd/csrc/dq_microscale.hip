@@ -163,9 +163,9 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 // (4.6 TB/s), 132 behind other work (with the XCDs' workgroups strewn 8 % more, 8000 x 5000 40 for 35), where the pool's runs of 64 bytes keep it from more: neither all of the pool asked for at once nor fewer
 // instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.  Blocks that have to be lowered are looked for while their columns
 // are encoded and taken behind the loop, where nothing else needs registers (in it: 2 to 6 % for every matrix); to the nearest four workgroups share a CU, which 65 registers would not let them.
-// A checkpoint's tile is twice as wide, 16 columns a lane: runs of 256 bytes of it as of a 16-bit matrix.
-template <int DT> constexpr uint32_t kColumns = DT == DQ_E4M3 ? 16 : 8; // of a lane
-inline uint32_t columns_tiles(int64_t cols, int dtype) { return dtype == DQ_E4M3 ? (uint32_t)((cols + 255) >> 8) : (uint32_t)((cols + 127) >> 7); }
+// A checkpoint's tile is twice as wide where that leaves a workgroup for each CU, 16 columns a lane: runs of 256 bytes of it as of a 16-bit matrix (8192 x 14336 rotated 53 us for 62,
+// to the nearest 42 for 55; 2560 x 2560, which it does not, 10.3 for 7.0).
+inline uint32_t columns_tiles(int64_t cols, uint32_t each) { return (uint32_t)((cols + 16 * each - 1) / (16 * each)); }
 template <uint32_t LINES> struct ColumnsLds {
     __attribute__((aligned(16))) uint8_t tile[LINES * 128];
     __attribute__((aligned(8))) uint8_t scales[LINES * 8];
@@ -177,10 +177,11 @@ __device__ __forceinline__ float byte_value(const uint32_t (&x)[4], int j)
     return j & 1 ? v.y : v.x;
 }
 
-template <int DT, int RAND, bool ROTATE, class LDS>
+// EACH: columns of a lane
+template <int DT, int RAND, bool ROTATE, uint32_t EACH, class LDS>
 __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t superchunks, const Division &tiles, uint32_t id, LDS &lds)
 {
-    constexpr uint32_t EACH = kColumns<DT>, LINES = 16 * EACH, TURN = EACH == 16 ? 4 : 3; // TURN: neighbouring lanes' lines lie in turned pieces
+    constexpr uint32_t LINES = 16 * EACH, TURN = EACH == 16 ? 4 : 3; // TURN: neighbouring lanes' lines lie in turned pieces
     uint8_t *tile = lds.tile, *tile_scales = lds.scales;
     const int lane = threadIdx.x & 63, block = threadIdx.x >> 6, g = lane & 3;
     const uint32_t superchunk = tiles(id), col0 = (id - superchunk * tiles.by) * LINES, col = col0 + EACH * (lane >> 2), all_cols = (uint32_t)a.cols, last_row = (uint32_t)a.rows - 1;
@@ -189,15 +190,23 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
     uint32_t x[8][WORDS]; // [row][column], as they are in memory
     float up[8];          // of a checkpoint's rows
     if constexpr (DT == DQ_E4M3) {
-        const uint32_t from = min(col, (uint32_t)a.stride - 16);
+        const uint32_t from = min(col, (uint32_t)a.stride - EACH);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int64_t r = min(row + j, last_row);
-            const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.x) + r * a.stride + from);
-            x[j][0] = w.x;
-            x[j][1] = w.y;
-            x[j][2] = w.z;
-            x[j][3] = w.w;
+            const uint8_t *at = static_cast<const uint8_t *>(a.x) + r * a.stride + from;
+            if constexpr (EACH == 16) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(at);
+                x[j][0] = w.x;
+                x[j][1] = w.y;
+                x[j][2] = w.z;
+                x[j][3] = w.w;
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2 *>(at);
+                x[j][0] = w.x;
+                x[j][1] = w.y;
+                x[j][2] = x[j][3] = 0u;
+            }
             up[j] = scale_up(a.x_scales[r * (a.stride >> 5) + (from >> 5)]);
         }
     } else if (all_cols >= 8) {
@@ -305,23 +314,34 @@ __device__ __forceinline__ void quantize_columns(const QuantizeArgs &a, uint32_t
         reinterpret_cast<uint2 *>(a.scales)[(int64_t)(col0 + threadIdx.x) * superchunks + superchunk] = reinterpret_cast<const uint2 *>(tile_scales)[threadIdx.x];
 }
 
-template <int DT, int RAND, bool ROTATE>
+template <int DT, int RAND, bool ROTATE, uint32_t EACH>
 __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : RAND == kNearest && ROTATE && DT != DQ_E4M3 ? 8 : 6) void mx4_columns_kernel(QuantizeArgs a, uint32_t superchunks, Division tiles)
 {
-    __shared__ ColumnsLds<16 * kColumns<DT>> lds;
-    quantize_columns<DT, RAND, ROTATE>(a, superchunks, tiles, unit_of(blockIdx.x, gridDim.x), lds);
+    __shared__ ColumnsLds<16 * EACH> lds;
+    quantize_columns<DT, RAND, ROTATE, EACH>(a, superchunks, tiles, unit_of(blockIdx.x, gridDim.x), lds);
 }
 
 template <int DT, int RAND> static hipError_t launch_quantize(const QuantizeArgs &a, bool columns, hipStream_t stream)
 {
     const uint32_t superchunks = (uint32_t)(((columns ? a.rows : a.cols) + 255) >> 8);
     if (columns) {
-        const Division tiles(columns_tiles(a.cols, DT));
+        if constexpr (DT == DQ_E4M3) {
+            const Division tiles(columns_tiles(a.cols, 16));
+            const dim3 grid(tiles.by * superchunks);
+            if (grid.x >= 256) {
+                if (a.sign)
+                    mx4_columns_kernel<DT, RAND, true, 16><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
+                else
+                    mx4_columns_kernel<DT, RAND, false, 16><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
+                return hipGetLastError();
+            }
+        }
+        const Division tiles(columns_tiles(a.cols, 8));
         const dim3 grid(tiles.by * superchunks);
         if (a.sign)
-            mx4_columns_kernel<DT, RAND, true><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
+            mx4_columns_kernel<DT, RAND, true, 8><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
         else
-            mx4_columns_kernel<DT, RAND, false><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
+            mx4_columns_kernel<DT, RAND, false, 8><<<grid, 512, 0, stream>>>(a, superchunks, tiles);
     } else {
         const uint32_t units = (uint32_t)(a.rows * superchunks * 32);
         const dim3 grid((units + 255) / 256);
@@ -367,17 +387,17 @@ struct QuantizeJobs {
     QuantizeJob job[kJobs];
 };
 
-template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void do_job(const QuantizeJob &j, bool columns, uint32_t id, ColumnsLds<256> &lds)
+template <int DT, int RAND, bool ROTATE> __device__ __forceinline__ void do_job(const QuantizeJob &j, bool columns, uint32_t id, ColumnsLds<128> &lds)
 {
     if (columns)
-        quantize_columns<DT, RAND, ROTATE>(j.a, j.superchunks, j.by, id, lds);
+        quantize_columns<DT, RAND, ROTATE, 8>(j.a, j.superchunks, j.by, id, lds);
     else if (id * 512 + threadIdx.x < j.units)
         quantize_rows<DT, RAND, ROTATE>(j.a, j.by, id * 512 + threadIdx.x);
 }
 
 template <int DT> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void mx4_jobs_kernel(QuantizeJobs jobs)
 {
-    __shared__ ColumnsLds<256> lds;
+    __shared__ ColumnsLds<128> lds;
     int k = 0;
 #pragma unroll
     for (int i = 1; i < kJobs; i++) k += blockIdx.x >= jobs.job[i].first ? 1 : 0;
@@ -403,7 +423,7 @@ template <int DT> __global__ __launch_bounds__(512, DT == DQ_F32 ? 4 : 6) void m
 hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStream_t stream)
 {
     const auto blocks_of = [](const QuantizeOne &q) {
-        return q.columns ? columns_tiles(q.a.cols, q.dtype) * ((q.a.rows + 255) >> 8) : (q.a.rows * ((q.a.cols + 255) >> 8) + 15) >> 4;
+        return q.columns ? columns_tiles(q.a.cols, 8) * ((q.a.rows + 255) >> 8) : (q.a.rows * ((q.a.cols + 255) >> 8) + 15) >> 4;
     };
     for (int next = 0; next < count;) {
         int take = 0, dtype = DQ_E4M3; // the type of what is no checkpoint
@@ -429,7 +449,7 @@ hipError_t launch_mx4_quantize_list(const QuantizeOne *list, int count, hipStrea
                 const QuantizeOne &q = list[next + k];
                 j.a = q.a;
                 j.superchunks = (uint32_t)(((q.columns ? q.a.rows : q.a.cols) + 255) >> 8);
-                j.by = Division(q.columns ? columns_tiles(q.a.cols, q.dtype) : j.superchunks);
+                j.by = Division(q.columns ? columns_tiles(q.a.cols, 8) : j.superchunks);
                 j.units = (uint32_t)(q.a.rows * j.superchunks * 32);
                 j.kind = (q.columns ? 16 : 0) + (q.dtype == DQ_E4M3 ? 10 : !q.stochastic ? 0 : !q.a.pool ? 2 : 4 + 2 * q.pool_dtype) + (q.a.sign ? 1 : 0);
                 first += (uint32_t)blocks_of(q);

@@ -19,7 +19,9 @@ hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t st
 {
     a.flags |= norm_threads(a.cols) << 16;
     if (norm_passing(a.rows, a.cols, dtype)) a.flags |= kNormPassing;
-    a.grid = std::min(a.rows, 4096 * 64 / norm_threads(a.cols)); // sixteen waves for each CU
+    // workgroups that the chip holds at once, sixteen waves a CU, with as many rows each
+    const uint32_t held = 256 * (1024 / norm_threads(a.cols)), turns = (a.rows + held - 1) / held;
+    a.grid = (a.rows + turns - 1) / turns;
     return dtype == DQ_F32 ? launch_norm_f32(a, stream32, stream) : dtype == DQ_BF16 ? launch_norm_bf16(a, stream32, stream) : launch_norm_f16(a, stream32, stream);
 }
 

@@ -11,7 +11,8 @@ peak).  ``python evaluate.py --config 1|2|3|4|5``.  A measurement tool beside
   5  2^30 fp32: compress / decompress / fused sweep, and the blocked transform
 ``--kernels`` times every entry point of the library on one 25 MB bucket.
 ``--training-step`` runs whole training steps of one rank: two 4-bit linear layers, their gradients through a dynamic-bitrate bucket,
-the clipping norm, and AdamW.
+the clipping norm, and AdamW; and the same around a block of norms, a gated activation and its two linear layers, what the backward
+pass keeps in 16 bits and in 8.
 ``--reference-benchmark`` prints the table of the reference's own microbenchmark
 (cuda_kernels/tests/benchmark_scaling_quantization.py:60-112: bf16, chunk 16, 268,435,456 elements,
 2/4/8 bits x strategy 2/3, eager launches through the eden_utils module) with the fraction of the HBM peak.
@@ -34,7 +35,7 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 import cpu_baselines                                                                       # noqa: E402
-from dynamiq_sigcomm_artifact_amd import bitrate, capi, microscale, optimizer              # noqa: E402
+from dynamiq_sigcomm_artifact_amd import activations, bitrate, capi, microscale, optimizer  # noqa: E402
 from dynamiq_sigcomm_artifact_amd.compressors import Aee_Dynamic_Range_GPU_kern, Mee_Dynamic_Range_GPU_kern   # noqa: E402
 from dynamiq_sigcomm_artifact_amd.dynamiq_pipeline import (dynamic_bitrate_allreduce,     # noqa: E402
                                                            dynamic_bitrate_allreduce_grouped,
@@ -815,6 +816,19 @@ def kernels(dev, n=6553600):
         a = microscale.quantize(torch.randn(m, cols, generator=g, device=dev))
         t = _time_us(lambda: microscale.product(a, q))
         _emit(kernel="mx4 product", us=round(t, 2), m=m, n=rows, k=cols, TFLOPs=round(2.0 * m * n / t / 1e6, 1))
+    # what lies between the linear layers
+    eight = 33 / 32
+    line("checkpoint compress", lambda: activations.compress(x), (2 + eight) * n, n=n)
+    c = activations.compress(x)
+    line("checkpoint restore", lambda: activations.restore(c, torch.bfloat16), (2 + eight) * n, n=n)
+    line("mx4 quantize (of a checkpoint, rotated)", lambda: microscale.quantize(c, True, sign=bits[1]), eight * n + padded * 17 / 32, n=n, columns=True)
+    y, weight = torch.randn(rows, cols, generator=g, device=dev).bfloat16(), torch.ones(cols, dtype=torch.bfloat16, device=dev)
+    line("residual_norm", lambda: activations.residual_norm(y, x, weight), 8 * n, n=n)
+    line("residual_norm (with the checkpoint)", lambda: activations.residual_norm(y, x, weight, checkpoint=True), (8 + eight) * n, n=n)
+    line("residual_norm (after and before, gate)", lambda: activations.residual_norm(y, x, weight, gate=weight, after=True, after_weight=weight), 8 * n, n=n)
+    for kind in ("silu", "gelu_tanh"):
+        line("gated " + kind, lambda: activations.gated(y, x, kind=kind), 6 * n, n=n)
+    line("gated (with the checkpoint)", lambda: activations.gated(y, x, checkpoint=True), (6 + eight) * n, n=n)
 
 
 def training_step(dev, tokens=4096, width=1600, hidden=2048, steps=20):
@@ -879,6 +893,82 @@ def training_step(dev, tokens=4096, width=1600, hidden=2048, steps=20):
           grad_nmse_of_4_bit_layers=_nmse(exact, bucket), grad_nmse_of_the_encoding=_nmse(bucket, reduced), norm=float(norm[0]))
     for name, fn in (("layers", layers), ("encode", encode), ("clip", clip), ("update", update), ("step", step)):
         _emit(training_step=name, us=round(_time_us(fn, warmup=3, iters=10), 2))
+
+
+def training_block(dev, tokens=4096, width=1600, hidden=2048, steps=20):
+    """One rank's training steps around a block as models have them: a norm, the linear layer with both halves of a gated activation, the activation, the linear layer back,
+    and a norm after it, a gate per channel, the residual and the next block's norm in one pass.  The 4-bit layers' 9,830,400 gradients and those of the norms go through a
+    dynamic-bitrate bucket, the clipping norm and AdamW.  Beside the times: what lies in memory between the two passes where it is kept in 16 bits and in 8, and what
+    4-bit products and 8-bit checkpoints change in the gradients."""
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(tokens, width, generator=g, device=dev).bfloat16()
+    shapes = ((2 * hidden, width), (width, hidden))
+    weights = [(torch.randn(r, c, generator=g, device=dev) / math.sqrt(c)).bfloat16() for r, c in shapes] + [torch.ones(width, dtype=torch.bfloat16, device=dev) for _ in range(4)]
+    true = [w.float() + torch.randn(w.shape, generator=g, device=dev) * 0.3 / math.sqrt(w.shape[-1]) for w in weights]
+    weights = [w.requires_grad_() for w in weights]
+
+    def plain(up, down, before, after, gate, following):
+        h = torch.nn.functional.rms_norm(x.float(), (width,), before, 1e-6) @ up.t()
+        y = (torch.nn.functional.silu(h[:, :hidden]) * h[:, hidden:]) @ down.t()
+        return torch.nn.functional.rms_norm(x.float() + gate * torch.nn.functional.rms_norm(y, (width,), after, 1e-6), (width,), following, 1e-6)
+    with torch.no_grad():
+        aim = plain(*true).bfloat16()
+    sizes = [w.numel() for w in weights]
+    total = -(-sum(sizes) // 256) * 256                              # a bucket is whole superchunks
+    bucket, reduced = (torch.zeros(total, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    parts, grads = ([v.view_as(w) for v, w in zip(flat[:sum(sizes)].split(sizes), weights)] for flat in (bucket, reduced))
+    signs = {}
+    for k, n in enumerate((tokens, width, 2 * hidden)):
+        signs[n] = torch.empty(-(-n // 256) * 8, dtype=torch.int32, device=dev)
+        capi.rand_diag_bits(signs[n], signs[n].numel() * 32, k + 1)
+    count = torch.zeros(1, dtype=torch.int64, device=dev)
+    pipe = SinglePassBuckets(dev, seed=3, u=45.0)
+    opt = optimizer.AdamW(weights, lr=1e-3, bits=8, capturable=True)
+    norm, loss = torch.empty(2, dtype=torch.float32, device=dev), torch.empty((), device=dev)
+
+    def forward(eight):
+        up, down, before, after, gate, following = weights
+        h, r, *c = activations.residual_norm(x, weight=before, checkpoint=eight)
+        both = microscale.linear(h, up, sign=(signs[2 * hidden], signs[tokens]), seed=1, step=count, checkpoint=c[0] if eight else None)
+        a = activations.gated(both, checkpoint=eight)
+        a, c = a if eight else (a, None)
+        y = microscale.linear(a, down, sign=(signs[width], signs[tokens]), seed=2, step=count, checkpoint=c)
+        return activations.residual_norm(y, r, following, gate=gate, after=True, after_weight=after, checkpoint=eight)[0]
+
+    def layers(eight=True):
+        value = (forward(eight) - aim).float().square().mean()
+        loss.copy_(value.detach())
+        for part, v in zip(parts, torch.autograd.grad(value * tokens, weights)):
+            part.copy_(v)
+        count.add_(1)
+
+    def step():
+        layers()
+        pipe.begin_step()
+        pipe.run(bucket, reduced)
+        optimizer.grad_norm(grads, 1.0, work=opt.work, out=norm)
+        for w, v in zip(weights, grads):
+            w.grad = v
+        opt.step(grad_scale=norm[1:])
+
+    losses, held, off = [], {}, {}
+    exact = [w.detach().float().requires_grad_() for w in weights]
+    exact = torch.cat([v.reshape(-1) for v in torch.autograd.grad((plain(*exact) - aim.float()).square().mean() * tokens, exact)])
+    for eight in (False, True):
+        layers(eight)
+        off[eight] = _nmse(exact, bucket[:sum(sizes)])
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(dev)
+        out = forward(eight)
+        held[eight] = torch.cuda.memory_allocated(dev) - before
+        del out
+    for k in range(steps):
+        step()
+        losses.append(float(loss))
+    _emit(training_block="run", tokens=tokens, width=width, hidden=hidden, steps=steps, loss_first=losses[0], loss_last=losses[-1], held_bytes_16_bits=held[False],
+          held_bytes_8_bits=held[True], grad_nmse=off[True], grad_nmse_16_bits=off[False], norm=float(norm[0]))
+    for name, fn in (("layers", layers), ("layers_16_bits", lambda: layers(False)), ("step", step)):
+        _emit(training_block=name, us=round(_time_us(fn, warmup=3, iters=10), 2))
 
 
 def quantiser_sizes(dev, nbits=4):
@@ -1073,7 +1163,8 @@ def main():
     ap.add_argument("--config", type=int, choices=[1, 2, 3, 4, 5])
     ap.add_argument("--kernels", action="store_true", help="time every entry point of the library on a 25 MB bucket")
     ap.add_argument("--training-step", action="store_true",
-                    help="whole training steps of one rank: 4-bit linear layers, a dynamic-bitrate bucket, the clipping norm, AdamW")
+                    help="whole training steps of one rank: 4-bit linear layers, a dynamic-bitrate bucket, the clipping norm, AdamW; around a block with "
+                         "norms, a gated activation and 8-bit checkpoints as well")
     ap.add_argument("--quantiser-sizes", action="store_true",
                     help="compress / decompress / fused step of the production quantiser (bf16, 4-bit, AEE and MEE) at 25 MB, at "
                          "the ring-chunk size of the 8-rank configuration and at 2^28 elements")
@@ -1097,6 +1188,7 @@ def main():
         return
     if args.training_step:
         training_step(dev)
+        training_block(dev)
         return
     if args.quantiser_sizes:
         quantiser_sizes(dev)
