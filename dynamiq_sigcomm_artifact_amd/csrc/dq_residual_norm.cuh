@@ -2,9 +2,11 @@
 //
 //   z = norm(y; after_weight, after_bias) or y,   r = residual_scale residual + block_scale gate z,   h = norm(r; weight, bias)
 //
-// A workgroup takes a row (64 to 1024 threads, eight elements of a thread together, up to four times), holds it in registers from the loads to the stores, and reduces through
-// LDS: every array moves once.  Backward it takes a run of rows and keeps what the weights' and the gate's gradients add up to in registers; what workgroups have of the same
-// columns is added in the order of the rows by a second launch.
+// A workgroup takes a row (64 to 1024 threads, eight elements of a thread together, from 8192 columns on twice, from 16384 four times), holds it in registers from the loads to the
+// stores, and reduces through LDS: every array moves once.  Backward it takes a run of rows and keeps what the weights' and the gate's gradients add up to in registers; what
+// workgroups have of the same columns is added in the order of the rows by a second launch.
+//
+// All arithmetic is in binary32, sums included; h, r and the gradients are rounded once, where they are stored, h from the r that is not rounded yet.
 #pragma once
 
 #include "dq_launch.h"
@@ -30,6 +32,16 @@ __device__ __forceinline__ float wave_sum_f32(float v)
            (__int_as_float(__builtin_amdgcn_readlane(u, 32)) + __int_as_float(__builtin_amdgcn_readlane(u, 48)));
 }
 
+// the elements that a lane has of a row, and zeros in place of the others
+__device__ __forceinline__ int lanes_own(uint32_t col, uint32_t cols) { return (int)min(cols - min(col, cols), 8u); }
+__device__ __forceinline__ void clip(float (&v)[8], int own)
+{
+    if (own < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = j < own ? v[j] : 0.0f;
+    }
+}
+
 // Sums over a workgroup's threads, in every one of them: a wave's, and then 16 lanes add what up to 16 waves have left.  Two buffers in turn: who writes one for the second time has
 // met, in the sum between, everybody who still read it.
 struct GroupSums {
@@ -49,6 +61,38 @@ struct GroupSums {
         const f32x2_t v = at[first + min(w, waves - 1)];
         a = row16_sum(w < waves ? v.x : 0.0f);
         b = row16_sum(w < waves ? v.y : 0.0f);
+    }
+    // The mean of a row of cols elements and the sum of the squares of what lies between them and it, where every thread has eight neighbours (0 behind the last one): each wave
+    // takes its own mean off first, and waves meet once: sum of squares = sum over the waves of (theirs + their count (their mean - the mean)^2).
+    __device__ __forceinline__ void moments(const float (&x)[8], int own, uint32_t cols, float &mean, float &squares)
+    {
+        const uint32_t wave = (threadIdx.x >> 6) - first;
+        const auto count = [&](uint32_t w) { return (float)min(cols - min(cols, 512 * w), 512u); };
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += x[j];
+        s = wave_sum_f32(s);
+        const float mine = s / fmaxf(count(wave), 1.0f);
+        float d[8], q = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) d[j] = x[j] - mine;
+        clip(d, own);
+#pragma unroll
+        for (int j = 0; j < 8; j++) q += d[j] * d[j];
+        q = wave_sum_f32(q);
+        mean = mine;
+        squares = q;
+        if (waves == 1) return;
+        f32x2_t *at = part[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = f32x2_t{s, q};
+        __syncthreads();
+        const uint32_t w = threadIdx.x & 15;
+        const f32x2_t v = at[first + min(w, waves - 1)];
+        const float n = count(w);
+        mean = row16_sum(w < waves ? v.x : 0.0f) / (float)cols;
+        const float off = v.x / fmaxf(n, 1.0f) - mean;
+        squares = row16_sum(w < waves ? v.y + n * (off * off) : 0.0f);
     }
 };
 
@@ -93,15 +137,6 @@ template <int DT> __device__ __forceinline__ void settle(uint32_t col, uint32_t 
 #pragma unroll
                 for (int w = 0; w < N; w++) x[w] = w + k < N ? x[(w + k) % N] : 0u;
             }
-    }
-}
-// the elements that a lane has of a row, and zeros in place of the others
-__device__ __forceinline__ int lanes_own(uint32_t col, uint32_t cols) { return (int)min(cols - min(col, cols), 8u); }
-__device__ __forceinline__ void clip(float (&v)[8], int own)
-{
-    if (own < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = j < own ? v[j] : 0.0f;
     }
 }
 template <int DT> __device__ __forceinline__ void row_values(uint32_t (&x)[kWords<DT>], uint32_t col, uint32_t cols, float (&v)[8])
@@ -176,7 +211,9 @@ template <int DT> struct Columns {
 };
 
 // FULL: there is a norm after the block, or a gate.  Rows up to 8192 wide, without these up to 16384, are taken in turn by as many workgroups as the chip holds, which keep the vectors and ask for a row
-// before they work on the one in front of it.
+// before they work on the one in front of it.  Bound by memory: 8192 x 4096 bf16 with the checkpoints of h and r in 55 us (6.1 TB/s; a workgroup for each row, which loads the weight
+// again, 60), with a norm after the block and gates, without checkpoints, 56 (4.8 TB/s; 65); 2048 x 14336 in 48 (4.9 TB/s; with the weight loaded again 94); 1 x 4096 in 2.7, a launch.
+// Twice or four times as many workgroups as fit at once take up to 10 % longer.
 template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global__ __launch_bounds__(THREADS, 4) void residual_norm_kernel(BlockNormArgs a)
 {
     constexpr bool HELD = V == 1 || (V == 2 && !FULL);
@@ -188,6 +225,11 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
     const auto statistics = [&](const float (&x)[V][8], float &mean, float &rs) {
         float s = 0.0f, none = 0.0f;
         mean = 0.0f;
+        if (V == 1 && center) {
+            sums.moments(x[0], lanes_own(8 * threadIdx.x, cols), cols, mean, s);
+            rs = inverse_root(s / (float)cols + a.eps);
+            return;
+        }
         if (center) {
 #pragma unroll
             for (int k = 0; k < V; k++)
@@ -342,6 +384,11 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
 //   xhat = (r - mean) rs, g = dh weight:   dr = rs (g - [mean g] - xhat mean(g xhat)) + the gradient of r itself
 //   dresidual = residual_scale dr, t = block_scale dr, dgate = sum t z, t gate through the norm of y likewise: dy
 //   dweight = sum dh xhat, dbias = sum dh, and of the norm of y with t gate in dh's place
+//
+// Bound by memory where few sums are kept: 8192 x 4096 bf16, weight's gradient, r in 8 bits, 44 us (5.3 TB/s): a row is asked for while the one in front of it is worked on (without
+// that 53 at three workgroups a CU, 59 at two), with the hint that nothing of it is wanted again (52 without; what the cache holds is loaded without it, 15.0 us for 17 at 4095 x 768).  With a norm after the
+// block and a gate, whose vectors, sums and arrays fill the 128 registers of two workgroups a CU, 76 us (5.3 TB/s; 121 at one workgroup a CU, with more registers each).  A checkpoint's
+// codes and the two-byte forms are kernels of their own (EIGHT): one kernel for both waited for each load where the two ways met, 103 us.
 //
 // SUMS: which of them registers are kept for, at least those that are wanted.  Narrow rows are shared by fewer threads than a workgroup has: those that share one, a team, have a
 // run of rows each, and add up what they have of the columns before it leaves.
