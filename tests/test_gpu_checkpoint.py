@@ -159,6 +159,28 @@ def test_in_four_bits(act, ms, capi, r, c, columns, rotate):
     assert torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales) and q.shape == want.shape
 
 
+@pytest.mark.parametrize("r,c", [(2100, 8200), (256 * 16, 4096), (65, 70001), (70001, 65)])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_in_four_bits_of_many(act, ms, capi, r, c, rotate):
+    """sizes that fill the chip: wide tiles, ragged at both ends"""
+    x = matrix(r, c, BF, 12)
+    x[r // 2, c // 3], x[r - 1, c - 1], x[r - 1, 0] = math.inf, math.nan, torch.finfo(BF).max
+    k = act.compress(x)
+    sign = signs(capi, r, 4) if rotate else None
+    q, want = ms.quantize(k, columns=True, sign=sign), ms.quantize(act.restore(k), columns=True, sign=sign)
+    live = torch.repeat_interleave(want.scales != 255, 16, 1)
+    assert torch.equal(q.scales, want.scales) and torch.equal(q.codes[live], want.codes[live]) and bool((want.scales == 255).any())
+
+
+def test_hinted_loads(act):
+    """what is beyond the cache, whose loads carry a hint, against parts of it that are not"""
+    x = matrix(9001, 8192, BF, 13)
+    whole = act.compress(x)
+    for part, codes, scales in zip(x.split(3000), whole.codes.split(3000), whole.scales.split(3000)):
+        c = act.compress(part)
+        assert torch.equal(c.codes, codes) and torch.equal(c.scales, scales)
+
+
 def test_in_four_bits_of_the_largest_numbers(act, ms, capi):
     """sums beyond 2^128 in the rotation, next to what is not finite"""
     x = matrix(300, 200, FP, 10, 0.5)

@@ -172,6 +172,21 @@ def test_partial_gradients_and_none(act):
         assert torch.equal(act.gated(g, u), out)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_hinted_loads(act, eight):
+    """what is beyond the cache against parts of it that are not"""
+    x, da = normal((3001, 2 * 8000), BF, 1), normal((3001, 8000), BF, 2)
+
+    def run(x, da):
+        leaf = x.detach().requires_grad_()
+        out = act.gated(leaf, checkpoint=eight)
+        out, c = out if eight else (out, None)
+        return [out.detach(), torch.autograd.grad(out, leaf, da)[0]] + ([c.codes, c.scales] if eight else [])
+    whole = run(x, da)
+    for k in range(0, 3001, 700):
+        assert all(torch.equal(a[k:k + 700], b) for a, b in zip(whole, run(x[k:k + 700], da[k:k + 700])))
+
+
 def test_empty(act):
     for shape in ((0, 10), (5, 0), (0,)):
         x = torch.empty(shape, device=DEV, requires_grad=True)

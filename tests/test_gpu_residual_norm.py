@@ -170,6 +170,49 @@ def test_widths(act, cols, center):
         against_definition(act, t, True, True, center=center, after=True, residual_scale=0.9, block_scale=1.2)
 
 
+@pytest.mark.parametrize("cols", [520, 2055, 4096, 4099, 8192, 8200, 14336, 16390])
+@pytest.mark.parametrize("eight", [False, True])
+def test_widths_of_few_sums(act, cols, eight):
+    """every width with the kernels that keep fewer sums: the weight's, the bias' too, the gate's, the norm after the block's"""
+    for k, (parts, gate, kw) in enumerate(((("residual", "weight"), None, {}), (("residual", "weight", "bias"), None, {"center": True}), (("residual",), (cols,), {}),
+                                           (("weight", "after_weight"), None, {"after": True}), (("residual", "after_weight"), (5, cols), {"after": True}),
+                                           (("residual", "weight", "bias"), (cols,), {"center": True}))):
+        dtype, stream = ((BF, BF), (HF, FP), (FP, FP))[k % 3]
+        against_definition(act, tensors((5, cols), dtype, stream, parts, cols + k, gate=gate), True, True, eight=eight, **kw)
+
+
+@pytest.mark.parametrize("rows,cols", [(5001, 4096), (4100, 5000), (40001, 512), (2001, 8200)])
+@pytest.mark.parametrize("parts,gate,kw", [(("residual", "weight"), False, {}), (("weight", "bias"), False, {"center": True}), (("residual", "weight", "after_weight"), True, {"after": True})],
+                         ids=["lean", "centred", "sandwich"])
+@pytest.mark.parametrize("eight", [False, True])
+def test_many_rows(act, rows, cols, parts, gate, kw, eight):
+    """what is beyond the cache, whose loads carry a hint and whose workgroups have many rows, against parts of it that are not"""
+    t = tensors((rows, cols), BF, BF, parts, 9, of=FP, gate=(cols,) if gate else None)
+    dh, dr = normal((rows, cols), BF, 10, 1e-2), normal((rows, cols), BF, 11, 1e-2)
+    vectors = [k for k in t if k not in ("y", "residual")]
+
+    def run(at):
+        leaf = {k: (v if k in vectors else v[at]).detach().requires_grad_() for k, v in t.items()}
+        got = act.residual_norm(leaf["y"], leaf.get("residual"), leaf.get("weight"), leaf.get("bias"), gate=leaf.get("gate"), after_weight=leaf.get("after_weight"),
+                                checkpoint=eight, **kw)
+        plain = got[1] is leaf["y"]
+        grads = torch.autograd.grad(got[:1] if plain else got[:2], list(leaf.values()), (dh[at],) if plain else (dh[at], dr[at]))
+        rows = [got[0].detach(), got[1].detach()] + [g for k, g in zip(leaf, grads) if k not in vectors] + ([got[2].codes, got[2].scales] if eight else [])
+        return rows, {k: g.double() for k, g in zip(leaf, grads) if k in vectors}
+    whole, sums = run(slice(0, rows))
+    step = 700 * 4096 // cols
+    total, size = {k: 0.0 for k in sums}, {k: 0.0 for k in sums}
+    for at in range(0, rows, step):
+        part, s = run(slice(at, at + step))
+        assert all(torch.equal(a[at:at + step], b) for a, b in zip(whole, part))
+        for k in s:
+            total[k], size[k] = total[k] + s[k], size[k] + s[k].abs()
+    # both are sums of the same terms; a chain of additions is off by 2^-24 of what it has passed at each: as many as rows at most, of terms whose magnitudes are ten times the parts' sums
+    # or less where the sign is random over hundreds of rows
+    for k in sums:
+        assert float(((sums[k] - total[k]).abs() - rows * U * 10 * (size[k] + 1.0)).max()) <= 0, k
+
+
 @pytest.mark.parametrize("dtype,stream", [(BF, BF), (BF, FP), (HF, HF), (HF, FP), (FP, FP)], ids=str)
 @pytest.mark.parametrize("eight", [False, True])
 def test_parts(act, dtype, stream, eight):
@@ -215,7 +258,7 @@ def test_partial_gradients(act):
         _, one = against_definition(act, t, True, True, wants=[k])
         assert torch.equal(one[k], both[k])
     _, scaled = against_definition(act, t, True, True, residual_scale=0.5)
-    assert torch.equal(scaled["y"], both["y"]) is False or scaled["residual"] is not scaled["y"]
+    assert scaled["y"].data_ptr() != scaled["residual"].data_ptr()
 
 
 def test_gradients_accumulate(act):
@@ -232,6 +275,16 @@ def test_gradients_accumulate(act):
     dz, = torch.autograd.grad(act.residual_norm(z, z)[0], z, dh)
     want = torch.autograd.grad(act.residual_norm(z.detach().requires_grad_(), z)[0], z, dh)[0]
     assert torch.equal(dz, 2 * want)
+
+
+def test_backward_twice(act):
+    """a graph that is kept gives the same gradients again"""
+    t = {k: v.requires_grad_() for k, v in tensors((30, 130), BF, FP, ALL, 2, gate=(130,)).items()}
+    h, r, _ = act.residual_norm(t["y"], t["residual"], t["weight"], t["bias"], gate=t["gate"], after=True, after_weight=t["after_weight"], after_bias=t["after_bias"], checkpoint=True)
+    loss = (h.float().square().sum() + r.square().sum())
+    first = torch.autograd.grad(loss, list(t.values()), retain_graph=True)
+    again = torch.autograd.grad(loss, list(t.values()))
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
 def test_not_differentiated(act):
