@@ -1343,9 +1343,9 @@ int dq_residual_norm_forward(const dq_residual_norm_t *o, int device, dq_stream_
 int64_t dq_residual_norm_work_floats(const dq_residual_norm_t *o)
 {
     if (norm_ok(o)) return -1;
-    const dq::NormShares s = dq::norm_shares(o->rows, o->gate ? o->rows_per_gate : 0, (uint32_t)o->cols);
+    const dq::NormShares s = dq::norm_shares(o->rows, o->gate ? o->rows_per_gate : 0, (uint32_t)o->cols, o->gate || o->after);
     const int sums = !!o->dweight + !!o->dbias + (o->dgate && s.parts > 1) + !!o->dafter_weight + !!o->dafter_bias;
-    return (int64_t)sums * s.grid * o->cols;
+    return (int64_t)sums * s.grid * o->cols + (s.wide ? 4 * o->rows : 0);
 }
 
 int dq_residual_norm_backward(const dq_residual_norm_t *o, int device, dq_stream_t stream)
@@ -1366,7 +1366,7 @@ int dq_residual_norm_backward(const dq_residual_norm_t *o, int device, dq_stream
     const uint8_t *kept_y = o->kept ? o->kept + (o->keep_r ? (dq_checkpoint_bytes(o->rows, o->cols) + 15) / 16 * 16 : 0) : nullptr;
     const bool eight = (wants_r && o->keep_r) || (wants_y && o->keep_y);
     dq::BlockNormBackArgs a = {o->dh, o->dr, wants_r ? (o->keep_r ? o->kept : o->r ? o->r : o->y) : nullptr, wants_y ? (o->keep_y ? kept_y : o->y) : nullptr, o->weight, o->gate, o->after_weight,
-                          o->after_bias, o->stats, o->dy, o->dresidual, nullptr, o->work, (uint32_t)o->rows, (uint32_t)o->cols, o->gate ? (uint32_t)o->rows_per_gate : 1,
+                          o->after_bias, o->stats, o->dy, o->dresidual, nullptr, o->work, nullptr, (uint32_t)o->rows, (uint32_t)o->cols, o->gate ? (uint32_t)o->rows_per_gate : 1,
                           norm_flags(o) | (eight ? dq::kNormEight : 0), 0, 0, 0, 0, 0, (float)o->residual_scale, (float)o->block_scale};
     const auto sum = [&](void *out, int bit) { return dq::NormSum{out, o->float32 & bit ? DQ_F32 : o->dtype}; };
     const dq::NormSum sums[5] = {sum(o->dweight, 1), sum(o->dbias, 2), sum(o->dgate, 4), sum(o->dafter_weight, 8), sum(o->dafter_bias, 16)};

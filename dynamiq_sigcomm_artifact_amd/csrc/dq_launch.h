@@ -455,19 +455,20 @@ struct BlockNormBackArgs {
     const void *dh, *dr, *r, *y, *weight, *gate, *after_weight, *after_bias;
     const float *stats;
     void *dy, *dresidual, *dgate;
-    float *work; // [sums][grid][cols]
+    float *work, *means; // [sums][grid][cols]; [rows][4], for rows that are met twice
     uint32_t rows, cols, per, flags, grid, teams, run, parts, sums;
     float residual_scale, block_scale;
 };
 struct NormShares {
     uint32_t grid, teams, run, parts;
+    bool wide; // sums of rows and of columns are a launch each
 };
 struct NormSum {
     void *out;
     int dtype;
 };
 constexpr int64_t kNormCols = 32768;
-NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols);
+NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols, bool between);
 hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t stream);
 hipError_t launch_norm_f16(const BlockNormArgs &a, bool stream32, hipStream_t stream);
 hipError_t launch_norm_bf16(const BlockNormArgs &a, bool stream32, hipStream_t stream);

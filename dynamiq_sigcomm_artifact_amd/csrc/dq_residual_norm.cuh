@@ -2,9 +2,13 @@
 //
 //   z = norm(y; after_weight, after_bias) or y,   r = residual_scale residual + block_scale gate z,   h = norm(r; weight, bias)
 //
-// A workgroup takes a row (64 to 1024 threads, eight elements of a thread together, from 8192 columns on twice, from 16384 four times), holds it in registers from the loads to the
-// stores, and reduces through LDS: every array moves once.  Backward it takes a run of rows and keeps what the weights' and the gate's gradients add up to in registers; what
-// workgroups have of the same columns is added in the order of the rows by a second launch.
+// A workgroup takes a row (64 to 1024 threads, eight elements of a thread together, from 8192 columns on twice), holds it in registers from the loads to the stores, and reduces
+// through LDS: every array moves once.  Backward it takes a run of rows and keeps what the weights' and the gate's gradients add up to in registers; what workgroups have of the same
+// columns is added in the order of the rows by a second launch.  Rows beyond 16384, or beyond 8192 with more than a residual between y and r, have kernels of their own.
+//
+// Column numbers are made afresh from the thread's where a loop over rows would spill (an empty asm): what follows from them alone, addresses and the shifts of a row's end, is else
+// kept from row to row for every array.  2048 x 14336 bf16 with a binary32 residual 73 us forward, 196 with it kept; all five sums of 4096 x 4096 77 backward, and 99; where
+// registers are left, keeping it is 2 % faster.
 //
 // All arithmetic is in binary32, sums included; h, r and the gradients are rounded once, where they are stored, h from the r that is not rounded yet.
 #pragma once
@@ -210,13 +214,13 @@ template <int DT> struct Columns {
     }
 };
 
-// FULL: there is a norm after the block, or a gate.  Rows up to 8192 wide, without these up to 16384, are taken in turn by as many workgroups as the chip holds, which keep the vectors and ask for a row
-// before they work on the one in front of it.  Bound by memory: 8192 x 4096 bf16 with the checkpoints of h and r in 55 us (6.1 TB/s; a workgroup for each row, which loads the weight
-// again, 60), with a norm after the block and gates, without checkpoints, 56 (4.8 TB/s; 65); 2048 x 14336 in 48 (4.9 TB/s; with the weight loaded again 94); 1 x 4096 in 2.7, a launch.
-// Twice or four times as many workgroups as fit at once take up to 10 % longer.
+// FULL: there is a norm after the block, or a gate.  Rows are taken in turn by as many workgroups as the chip holds, which keep the vectors and ask for a row before they work on the
+// one in front of it.  Bound by memory: 8192 x 4096 bf16 with the checkpoints of h and r in 55 us (6.1 TB/s; a workgroup for each row, which loads the weight again, 60), with a norm
+// after the block and gates, without checkpoints, 56 (4.8 TB/s; 65); 2048 x 14336 in 46 (5.1 TB/s; in LDS 55); 1 x 4096 in 2.7, a launch.  Twice or four times as many workgroups as
+// fit at once take up to 10 % longer.
 template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global__ __launch_bounds__(THREADS, 4) void residual_norm_kernel(BlockNormArgs a)
 {
-    constexpr bool HELD = V == 1 || (V == 2 && !FULL);
+    static_assert(V == 1 || !FULL, "the vectors between r and y are held of eight columns");
     __shared__ f32x2_t part[2][16];
     const uint32_t threads = a.flags >> 16, cols = a.cols;
     const bool center = a.flags & kNormCenter, after = FULL && a.flags & kNormAfter, before = a.flags & kNormBefore;
@@ -251,7 +255,7 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
         sums(s, none);
         rs = inverse_root(s / (float)cols + a.eps);
     };
-    Columns<DT> weight[HELD ? V : 1], bias[HELD ? V : 1], after_weight, after_bias, gate;
+    Columns<DT> weight[V], bias[V], after_weight, after_bias, gate;
     const auto ask_gate = [&](uint32_t row, uint32_t col) { gate.ask(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols); };
     const auto take_gate = [&](uint32_t col) { gate.take(a.gate, a.flags & kNormGate32, col, cols, 1.0f); };
     const auto ask_after = [&](uint32_t col) {
@@ -273,50 +277,46 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
     struct Raw {
         uint32_t y[V][kWords<DT>], residual[V][kWords<RT>];
     };
+    const auto col_of = [&](int k) {
+        uint32_t thread = threadIdx.x;
+        if (V > 1) asm volatile("" : "+v"(thread));
+        return 8 * (thread + k * threads);
+    };
     const auto load = [&](Raw &raw, uint32_t row) {
         const int64_t base = (int64_t)row * cols;
 #pragma unroll
-        for (int k = 0; k < V; k++) load_row<DT, PASSING>(row_of<DT>(a.y, base), 8 * (threadIdx.x + k * threads), cols, raw.y[k]);
+        for (int k = 0; k < V; k++) load_row<DT, PASSING>(row_of<DT>(a.y, base), col_of(k), cols, raw.y[k]);
         if (a.residual) {
 #pragma unroll
-            for (int k = 0; k < V; k++) load_row<RT, PASSING>(row_of<RT>(a.residual, base), 8 * (threadIdx.x + k * threads), cols, raw.residual[k]);
+            for (int k = 0; k < V; k++) load_row<RT, PASSING>(row_of<RT>(a.residual, base), col_of(k), cols, raw.residual[k]);
         }
     };
     uint32_t gated = blockIdx.x / a.per; // the gate that is held
     const auto step = [&](Raw &now, Raw &next, uint32_t row) {
         const int64_t base = (int64_t)row * cols;
-        if (HELD && row + a.grid < a.rows) load(next, row + a.grid);
-        if (!HELD) load(now, row);
+        if (row + a.grid < a.rows) load(next, row + a.grid);
         float x[V][8], mean_y = 0.0f, rs_y = 1.0f;
 #pragma unroll
-        for (int k = 0; k < V; k++) row_values<DT>(now.y[k], 8 * (threadIdx.x + k * threads), cols, x[k]);
+        for (int k = 0; k < V; k++) row_values<DT>(now.y[k], col_of(k), cols, x[k]);
         if (a.flags & kNormKeepY) {
             uint8_t *data = a.kept + (a.flags & kNormKeepR ? (((int64_t)a.rows * ((cols + 31) >> 5) * 33 + 15) & ~(int64_t)15) : 0);
 #pragma unroll
-            for (int k = 0; k < V; k++) keep_row<DT>(data, a.rows, row, 8 * (threadIdx.x + k * threads), cols, x[k]);
+            for (int k = 0; k < V; k++) keep_row<DT>(data, a.rows, row, col_of(k), cols, x[k]);
         }
         if (after) statistics(x, mean_y, rs_y);
-        if (FULL && HELD && a.gate && row / a.per != gated) {
+        if (FULL && a.gate && row / a.per != gated) {
             gated = row / a.per;
             ask_gate(row, 8 * threadIdx.x);
             take_gate(8 * threadIdx.x);
         }
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const uint32_t col = 8 * (threadIdx.x + k * threads);
+            const uint32_t col = col_of(k);
             if (after) {
-                if (!HELD) {
-                    ask_after(col);
-                    take_after(col);
-                }
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[k][j] = (x[k][j] - mean_y) * rs_y * after_weight.v[j] + after_bias.v[j];
             }
             if (FULL && a.gate) {
-                if (!HELD) {
-                    ask_gate(row, col);
-                    take_gate(col);
-                }
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[k][j] *= gate.v[j];
             }
@@ -341,13 +341,9 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
             statistics(x, mean, rs);
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                const uint32_t col = 8 * (threadIdx.x + k * threads);
-                if (!HELD) {
-                    ask_before(0, col);
-                    take_before(0, col);
-                }
+                const uint32_t col = col_of(k);
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[k][j] = ElemIO<DT>::round((x[k][j] - mean) * rs * weight[HELD ? k : 0].v[j] + bias[HELD ? k : 0].v[j]);
+                for (int j = 0; j < 8; j++) x[k][j] = ElemIO<DT>::round((x[k][j] - mean) * rs * weight[k].v[j] + bias[k].v[j]);
                 store_row<DT>(row_of<DT>(a.h, base), col, cols, x[k]);
                 if (a.h8) keep_row<DT>(a.h8, a.rows, row, col, cols, x[k]);
             }
@@ -355,27 +351,161 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
         if (a.stats && threadIdx.x == 0) reinterpret_cast<float4 *>(a.stats)[row] = make_float4(mean, rs, mean_y, rs_y);
     };
     Raw one, other;
-    if (HELD) {
-        const uint32_t col = 8 * threadIdx.x;
-        load(one, blockIdx.x);
-        if (FULL) {
-            ask_after(col);
-            ask_gate(blockIdx.x, col);
-        }
+    const uint32_t col = 8 * threadIdx.x;
+    load(one, blockIdx.x);
+    if (FULL) {
+        ask_after(col);
+        ask_gate(blockIdx.x, col);
+    }
 #pragma unroll
-        for (int k = 0; k < V; k++) ask_before(k, col + 8 * k * threads);
-        if (FULL) {
-            take_after(col);
-            take_gate(col);
-        }
+    for (int k = 0; k < V; k++) ask_before(k, col + 8 * k * threads);
+    if (FULL) {
+        take_after(col);
+        take_gate(col);
+    }
 #pragma unroll
-        for (int k = 0; k < V; k++) take_before(k, col + 8 * k * threads);
-        for (uint32_t row = blockIdx.x; row < a.rows; row += 2 * a.grid) {
-            step(one, other, row);
-            if (row + a.grid < a.rows) step(other, one, row + a.grid);
+    for (int k = 0; k < V; k++) take_before(k, col + 8 * k * threads);
+    for (uint32_t row = blockIdx.x; row < a.rows; row += 2 * a.grid) {
+        step(one, other, row);
+        if (row + a.grid < a.rows) step(other, one, row + a.grid);
+    }
+}
+
+// Wider rows lie in LDS, each thread's own columns of them, from the loads of y to the stores of h; two workgroups a CU, or one beyond 16384.  Bound by vector instructions and LDS beside
+// memory: 2048 x 14336 bf16 with both norms and a gate 63 us (3.7 TB/s), 1000 x 32768 with one norm 50 (5.2 TB/s).
+template <int DT, int RT, int THREADS> __global__ __launch_bounds__(THREADS, 4) void residual_norm_wide_kernel(BlockNormArgs a)
+{
+    constexpr int V = 4;
+    __shared__ f32x2_t part[2][16];
+    __shared__ float4 held[2 * V][THREADS];
+    const uint32_t cols = a.cols;
+    const bool center = a.flags & kNormCenter, after = a.flags & kNormAfter, before = a.flags & kNormBefore;
+    GroupSums sums = {part, THREADS / 64, 0};
+    const auto col_of = [](int k) { // afresh
+        uint32_t thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        return 8 * (thread + k * THREADS);
+    };
+    const auto hold = [&](int k, const float (&v)[8]) {
+        held[2 * k][threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+        held[2 * k + 1][threadIdx.x] = make_float4(v[4], v[5], v[6], v[7]);
+    };
+    const auto look = [&](int k, float (&v)[8]) {
+        const float4 x = held[2 * k][threadIdx.x], y = held[2 * k + 1][threadIdx.x];
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    };
+    // mean and 1 / sqrt(var + eps) of what is held, from the sum of it, or of its squares
+    const auto statistics = [&](float s, float &mean, float &rs) {
+        float none = 0.0f;
+        sums(s, none);
+        mean = 0.0f;
+        if (center) {
+            mean = s / (float)cols;
+            s = none = 0.0f;
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                if (8 * k * THREADS >= cols) break;
+                float v[8];
+                look(k, v);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] -= mean;
+                clip(v, lanes_own(col_of(k), cols));
+#pragma unroll
+                for (int j = 0; j < 8; j++) s += v[j] * v[j];
+            }
+            sums(s, none);
         }
-    } else {
-        for (uint32_t row = blockIdx.x; row < a.rows; row += a.grid) step(one, one, row);
+        rs = inverse_root(s / (float)cols + a.eps);
+    };
+    const auto add_up = [&](const float (&v)[8], float &s) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += center ? v[j] : v[j] * v[j];
+    };
+    for (uint32_t row = blockIdx.x; row < a.rows; row += a.grid) {
+        const int64_t base = (int64_t)row * cols;
+        uint32_t y[V][kWords<DT>], residual[V][kWords<RT>];
+#pragma unroll
+        for (int k = 0; k < V; k++) load_row<DT, true>(row_of<DT>(a.y, base), col_of(k), cols, y[k]);
+        if (a.residual) {
+#pragma unroll
+            for (int k = 0; k < V; k++) load_row<RT, true>(row_of<RT>(a.residual, base), col_of(k), cols, residual[k]);
+        }
+        float mean_y = 0.0f, rs_y = 1.0f, mean = 0.0f, rs = 1.0f, s = 0.0f;
+        uint8_t *data = a.kept + (a.flags & kNormKeepR ? (((int64_t)a.rows * ((cols + 31) >> 5) * 33 + 15) & ~(int64_t)15) : 0);
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            if (8 * k * THREADS >= cols) break;
+            float v[8];
+            const uint32_t col = col_of(k);
+            row_values<DT>(y[k], col, cols, v);
+            if (a.flags & kNormKeepY) keep_row<DT>(data, a.rows, row, col, cols, v);
+            hold(k, v);
+            add_up(v, s);
+        }
+        if (after) statistics(s, mean_y, rs_y);
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            if (8 * k * THREADS >= cols) break;
+            const uint32_t col = col_of(k);
+            float x[8];
+            Columns<DT> weight, bias, gate;
+            if (after) {
+                weight.ask(a.after_weight, a.flags & kNormAfterWeight32, 0, col, cols);
+                bias.ask(a.after_bias, a.flags & kNormAfterBias32, 0, col, cols);
+            }
+            gate.ask(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols);
+            look(k, x);
+            if (after) {
+                weight.take(a.after_weight, a.flags & kNormAfterWeight32, col, cols, 1.0f);
+                bias.take(a.after_bias, a.flags & kNormAfterBias32, col, cols, 0.0f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = (x[j] - mean_y) * rs_y * weight.v[j] + bias.v[j];
+            }
+            if (a.gate) {
+                gate.take(a.gate, a.flags & kNormGate32, col, cols, 1.0f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] *= gate.v[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= a.block_scale;
+            if (a.residual) {
+                float v[8];
+                row_values<RT>(residual[k], col, cols, v);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = v[j] * a.residual_scale + x[j];
+            }
+            if (a.r) store_row<RT>(row_of<RT>(a.r, base), col, cols, x);
+            if (a.flags & kNormKeepR) { // of r as it is stored
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = ElemIO<RT>::round(x[j]);
+                keep_row<RT>(a.kept, a.rows, row, col, cols, v);
+            }
+            hold(k, x);
+            add_up(x, s);
+        }
+        if (before) {
+            statistics(s, mean, rs);
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                if (8 * k * THREADS >= cols) break;
+                const uint32_t col = col_of(k);
+                float x[8];
+                Columns<DT> weight, bias;
+                weight.ask(a.weight, a.flags & kNormWeight32, 0, col, cols);
+                bias.ask(a.bias, a.flags & kNormBias32, 0, col, cols);
+                look(k, x);
+                weight.take(a.weight, a.flags & kNormWeight32, col, cols, 1.0f);
+                bias.take(a.bias, a.flags & kNormBias32, col, cols, 0.0f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = ElemIO<DT>::round((x[j] - mean) * rs * weight.v[j] + bias.v[j]);
+                store_row<DT>(row_of<DT>(a.h, base), col, cols, x);
+                if (a.h8) keep_row<DT>(a.h8, a.rows, row, col, cols, x);
+            }
+        }
+        if (a.stats && threadIdx.x == 0) reinterpret_cast<float4 *>(a.stats)[row] = make_float4(mean, rs, mean_y, rs_y);
     }
 }
 
@@ -392,16 +522,20 @@ template <int DT, int RT, int V, int THREADS, bool FULL, bool PASSING> __global_
 //
 // SUMS: which of them registers are kept for, at least those that are wanted.  Narrow rows are shared by fewer threads than a workgroup has: those that share one, a team, have a
 // run of rows each, and add up what they have of the columns before it leaves.
+struct RowMeans { // of g and g xhat, and of the norm of y likewise
+    float mean, mean_xhat, mean_after, mean_yhat;
+};
 enum { kSumWeight = 1, kSumBias = 2, kSumGate = 4, kSumAfterWeight = 8, kSumAfterBias = 16 };
 
-template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING> __global__ __launch_bounds__(THREADS, 4) void residual_norm_backward_kernel(BlockNormBackArgs a)
+template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING, bool WIDE> __global__ __launch_bounds__(THREADS, 4) void residual_norm_backward_kernel(BlockNormBackArgs a)
 {
     constexpr bool AHEAD = V == 1 && !(SUMS & ~(kSumWeight | kSumBias));
     constexpr bool AFTER = SUMS & (kSumAfterWeight | kSumAfterBias), BETWEEN = SUMS & ~(kSumWeight | kSumBias);
     __shared__ f32x2_t part[2][16];
     const uint32_t threads = a.flags >> 16, cols = a.cols;
     const bool center = a.flags & kNormCenter, after = AFTER && a.flags & kNormAfter;
-    const uint32_t team = V == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / threads) : 0, lane = threadIdx.x - team * threads;
+    const uint32_t team = V == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / threads) : 0, lane = threadIdx.x - team * threads + (WIDE ? blockIdx.x * threads : 0);
+    const uint32_t workgroup = WIDE ? blockIdx.y : blockIdx.x; // of those that share the rows
     GroupSums sums = {part, threads >> 6, team * (threads >> 6)};
     const float share = 1.0f / (float)cols;
     float acc[5][V][8];
@@ -415,12 +549,12 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
     for (int s = 0; s < 5; s++)
         if (SUMS >> s & 1) clear(s);
     // a team's rows: of one gate, or of whole ones
-    const uint32_t id = blockIdx.x * a.teams + team, of = a.parts > 1 ? id / a.parts : 0;
+    const uint32_t id = workgroup * a.teams + team, of = a.parts > 1 ? id / a.parts : 0;
     const uint32_t start = a.parts > 1 ? of * a.per + (id - of * a.parts) * a.run : id * a.run;
     const uint32_t end = min(start + a.run, a.parts > 1 ? (of + 1) * a.per : a.rows);
     uint32_t left = a.per;
-    // What the columns are multiplied by, in registers where they hold it all along (1 where there is no weight; 0 behind the last column, where nothing else need be).
-    constexpr bool HELD = V == 1 || (V == 2 && !BETWEEN);
+    // What the columns are multiplied by, in registers all along (1 where there is no weight; 0 behind the last column, where nothing else need be).
+    static_assert(V == 1 || !BETWEEN, "the vectors between r and y are held of eight columns");
     float weight[V][8], after_weight[V][8], gate[V][8];
     const auto load_weight = [&](const void *p, bool in32, int64_t base, uint32_t col, float (&v)[8]) {
         if (p) {
@@ -431,12 +565,10 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
             clip(v, lanes_own(col, cols));
         }
     };
-    if (HELD) {
 #pragma unroll
-        for (int k = 0; k < V; k++) load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * (lane + k * threads), weight[k]);
-        if (AFTER) load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, 8 * lane, after_weight[0]);
-        if (BETWEEN && a.gate) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(min(start, a.rows - 1) / a.per) * cols, 8 * lane, cols, gate[0]); // (a team may have no rows)
-    }
+    for (int k = 0; k < V; k++) load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * (lane + k * threads), weight[k]);
+    if (AFTER) load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, 8 * lane, after_weight[0]);
+    if (BETWEEN && a.gate) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(min(start, a.rows - 1) / a.per) * cols, 8 * lane, cols, gate[0]); // (a team may have no rows)
     const auto load_kept = [&](const void *p, auto &x, uint32_t row, uint32_t col, auto type) {
         constexpr int T = decltype(type)::value;
         if (EIGHT) {
@@ -465,12 +597,18 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
     struct Raw {
         uint32_t dh[V][kWords<DT>], dr[V][kWords<RT>], r[V][kWords<RT>], y[V][kWords<DT>];
         float4 stats;
+        RowMeans means;
+    };
+    const auto col_of = [&](int k) {
+        uint32_t mine = lane;
+        if (V > 1 || SUMS == 31 || (AFTER && RT == DQ_F32)) asm volatile("" : "+v"(mine));
+        return 8 * (mine + k * threads);
     };
     const auto load = [&](Raw &x, uint32_t row) {
         const int64_t base = (int64_t)row * cols;
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const uint32_t col = 8 * (lane + k * threads);
+            const uint32_t col = col_of(k);
             if (a.dh) {
                 load_row<DT, PASSING>(row_of<DT>(a.dh, base), col, cols, x.dh[k]);
                 load_kept(a.r, x.r[k], row, col, R());
@@ -479,6 +617,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
             if (BETWEEN && a.y) load_kept(a.y, x.y[k], row, col, Y());
         }
         x.stats = reinterpret_cast<const float4 *>(a.stats)[row];
+        if (WIDE) x.means = reinterpret_cast<const RowMeans *>(a.means)[row];
     };
     // what becomes of row start + i (as many for every team: they meet), while `next` is on its way
     const auto step = [&](Raw &now, Raw &next, uint32_t i) {
@@ -499,6 +638,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                 for (int w = 0; w < kWords<RT>; w++) now.dr[k][w] = now.r[k][w] = 0u;
             }
             now.stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            now.means = {0.0f, 0.0f, 0.0f, 0.0f};
         }
         const float4 stats = now.stats;
         float t[V][8];
@@ -506,9 +646,8 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
             float xhat[V][8], first = 0.0f, second = 0.0f;
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                kept_values(now.r[k], 8 * (lane + k * threads), xhat[k], R());
-                row_values<DT>(now.dh[k], 8 * (lane + k * threads), cols, t[k]);
-                if (!HELD) load_weight(a.weight, a.flags & kNormWeight32, 0, 8 * (lane + k * threads), weight[k]);
+                kept_values(now.r[k], col_of(k), xhat[k], R());
+                row_values<DT>(now.dh[k], col_of(k), cols, t[k]);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     xhat[k][j] = (xhat[k][j] - stats.x) * stats.y;
@@ -519,9 +658,14 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                     second += t[k][j] * xhat[k][j];
                 }
             }
-            sums(first, second);
-            first = center ? first * share : 0.0f;
-            second *= share;
+            if (WIDE) {
+                first = now.means.mean;
+                second = now.means.mean_xhat;
+            } else {
+                sums(first, second);
+                first = center ? first * share : 0.0f;
+                second *= share;
+            }
 #pragma unroll
             for (int k = 0; k < V; k++)
 #pragma unroll
@@ -534,7 +678,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
         }
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const uint32_t col = 8 * (lane + k * threads);
+            const uint32_t col = col_of(k);
             float v[8];
             if (a.dr) {
                 row_values<RT>(now.dr[k], col, cols, v);
@@ -553,7 +697,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
             float yhat[V][8], first = 0.0f, second = 0.0f;
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                const uint32_t col = 8 * (lane + k * threads);
+                const uint32_t col = col_of(k);
                 if (a.y) {
                     kept_values(now.y[k], col, yhat[k], Y());
                 } else {
@@ -563,7 +707,6 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                 if (after) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) yhat[k][j] = (yhat[k][j] - stats.z) * stats.w;
-                    if (!HELD) load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, col, after_weight[k]);
                 }
                 if (SUMS & kSumGate) {
 #pragma unroll
@@ -576,7 +719,6 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                     }
                 }
                 if (a.gate) {
-                    if (!HELD) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(min(row, a.rows - 1) / a.per) * cols, col, cols, gate[k]);
 #pragma unroll
                     for (int j = 0; j < 8; j++) t[k][j] *= gate[k][j];
                 }
@@ -592,9 +734,14 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                 }
             }
             if (after) {
-                sums(first, second);
-                first = center ? first * share : 0.0f;
-                second *= share;
+                if (WIDE) {
+                    first = now.means.mean_after;
+                    second = now.means.mean_yhat;
+                } else {
+                    sums(first, second);
+                    first = center ? first * share : 0.0f;
+                    second *= share;
+                }
 #pragma unroll
                 for (int k = 0; k < V; k++)
 #pragma unroll
@@ -603,7 +750,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
         }
         if (a.dy && there) {
 #pragma unroll
-            for (int k = 0; k < V; k++) store_row<DT>(row_of<DT>(a.dy, base), 8 * (lane + k * threads), cols, t[k]);
+            for (int k = 0; k < V; k++) store_row<DT>(row_of<DT>(a.dy, base), col_of(k), cols, t[k]);
         }
         if (SUMS & kSumGate && a.gate && --left == 0) { // the last row of a gate; where all of its rows are this team's, its gradient is whole
             left = a.per;
@@ -611,7 +758,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                 const int64_t to = (int64_t)(row / a.per) * cols;
 #pragma unroll
                 for (int k = 0; k < V; k++) {
-                    const uint32_t col = 8 * (lane + k * threads);
+                    const uint32_t col = col_of(k);
                     if (DT == DQ_F32 || a.flags & kNormGate32)
                         store_row<DQ_F32>(row_of<DQ_F32>(a.dgate, to), col, cols, acc[2][k]);
                     else
@@ -619,7 +766,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                 }
                 clear(2);
             }
-            if (HELD && row + 1 < end) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)((row + 1) / a.per) * cols, 8 * lane, cols, gate[0]);
+            if (row + 1 < end) load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)((row + 1) / a.per) * cols, 8 * lane, cols, gate[0]);
         }
     };
     Raw one, other;
@@ -636,7 +783,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
 #pragma unroll
     for (int s = 0; s < 5; s++) {
         if (!(SUMS >> s & 1) || !(a.sums >> s & 1) || (s == 2 && a.dgate)) continue;
-        char *to = row_of<DQ_F32>(a.work, ((int64_t)slot++ * a.grid + blockIdx.x) * cols);
+        char *to = row_of<DQ_F32>(a.work, ((int64_t)slot++ * a.grid + workgroup) * cols);
         if constexpr (V == 1 && THREADS == 512) {
             if (a.teams > 1) {
                 __shared__ float4 both[2][512];
@@ -646,7 +793,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
                 __syncthreads();
                 if (team == 0) {
                     for (uint32_t m = 1; m < a.teams; m++) {
-                        const float4 x = both[0][m * threads + lane], y = both[1][m * threads + lane];
+                        const float4 x = both[0][m * threads + threadIdx.x], y = both[1][m * threads + threadIdx.x];
                         acc[s][0][0] += x.x; acc[s][0][1] += x.y; acc[s][0][2] += x.z; acc[s][0][3] += x.w;
                         acc[s][0][4] += y.x; acc[s][0][5] += y.y; acc[s][0][6] += y.z; acc[s][0][7] += y.w;
                     }
@@ -660,6 +807,146 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
     }
 }
 
+// The means of rows that are too wide for a thread to hold its part of all arrays and sums: a workgroup goes over a row, and with a norm after the block over it again, from the cache.
+// Then the kernel above takes the columns in tiles of 512 (WIDE), a wave each with a run of rows: it meets nobody.  2048 x 14336 bf16 with both norms and a gate 72 us, bound by what
+// each element has to be unpacked and multiplied with more than by memory (3.3 TB/s; the same at 8 to 24 waves a CU, with one vector or two at a time), and 62 us (5.7 TB/s).
+template <int DT, int RT, bool EIGHT> __global__ __launch_bounds__(512, 4) void residual_norm_means_kernel(BlockNormBackArgs a)
+{
+    __shared__ f32x2_t part[2][16];
+    const uint32_t cols = a.cols;
+    const bool center = a.flags & kNormCenter, after = a.flags & kNormAfter;
+    const float share = 1.0f / (float)cols;
+    GroupSums sums = {part, 8, 0};
+    typedef std::integral_constant<int, DT> Y;
+    typedef std::integral_constant<int, RT> R;
+    const auto load_kept = [&](const void *p, auto &x, uint32_t row, uint32_t col, auto type) {
+        constexpr int T = decltype(type)::value;
+        if (EIGHT) {
+            const CheckpointOf<const uint8_t> c(static_cast<const uint8_t *>(p), a.rows, cols);
+            const uint32_t from = min(col, 32 * c.blocks - 8);
+            const u32x2_t w = *reinterpret_cast<const u32x2_t *>(c.codes + (int64_t)row * 32 * c.blocks + from);
+            x[0] = w[0];
+            x[1] = w[1];
+            x[2] = (c.scales + (int64_t)row * c.blocks)[from >> 5];
+        } else {
+            load_row<T>(row_of<T>(p, (int64_t)row * cols), col, cols, x);
+        }
+    };
+    const auto kept_values = [&](auto &x, uint32_t col, float (&v)[8], auto type) {
+        constexpr int T = decltype(type)::value;
+        if (EIGHT) {
+            const u32x2_t w = {x[0], x[1]};
+            decode_e4m3(w, x[2], v);
+            clip(v, lanes_own(col, cols));
+        } else {
+            row_values<T>(x, col, cols, v);
+        }
+    };
+    // 1 where there is no such vector, and 0 behind the last column
+    const auto load_weight = [&](const void *p, bool in32, int64_t base, uint32_t col, float (&v)[8]) {
+        if (p) {
+            load_columns<DT>(p, in32, base, col, cols, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = 1.0f;
+            clip(v, lanes_own(col, cols));
+        }
+    };
+    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t base = (int64_t)row * cols;
+        const float4 stats = reinterpret_cast<const float4 *>(a.stats)[row];
+        RowMeans means = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.dh) {
+            float first = 0.0f, second = 0.0f;
+            for (uint32_t at = 8 * threadIdx.x; at < cols; at += 8192) {
+                uint32_t dh[2][kWords<DT>], r[2][kWords<RT>];
+                float weight[2][8];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    load_row<DT>(row_of<DT>(a.dh, base), at + 4096 * k, cols, dh[k]);
+                    load_kept(a.r, r[k], row, at + 4096 * k, R());
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) load_weight(a.weight, a.flags & kNormWeight32, 0, at + 4096 * k, weight[k]);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    float g[8], xhat[8];
+                    row_values<DT>(dh[k], at + 4096 * k, cols, g);
+                    kept_values(r[k], at + 4096 * k, xhat, R());
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        g[j] *= weight[k][j];
+                        first += g[j];
+                        second += g[j] * ((xhat[j] - stats.x) * stats.y);
+                    }
+                }
+            }
+            sums(first, second);
+            means.mean = center ? first * share : 0.0f;
+            means.mean_xhat = second * share;
+        }
+        if (after) {
+            float first = 0.0f, second = 0.0f;
+            for (uint32_t at = 8 * threadIdx.x; at < cols; at += 8192) {
+                uint32_t dh[2][kWords<DT>], r[2][kWords<RT>], dr[2][kWords<RT>], y[2][kWords<DT>];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t col = at + 4096 * k;
+                    if (a.dh) {
+                        load_row<DT>(row_of<DT>(a.dh, base), col, cols, dh[k]);
+                        load_kept(a.r, r[k], row, col, R());
+                    }
+                    if (a.dr) load_row<RT>(row_of<RT>(a.dr, base), col, cols, dr[k]);
+                    if (a.y) load_kept(a.y, y[k], row, col, Y());
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t col = at + 4096 * k;
+                    float t[8], v[8];
+                    if (a.dh) {
+                        row_values<DT>(dh[k], col, cols, t);
+                        kept_values(r[k], col, v, R());
+                        float weight[8];
+                        load_weight(a.weight, a.flags & kNormWeight32, 0, col, weight);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) t[j] = (t[j] * weight[j] - means.mean - (v[j] - stats.x) * stats.y * means.mean_xhat) * stats.y;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) t[j] = 0.0f;
+                    }
+                    if (a.dr) {
+                        row_values<RT>(dr[k], col, cols, v);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) t[j] += v[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++) t[j] *= a.block_scale;
+                    if (a.gate) {
+                        load_columns<DT>(a.gate, a.flags & kNormGate32, (int64_t)(row / a.per) * cols, col, cols, v);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) t[j] *= v[j];
+                    }
+                    load_weight(a.after_weight, a.flags & kNormAfterWeight32, 0, col, v);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        t[j] *= v[j]; // (0 behind the last column)
+                        first += t[j];
+                    }
+                    if (a.y) {
+                        kept_values(y[k], col, v, Y());
+#pragma unroll
+                        for (int j = 0; j < 8; j++) second += t[j] * ((v[j] - stats.z) * stats.w);
+                    }
+                }
+            }
+            sums(first, second);
+            means.mean_after = center ? first * share : 0.0f;
+            means.mean_yhat = second * share;
+        }
+        if (threadIdx.x == 0) reinterpret_cast<RowMeans *>(a.means)[row] = means;
+    }
+}
+
 // ---- launches for one type of activations --------------------------------------------------------------------
 
 template <int DT, int RT> static hipError_t launch_norm_of(const BlockNormArgs &a, hipStream_t stream)
@@ -667,9 +954,9 @@ template <int DT, int RT> static hipError_t launch_norm_of(const BlockNormArgs &
     const uint32_t threads = a.flags >> 16;
     const dim3 grid(a.grid), block(threads);
     const bool full = a.gate || a.flags & kNormAfter, passing = a.flags & kNormPassing;
-    if (a.cols > 16384) return launch_with(residual_norm_kernel<DT, RT, 4, 1024, true, false>, grid, block, stream, a);
-    if (a.cols > 8192)
-        return full ? launch_with(residual_norm_kernel<DT, RT, 2, 1024, true, false>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 2, 1024, false, true>, grid, block, stream, a);
+    if (a.cols > 16384) return launch_with(residual_norm_wide_kernel<DT, RT, 1024>, grid, dim3(1024), stream, a);
+    if (a.cols > 8192 && full) return launch_with(residual_norm_wide_kernel<DT, RT, 512>, grid, dim3(512), stream, a);
+    if (a.cols > 8192) return launch_with(residual_norm_kernel<DT, RT, 2, 1024, false, true>, grid, block, stream, a);
     if (threads > 512)
         return full ? passing ? launch_with(residual_norm_kernel<DT, RT, 1, 1024, true, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 1024, true, false>, grid, block, stream, a)
                     : passing ? launch_with(residual_norm_kernel<DT, RT, 1, 1024, false, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 1024, false, false>, grid, block, stream, a);
@@ -677,26 +964,30 @@ template <int DT, int RT> static hipError_t launch_norm_of(const BlockNormArgs &
                 : passing ? launch_with(residual_norm_kernel<DT, RT, 1, 512, false, true>, grid, block, stream, a) : launch_with(residual_norm_kernel<DT, RT, 1, 512, false, false>, grid, block, stream, a);
 }
 
-template <int DT, int RT, int V, int THREADS, int SUMS> static hipError_t launch_norm_backward_with(const BlockNormBackArgs &a, hipStream_t stream)
+template <int DT, int RT, int V, int THREADS, int SUMS, bool WIDE = false> static hipError_t launch_norm_backward_with(const BlockNormBackArgs &a, hipStream_t stream)
 {
-    const dim3 grid(a.grid), block((a.flags >> 16) * a.teams);
+    const dim3 grid = WIDE ? dim3((a.cols + 511) / 512, a.grid) : dim3(a.grid), block((a.flags >> 16) * a.teams);
     if constexpr (V == 1) {
         if (a.flags & kNormPassing)
-            return a.flags & kNormEight ? launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, true, true>, grid, block, stream, a)
-                                        : launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, false, true>, grid, block, stream, a);
+            return a.flags & kNormEight ? launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, true, true, WIDE>, grid, block, stream, a)
+                                        : launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, false, true, WIDE>, grid, block, stream, a);
     }
-    return a.flags & kNormEight ? launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, true, false>, grid, block, stream, a)
-                                : launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, false, false>, grid, block, stream, a);
+    return a.flags & kNormEight ? launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, true, false, WIDE>, grid, block, stream, a)
+                                : launch_with(residual_norm_backward_kernel<DT, RT, V, THREADS, SUMS, false, false, WIDE>, grid, block, stream, a);
 }
 template <int DT, int RT> static hipError_t launch_norm_backward_of(const BlockNormBackArgs &a, hipStream_t stream)
 {
     // the block between r and y takes part only in kernels that keep sums of it
     const uint32_t want = a.sums | (a.gate ? kSumGate : 0) | (a.flags & kNormAfter ? kSumAfterWeight : 0);
     const auto within = [&](uint32_t of) { return !(want & ~of); };
-    if (a.cols > 16384) return within(3) ? launch_norm_backward_with<DT, RT, 4, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 4, 1024, 31>(a, stream);
-    if (a.cols > 8192)
-        return within(1) ? launch_norm_backward_with<DT, RT, 2, 1024, 1>(a, stream)
-             : within(3) ? launch_norm_backward_with<DT, RT, 2, 1024, 3>(a, stream) : launch_norm_backward_with<DT, RT, 2, 1024, 31>(a, stream);
+    if (a.means) {
+        const dim3 grid(std::min(a.rows, 1024u)), block(512); // (as many as the chip holds, and as many again)
+        const hipError_t e = a.flags & kNormEight ? launch_with(residual_norm_means_kernel<DT, RT, true>, grid, block, stream, a) : launch_with(residual_norm_means_kernel<DT, RT, false>, grid, block, stream, a);
+        if (e != hipSuccess) return e;
+        return within(3) ? launch_norm_backward_with<DT, RT, 1, 512, 3, true>(a, stream)
+             : within(13) ? launch_norm_backward_with<DT, RT, 1, 512, 13, true>(a, stream) : launch_norm_backward_with<DT, RT, 1, 512, 31, true>(a, stream);
+    }
+    if (a.cols > 8192) return within(1) ? launch_norm_backward_with<DT, RT, 2, 1024, 1>(a, stream) : launch_norm_backward_with<DT, RT, 2, 1024, 3>(a, stream);
     if (a.cols > 4096)
         return within(3) ? launch_norm_backward_with<DT, RT, 1, 1024, 3>(a, stream)
              : within(13) ? launch_norm_backward_with<DT, RT, 1, 1024, 13>(a, stream) : launch_norm_backward_with<DT, RT, 1, 1024, 31>(a, stream);

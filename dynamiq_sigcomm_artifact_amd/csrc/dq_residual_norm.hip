@@ -4,13 +4,17 @@
 
 namespace dq {
 
-// Threads of a row: eight elements each as far as 1024 of them go, then twice and four times eight.
+// Threads of a row that lies in registers: eight elements each as far as 1024 of them go, then twice eight.
 static uint32_t norm_threads(uint32_t cols)
 {
     const uint32_t vectors = (cols + 7) >> 3;
-    const uint32_t each = vectors <= 1024 ? 1 : vectors <= 2048 ? 2 : 4;
-    return ((vectors + each - 1) / each + 63) & ~63u;
+    const uint32_t each = vectors <= 1024 ? 1 : 2;
+    return std::min(((vectors + each - 1) / each + 63) & ~63u, 1024u);
 }
+
+// Rows of which a thread would have more than its registers hold: in LDS forward, and read twice backward.  2048 x 14336 bf16 with both norms and a gate, forward 63 us and backward 139
+// (registers that spill 90 and 344), 1000 x 32768 with one norm 50 and 80 (118 and 281); 4096 x 8192 with both norms and a gate would take 150 backward in place of 96.
+static bool norm_wide(uint32_t cols, bool between) { return cols > 16384 || (between && cols > 8192); }
 
 // Whether a pass' arrays, four or so, are more than half of the 256 MB cache: then its loads carry the hint that nothing of them is wanted again soon.
 static bool norm_passing(int64_t rows, uint32_t cols, int dtype) { return rows * cols * 4 * (dtype == DQ_F32 ? 4 : 2) > (int64_t)128 << 20; }
@@ -20,20 +24,23 @@ hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t st
     a.flags |= norm_threads(a.cols) << 16;
     if (norm_passing(a.rows, a.cols, dtype)) a.flags |= kNormPassing;
     // workgroups that the chip holds at once, sixteen waves a CU, with as many rows each
-    const uint32_t held = 256 * (1024 / norm_threads(a.cols)), turns = (a.rows + held - 1) / held;
+    const bool halves = a.cols <= 16384 && norm_wide(a.cols, a.gate || a.flags & kNormAfter); // half a CU's LDS each
+    const uint32_t held = 256 * (halves ? 2 : 1024 / norm_threads(a.cols)), turns = (a.rows + held - 1) / held;
     a.grid = (a.rows + turns - 1) / turns;
     return dtype == DQ_F32 ? launch_norm_f32(a, stream32, stream) : dtype == DQ_BF16 ? launch_norm_bf16(a, stream32, stream) : launch_norm_f16(a, stream32, stream);
 }
 
 // How a backward pass shares its rows out.  As many workgroups as the chip holds at once, two a CU, or one of a thousand threads (1024 x 8192 in 20 us, with two in turn 26); more
-// would leave more sums to add up, fewer take longer than what that saves (with at least 4, 8 or 16 rows each 1024 x 4096 takes 1 % less, 7 and 60 % more).  Teams of as many threads as a row takes, up to 512 together in a workgroup, have runs of `run` rows -- `parts` of them (the last ones
-// shorter) to the rows of a gate, all of a workgroup's of the same one, or one of whole gates.
-NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols)
+// would leave more sums to add up, fewer take longer than what that saves (with at least 4, 8 or 16 rows each 1024 x 4096 takes 1 % less, 7 and 60 % more).  Teams of as many threads as
+// a row takes, or the 64 of a tile of a wide one, up to 512 together in a workgroup, have runs of `run` rows -- `parts` of them (the last ones shorter) to the rows of a gate, all of a
+// workgroup's of the same one, or one of whole gates.
+NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols, bool between)
 {
     NormShares s;
-    const uint32_t threads = norm_threads(cols);
+    s.wide = norm_wide(cols, between);
+    const uint32_t threads = s.wide ? 64 : norm_threads(cols), tiles = s.wide ? (cols + 511) / 512 : 1;
     s.teams = std::max(1u, 512 / threads);
-    const int64_t runs = (threads > 512 ? 256 : 512) * (int64_t)s.teams;
+    const int64_t runs = std::max(1u, (threads > 512 ? 256 : 512) / tiles) * (int64_t)s.teams;
     int64_t run = (rows + runs - 1) / runs;
     if (per == 0 || per <= run) {
         if (per) run = run / per * per;
@@ -94,8 +101,10 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSums a)
 
 hipError_t launch_norm_backward(BlockNormBackArgs a, const NormSum (&sums)[5], int dtype, bool stream32, hipStream_t stream)
 {
-    const NormShares s = norm_shares(a.rows, a.gate ? a.per : 0, a.cols);
-    a.flags |= norm_threads(a.cols) << 16;
+    const NormShares s = norm_shares(a.rows, a.gate ? a.per : 0, a.cols, a.gate || a.flags & kNormAfter);
+    a.flags |= (s.wide ? 64 : norm_threads(a.cols)) << 16;
+    a.means = s.wide ? a.work : nullptr;
+    a.work += s.wide ? 4 * (int64_t)a.rows : 0;
     if (norm_passing(a.rows, a.cols, dtype)) a.flags |= kNormPassing;
     a.grid = s.grid;
     a.teams = s.teams;

@@ -498,3 +498,77 @@ def test_behind_the_results(act):
         grads = dict(zip(leaf, torch.autograd.grad((h, r), list(leaf.values()), (dh, dr))))
         for k, v in {"h": h, "r": r, "h8": c.data, **{"d" + k: g for k, g in grads.items()}}.items():
             assert torch.equal(buffers[k][32:32 + sizes[k]].view(v.shape), v), k
+
+
+@pytest.mark.parametrize("shape,gate", [((6, 8200), (6, 8200)), ((2, 3, 9001), (2, 1, 9001)), ((130, 2, 8195), (130, 1, 8195)), ((500, 8193), (500, 8193)), ((1, 32768), (32768,)), ((3, 16400), (16400,))])
+@pytest.mark.parametrize("after", [False, True])
+@pytest.mark.parametrize("eight", [False, True])
+def test_wide_gates(act, shape, gate, after, eight):
+    """rows that are wider than registers hold, whose gates are of one row, of some, of all"""
+    if eight:
+        shape, gate = (shape[0] * (shape[1] if len(shape) == 3 else 1), shape[-1]), gate[-1:]
+    t = tensors(shape, BF, FP, ("residual", "weight", "bias") + ("after_weight",) * after, 3, gate=gate)
+    against_definition(act, t, True, True, after=after, eight=eight, center=True)
+
+
+def test_wide_parts(act):
+    """whatever takes part, and whatever does not, in such rows"""
+    rng = random.Random(6)
+    for case in range(24):
+        after, before, center, eight = rng.random() < 0.7, rng.random() < 0.7, rng.random() < 0.5, rng.random() < 0.5
+        dtype, stream = rng.choice(((BF, BF), (BF, FP), (HF, HF), (HF, FP), (FP, FP)))
+        parts = [p for p in ALL if rng.random() < 0.6 and (after or "after" not in p) and (before or p not in ("weight", "bias"))]
+        rows, cols = rng.choice(((1, 8201), (7, 9000), (3, 16385), (2, 20003)))
+        gate = rng.choice((None, (cols,), (rows, cols)))
+        t = tensors((rows, cols), dtype, stream, parts, 10 * case, rng.choice((None, FP)), gate)
+        plain = "residual" not in parts and gate is None and not after
+        which = rng.choice(((True, True), (True, False), (False, True))) if before else (False, True)
+        if plain and before and which == (False, True):
+            which = (True, True)
+        against_definition(act, t, *which, eight=eight, after=after, before=before, center=center, residual_scale=0.7, block_scale=1.0 if plain else 0.5)
+
+
+def test_wide_rows_keep_apart(act):
+    """a row with what is no number, or beyond the largest, makes no other row so"""
+    t = tensors((5, 9003), BF, BF, ("residual", "weight", "after_weight"), 4, gate=(5, 9003))
+    dh, dr = normal((5, 9003), BF, 5), normal((5, 9003), BF, 6)
+
+    def run():
+        leaf = {k: v.clone().requires_grad_() for k, v in t.items()}
+        h, r = act.residual_norm(leaf["y"], leaf["residual"], leaf["weight"], gate=leaf["gate"], after=True, after_weight=leaf["after_weight"])
+        return [h.detach(), r.detach(), *torch.autograd.grad((h, r), [leaf[k] for k in ("y", "residual", "gate")], (dh, dr))]
+    clean = run()
+    t["y"][1, 77], t["residual"][3, 9002] = float("nan"), float("inf")
+    for a, b in zip(clean, run()):
+        assert torch.equal(a[[0, 2, 4]], b[[0, 2, 4]])
+        assert not torch.isfinite(b[[1, 3]]).all()
+
+
+def test_wide_work(act):
+    """the work buffer of such rows: nothing is written outside of it, and one that is smaller is refused"""
+    from dynamiq_sigcomm_artifact_amd import capi
+    L, s = capi.lib(), torch.cuda.current_stream().cuda_stream
+    for rows, cols, gate in ((9, 8200, (8200,)), (9, 16392, None), (600, 8200, (600, 8200))):
+        t = tensors((rows, cols), BF, BF, ("residual", "weight"), 1, gate=gate)
+        leaf = {k: v.detach().requires_grad_() for k, v in t.items()}
+        h, r = act.residual_norm(leaf["y"], leaf["residual"], leaf["weight"], gate=leaf.get("gate"), eps=1e-5)
+        dh, dr = normal((rows, cols), BF, 2), normal((rows, cols), BF, 3)
+        want = dict(zip(leaf, torch.autograd.grad((h, r), list(leaf.values()), (dh, dr))))
+        stats = torch.empty(rows, 4, device=DEV)
+        h2, r2 = torch.empty_like(h), torch.empty_like(r)
+        got = {k: torch.empty_like(v) for k, v in want.items()}
+        both = dict({k: v.data_ptr() for k, v in t.items()}, rows=rows, cols=cols, rows_per_gate=rows // (gate[0] if gate and len(gate) == 2 else 1), eps=1e-5, residual_scale=1.0, block_scale=1.0,
+                    dtype=1, stream_dtype=1, before=1, stats=stats.data_ptr(), r=r2.data_ptr())
+        assert L.dq_residual_norm_forward(ctypes.byref(capi.ResidualNorm(**both, h=h2.data_ptr())), 0, s) == 0, L.dq_last_error()
+        o = capi.ResidualNorm(**both, dh=dh.data_ptr(), dr=dr.data_ptr(), dy=got["y"].data_ptr(), dresidual=got["residual"].data_ptr(), dweight=got["weight"].data_ptr(),
+                              dgate=got["gate"].data_ptr() if gate else None)
+        n = L.dq_residual_norm_work_floats(ctypes.byref(o))
+        work = torch.full((n + 64,), 77.0, device=DEV)
+        o.work, o.work_floats = work.data_ptr() + 128, n - 1
+        assert L.dq_residual_norm_backward(ctypes.byref(o), 0, s) != 0 and b"too small" in L.dq_last_error()
+        o.work_floats = n
+        assert L.dq_residual_norm_backward(ctypes.byref(o), 0, s) == 0, L.dq_last_error()
+        assert bool((work[:32] == 77).all()) and bool((work[-32:] == 77).all())
+        assert torch.equal(h2, h) and torch.equal(r2, r)
+        for k in want:
+            assert torch.equal(got[k], want[k]), k
