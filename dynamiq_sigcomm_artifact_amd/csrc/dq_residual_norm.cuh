@@ -810,6 +810,7 @@ template <int DT, int RT, int V, int THREADS, int SUMS, bool EIGHT, bool PASSING
 // The means of rows that are too wide for a thread to hold its part of all arrays and sums: a workgroup goes over a row, and with a norm after the block over it again, from the cache.
 // Then the kernel above takes the columns in tiles of 512 (WIDE), a wave each with a run of rows: it meets nobody.  2048 x 14336 bf16 with both norms and a gate 72 us, bound by what
 // each element has to be unpacked and multiplied with more than by memory (3.3 TB/s; the same at 8 to 24 waves a CU, with one vector or two at a time), and 62 us (5.7 TB/s).
+constexpr uint32_t kMeansGrid = 1024; // as many as the chip holds, and as many again
 template <int DT, int RT, bool EIGHT> __global__ __launch_bounds__(512, 4) void residual_norm_means_kernel(BlockNormBackArgs a)
 {
     __shared__ f32x2_t part[2][16];
@@ -852,7 +853,7 @@ template <int DT, int RT, bool EIGHT> __global__ __launch_bounds__(512, 4) void 
             clip(v, lanes_own(col, cols));
         }
     };
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    for (uint32_t row = blockIdx.x; row < a.rows; row += kMeansGrid) {
         const int64_t base = (int64_t)row * cols;
         const float4 stats = reinterpret_cast<const float4 *>(a.stats)[row];
         RowMeans means = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -981,7 +982,7 @@ template <int DT, int RT> static hipError_t launch_norm_backward_of(const BlockN
     const uint32_t want = a.sums | (a.gate ? kSumGate : 0) | (a.flags & kNormAfter ? kSumAfterWeight : 0);
     const auto within = [&](uint32_t of) { return !(want & ~of); };
     if (a.means) {
-        const dim3 grid(std::min(a.rows, 1024u)), block(512); // (as many as the chip holds, and as many again)
+        const dim3 grid(std::min(a.rows, kMeansGrid)), block(512);
         const hipError_t e = a.flags & kNormEight ? launch_with(residual_norm_means_kernel<DT, RT, true>, grid, block, stream, a) : launch_with(residual_norm_means_kernel<DT, RT, false>, grid, block, stream, a);
         if (e != hipSuccess) return e;
         return within(3) ? launch_norm_backward_with<DT, RT, 1, 512, 3, true>(a, stream)
