@@ -572,3 +572,33 @@ def test_wide_work(act):
         assert torch.equal(h2, h) and torch.equal(r2, r)
         for k in want:
             assert torch.equal(got[k], want[k]), k
+
+
+def test_wide_graph(act):
+    """two graphs of such rows, each with its own workspace, between the program's own work"""
+    t = tensors((70, 8300), BF, FP, ALL, 1, gate=(70, 8300))
+    dh, dr = normal((70, 8300), BF, 2), normal((70, 8300), FP, 3)
+
+    def work():
+        leaf = {k: v.detach().requires_grad_() for k, v in t.items()}
+        h, r, c = act.residual_norm(leaf["y"], leaf["residual"], leaf["weight"], leaf["bias"], gate=leaf["gate"], after=True, after_weight=leaf["after_weight"],
+                                    after_bias=leaf["after_bias"], checkpoint=True)
+        return [h.detach(), r.detach(), c.data] + list(torch.autograd.grad((h, r), list(leaf.values()), (dh, dr)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(work())
+    for k in range(4):
+        t["y"].normal_()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = work()
+        for out in outs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want)), k
+        torch.cuda.synchronize()
