@@ -1667,6 +1667,7 @@ struct GatedOf : public torch::autograd::Function<GatedOf> {
         o.out = out.data_ptr();
         if (o.rows && o.cols) check(dq_gated_forward(&o, x.device().index(), c10::hip::getCurrentHIPStream(x.device().index()).stream()));
         if (kept) {
+            ctx->set_materialize_grads(false); // (the engine would fill one of the checkpoint's size, which nobody reads)
             if (eight)
                 ctx->save_for_backward({keep});
             else if (up)

@@ -284,3 +284,19 @@ def test_c_interface_writes_where_it_is_told(act):
     o = capi.Gated(gate=g.data_ptr(), up=u.data_ptr(), gate_stride=c, up_stride=c, out=da.data_ptr(), dgate=room.data_ptr() + 6, dgate_stride=100, rows=r, cols=c, dtype=1, kind=0)
     assert L.dq_gated_backward(ctypes.byref(o), 0, s) == 0
     assert torch.equal(room[:, 3:40], want[0]) and bool((room[:, :3] == 7).all()) and bool((room[:, 40:] == 7).all())
+
+
+def test_backward_makes_its_gradients_and_no_more(act):
+    """what a backward pass takes of memory beside its results: nothing of the checkpoint's size"""
+    x, da = normal((2048, 4096), BF, 1).requires_grad_(), normal((2048, 2048), BF, 2)
+    for up in (None, normal((2048, 4096), BF, 3).requires_grad_()):
+        d = da if up is None else normal((2048, 4096), BF, 4)
+        a, c = act.gated(x, up, checkpoint=True)
+        leaves = [x] if up is None else [x, up]
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(a, leaves, d)
+        peak = torch.cuda.max_memory_allocated() - before
+        assert peak <= sum(g.numel() * 2 for g in grads) + 65536
+        del a, c, grads
