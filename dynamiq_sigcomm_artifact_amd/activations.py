@@ -75,7 +75,7 @@ def residual_norm(y, residual=None, weight=None, bias=None, gate=None, residual_
 
     -> (h, r), r being y itself where nothing is added to it or done with it; r alone without ``before``.
     checkpoint: (h, r, c) with c the Checkpoint of h, for the layers that take it, and the backward pass keeps r and y in 8 bits.
-    What is not contiguous is copied.  The gradients cannot be differentiated again."""
+    What is not contiguous is copied.  The gradients cannot be differentiated again, and there is no forward mode."""
     h, r, data = capi.host().residual_norm(y, residual, weight, bias, gate, after_weight, after_bias, residual_scale, block_scale, eps, after, before, center, checkpoint)
     if not before:
         return r
@@ -93,7 +93,7 @@ def gated(x, up=None, kind="silu", checkpoint=False):
 
     kind: "silu", g sigmoid(g), or "gelu_tanh", g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3)) = g / 2 (1 + tanh(...)).
     checkpoint: also the Checkpoint of the result, for the layers that take it -- the answer is (out, Checkpoint) -- and the backward pass keeps gate and up in 8 bits.
-    The gradients cannot be differentiated again."""
+    The gradients cannot be differentiated again, and there is no forward mode."""
     if kind not in _KINDS:
         raise RuntimeError("gated: unknown activation %r" % (kind,))
     out, data = capi.host().gated(x, up, _KINDS[kind], checkpoint)

@@ -1558,6 +1558,13 @@ void leaves_can_be_recorded(const char *what, const c10::Device &device, std::in
     }
 }
 
+// A tensor with a tangent need not require a gradient, and where nothing does no node is made that would refuse it: the tangent would be dropped without a word.
+void no_tangents(const char *what, std::initializer_list<const at::Tensor *> tensors)
+{
+    for (const at::Tensor *t : tensors)
+        if (t->_fw_grad(0).defined()) refuse(std::string(what) + ": there are no derivatives in forward mode");
+}
+
 // x, weight, signs of the outputs and of the tokens, pools of the gradient's rows and columns, seed (None: no random stream), step, checkpoint (None, True or the data of one)
 PyObject *mx4_linear(PyObject *, PyObject *const *v, Py_ssize_t have)
 {
@@ -1738,6 +1745,7 @@ PyObject *gated(PyObject *, PyObject *const *v, Py_ssize_t have)
         }
         need(x.dim() >= 1 && (up || x.size(-1) % 2 == 0), "gated: x [..., 2 cols], or two tensors, are required");
         const bool eight = PyObject_IsTrue(v[3]), kept = at::GradMode::is_enabled() && (x.requires_grad() || (up && up->requires_grad()));
+        no_tangents("gated", {&x, up ? &*up : &x});
         leaves_can_be_recorded("gated", x.device(), {&x, up ? &*up : &x});
         const torch::autograd::variable_list out = kept ? GatedOf::apply(x, up, integer(v[2]), eight, true) : GatedOf::forward(nullptr, x, up, integer(v[2]), eight, false);
         const py::object a = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[0]));
@@ -1939,7 +1947,9 @@ PyObject *residual_norm(PyObject *, PyObject *const *v, Py_ssize_t have)
             need(fits, "residual_norm: a gate is [cols], or of y's shape with ones in place of the dimensions, the last of them before cols, that share it");
             s.per = rows ? rows / (gate.numel() / cols) : 1;
         }
-        leaves_can_be_recorded("residual_norm", y.device(), {&y, in[1] ? &*in[1] : &y, in[2] ? &*in[2] : &y, in[3] ? &*in[3] : &y, in[4] ? &*in[4] : &y, in[5] ? &*in[5] : &y, in[6] ? &*in[6] : &y});
+        const std::initializer_list<const at::Tensor *> inputs = {&y, in[1] ? &*in[1] : &y, in[2] ? &*in[2] : &y, in[3] ? &*in[3] : &y, in[4] ? &*in[4] : &y, in[5] ? &*in[5] : &y, in[6] ? &*in[6] : &y};
+        no_tangents("residual_norm", inputs);
+        leaves_can_be_recorded("residual_norm", y.device(), inputs);
         const torch::autograd::variable_list out = any ? F::apply(y, in[1], in[2], in[3], in[4], in[5], in[6], s) : F::forward(nullptr, y, in[1], in[2], in[3], in[4], in[5], in[6], s);
         const bool plain = !in[F::RESIDUAL] && !in[F::GATE] && !s.after && s.block_scale == 1.0;
         size_t next = 0;

@@ -300,3 +300,19 @@ def test_backward_makes_its_gradients_and_no_more(act):
         peak = torch.cuda.max_memory_allocated() - before
         assert peak <= sum(g.numel() * 2 for g in grads) + 65536
         del a, c, grads
+
+
+def test_forward_mode_is_refused(act):
+    """a tangent is not dropped without a word, whoever else wants a gradient"""
+    import torch.autograd.forward_ad as forward
+    g, u, t = normal((4, 64), BF, 1), normal((4, 64), BF, 2), normal((4, 64), BF, 3)
+    with forward.dual_level():
+        dual = forward.make_dual(g, t)
+        for wanted in (False, True):
+            other = u.clone().requires_grad_(wanted)
+            for call in (lambda: act.gated(dual), lambda: act.gated(dual, checkpoint=True), lambda: act.gated(dual, other), lambda: act.gated(other, dual), lambda: act.gated(dual.view(2, 2, 64))):
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                    call()
+        assert torch.equal(act.gated(forward.unpack_dual(dual).primal, u), act.gated(g, u))

@@ -602,3 +602,25 @@ def test_wide_graph(act):
         for out in outs:
             assert all(torch.equal(p, q) for p, q in zip(out, want)), k
         torch.cuda.synchronize()
+
+
+def test_forward_mode_is_refused(act):
+    """a tangent of any input is not dropped without a word, whoever else wants a gradient"""
+    import torch.autograd.forward_ad as forward
+    t = tensors((6, 64), BF, FP, ALL, 1, gate=(64,))
+
+    def call(t):
+        return act.residual_norm(t["y"], t["residual"], t["weight"], t["bias"], gate=t["gate"], after=True, after_weight=t["after_weight"], after_bias=t["after_bias"])
+    with forward.dual_level():
+        for name in t:
+            for wanted in (False, True):
+                mine = {k: v.detach().requires_grad_(wanted) for k, v in t.items()}
+                mine[name] = forward.make_dual(t[name], torch.ones_like(t[name]))
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call(mine)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                    call(mine)
+        plain = forward.make_dual(t["y"], torch.ones_like(t["y"]))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            act.residual_norm(plain)
+        call(t)
