@@ -1314,6 +1314,7 @@ static int norm_ok(const dq_residual_norm_t *o)
     if (!(o->eps >= 0) || !__builtin_isfinite(o->eps) || !__builtin_isfinite(o->residual_scale) || !__builtin_isfinite(o->block_scale))
         return fail(DQ_ERR_SIZE, "eps must be a number and not negative, the scales numbers");
     if ((o->keep_r || o->keep_y) && !o->kept) return fail(DQ_ERR_NULL);
+    if ((o->h8 || o->keep_r || o->keep_y) && !checkpoint_size_ok(o->rows, o->cols)) return fail(DQ_ERR_SIZE, kCheckpointSizes);
     if ((reinterpret_cast<uintptr_t>(o->h8) | reinterpret_cast<uintptr_t>(o->kept) | reinterpret_cast<uintptr_t>(o->stats)) & 15)
         return fail(DQ_ERR_SIZE, "checkpoints and stats must be 16-byte aligned");
     return 0;

@@ -925,7 +925,7 @@ int dq_gated_backward(const dq_gated_t *gated, int device, dq_stream_t stream);
  * gradient; every result that is not wanted.
  * 8 bits: h8 takes the checkpoint of h as it is stored, kept those of r as it is stored (keep_r) and, at the next
  * multiple of 16 bytes, of y (keep_y): the backward pass reads them where keep_r or keep_y is set, in place of r
- * and y.  It needs r with `before`, y with `after` and for dgate.
+ * and y.  It needs r with `before`, y with `after` and for dgate.  rows and cols within a checkpoint's limits then.
  * Where r is y, the backward pass takes it as r. */
 typedef struct dq_residual_norm {
     const void *y, *residual;                               /* [rows][cols]: dtype, stream_dtype */

@@ -156,3 +156,22 @@ def test_residual_norm_refuses(L):
     for rows in (1, 2, 1000, 4097, 100003):
         for per in (1, rows):
             assert 0 < room(rows=rows, gate=0x1000, dgate=0x1000, rows_per_gate=per) <= 2 * 40 * min(rows, 2048)
+
+
+def test_residual_norm_refuses_checkpoints_beyond_their_size(L):
+    """one of 2^35 elements, which no reader of a checkpoint takes; what keeps nothing in 8 bits has no such limit"""
+    from dynamiq_sigcomm_artifact_amd import capi
+    both = dict(y=0x1000, residual=0x1000, r=0x1000, rows=1 << 20, cols=32768, eps=1e-5, residual_scale=1.0, block_scale=1.0, dtype=1, stream_dtype=1, before=1)
+    forward = dict(both, h=0x1000)
+    backward = dict(both, stats=0x1000, dh=0x1000, dr=0x1000, dy=0x1000, dweight=0x1000, work=0x1000, work_floats=1 << 40)
+
+    def call(fn, base, **kw):
+        return fn(ctypes.byref(capi.ResidualNorm(**{**base, **kw})), 0, S)
+    for kw in (dict(h8=0x1000), dict(keep_r=1, kept=0x1000), dict(after=1, keep_y=1, kept=0x1000), dict(after=1, keep_r=1, keep_y=1, kept=0x1000)):
+        refused(L, call(L.dq_residual_norm_forward, forward, **kw), "2^35")
+        if "kept" in kw:
+            refused(L, call(L.dq_residual_norm_backward, backward, **kw), "2^35")
+            assert L.dq_residual_norm_work_floats(ctypes.byref(capi.ResidualNorm(**{**backward, **kw}))) == -1
+    assert L.dq_residual_norm_work_floats(ctypes.byref(capi.ResidualNorm(**backward))) > 0
+    small = dict(backward, rows=(1 << 20) - 1, after=1, keep_r=1, keep_y=1, kept=0x1000)
+    assert L.dq_residual_norm_work_floats(ctypes.byref(capi.ResidualNorm(**small))) > 0
