@@ -89,7 +89,7 @@ _KINDS = {"silu": 0, "gelu_tanh": 1}
 
 def gated(x, up=None, kind="silu", checkpoint=False):
     """act(gate) * up, [..., cols]: gate and up are the halves of x [..., 2 cols], side by side as a linear layer with both weights gives them, or x and up, of one shape.
-    Views whose elements of a row are consecutive are read in place, others are copied.
+    Views whose elements of a row are consecutive, and whose rows lie one distance apart, are read in place, others are copied.
 
     kind: "silu", g sigmoid(g), or "gelu_tanh", g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3)) = g / 2 (1 + tanh(...)).
     checkpoint: also the Checkpoint of the result, for the layers that take it -- the answer is (out, Checkpoint) -- and the backward pass keeps gate and up in 8 bits.

@@ -1282,12 +1282,13 @@ const uint8_t *checkpoint_of(const at::Tensor &data, int64_t rows, int64_t cols)
     return static_cast<const uint8_t *>(data.data_ptr());
 }
 
-// x as rows of consecutive elements (a matrix whose rows are apart is taken as it is)
+// x as rows of consecutive elements: views whose rows are apart, by one distance, are taken as they are
 at::Tensor as_rows(const at::Tensor &x)
 {
-    if (x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1) && (x.stride(0) >= x.size(1) || x.size(0) <= 1)) return x;
-    const int64_t cols = x.size(-1);
-    return x.reshape({c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)), cols}).contiguous();
+    const auto apart = [](const at::Tensor &t) { return (t.stride(1) == 1 || t.size(1) <= 1) && (t.stride(0) >= t.size(1) || t.size(0) <= 1); };
+    if (x.dim() == 2 && apart(x)) return x;
+    const at::Tensor rows = x.reshape({c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)), x.size(-1)}); // (a view where there is one)
+    return apart(rows) ? rows : rows.contiguous();
 }
 int64_t row_stride(const at::Tensor &x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
 

@@ -302,3 +302,16 @@ def test_graph_and_streams(act, ms, capi):
         want = step(k)
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         torch.cuda.synchronize()
+
+
+def test_views_of_a_batch_are_read_in_place(act):
+    """views with consecutive rows of more dimensions than two: right, and nothing of their size is made beside the result"""
+    big = matrix(24, 400, BF, 4).view(2, 3, 4, 400)
+    for x in (big[..., 8:300], big[..., :257], big[:, :, ::2], big.transpose(0, 1)[..., 3:90], big[..., ::3], big[:1, :1, :1, :33], big[:, :1].expand(2, 3, 4, 400)):
+        same(act.compress(x), x.contiguous())
+    x = matrix(2048, 4096, BF, 5).view(8, 256, 4096)[..., :2048]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    c = act.compress(x)
+    assert torch.cuda.max_memory_allocated() - before <= c.data.numel() + 65536

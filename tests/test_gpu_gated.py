@@ -316,3 +316,30 @@ def test_forward_mode_is_refused(act):
                 with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
                     call()
         assert torch.equal(act.gated(forward.unpack_dual(dual).primal, u), act.gated(g, u))
+
+
+def test_halves_of_a_batch_are_read_in_place(act):
+    """as two tensors, each a view with consecutive rows of more dimensions than two: right, and nothing of their size is made beside the results"""
+    x, da = normal((3, 5, 140), BF, 1), normal((3, 5, 70), BF, 2)
+    for gate, up in (x.chunk(2, -1), normal((3, 5, 300), BF, 3)[:, :, 8:288].chunk(2, -1), [v.transpose(0, 1) for v in normal((5, 3, 280), BF, 4).chunk(2, -1)],
+                     normal((3, 10, 280), BF, 5)[:, ::2].chunk(2, -1), normal((3, 5, 560), BF, 6)[:, :, ::2].chunk(2, -1), normal((1, 1, 280), BF, 7).expand(3, 5, 280).chunk(2, -1)):
+        d = da if gate.shape[-1] == 70 else normal(gate.shape, BF, 8)
+        for eight in (False, True):
+            against_definition(act, None, d, "silu", eight, gate, up)
+        assert torch.equal(act.gated(gate, up), act.gated(gate.contiguous(), up.contiguous()))
+    x, da = normal((8, 256, 4096), BF, 1), normal((8, 256, 2048), BF, 2)
+    for eight in (False, True):
+        gate, up = (v.detach().requires_grad_() for v in x.chunk(2, -1))
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = act.gated(gate, up, checkpoint=eight)
+        held = torch.cuda.memory_allocated() - before
+        assert torch.cuda.max_memory_allocated() - before == held
+        a = got[0] if eight else got
+        assert held <= a.numel() * 2 + eight * 3 * (a.numel() * 33 // 32) + 65536
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(a, (gate, up), da)
+        assert torch.cuda.max_memory_allocated() - before <= 2 * 2 * a.numel() + 65536
+        del got, a, grads
