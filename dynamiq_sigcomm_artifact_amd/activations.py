@@ -68,7 +68,8 @@ def residual_norm(y, residual=None, weight=None, bias=None, gate=None, residual_
       r = residual_scale * residual + block_scale * gate * z
       h = norm(r) * weight + bias                 the norm before the next block, unless ``before`` is False
 
-    norm(x) = x / sqrt(mean(x^2) + eps), or with ``center`` (x - mean(x)) / sqrt(variance(x) + eps), in float32: elements from 10^18 on give NaN.  Everything but y may be missing.
+    norm(x) = x / sqrt(mean(x^2) + eps), or with ``center`` (x - mean(x)) / sqrt(variance(x) + eps), in float32: a row whose squares add up to 2^128 or more
+    gives NaN (10^17 in every element of the widest row, 6 10^18 in the narrowest).  Everything but y may be missing.
 
     residual: of y's shape; its type, y's or float32, is r's.  gate: [cols], or of y's shape with ones in place of the last dimensions that share it: [batch, 1, cols] is a gate
     for each sequence.  weights, biases, gate: of y's type or float32, and so are their gradients.  cols: 8 to 32768.

@@ -914,7 +914,8 @@ int dq_gated_backward(const dq_gated_t *gated, int device, dq_stream_t stream);
  *   r = residual_scale residual + block_scale gate z
  *   h = norm(r) with weight and bias, where `before` (the next block) is set
  * norm(x) = x / sqrt(mean(x^2) + eps) w + b, or with `center` (x - mean) / sqrt(variance + eps) w + b.
- * In binary32 (a row whose mean square, eps included, lies outside of [2^-126, 2^128) may come out as NaN): r is
+ * In binary32: a row whose squares (with `center` those of the distances from the mean, or the elements) add up to
+ * 2^128 or more, or whose mean square, eps included, is below 2^-126, may come out as NaN.  r is
  * rounded once where it is stored, h once, from the unrounded r.  Backward, with the mean and
  * 1 / sqrt(..) that the forward pass has left in stats:
  *   dr' = dr + the norm's part of dh,  dresidual = residual_scale dr',  t = block_scale dr',  dgate = sum t z,

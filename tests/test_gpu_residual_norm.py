@@ -624,3 +624,20 @@ def test_forward_mode_is_refused(act):
         with pytest.raises(RuntimeError, match="forward mode"):
             act.residual_norm(plain)
         call(t)
+
+
+@pytest.mark.parametrize("cols", [90, 513, 4096, 8192, 9000, 16400, 32768])
+def test_rows_near_the_largest_sum_of_squares(act, cols):
+    """rows whose squares add up to somewhat less than 2^128, at every width, are like others; from there on they are NaN, and their neighbours are not"""
+    for dtype, parts, kw in ((FP, ("weight",), {}), (BF, ("weight",), {"center": True}), (FP, ("residual", "weight", "after_weight"), {"after": True})):
+        t = tensors((6, cols), dtype, dtype, parts, 1)
+        v = t["y"].double()
+        # (a norm takes the squares of y, and the other those of r: the same here, as the residual is small beside them)
+        t["y"] = (v * (0.9 * 2.0 ** 64 / v.square().sum(-1, keepdim=True).sqrt())).to(dtype)
+        if "after" not in kw:
+            against_definition(act, t, True, False, eps=0.0, **kw)
+        else:
+            against_definition(act, t, True, True, eps=1e-5, **kw)
+        t["y"][2] *= 4
+        h = act.residual_norm(t["y"], t.get("residual"), t["weight"], after_weight=t.get("after_weight"), eps=1e-5, **kw)[0]
+        assert bool(torch.isnan(h[2]).all()) and bool(torch.isfinite(h[[0, 1, 3, 4, 5]]).all())
