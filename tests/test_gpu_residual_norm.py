@@ -641,3 +641,47 @@ def test_rows_near_the_largest_sum_of_squares(act, cols):
         t["y"][2] *= 4
         h = act.residual_norm(t["y"], t.get("residual"), t["weight"], after_weight=t.get("after_weight"), eps=1e-5, **kw)[0]
         assert bool(torch.isnan(h[2]).all()) and bool(torch.isfinite(h[[0, 1, 3, 4, 5]]).all())
+
+
+@pytest.mark.parametrize("shape,gate", [((40001, 512), (512,)), ((30001, 256), (256,)), ((8190, 3, 512), (8190, 1, 512)), ((20000, 768), (768,)), ((40, 900, 768), (40, 1, 768)), ((4095, 64), (4095, 64)),
+                                        ((5001, 4096), (4096,)), ((16, 300, 4096), (16, 1, 4096)), ((4100, 5000), (5000,)), ((1201, 8192), (8192,)), ((2001, 8200), (8200,)), ((7, 160, 8200), (7, 1, 8200)),
+                                        ((601, 16390), (16390,))])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("stream", [BF, FP], ids=str)
+def test_every_row_counts_once(act, shape, gate, eight, stream):
+    """The sums over the rows of numbers that binary32 adds without rounding: a row that is lost, or taken twice, changes them.  Rows of +1 and -1, as many of each, have a mean of 0, a
+    mean square of 1 and, with eps 0, are their own norm; what is multiplied with them are whole numbers up to 7, of which 2^24 / 7 add up exactly.  The weight is 0 and its gradient is
+    not: nothing but the gradient of r reaches the gate and the norm after the block."""
+    cols, flat = shape[-1], (-1, shape[-1])
+    rows = math.prod(shape[:-1])
+    g = torch.Generator(device=DEV).manual_seed(rows)
+
+    def signs(*size):
+        return 1.0 - 2.0 * torch.randint(0, 2, size, generator=g, device=DEV).float()
+
+    def whole():
+        return torch.randint(1, 8, shape, generator=g, device=DEV).float()
+    # each pair of columns has both signs, which gate and weight change together
+    y = torch.stack((signs(*shape[:-1], cols // 2),) * 2, -1).mul_(torch.tensor([1.0, -1.0], device=DEV)).view(shape)
+    t = {"y": y.to(BF), "weight": torch.zeros(cols, device=DEV), "bias": torch.zeros(cols, device=DEV), "after_bias": torch.zeros(cols, device=DEV),
+         "gate": signs(*gate[:-1], cols // 2).repeat_interleave(2, -1), "after_weight": signs(cols // 2).repeat_interleave(2)}
+    dh, dr = whole(), whole()
+    per = t["gate"] if len(gate) == 1 else t["gate"].expand(shape)
+    after = y * t["after_weight"]
+    r = after * per
+    want = {"weight": dh * r, "bias": dh, "gate": dr * after, "after_weight": dr * per * y, "after_bias": dr * per}
+    for names in (list(want), ["weight", "bias"], ["gate", "after_weight"]):
+        # without the norm after the block where nothing of it is wanted
+        sandwich = "after_weight" in names
+        leaf = {k: v.detach().requires_grad_(k in names) for k, v in t.items()}
+        residual = torch.zeros(shape, dtype=stream, device=DEV)
+        kw = dict(gate=leaf["gate"], after=True, after_weight=leaf["after_weight"], after_bias=leaf["after_bias"]) if sandwich else {}
+        for center in (False, True):
+            got = act.residual_norm(leaf["y"], residual, leaf["weight"], leaf["bias"], center=center, eps=0.0, checkpoint=eight, **kw)
+            assert torch.equal(got[1].float(), r if sandwich else y)
+            grads = dict(zip(names, torch.autograd.grad(got[:2], [leaf[k] for k in names], (dh.to(BF), dr.to(stream)))))
+            for k in names:
+                v = want[k] if sandwich or k != "weight" else dh * y
+                v = v.double().view(shape)
+                v = v.sum(1, keepdim=True) if k == "gate" and len(gate) == 3 else v if k == "gate" and len(gate) == len(shape) else v.reshape(flat).sum(0)
+                assert torch.equal(grads[k].double(), v), (k, center, names)
