@@ -33,7 +33,9 @@ hipError_t launch_norm(BlockNormArgs a, int dtype, bool stream32, hipStream_t st
 // How a backward pass shares its rows out.  As many workgroups as the chip holds at once, two a CU, or one of a thousand threads (1024 x 8192 in 20 us, with two in turn 26); more
 // would leave more sums to add up, fewer take longer than what that saves (with at least 4, 8 or 16 rows each 1024 x 4096 takes 1 % less, 7 and 60 % more).  Teams of as many threads as
 // a row takes, or the 64 of a tile of a wide one, up to 512 together in a workgroup, have runs of `run` rows -- `parts` of them (the last ones shorter) to the rows of a gate, all of a
-// workgroup's of the same one, or one of whole gates.
+// workgroup's of the same one, or one of whole gates (then up to twice as many workgroups).  A gate that would be two runs or less is one: shared out among all of a workgroup's teams it
+// would take a workgroup, most of whose teams had nothing to do (both passes over 8190 x 512 with 3 rows a gate 31 us, 83 shared out, with 2 rows 28; 12288 x 256 with 4 rows 30 and 66;
+// 4096 x 14336 with 32 rows 397 and 454; nothing measured is slower).  At three runs 8190 x 512 with 5 rows would gain as well (59 to 31), but 30000 x 64 with 24 lose (52 to 65).
 NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols, bool between)
 {
     NormShares s;
@@ -42,8 +44,8 @@ NormShares norm_shares(int64_t rows, int64_t per, uint32_t cols, bool between)
     s.teams = std::max(1u, 512 / threads);
     const int64_t runs = std::max(1u, (threads > 512 ? 256 : 512) / tiles) * (int64_t)s.teams;
     int64_t run = (rows + runs - 1) / runs;
-    if (per == 0 || per <= run) {
-        if (per) run = run / per * per;
+    if (per == 0 || per <= run || (s.teams > 2 && per <= 2 * run)) {
+        if (per) run = std::max(run / per, (int64_t)1) * per;
         s.parts = 1;
         s.grid = (uint32_t)((rows + run * s.teams - 1) / (run * s.teams));
     } else {

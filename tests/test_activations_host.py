@@ -175,3 +175,15 @@ def test_residual_norm_refuses_checkpoints_beyond_their_size(L):
     assert L.dq_residual_norm_work_floats(ctypes.byref(capi.ResidualNorm(**backward))) > 0
     small = dict(backward, rows=(1 << 20) - 1, after=1, keep_r=1, keep_y=1, kept=0x1000)
     assert L.dq_residual_norm_work_floats(ctypes.byref(capi.ResidualNorm(**small))) > 0
+
+
+def test_residual_norm_shares_its_rows_out(L):
+    """A gate with somewhat more rows than a team would take makes no more workgroups, and partial sums of theirs, than others do: two a CU, in wide rows for all of their tiles together,
+    and twice as many where runs of whole gates are shorter than the others, by less than half"""
+    from dynamiq_sigcomm_artifact_amd import capi
+    for cols, rows, pers in ((512, 8190, (1, 2, 3)), (512, 8192, (4,)), (256, 12288, (1, 2, 3, 4, 6)), (64, 30000, (1, 6, 8, 12)), (1024, 2048, (1, 2)), (14336, 4096, (1, 16, 32)), (32768, 984, (8, 24))):
+        for per in pers:
+            o = capi.ResidualNorm(y=0x1000, residual=0x1000, gate=0x1000, h=0x1000, r=0x1000, rows=rows, cols=cols, rows_per_gate=per, eps=1e-5, residual_scale=1.0, block_scale=1.0, dtype=1,
+                                  stream_dtype=1, before=1, stats=0x1000, dh=0x1000, dweight=0x1000)
+            workgroups = (L.dq_residual_norm_work_floats(ctypes.byref(o)) - (4 * rows if cols > 8192 else 0)) / cols
+            assert workgroups <= 2 * (512 if cols <= 8192 else 512 // -(-cols // 512)), (cols, rows, per, workgroups)
