@@ -79,7 +79,9 @@ hipError_t launch_checkpoint_restore(const uint8_t *data, void *out, int64_t row
 
 // ---- the gated activation -----------------------------------------------------------------------------------
 
-// sigmoid(q) and 1 - sigmoid(q), both to their own precision: with e = exp(-|q|) they are 1 / (1 + e) and e / (1 + e)
+// sigmoid(q) and 1 - sigmoid(q), neither from the other: with e = exp(-|q|) they are 1 / (1 + e) and e / (1 + e).  For 16-bit types e is the machine's power of two of -|q| log2(e), off by
+// (2 + 2 |q|) 2^-24 of itself, and the quotient its reciprocal, by 2^-23: 2^-16 at |q| = 88, the largest, a fortieth at most of the rounding to 16 bits that follows.  With the functions that
+// binary32 takes 8192 x 14336 bf16 is 141 us for 112 forward (160 for 129 with the checkpoint), 363 for 351 in both passes with checkpoints.
 template <int DT> __device__ __forceinline__ void sigmoids(float q, float &s, float &rest)
 {
     const float e = DT == DQ_F32 ? expf(-__builtin_fabsf(q)) : __expf(-__builtin_fabsf(q));
@@ -108,8 +110,8 @@ struct GatedCall {
 static_assert(sizeof(GatedCall) <= 128, "a launch whose arguments are longer takes longer");
 
 // A lane takes eight elements, four of them a block of 32, padding included: the last block of a row may be a part.  Bound by memory: 8192 x 14336 bf16 with all three checkpoints
-// in 158 to 170 us by the box (6.3 to 6.8 TB/s, where loads and the result carry the hint; 178 without, and 175 with it on the checkpoints too), backward from them in 165 to 174
-// (5.4 to 5.7 TB/s): half of that is stores, in two streams.  The hint on its stores takes 161 on one box and 190 on another, on its loads 173 and 170; two units a lane 8 % more,
+// in 158 to 170 us by the box (6.3 to 6.8 TB/s, where loads and the result carry the hint; 178 without, and 175 with it on the checkpoints too), backward from them in 165 to 179
+// (5.3 to 5.7 TB/s): half of that is stores, in two streams.  Without checkpoints 112 (6.3 TB/s) and 205 (5.7 TB/s); fp32 4096 x 14336 138 and 203.  The hint on its stores takes 161 on one box and 190 on another, on its loads 173 and 170; two units a lane 8 % more,
 // workgroups of 1024 5 %.
 template <int DT, int KIND, bool EIGHT, bool PASSING> __global__ __launch_bounds__(256) void gated_kernel(GatedCall call)
 {

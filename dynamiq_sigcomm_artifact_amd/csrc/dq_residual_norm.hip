@@ -14,6 +14,8 @@ static uint32_t norm_threads(uint32_t cols)
 
 // Rows of which a thread would have more than its registers hold: in LDS forward, and read twice backward.  2048 x 14336 bf16 with both norms and a gate, forward 63 us and backward 139
 // (registers that spill 90 and 344), 1000 x 32768 with one norm 50 and 80 (118 and 281); 4096 x 8192 with both norms and a gate would take 150 backward in place of 96.
+// With a residual alone registers are the better place as far as they go, though they spill 52 to 140 values of fp32, and of a 32-bit stream with a bias: both passes over 2048 x 14336 bf16
+// 100 us (113 read twice), with a 32-bit stream 177 (187), fp32 228 (247), 4096 x 8200 with a 32-bit stream and a bias 241 (260); that form alone is slower in the widest, 208 for 193.
 static bool norm_wide(uint32_t cols, bool between) { return cols > 16384 || (between && cols > 8192); }
 
 // Whether a pass' arrays, four or so, are more than half of the 256 MB cache: then its loads carry the hint that nothing of them is wanted again soon.

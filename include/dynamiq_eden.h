@@ -891,7 +891,7 @@ int dq_checkpoint_restore(const uint8_t *data, void *out, int dtype, int64_t row
  *   DQ_SILU       q = g
  *   DQ_GELU_TANH  q = 2 sqrt(2 / pi) (g + 0.044715 g^3)
  * and backward, of d = the gradient of out:  dgate = d up (s + g s (1 - s) q'),  dup = d act(gate).
- * In binary32, rounded once. */
+ * In binary32, rounded once; for 16-bit types the sigmoid is off by up to (6 + 6 |q|) 2^-24 of itself before that. */
 enum dq_activation { DQ_SILU = 0, DQ_GELU_TANH = 1 };
 typedef struct dq_gated {
     const void *gate, *up;           /* `dtype` [rows][cols], row i from element i * stride on (halves of one matrix, for one) */

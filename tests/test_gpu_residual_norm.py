@@ -632,7 +632,7 @@ def test_rows_near_the_largest_sum_of_squares(act, cols):
     for dtype, parts, kw in ((FP, ("weight",), {}), (BF, ("weight",), {"center": True}), (FP, ("residual", "weight", "after_weight"), {"after": True})):
         t = tensors((6, cols), dtype, dtype, parts, 1)
         v = t["y"].double()
-        # (a norm takes the squares of y, and the other those of r: the same here, as the residual is small beside them)
+        # (with a norm after the block it is that one which takes them)
         t["y"] = (v * (0.9 * 2.0 ** 64 / v.square().sum(-1, keepdim=True).sqrt())).to(dtype)
         if "after" not in kw:
             against_definition(act, t, True, False, eps=0.0, **kw)
