@@ -164,8 +164,8 @@ template <int DT, int RAND, bool ROTATE> __global__ __launch_bounds__(256) void 
 // instructions change it.  Half as wide a tile, with runs of 128 bytes of x, takes half as long again to the nearest.  Blocks that have to be lowered are looked for while their columns
 // are encoded and taken behind the loop, where nothing else needs registers (in it: 2 to 6 % for every matrix); to the nearest four workgroups share a CU, which 65 registers would not let them.
 // A checkpoint's tile is twice as wide where that leaves a workgroup for each CU, 16 columns a lane: runs of 256 bytes of it as of a 16-bit matrix (8192 x 14336 rotated 53 us for 62,
-// to the nearest 42 for 55; 2560 x 2560, which it does not, 10.3 for 7.0).  Vector instructions take nine tenths of that time rotated, the butterflies in front (the same on the matrix
-// cores has not been built), and to the nearest six tenths, beside 4.0 TB/s.
+// to the nearest 42 for 55; 2560 x 2560, which it does not, 10.3 for 7.0).  Vector instructions, at four cycles each, are nine tenths of that time rotated, the butterflies in front (the
+// same on the matrix cores has not been built), and six tenths to the nearest, beside 4.0 TB/s.
 inline uint32_t columns_tiles(int64_t cols, uint32_t each) { return (uint32_t)((cols + 16 * each - 1) / (16 * each)); }
 template <uint32_t LINES> struct ColumnsLds {
     __attribute__((aligned(16))) uint8_t tile[LINES * 128];
