@@ -645,7 +645,7 @@ def test_rows_near_the_largest_sum_of_squares(act, cols):
 
 @pytest.mark.parametrize("shape,gate", [((40001, 512), (512,)), ((30001, 256), (256,)), ((20000, 768), (768,)), ((5001, 4096), (4096,)), ((4100, 5000), (5000,)), ((1201, 8192), (8192,)),
                                         ((2001, 8200), (8200,)), ((601, 16390), (16390,)), ((4095, 64), (4095, 64)), ((8190, 3, 512), (8190, 1, 512)), ((2730, 3, 512), (2730, 1, 512)),
-                                        ((3072, 4, 256), (3072, 1, 256)), ((1001, 5, 512), (1001, 1, 512)), ((90, 3, 8200), (90, 1, 8200)), ((40, 900, 768), (40, 1, 768)),
+                                        ((3000, 4, 256), (3000, 1, 256)), ((1001, 5, 512), (1001, 1, 512)), ((90, 3, 8200), (90, 1, 8200)), ((40, 900, 768), (40, 1, 768)),
                                         ((16, 300, 4096), (16, 1, 4096)), ((7, 160, 8200), (7, 1, 8200))])
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("stream", [BF, FP], ids=str)
