@@ -111,8 +111,8 @@ static_assert(sizeof(GatedCall) <= 128, "a launch whose arguments are longer tak
 
 // A lane takes eight elements, four of them a block of 32, padding included: the last block of a row may be a part.  Bound by memory: 8192 x 14336 bf16 with all three checkpoints
 // in 158 to 170 us by the box (6.3 to 6.8 TB/s, where loads and the result carry the hint; 178 without, and 175 with it on the checkpoints too), backward from them in 165 to 179
-// (5.3 to 5.7 TB/s): half of that is stores, in two streams.  Without checkpoints 112 (6.3 TB/s) and 205 (5.7 TB/s); fp32 4096 x 14336 138 and 203.  The hint on its stores takes 161 on one box and 190 on another, on its loads 173 and 170; two units a lane 8 % more,
-// workgroups of 1024 5 %.
+// (5.3 to 5.7 TB/s): half of that is stores, in two streams.  The hint on its stores takes 161 on one box and 190 on another, on its loads 173 and 170; two units a lane 8 % more,
+// workgroups of 1024 5 %.  Without checkpoints 112 (6.3 TB/s) and 205 (5.7 TB/s); fp32 4096 x 14336 138 and 203.
 template <int DT, int KIND, bool EIGHT, bool PASSING> __global__ __launch_bounds__(256) void gated_kernel(GatedCall call)
 {
     const GatedArgs &a = call.a;
